@@ -511,6 +511,110 @@ int64_t vapi_spill_promote(vapi_spill_store* store, const vapi_kv_pool* pool,
                            const uint8_t* hashes, const uint32_t* ids, uint32_t n,
                            void* pinned, size_t pinned_bytes, vapi_stream_t stream);
 
+/* ---- 8-bit caches --------------------------------------------------------- */
+
+/*
+ * A paged K/V pool held in 8 bits: codes as in vapi_kv_pool (same layouts,
+ * same slots), and one f32 scale for each (block, kv head) of K and of V. A
+ * code c stands for c * scale. Half the bytes of a 16-bit pool, so twice the
+ * context per GPU and about twice the decode rate. No counterpart in the
+ * reference, whose pools hold the model's own dtype (cache.rs:12-118).
+ *
+ * Scales are powers of two (0: the block holds only zeros): codes times
+ * scale is then exact in the rows' dtype, and taking a block's codes to a
+ * larger scale is an exact shift (e4m3, above its subnormals) or a single
+ * rounding of the last bits (int8).
+ *
+ * VAPI_KV_Q8_E4M3: OCP e4m3 (3 bits of mantissa; a value is off by at most
+ *   2^-4 of itself), which suits rows whose channels differ much in size.
+ * VAPI_KV_Q8_INT8: -127 .. 127; a value is off by at most half a step, 2^-7
+ *   to 2^-8 of the block's largest (a whole step at the largest itself).
+ *
+ * dtype is that of the rows appended and gathered, of q and of out:
+ * VAPI_KV_F16 or VAPI_KV_BF16. head_dim is a multiple of 16 up to 256,
+ * block_size a power of two from 16 to 256 (else VAPI_KV_EUNSUP).
+ *
+ * Layer l's codes start at k/v + l * layer_stride_bytes, its scales at
+ * k_scale/v_scale + l * scale_layer_stride_bytes; block b's scale of head h
+ * is element b * scale_block_stride + h. k, v and layer_stride_bytes are
+ * multiples of 16 bytes, the scales of 4.
+ */
+typedef enum { VAPI_KV_Q8_E4M3 = 0, VAPI_KV_Q8_INT8 = 1 } vapi_kv_q8_format;
+
+typedef struct vapi_kv_q8_pool {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  uint64_t layer_stride_bytes;
+  uint64_t scale_layer_stride_bytes;
+  uint32_t scale_block_stride; /* in f32, at least num_kv_heads */
+  uint32_t num_layers;
+  uint32_t num_blocks;
+  uint32_t block_size;
+  uint32_t num_kv_heads;
+  uint32_t head_dim;
+  uint32_t dtype;  /* VAPI_KV_F16 or VAPI_KV_BF16 */
+  uint32_t format; /* vapi_kv_q8_format */
+  uint32_t layout; /* vapi_kv_layout */
+} vapi_kv_q8_pool;
+
+/*
+ * vapi_kv_append into an 8-bit pool: k_src, v_src [n_tokens, num_kv_heads,
+ * head_dim] of the pool's dtype, 16-byte aligned, to slots slot_mapping[i]
+ * (VAPI_KV_SLOT_SKIP and slots past the pool are dropped). Per block touched,
+ * kv head, K and V:
+ *   - a call that writes the block's first slot starts the block: what it
+ *     held before counts for nothing, and its slots not written become 0;
+ *     any other call adds to what the block holds;
+ *   - the scale becomes the least power of two, no smaller than the one the
+ *     block had, that takes the largest new magnitude into the format (at
+ *     most 448 in e4m3, below 128 in int8);
+ *   - new rows are rounded to nearest (ties to even) under it, and where it
+ *     grew the codes already there are rounded to it.
+ * NaN is stored as 0 and infinities as the largest value of the format at
+ * the largest scale, so a pool written by this call alone holds finite
+ * values. The result does not depend on the order of tokens within a call.
+ *
+ * The tokens of one block must follow one another in slot_mapping (skipped
+ * tokens between them aside), as a step's tokens do sequence by sequence;
+ * duplicate slots, or a block's tokens in two places, leave that block's
+ * contents undefined.
+ */
+int vapi_kv_q8_append(const vapi_kv_q8_pool* pool, uint32_t layer, const void* k_src,
+                      const void* v_src, const uint32_t* slot_mapping, uint32_t n_tokens,
+                      vapi_stream_t stream);
+
+/* vapi_kv_gather from an 8-bit pool: the values in the pool's dtype. k_out
+ * and v_out (either may be NULL) are 16-byte aligned. */
+int vapi_kv_q8_gather(const vapi_kv_q8_pool* pool, uint32_t layer, const uint32_t* block_table,
+                      uint32_t n_table, uint32_t len_k, void* k_out, void* v_out,
+                      vapi_stream_t stream);
+
+/*
+ * vapi_paged_attention_prepared over an 8-bit pool: the attention of the
+ * values the codes stand for, computed in the pool's dtype on matrix cores
+ * with f32 sums as for a 16-bit pool. Same arguments (q and out of the
+ * pool's dtype), same flags, same meaning of prefill_seqs, same rules for
+ * the workspace (zero-fill it once; one per stream; calls sharing one must
+ * not overlap), except that prefill_seqs == NULL with n_prefill == 0 and
+ * max_seqlen_q > 1 covers every sequence, and that a call with prefill rows
+ * needs the whole size that _workspace_size returns: their codes are
+ * expanded there once, n_prefill * max_seqlen_k keys of the layer in the
+ * pool's dtype. n_prefill is the list's length, or batch without a list.
+ * Groups of up to 256 query heads per kv head.
+ */
+size_t vapi_kv_q8_attention_workspace_size(const vapi_kv_q8_pool* pool, uint32_t batch,
+                                           uint32_t n_prefill, uint32_t num_heads,
+                                           uint32_t max_seqlen_q, uint32_t max_seqlen_k);
+int vapi_kv_q8_attention(const vapi_kv_q8_pool* pool, uint32_t layer, const void* q, void* out,
+                         const uint32_t* cu_seqlens_q, const uint32_t* cu_seqlens_k,
+                         const uint32_t* block_table, uint32_t batch, uint32_t max_blocks,
+                         uint32_t max_seqlen_q, uint32_t max_seqlen_k, uint32_t num_heads,
+                         float scale, int32_t window_left, int32_t window_right, uint32_t flags,
+                         const uint32_t* prefill_seqs, uint32_t n_prefill, void* workspace,
+                         size_t workspace_bytes, vapi_stream_t stream);
+
 /*
  * Host-side check of a step descriptor: ForwardBatch::validate
  * (crates/vapi-engine/src/backend.rs:96-204). All arrays are host memory.

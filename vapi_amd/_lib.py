@@ -19,6 +19,7 @@ OK, EINVAL, EUNSUP, EHIP, ESPACE = 0, -1, -2, -3, -4
 ATTN_DETERMINISTIC, ATTN_NO_DECODE_ROWS = 0x1, 0x2
 ATTN_SCRATCH_BYTES = 16 << 20  # VAPI_ATTN_SCRATCH_BYTES
 APPEND_COLD_SOURCE = 0x1  # VAPI_APPEND_COLD_SOURCE
+Q8_E4M3, Q8_INT8 = 0, 1  # vapi_kv_q8_format
 
 # Every symbol include/vapi_kv.h declares.
 EXPORTS = (
@@ -38,6 +39,8 @@ EXPORTS = (
     "vapi_paged_attention_ex", "vapi_paged_attention_append_ex",
     "vapi_paged_attention_noalloc",
     "vapi_paged_attention_prepared", "vapi_paged_attention_prepared_workspace_size",
+    "vapi_kv_q8_append", "vapi_kv_q8_gather", "vapi_kv_q8_attention",
+    "vapi_kv_q8_attention_workspace_size",
 )
 
 
@@ -65,6 +68,27 @@ class Pool(ctypes.Structure):
     ]
 
 
+class Q8Pool(ctypes.Structure):
+    """vapi_kv_q8_pool."""
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("layer_stride_bytes", ctypes.c_uint64),
+        ("scale_layer_stride_bytes", ctypes.c_uint64),
+        ("scale_block_stride", ctypes.c_uint32),
+        ("num_layers", ctypes.c_uint32),
+        ("num_blocks", ctypes.c_uint32),
+        ("block_size", ctypes.c_uint32),
+        ("num_kv_heads", ctypes.c_uint32),
+        ("head_dim", ctypes.c_uint32),
+        ("dtype", ctypes.c_uint32),
+        ("format", ctypes.c_uint32),
+        ("layout", ctypes.c_uint32),
+    ]
+
+
 _lib = None
 _vp = ctypes.c_void_p
 _u32 = ctypes.c_uint32
@@ -72,6 +96,7 @@ _i32 = ctypes.c_int32
 _sz = ctypes.c_size_t
 _u32p = ctypes.POINTER(ctypes.c_uint32)
 _poolp = ctypes.POINTER(Pool)
+_q8p = ctypes.POINTER(Q8Pool)
 
 
 class SpillStats(ctypes.Structure):
@@ -146,6 +171,13 @@ def lib():
     L.vapi_cache_export_block.argtypes = [_vp, _u32, _vp, _sz]
     L.vapi_cache_import_block.argtypes = [_vp, _u32, _vp, _sz]
     L.vapi_cache_copy_blocks.argtypes = [_vp, _u32p, _u32]
+    L.vapi_kv_q8_append.argtypes = [_q8p, _u32, _vp, _vp, _vp, _u32, _vp]
+    L.vapi_kv_q8_gather.argtypes = [_q8p, _u32, _vp, _u32, _u32, _vp, _vp, _vp]
+    L.vapi_kv_q8_attention_workspace_size.argtypes = [_q8p, _u32, _u32, _u32, _u32, _u32]
+    L.vapi_kv_q8_attention_workspace_size.restype = _sz
+    L.vapi_kv_q8_attention.argtypes = [
+        _q8p, _u32, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32,
+        ctypes.c_float, _i32, _i32, _u32, _vp, _u32, _vp, _sz, _vp]
     L.vapi_spill_open.argtypes = [ctypes.c_char_p, ctypes.c_uint64, ctypes.c_uint64,
                                   ctypes.POINTER(_vp)]
     L.vapi_spill_close.argtypes = [_vp]

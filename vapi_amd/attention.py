@@ -15,7 +15,7 @@ import numpy as np
 import torch
 
 from ._lib import ESPACE, check, lib
-from .cache import PagedKvCache, _per_layer, stream_handle
+from .cache import PagedKvCache, _is_quantised, _per_layer, stream_handle, write_rows_indexed
 
 _u32p = ctypes.POINTER(ctypes.c_uint32)
 
@@ -146,20 +146,27 @@ class PreparedAttention:
         max_q, max_k = max(self.max_seqlen_q, 1), max(self.max_seqlen_k, 1)
         layers = ([cache.layer_view(l) for l, s in enumerate(cache.layouts) if s[0] == "kv"]
                   if isinstance(cache, HybridKvCache) else [cache])
-        need = max(workspace_bytes(c, b, num_heads, max_q, max_k, self.n_prefill_arg())
+        need = max(workspace_bytes(c, b, num_heads, max_q, max_k, self.n_prefill_arg(c))
                    for c in layers)
         if need and (self.workspace is None or self.workspace.numel() < need):
             self.workspace = torch.zeros(need, dtype=torch.uint8, device=device)
 
-    def n_prefill_arg(self) -> int | None:
-        """The prefill sequence count the calls pass (None: no list)."""
+    def n_prefill_arg(self, cache=None) -> int | None:
+        """The prefill sequence count the calls pass (None: no list). Over an
+        8-bit cache a prefill-only step covers every sequence of the batch."""
+        if cache is not None and _is_quantised(cache) and self.flags & ATTN_NO_DECODE_ROWS:
+            return None
         return self.n_prefill if self.prefill_seqs is not None else None
 
 
 def workspace_bytes(cache: PagedKvCache, batch: int, num_heads: int, max_q: int,
                     max_k: int, n_prefill: int | None = None) -> int:
     """vapi_paged_attention_workspace_size, or with `n_prefill` (a call that
-    names its prefill sequences) vapi_paged_attention_prepared_workspace_size."""
+    names its prefill sequences) vapi_paged_attention_prepared_workspace_size;
+    vapi_kv_q8_attention_workspace_size of a QuantKvCache."""
+    if _is_quantised(cache):
+        return lib().vapi_kv_q8_attention_workspace_size(
+            cache.q8, batch, batch if n_prefill is None else n_prefill, num_heads, max_q, max_k)
     if n_prefill is None:
         return lib().vapi_paged_attention_workspace_size(cache.pool, batch, num_heads,
                                                           max_q, max_k)
@@ -169,7 +176,7 @@ def workspace_bytes(cache: PagedKvCache, batch: int, num_heads: int, max_q: int,
 
 def _workspace(cache, prepared: PreparedAttention, b: int, num_heads: int, max_q: int,
                max_k: int, device):
-    need = workspace_bytes(cache, b, num_heads, max_q, max_k, prepared.n_prefill_arg())
+    need = workspace_bytes(cache, b, num_heads, max_q, max_k, prepared.n_prefill_arg(cache))
     ws = prepared.workspace
     if need and (ws is None or ws.numel() < need):
         # Zero-filled once: a zeroed workspace starts the decode from equal
@@ -204,8 +211,8 @@ def paged_attention_prepared(q: torch.Tensor, cache: PagedKvCache, layer: int,
                              out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """attention.rs:262-288 on libvapi_kv.so. None for a window side means
     unlimited (flash convention); the default right window 0 is causal.
-    `cache` may be a HybridKvCache: `layer` then names one of its K/V
-    layers."""
+    `cache` may be a HybridKvCache (`layer` then names one of its K/V layers)
+    or a QuantKvCache."""
     cache, layer = _per_layer(cache, layer)
     if q.dim() != 3 or q.shape[2] != cache.head_dim:
         raise ValueError(f"q must be (tokens, heads, {cache.head_dim}), got {tuple(q.shape)}")
@@ -224,7 +231,15 @@ def paged_attention_prepared(q: torch.Tensor, cache: PagedKvCache, layer: int,
             -1 if window_size_left is None else int(window_size_left),
             -1 if window_size_right is None else int(window_size_right), prepared.flags)
     handle = stream_handle(stream)
-    if prepared.prefill_seqs is None:
+    if _is_quantised(cache):
+        from .quant import check_on_device
+        check_on_device(cache.device, q, out, prepared.block_table, prepared.seqlens_q,
+                        prepared.seqlens_k)
+        listed = prepared.prefill_seqs is not None
+        args = (cache.q8,) + args[1:] + (prepared.prefill_seqs.data_ptr() if listed else None,
+                                         prepared.n_prefill if listed else 0)
+        fn = lib().vapi_kv_q8_attention
+    elif prepared.prefill_seqs is None:
         fn = lib().vapi_paged_attention_ex
     else:
         fn = lib().vapi_paged_attention_prepared
@@ -285,6 +300,14 @@ def paged_attention_append_prepared(q: torch.Tensor, k: torch.Tensor, v: torch.T
     num_heads = q.shape[1]
     max_q = max(int(prepared.max_seqlen_q), 1)
     max_k = max(int(prepared.max_seqlen_k), 1)
+    if _is_quantised(cache):
+        # Two calls; what the second would refuse is refused before the first.
+        if num_heads % cache.num_kv_heads or num_heads > 256 * cache.num_kv_heads:
+            raise ValueError(f"{num_heads} query heads over {cache.num_kv_heads} kv heads")
+        write_rows_indexed(cache, layer, k, v, slot_mapping, stream=stream)
+        return paged_attention_prepared(q, cache, layer, prepared, softmax_scale,
+                                        window_size_left, window_size_right, out=out,
+                                        stream=stream)
     if max_q > 1 and prepared.prefill_seqs is not None and cache.pool.v:
         # (A K-only pool goes to the library call below, which refuses it
         # before writing anything.)

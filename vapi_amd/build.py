@@ -38,7 +38,8 @@ COMMON_FLAGS = [
 ]
 
 SOURCES = ["kv_ops.hip", "attention.hip", "attn_decode.hip", "attn_decode_small.hip",
-           "attn_prefill.hip", "attn_prefill_f32.hip", "attn_generic.hip", "host.cpp", "spill.cpp"]
+           "attn_prefill.hip", "attn_prefill_f32.hip", "attn_generic.hip", "q8_ops.hip",
+           "attn_q8.hip", "host.cpp", "spill.cpp"]
 
 # The MFMA attention kernels never produce NaN from finite K/V/Q (masked
 # scores are -inf, running maxima start finite), so fmaxf on MFMA results
@@ -48,7 +49,8 @@ EXTRA_FLAGS = {"attn_decode.hip": ["-fno-honor-nans", "-Rpass-analysis=kernel-re
                                          "-Rpass-analysis=kernel-resource-usage"],
                "attn_prefill.hip": ["-fno-honor-nans", "-Rpass-analysis=kernel-resource-usage"],
                "attn_prefill_f32.hip": ["-fno-honor-nans",
-                                        "-Rpass-analysis=kernel-resource-usage"]}
+                                        "-Rpass-analysis=kernel-resource-usage"],
+               "attn_q8.hip": ["-fno-honor-nans", "-Rpass-analysis=kernel-resource-usage"]}
 
 # The prefill kernel's step barrier counts its own vector-memory operations
 # (the direct loads into LDS) with an explicit vmcnt wait, and the decode
@@ -58,7 +60,8 @@ EXTRA_FLAGS = {"attn_decode.hip": ["-fno-honor-nans", "-Rpass-analysis=kernel-re
 NO_SCRATCH = {"attn_prefill.hip": ("paged_prefill_tiled", "paged_mixed_stream"),
               "attn_decode.hip": ("paged_decode_stream",),
               "attn_decode_small.hip": ("paged_decode_small",),
-              "attn_prefill_f32.hip": ("paged_prefill_f32",)}
+              "attn_prefill_f32.hip": ("paged_prefill_f32",),
+              "attn_q8.hip": ("q8_decode_stream",)}
 
 # Half of a CU's 160 KiB of LDS less the dynamic part (4 bytes for each of the
 # 4,000 sequences that the launch takes, and one more): a workgroup of the mixed

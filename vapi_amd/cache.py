@@ -226,9 +226,34 @@ def _per_layer(cache, layer: int):
     return cache, layer
 
 
+def _is_quantised(cache) -> bool:
+    """Whether `cache` is a QuantKvCache (its per-layer calls are the 8-bit ones)."""
+    return getattr(cache, "q8", None) is not None
+
+
+def _write_quantised(cache, layer: int, k: torch.Tensor, v: torch.Tensor, idx: torch.Tensor,
+                     stream) -> None:
+    """write_rows_indexed into a QuantKvCache (vapi_kv_q8_append)."""
+    from .quant import check_on_device
+    want = (cache.num_kv_heads, cache.head_dim)
+    if v is None:
+        raise ValueError("an 8-bit cache is written K and V together")
+    if k.dim() != 3 or tuple(k.shape) != tuple(v.shape) or tuple(k.shape[1:]) != want:
+        raise ValueError(f"k/v must be (n, {want[0]}, {want[1]}), got {tuple(k.shape)} and "
+                         f"{tuple(v.shape)}")
+    if k.dtype != cache.dtype or v.dtype != cache.dtype:
+        raise ValueError(f"cache is {cache.dtype} but the rows are {k.dtype} and {v.dtype}")
+    check_on_device(cache.device, k, v, idx)
+    k, v, idx = k.contiguous(), v.contiguous(), idx.contiguous()
+    check(lib().vapi_kv_q8_append(cache.q8, layer, k.data_ptr(), v.data_ptr(), idx.data_ptr(),
+                                  k.shape[0], stream_handle(stream)))
+
+
 def _k_only(cache, which: str = "k"):
     """A view of `cache`'s pool that moves one buffer only (K, or V as if it
     were K): the single-buffer writes of cache.rs:150-159, 186-204."""
+    if _is_quantised(cache):
+        raise ValueError("an 8-bit cache is written K and V together")
     p = cache.pool
     base = p.k if which == "k" else p.v
     if base is None:
@@ -275,6 +300,9 @@ def write_kv_to_cache(cache: PagedKvCache, layer: int, k: torch.Tensor, v: torch
     real = slots[slots != _lib.SLOT_SKIP]
     if real.size and int(real.max()) >= cache.num_slots():
         raise ValueError(f"slot {int(real.max())} is past the end of the cache")
+    if _is_quantised(cache):
+        from .quant import check_block_runs
+        check_block_runs(slots, cache.block_size)
     if n == 0:
         return
     dev_slots = torch.from_numpy(slots.view(np.int32)).to(k.device, non_blocking=False)
@@ -322,13 +350,17 @@ def write_rows_indexed(cache, layer: int, k: torch.Tensor, v: torch.Tensor | Non
     launch for K and V, or for K alone when v is None (the reference's
     write_rows_indexed, cache.rs:176-185). Out-of-range slots are dropped
     on the device. cold_source: the rows are not in the GPU's caches (read
-    with streaming loads, VAPI_APPEND_COLD_SOURCE); same result."""
+    with streaming loads, VAPI_APPEND_COLD_SOURCE); same result. A
+    QuantKvCache takes K and V together, the tokens of a block one after the
+    other (vapi_kv_q8_append), and ignores cold_source."""
     cache, layer = _per_layer(cache, layer)
     if idx.dim() != 1 or idx.shape[0] != k.shape[0]:
         raise ValueError(f"scatter index {tuple(idx.shape)} does not match rows "
                          f"{tuple(k.shape)}")
     if idx.dtype not in (torch.int32, torch.uint32):
         raise TypeError("scatter index must be 32-bit")
+    if _is_quantised(cache):
+        return _write_quantised(cache, layer, k, v, idx, stream)
     k = k.contiguous()
     if v is None:
         check(lib().vapi_kv_append(_k_only(cache), layer, k.data_ptr(), None,
@@ -364,6 +396,8 @@ def write_kv_to_cache_layers(cache: PagedKvCache, layer0: int, k: torch.Tensor,
     separate pools: append to them one layer at a time.)"""
     if isinstance(cache, HybridKvCache):
         raise ValueError("a mixed cache's layers are separate pools: append per layer")
+    if _is_quantised(cache):
+        raise ValueError("an 8-bit cache is written one layer at a time")
     if k.dim() != 4 or tuple(k.shape) != tuple(v.shape):
         raise ValueError(f"k/v must be (layers, n, heads, width), got {tuple(k.shape)} "
                          f"and {tuple(v.shape)}")
@@ -385,7 +419,7 @@ def write_kv_to_cache_layers(cache: PagedKvCache, layer0: int, k: torch.Tensor,
 def gather_kv(cache: PagedKvCache, layer: int, block_table, len_k: int,
               which: str = "k", stream=None) -> torch.Tensor:
     """One sequence's K (or V) rows in logical order, [len_k, kvh, d]
-    (cache.rs:283-290)."""
+    (cache.rs:283-290); of a QuantKvCache the values, in its dtype."""
     cache, layer = _per_layer(cache, layer)
     if which == "v" and getattr(cache, "has_v", True) is False:
         raise ValueError("a rows layer stores no V")
@@ -398,6 +432,12 @@ def gather_kv(cache: PagedKvCache, layer: int, block_table, len_k: int,
         return out
     kp = out.data_ptr() if which == "k" else None
     vp = out.data_ptr() if which == "v" else None
+    if _is_quantised(cache):
+        from .quant import check_on_device
+        check_on_device(cache.device, table)
+        check(lib().vapi_kv_q8_gather(cache.q8, layer, table.data_ptr(), table.shape[0], len_k,
+                                      kp, vp, stream_handle(stream)))
+        return out
     check(lib().vapi_kv_gather(cache.pool, layer, table.data_ptr(), table.shape[0],
                                len_k, kp, vp, stream_handle(stream)))
     return out

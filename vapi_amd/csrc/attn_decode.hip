@@ -94,28 +94,36 @@ void decode_bind(AttnArgs& c, void* workspace, uint32_t head_dim) {
 uint32_t decode_max_plan_seqs() { return kMaxPlanSeqs; }
 
 // The merge launch of a (non-fused) decode whose stream ran in another
-// launch (the mixed step's): c is bound to its workspace, nwg the stream's
-// decode workgroups.
+// launch (the mixed step's, an 8-bit pool's): c is bound to its workspace, nwg
+// the stream's decode workgroups.
 void launch_decode_merge(const AttnArgs& c, uint32_t nwg, uint32_t head_dim, bool bf16,
-                         hipStream_t s) {
+                         hipStream_t s, uint32_t ns) {
   bool wide = false;
-  const uint32_t merge_wgs = decode_merge_wgs(c.batch, c.kvh, &wide);
+  const uint32_t merge_wgs = decode_merge_wgs(c.batch, c.kvh, &wide, ns);
 #define VK_MRG(T, DD, PAD)                                                                   \
   do {                                                                                       \
     if (wide && c.batch * c.kvh <= kFewSegs)                                                 \
       hipLaunchKernelGGL((paged_decode_merge<T, DD, false, 8, PAD>), dim3(merge_wgs),        \
-                         dim3(merge_threads(8)), 0, s, c, nwg, merge_wgs, 1u);               \
+                         dim3(merge_threads(8)), 0, s, c, nwg, merge_wgs, ns);               \
     else if (wide)                                                                           \
       hipLaunchKernelGGL((paged_decode_merge<T, DD, false, kMergeWaves, PAD>),               \
                          dim3(merge_wgs), dim3(merge_threads(kMergeWaves)), 0, s, c, nwg,    \
-                         merge_wgs, 1u);                                                     \
+                         merge_wgs, ns);                                                     \
     else                                                                                     \
       hipLaunchKernelGGL((paged_decode_merge<T, DD, false, 1, PAD>), dim3(merge_wgs),        \
-                         dim3(64 * kMergeWaves), 0, s, c, nwg, merge_wgs, 1u);               \
+                         dim3(64 * kMergeWaves), 0, s, c, nwg, merge_wgs, ns);               \
   } while (0)
   // A head_dim below the kernel's D: the padded merge.
   const bool pad = c.hd != head_dim;
-  if (bf16) {
+  if (head_dim == 256) {
+    if (bf16) {
+      if (pad) VK_MRG(bf16_t, 256, true);
+      else VK_MRG(bf16_t, 256, false);
+    } else {
+      if (pad) VK_MRG(f16_t, 256, true);
+      else VK_MRG(f16_t, 256, false);
+    }
+  } else if (bf16) {
     if (head_dim == 128) {
       if (pad) VK_MRG(bf16_t, 128, true);
       else VK_MRG(bf16_t, 128, false);

@@ -60,7 +60,9 @@ constexpr uint32_t kBalStats = 64;
 constexpr uint32_t kMinStepsPerWave = 8;  // launches that move the shares
 constexpr uint32_t kStatWords = 4;
 
-// Steps of sequence s (0 for rows that are not decode rows).
+// Steps of sequence s (0 for rows that are not decode rows). KS: keys per step
+// (a power of two; 32 but for the streams of 8-bit pools).
+template <int KS = 32>
 __device__ __forceinline__ uint32_t decode_steps(const AttnArgs& a,
                                                  const uint32_t* __restrict__ cu_q,
                                                  const uint32_t* __restrict__ cu_k, uint32_t s) {
@@ -68,7 +70,7 @@ __device__ __forceinline__ uint32_t decode_steps(const AttnArgs& a,
   const int32_t len_k = (int32_t)(cu_k[s + 1] - cu_k[s]);
   if (len_k <= 0) return 0;
   const int32_t lo = a.wl >= 0 ? max(0, len_k - 1 - a.wl) : 0;
-  return (uint32_t)(len_k - (lo & ~31) + 31) >> 5;
+  return (uint32_t)(len_k - (lo & ~(KS - 1)) + KS - 1) / KS;
 }
 
 // Fused append: whether decode row s's new key (position len_k - 1) comes
@@ -134,6 +136,7 @@ struct DecodePos {
 // kvh_plan: the kv heads the step order counts (a.kvh, or with a split
 // group's parts side by side the pool heads: then the position is part
 // `part` of pool head kp, virtual head kp * n + part).
+template <int KS = 32>
 __device__ __forceinline__ DecodePos locate(const AttnArgs& a, const uint32_t* __restrict__ cu_q,
                                             const uint32_t* __restrict__ cu_k, const uint32_t* P,
                                             const uint32_t* FZ, uint32_t t,
@@ -155,7 +158,7 @@ __device__ __forceinline__ DecodePos locate(const AttnArgs& a, const uint32_t* _
   p.q0 = cu_q[p.seq];
   p.len_k = (int32_t)(cu_k[p.seq + 1] - cu_k[p.seq]);
   p.lo = a.wl >= 0 ? max(0, p.len_k - 1 - a.wl) : 0;
-  p.key0 = (p.lo & ~31) + 32 * (int32_t)ks;
+  p.key0 = (p.lo & ~(KS - 1)) + KS * (int32_t)ks;
   p.seg_first = ks == 0;
   p.fuse = FZ ? FZ[lo_i] : 0u;
   return p;
@@ -165,6 +168,7 @@ __device__ __forceinline__ DecodePos locate(const AttnArgs& a, const uint32_t* _
 // or kv head 0 of the next sequence that has decode steps. A wave's slice
 // is contiguous, so the step after a segment's last is always this one,
 // and a wave that moves on from a finished segment needs no search.
+template <int KS = 32>
 __device__ __forceinline__ DecodePos next_segment(const AttnArgs& a,
                                                   const uint32_t* __restrict__ cu_q,
                                                   const uint32_t* __restrict__ cu_k,
@@ -186,7 +190,7 @@ __device__ __forceinline__ DecodePos next_segment(const AttnArgs& a,
     p.lo = a.wl >= 0 ? max(0, p.len_k - 1 - a.wl) : 0;
     p.fuse = FZ ? FZ[s] : 0u;
   }
-  p.key0 = p.lo & ~31;
+  p.key0 = p.lo & ~(KS - 1);
   p.seg_first = 1u;
   return p;
 }
@@ -842,9 +846,9 @@ DecodeWs decode_ws(uint32_t b, uint32_t kvh, uint32_t group, uint32_t head_dim,
                    uint32_t num_waves);
 // Points a's decode workspace fields into `workspace` (layout decode_ws).
 void decode_bind(AttnArgs& c, void* workspace, uint32_t head_dim);
-// The decode's merge launch alone (non-fused), after a stream of nwg
-// workgroups that ran inside another launch.
+// The decode's merge launch alone (non-fused, 16-bit outputs), after a stream
+// of nwg workgroups of another kernel; ns: slices per segment.
 void launch_decode_merge(const AttnArgs& c, uint32_t nwg, uint32_t head_dim, bool bf16,
-                         hipStream_t s);
+                         hipStream_t s, uint32_t ns = 1);
 
 }  // namespace vk
