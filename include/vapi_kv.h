@@ -615,6 +615,99 @@ int vapi_kv_q8_attention(const vapi_kv_q8_pool* pool, uint32_t layer, const void
                          const uint32_t* prefill_seqs, uint32_t n_prefill, void* workspace,
                          size_t workspace_bytes, vapi_stream_t stream);
 
+/* ---- attention weights and eviction ---------------------------------------- */
+
+/*
+ * A state of running attention weights: for each of `rows` sequences and each
+ * kv head one f32 per key position, `width` of them; element (r, h, k) is
+ * data[r * row_stride + h * head_stride + k]. index: device u32[batch], the
+ * row of each sequence of the call (NULL: sequence i has row i); the rows of
+ * a call must be distinct. A row index past `rows` leaves that sequence out.
+ * Such a state belongs to one layer; zero a row before a new sequence takes it.
+ */
+typedef struct vapi_kv_weights {
+  float* data;
+  const uint32_t* index;
+  uint64_t row_stride;
+  uint64_t head_stride;
+  uint32_t rows;
+  uint32_t width;
+} vapi_kv_weights;
+
+/*
+ * Adds to a state what a step's queries attend to. With p[j, h, k] the
+ * softmax of vapi_paged_attention (same arguments) for query j and query head
+ * h, for every sequence with queries, kv head g and key k < len_k:
+ *   w[g, k] = decay * w[g, k] + sum over the queries j taken and the query
+ *             heads h of g of p[j, h, k]
+ * last_queries: only the last min(len_q, last_queries) queries of a sequence
+ * are taken (0: all). decay 0 replaces what was there (whatever it holds).
+ * Positions from len_k on, and sequences with no query, stay as they were; a
+ * query that sees no key adds nothing. len_k is at most `width`
+ * (max_seqlen_k past it is refused). The sums run in f32, in an order fixed
+ * by the sizes: equal calls give equal bits.
+ *
+ * The pool's K alone is read: f16 or bf16, head_dim a multiple of 8 up to
+ * 256, block_size a power of two from 16 (else VAPI_KV_EUNSUP), or an 8-bit
+ * pool. q: 16-byte aligned. workspace: device scratch of
+ * vapi_kv_attention_weights_workspace_size bytes, 16-byte aligned, nothing in
+ * it kept between calls; calls sharing one must not overlap. No counterpart
+ * in the reference.
+ */
+size_t vapi_kv_attention_weights_workspace_size(uint32_t batch, uint32_t num_kv_heads,
+                                                uint32_t num_heads, uint32_t head_dim,
+                                                uint32_t max_seqlen_q, uint32_t max_seqlen_k,
+                                                uint32_t last_queries);
+int vapi_kv_attention_weights(const vapi_kv_pool* pool, uint32_t layer, const void* q,
+                              const uint32_t* cu_seqlens_q, const uint32_t* cu_seqlens_k,
+                              const uint32_t* block_table, uint32_t batch, uint32_t max_blocks,
+                              uint32_t max_seqlen_q, uint32_t max_seqlen_k, uint32_t num_heads,
+                              float scale, int32_t window_left, int32_t window_right,
+                              uint32_t last_queries, float decay, const vapi_kv_weights* weights,
+                              void* workspace, size_t workspace_bytes, vapi_stream_t stream);
+int vapi_kv_q8_attention_weights(const vapi_kv_q8_pool* pool, uint32_t layer, const void* q,
+                                 const uint32_t* cu_seqlens_q, const uint32_t* cu_seqlens_k,
+                                 const uint32_t* block_table, uint32_t batch, uint32_t max_blocks,
+                                 uint32_t max_seqlen_q, uint32_t max_seqlen_k, uint32_t num_heads,
+                                 float scale, int32_t window_left, int32_t window_right,
+                                 uint32_t last_queries, float decay,
+                                 const vapi_kv_weights* weights, void* workspace,
+                                 size_t workspace_bytes, vapi_stream_t stream);
+
+/*
+ * Moves the keys worth keeping of one layer's sequences into other blocks.
+ * A sequence of lens[i] keys (device u32[batch], each at most max_len) keeps
+ * n = min(lens[i], budget) of them per kv head: its first `sinks`, its last
+ * `recent`, and of the others those with the largest weights (ties: the
+ * earlier key; a NaN ranks below every number). Kept key number j of a head,
+ * in order of position, goes to position j of the sequence's dst table:
+ *   kept[(i * kvh + h) * max_keep + j]  its position before (-1 from n on),
+ *     max_keep = min(budget, max_len); device i32, required
+ *   K and V rows, bit for bit; in an 8-bit pool the codes under the new
+ *     block's scale (the least power of two that holds them; a code is rounded
+ *     again only where its scale grows), slots past n of the last block 0
+ *   out (may be NULL): w[h, j] = the key's weight, 0 from n to `width`
+ * The heads of a sequence keep different keys; attention over the dst table
+ * with len_k = n sees each head's own. Every layer of a sequence is evicted
+ * with the same tables. budget is at least sinks + recent, and at least 1.
+ *
+ * dst blocks must not be named twice, nor be src blocks; the src blocks (which
+ * other sequences may share) stay as they were. out may be the same rows as
+ * in, or must not overlap it. A dst entry past the pool is not written, a src
+ * entry past it reads its last block. Any pool dtype, with or without V.
+ * No counterpart in the reference.
+ */
+int vapi_kv_evict(const vapi_kv_pool* pool, uint32_t layer, const vapi_kv_weights* in,
+                  const vapi_kv_weights* out, const uint32_t* lens, const uint32_t* src_table,
+                  uint32_t src_blocks, const uint32_t* dst_table, uint32_t dst_blocks,
+                  uint32_t batch, uint32_t max_len, uint32_t budget, uint32_t sinks,
+                  uint32_t recent, int32_t* kept, vapi_stream_t stream);
+int vapi_kv_q8_evict(const vapi_kv_q8_pool* pool, uint32_t layer, const vapi_kv_weights* in,
+                     const vapi_kv_weights* out, const uint32_t* lens, const uint32_t* src_table,
+                     uint32_t src_blocks, const uint32_t* dst_table, uint32_t dst_blocks,
+                     uint32_t batch, uint32_t max_len, uint32_t budget, uint32_t sinks,
+                     uint32_t recent, int32_t* kept, vapi_stream_t stream);
+
 /*
  * Host-side check of a step descriptor: ForwardBatch::validate
  * (crates/vapi-engine/src/backend.rs:96-204). All arrays are host memory.

@@ -41,6 +41,8 @@ EXPORTS = (
     "vapi_paged_attention_prepared", "vapi_paged_attention_prepared_workspace_size",
     "vapi_kv_q8_append", "vapi_kv_q8_gather", "vapi_kv_q8_attention",
     "vapi_kv_q8_attention_workspace_size",
+    "vapi_kv_attention_weights", "vapi_kv_attention_weights_workspace_size",
+    "vapi_kv_q8_attention_weights", "vapi_kv_evict", "vapi_kv_q8_evict",
 )
 
 
@@ -89,6 +91,18 @@ class Q8Pool(ctypes.Structure):
     ]
 
 
+class Weights(ctypes.Structure):
+    """vapi_kv_weights."""
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("index", ctypes.c_void_p),
+        ("row_stride", ctypes.c_uint64),
+        ("head_stride", ctypes.c_uint64),
+        ("rows", ctypes.c_uint32),
+        ("width", ctypes.c_uint32),
+    ]
+
+
 _lib = None
 _vp = ctypes.c_void_p
 _u32 = ctypes.c_uint32
@@ -97,6 +111,7 @@ _sz = ctypes.c_size_t
 _u32p = ctypes.POINTER(ctypes.c_uint32)
 _poolp = ctypes.POINTER(Pool)
 _q8p = ctypes.POINTER(Q8Pool)
+_wp = ctypes.POINTER(Weights)
 
 
 class SpillStats(ctypes.Structure):
@@ -178,6 +193,15 @@ def lib():
     L.vapi_kv_q8_attention.argtypes = [
         _q8p, _u32, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32,
         ctypes.c_float, _i32, _i32, _u32, _vp, _u32, _vp, _sz, _vp]
+    L.vapi_kv_attention_weights_workspace_size.argtypes = [_u32] * 7
+    L.vapi_kv_attention_weights_workspace_size.restype = _sz
+    weights = [_u32, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, ctypes.c_float, _i32,
+               _i32, _u32, ctypes.c_float, _wp, _vp, _sz, _vp]
+    L.vapi_kv_attention_weights.argtypes = [_poolp] + weights
+    L.vapi_kv_q8_attention_weights.argtypes = [_q8p] + weights
+    evict = [_u32, _wp, _wp, _vp, _vp, _u32, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _vp, _vp]
+    L.vapi_kv_evict.argtypes = [_poolp] + evict
+    L.vapi_kv_q8_evict.argtypes = [_q8p] + evict
     L.vapi_spill_open.argtypes = [ctypes.c_char_p, ctypes.c_uint64, ctypes.c_uint64,
                                   ctypes.POINTER(_vp)]
     L.vapi_spill_close.argtypes = [_vp]

@@ -114,6 +114,7 @@ class PreparedAttention:
     flags: int = 0
     prefill_seqs: torch.Tensor | None = None
     n_prefill: int = 0
+    weights_workspace: torch.Tensor | None = None  # accumulate_attention_weights
 
     @classmethod
     def from_batch(cls, batch: ForwardBatch, device, cache=None, num_heads: int | None = None,

@@ -39,7 +39,7 @@ COMMON_FLAGS = [
 
 SOURCES = ["kv_ops.hip", "attention.hip", "attn_decode.hip", "attn_decode_small.hip",
            "attn_prefill.hip", "attn_prefill_f32.hip", "attn_generic.hip", "q8_ops.hip",
-           "attn_q8.hip", "host.cpp", "spill.cpp"]
+           "attn_q8.hip", "kv_weights.hip", "kv_evict.hip", "host.cpp", "spill.cpp"]
 
 # The MFMA attention kernels never produce NaN from finite K/V/Q (masked
 # scores are -inf, running maxima start finite), so fmaxf on MFMA results
@@ -50,7 +50,8 @@ EXTRA_FLAGS = {"attn_decode.hip": ["-fno-honor-nans", "-Rpass-analysis=kernel-re
                "attn_prefill.hip": ["-fno-honor-nans", "-Rpass-analysis=kernel-resource-usage"],
                "attn_prefill_f32.hip": ["-fno-honor-nans",
                                         "-Rpass-analysis=kernel-resource-usage"],
-               "attn_q8.hip": ["-fno-honor-nans", "-Rpass-analysis=kernel-resource-usage"]}
+               "attn_q8.hip": ["-fno-honor-nans", "-Rpass-analysis=kernel-resource-usage"],
+               "kv_weights.hip": ["-fno-honor-nans"]}
 
 # The prefill kernel's step barrier counts its own vector-memory operations
 # (the direct loads into LDS) with an explicit vmcnt wait, and the decode
