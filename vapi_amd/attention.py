@@ -15,7 +15,8 @@ import numpy as np
 import torch
 
 from ._lib import ESPACE, check, lib
-from .cache import PagedKvCache, _is_quantised, _per_layer, stream_handle, write_rows_indexed
+from .cache import (PagedKvCache, _is_quantised, _per_layer, check_on_device, stream_handle,
+                    write_rows_indexed)
 
 _u32p = ctypes.POINTER(ctypes.c_uint32)
 
@@ -233,9 +234,7 @@ def paged_attention_prepared(q: torch.Tensor, cache: PagedKvCache, layer: int,
             -1 if window_size_right is None else int(window_size_right), prepared.flags)
     handle = stream_handle(stream)
     if _is_quantised(cache):
-        from .quant import check_on_device
-        check_on_device(cache.device, q, out, prepared.block_table, prepared.seqlens_q,
-                        prepared.seqlens_k)
+        check_on_device(cache.k[0], q, out, prepared.block_table, prepared.seqlens_q)
         listed = prepared.prefill_seqs is not None
         args = (cache.q8,) + args[1:] + (prepared.prefill_seqs.data_ptr() if listed else None,
                                          prepared.n_prefill if listed else 0)

@@ -51,7 +51,7 @@ EXTRA_FLAGS = {"attn_decode.hip": ["-fno-honor-nans", "-Rpass-analysis=kernel-re
                "attn_prefill_f32.hip": ["-fno-honor-nans",
                                         "-Rpass-analysis=kernel-resource-usage"],
                "attn_q8.hip": ["-fno-honor-nans", "-Rpass-analysis=kernel-resource-usage"],
-               "kv_weights.hip": ["-fno-honor-nans"]}
+               "kv_weights.hip": ["-fno-honor-nans", "-Rpass-analysis=kernel-resource-usage"]}
 
 # The prefill kernel's step barrier counts its own vector-memory operations
 # (the direct loads into LDS) with an explicit vmcnt wait, and the decode
@@ -62,7 +62,8 @@ NO_SCRATCH = {"attn_prefill.hip": ("paged_prefill_tiled", "paged_mixed_stream"),
               "attn_decode.hip": ("paged_decode_stream",),
               "attn_decode_small.hip": ("paged_decode_small",),
               "attn_prefill_f32.hip": ("paged_prefill_f32",),
-              "attn_q8.hip": ("q8_decode_stream",)}
+              "attn_q8.hip": ("q8_decode_stream",),
+              "kv_weights.hip": ("weights_lse", "weights_sum")}
 
 # Half of a CU's 160 KiB of LDS less the dynamic part (4 bytes for each of the
 # 4,000 sequences that the launch takes, and one more): a workgroup of the mixed

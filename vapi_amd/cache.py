@@ -226,6 +226,20 @@ def _per_layer(cache, layer: int):
     return cache, layer
 
 
+def check_on_device(*tensors) -> None:
+    """Every tensor on one GPU, and that the current one: the library launches
+    on the current device's stream."""
+    if tensors[0].is_cuda:
+        now = torch._C._cuda_getDevice()
+        for t in tensors:
+            if t.get_device() != now:
+                break
+        else:
+            return
+    raise ValueError(f"tensors on {', '.join(sorted({str(t.device) for t in tensors}))}: the "
+                     "kernels run on the current GPU")
+
+
 def _is_quantised(cache) -> bool:
     """Whether `cache` is a QuantKvCache (its per-layer calls are the 8-bit ones)."""
     return getattr(cache, "q8", None) is not None
@@ -234,16 +248,15 @@ def _is_quantised(cache) -> bool:
 def _write_quantised(cache, layer: int, k: torch.Tensor, v: torch.Tensor, idx: torch.Tensor,
                      stream) -> None:
     """write_rows_indexed into a QuantKvCache (vapi_kv_q8_append)."""
-    from .quant import check_on_device
-    want = (cache.num_kv_heads, cache.head_dim)
     if v is None:
         raise ValueError("an 8-bit cache is written K and V together")
-    if k.dim() != 3 or tuple(k.shape) != tuple(v.shape) or tuple(k.shape[1:]) != want:
-        raise ValueError(f"k/v must be (n, {want[0]}, {want[1]}), got {tuple(k.shape)} and "
-                         f"{tuple(v.shape)}")
+    if k.dim() != 3 or k.shape != v.shape or k.shape[1] != cache.num_kv_heads or \
+            k.shape[2] != cache.head_dim:
+        raise ValueError(f"k/v must be (n, {cache.num_kv_heads}, {cache.head_dim}), got "
+                         f"{tuple(k.shape)} and {tuple(v.shape)}")
     if k.dtype != cache.dtype or v.dtype != cache.dtype:
         raise ValueError(f"cache is {cache.dtype} but the rows are {k.dtype} and {v.dtype}")
-    check_on_device(cache.device, k, v, idx)
+    check_on_device(cache.k[0], k, v, idx)
     k, v, idx = k.contiguous(), v.contiguous(), idx.contiguous()
     check(lib().vapi_kv_q8_append(cache.q8, layer, k.data_ptr(), v.data_ptr(), idx.data_ptr(),
                                   k.shape[0], stream_handle(stream)))
@@ -433,8 +446,7 @@ def gather_kv(cache: PagedKvCache, layer: int, block_table, len_k: int,
     kp = out.data_ptr() if which == "k" else None
     vp = out.data_ptr() if which == "v" else None
     if _is_quantised(cache):
-        from .quant import check_on_device
-        check_on_device(cache.device, table)
+        check_on_device(cache.k[0], table)
         check(lib().vapi_kv_q8_gather(cache.q8, layer, table.data_ptr(), table.shape[0], len_k,
                                       kp, vp, stream_handle(stream)))
         return out

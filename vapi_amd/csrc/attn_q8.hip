@@ -84,22 +84,28 @@ __device__ __forceinline__ void q8_load(Q8Step<D>& st, const AttnArgs& a, const 
     const uint64_t si = (uint64_t)blk * sc.sblk + kh;
     st.ks[tt] = ((ConstF32*)sc.k)[si];
     st.vs[tt] = ((ConstF32*)sc.v)[si];
-    const char* kp = a.k + tile + (uint32_t)min((int32_t)col, lim) * a.tok_e + 16 * g;
+    // Every load is unconditional (one under a branch makes the compiler wait
+    // for the whole prefetch). Pieces past head_dim repeat the row's last: K's
+    // meet zeros of Q, V's make output columns that are not stored (codes are
+    // finite).
+    const char* kp = a.k + tile + (uint32_t)min((int32_t)col, lim) * a.tok_e;
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c)
-      st.k[tt][c] = !kPad || 64 * c + 16 * g < a.hd ? load_kv<kNt>((const uint4*)(kp + 64 * c))
-                                                     : make_uint4(0u, 0u, 0u, 0u);
-    const char* vp = a.v + tile + v_col0<D>(col);
+    for (int c = 0; c < D / 64; ++c) {
+      const uint32_t d = 64 * c + 16 * g;
+      st.k[tt][c] = load_kv<kNt>((const uint4*)(kp + (kPad ? min(d, a.hd - 16) : d)));
+    }
+    const char* vp = a.v + tile;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const char* row = vp + (uint32_t)min((int32_t)(4 * g + i), lim) * a.tok_e;
       if constexpr (D == 64) {
-        st.v[tt][i][0] = !kPad || 4 * col < a.hd ? load_kv<kNt>((const uint32_t*)row) : 0u;
+        const uint32_t d = 4 * col;
+        st.v[tt][i][0] = load_kv<kNt>((const uint32_t*)(row + (kPad ? min(d, a.hd - 4) : d)));
       } else {
 #pragma unroll
         for (int h = 0; h < D / 128; ++h) {
-          const uint2 w = !kPad || v_d<D>(col, 8 * h) < a.hd
-                              ? load_kv<kNt>((const uint2*)(row + 128 * h)) : make_uint2(0u, 0u);
+          const uint32_t d = v_d<D>(col, 8 * h);
+          const uint2 w = load_kv<kNt>((const uint2*)(row + (kPad ? min(d, a.hd - 8) : d)));
           st.v[tt][i][2 * h] = w.x, st.v[tt][i][2 * h + 1] = w.y;
         }
       }

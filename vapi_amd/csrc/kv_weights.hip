@@ -25,6 +25,8 @@
 
 namespace vk {
 
+typedef uint32_t uint32x4 __attribute__((ext_vector_type(4)));
+
 // What K is stored as: the rows' own 16-bit type or a format of 8-bit codes.
 constexpr int kK16 = -1;
 
@@ -41,7 +43,9 @@ struct WeightArgs {
   uint32_t n_rows, width;
   uint32_t kvh, num_heads, hd, last_queries;
   FastDiv group;
-  uint32_t row_cap, n_chunk, chunk_keys;
+  uint32_t row_cap, n_chunk, chunk_keys, key_cap, part_rows;
+  float* part;    // [part][segment][key_cap] sums of pass 2
+  float* scores;  // [segment][row_cap][key_cap] (kept scores)
   float scale_log2, decay;
   int32_t wl, wr;
 };
@@ -89,48 +93,79 @@ __device__ __forceinline__ void weight_q(uint4 (&q)[D / 32], const WeightArgs& a
 #pragma unroll
   for (int c2 = 0; c2 < D / 32; ++c2) {
     const uint32_t d = weight_d<F>(c2, g);
-    q[c2] = d < a.hd ? *(const uint4*)(p + d) : make_uint4(0u, 0u, 0u, 0u);
+    q[c2] = *(const uint4*)(p + min(d, a.hd - 8));
+    if (d >= a.hd) q[c2] = make_uint4(0u, 0u, 0u, 0u);
   }
 }
 
-// A 16-key tile as it is stored, and its scale. Keys past the last repeat it.
+// A 16-key tile as it is stored, and its scale, on its way to MFMA operands
+// through LDS. An operand's lane wants 16 bytes of one of 16 rows, so loading it
+// straight takes two instructions (or four) for each 128-byte line, and L1 stalls
+// on the second while the first is on its way: with 8 KiB a wave outstanding, the
+// latency of 1,155 cycles held a read of K to 4.2 TB/s. Here consecutive lanes
+// load consecutive 16-byte pieces (each line by one instruction); the wave writes
+// them to its own LDS, piece c of row r at c ^ swizzle(r) so that the reads meet
+// no bank twice, and reads the operands back.
 template <int F, int D>
 struct WeightTile {
-  uint4 w[F == kK16 ? D / 32 : D / 64];
+  static constexpr int kPieces = D / (F == kK16 ? 8 : 16);  // of a row
+  static constexpr int N = kPieces / 4;
+  uint32x4 w[N];
   float scale;
+  __device__ static __forceinline__ uint32_t place(uint32_t row, uint32_t piece) {
+    return row * kPieces + (piece ^ (kPieces == 4 ? row >> 1 & 3 : row & 7));
+  }
 };
+// Keys past the last repeat it, pieces past head_dim the row's last (they meet
+// zeros of Q). Every load is unconditional: one under a branch makes the
+// compiler wait for all loads in flight.
 template <int F, int D>
 __device__ __forceinline__ void weight_load(WeightTile<F, D>& t, const WeightArgs& a,
-                                            const WeightSeg& s, int32_t key, uint32_t col,
-                                            uint32_t g) {
+                                            const WeightSeg& s, int32_t key, uint32_t lane) {
   using ConstU32 = const __attribute__((address_space(4))) uint32_t;
   using ConstF32 = const __attribute__((address_space(4))) float;
+  using Tile = WeightTile<F, D>;
   const int32_t last = s.len_k - 1;
   const int32_t ts = __builtin_amdgcn_readfirstlane(min(key, last & ~15));
   ConstU32* tab = (ConstU32*)(a.table + (uint64_t)s.seq * a.max_blocks);
   const uint32_t blk = min(tab[min((uint32_t)ts >> a.bs_shift, a.max_blocks - 1)], a.last_blk);
   const uint32_t off = (uint32_t)ts & ((1u << a.bs_shift) - 1);
-  const char* p = a.k + blk * a.blk_b + s.h * a.head_b + (uint64_t)off * a.tok_b +
-                  (uint32_t)min((int32_t)col, last - ts) * a.tok_b;
+  const char* p = a.k + blk * a.blk_b + s.h * a.head_b + (uint64_t)off * a.tok_b;
   t.scale = 1.f;
   if constexpr (F != kK16) t.scale = ((ConstF32*)a.k_scale)[(uint64_t)blk * a.sblk + s.h];
-  constexpr int N = F == kK16 ? D / 32 : D / 64;
+  const uint32_t end = a.hd * (F == kK16 ? 2 : 1) - 16;
 #pragma unroll
-  for (int c = 0; c < N; ++c) {
-    const uint32_t b = 64 * c + 16 * g;  // bytes into the row
-    t.w[c] = b < a.hd * (F == kK16 ? 2 : 1) ? *(const uint4*)(p + b) : make_uint4(0u, 0u, 0u, 0u);
+  for (int i = 0; i < Tile::N; ++i) {
+    const uint32_t row = (64 * i + lane) / Tile::kPieces, piece = lane % Tile::kPieces;
+    t.w[i] = *(const uint32x4*)(p + min((int32_t)row, last - ts) * a.tok_b + min(16 * piece, end));
   }
 }
-// The tile as MFMA operands (codes unscaled).
+template <int F, int D>
+__device__ __forceinline__ void weight_stage(uint32x4* lds, const WeightTile<F, D>& t,
+                                             uint32_t lane) {
+  using Tile = WeightTile<F, D>;
+#pragma unroll
+  for (int i = 0; i < Tile::N; ++i)
+    lds[Tile::place((64 * i + lane) / Tile::kPieces, lane % Tile::kPieces)] = t.w[i];
+}
+// The staged tile as MFMA operands (codes unscaled). A 16-bit pool's pieces past
+// head_dim are zeroed: they may repeat an infinity (codes are finite).
 template <typename T, int F, int D>
-__device__ __forceinline__ void weight_operand(const WeightTile<F, D>& t, uint4 (&k)[D / 32]) {
+__device__ __forceinline__ void weight_operand(const uint32x4* lds, uint4 (&k)[D / 32], uint32_t hd,
+                                               uint32_t col, uint32_t g) {
+  using Tile = WeightTile<F, D>;
   if constexpr (F == kK16) {
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) k[c] = t.w[c];
+    for (int c = 0; c < D / 32; ++c) k[c] = __builtin_bit_cast(uint4, lds[Tile::place(col, 4 * c + g)]);
+    if (hd < D) {
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c)
+        if (32 * c + 8 * g >= hd) k[c] = make_uint4(0u, 0u, 0u, 0u);
+    }
   } else {
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) {
-      const uint4 w = t.w[c];
+      const uint4 w = __builtin_bit_cast(uint4, lds[Tile::place(col, 4 * c + g)]);
       const uint2 a0 = q8_expand4<T, F, false>(w.x, 1.f), a1 = q8_expand4<T, F, false>(w.y, 1.f);
       const uint2 b0 = q8_expand4<T, F, false>(w.z, 1.f), b1 = q8_expand4<T, F, false>(w.w, 1.f);
       k[2 * c] = make_uint4(a0.x, a0.y, a1.x, a1.y);
@@ -138,12 +173,10 @@ __device__ __forceinline__ void weight_operand(const WeightTile<F, D>& t, uint4 
     }
   }
 }
-template <typename T, int D>
-__device__ __forceinline__ floatx4 weight_dot(const uint4 (&k)[D / 32], const uint4 (&q)[D / 32]) {
-  floatx4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int c = 0; c < D / 32; ++c) acc = mfma16x16x32<T>(k[c], q[c], acc);
-  return acc;
+// The wave's LDS writes before its reads (a wave's LDS operations run in order;
+// this holds the compiler to it).
+__device__ __forceinline__ void weight_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
 }
 
 // Keys that a query at `pos` sees: [lo, hi].
@@ -156,16 +189,32 @@ __device__ __forceinline__ int32_t weight_hi(const WeightArgs& a, int32_t pos, i
 
 constexpr int kWeightWaves = 4;
 
+// Tiles a wave of pass 1 loads at a time: 8 KiB of K where few rows use them
+// (the load is the work), fewer where many rows do.
+template <int F, int D, int MT>
+constexpr int weight_step() {
+  const int n = MT == 1 ? 8192 / (16 * D * (F == kK16 ? 2 : 1)) : 1;
+  return n < 1 ? 1 : n > 4 ? 4 : n;
+}
+
 // ---- pass 1 --------------------------------------------------------------------
 
-// Grid: (row tiles x chunks, segments).
-template <typename T, int F, int D, int MT>
+// Every grid has the segments fastest, so that the round-robin dealing over the
+// XCDs gives each of them work of every sequence (with the chunks fastest, eight
+// chunks put the ends of all long sequences on one XCD: 16 sequences of
+// 256-8,192 keys 47.9 us against @ORDER@).
+// Grid: (segments, row tiles x chunks). kStore: the scores are kept (then one
+// row tile, MT = 1).
+template <typename T, int F, int D, int MT, bool kStore>
 __global__ __launch_bounds__(64 * kWeightWaves) void weights_lse(WeightArgs a) {
+  constexpr int ST = weight_step<F, D, MT>();
   __shared__ float2 part[kWeightWaves][16 * MT];
-  const WeightSeg s = weight_seg(a, blockIdx.y);
+  __shared__ uint32x4 stage[kWeightWaves][ST][16 * WeightTile<F, D>::kPieces];
+  const WeightSeg s = weight_seg(a, blockIdx.x);
   if (!s.ok) return;
-  const uint32_t tile = blockIdx.x / a.n_chunk, chunk = blockIdx.x - tile * a.n_chunk;
-  const uint32_t row0 = tile * 16 * MT;
+  // The last rows see the most keys: their workgroups start first.
+  const uint32_t back = blockIdx.y / a.n_chunk, chunk = blockIdx.y - back * a.n_chunk;
+  const uint32_t row0 = (gridDim.y / a.n_chunk - 1 - back) * 16 * MT;
   if (row0 >= s.n_rows) return;
   const uint32_t lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int32_t wave = (int32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -187,33 +236,85 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_lse(WeightArgs a) {
   const int32_t c0 = (int32_t)(chunk * a.chunk_keys);
   const int32_t c1 = (int32_t)min((int64_t)c0 + a.chunk_keys, (int64_t)s.len_k) - 1;
   const int32_t k0 = max(c0, weight_lo(a, p0) & ~15), k1 = min(c1, weight_hi(a, p1, s.len_k));
-  WeightTile<F, D> next;
-  int32_t key = k0 + 16 * wave;
-  weight_load<F, D>(next, a, s, key, col, g);
-  for (; key <= k1; key += 16 * kWeightWaves) {
-    uint4 k[D / 32];
-    weight_operand<T, F, D>(next, k);
-    const float by = next.scale * a.scale_log2;
-    weight_load<F, D>(next, a, s, key + 16 * kWeightWaves, col, g);
-    const bool whole = key >= all_lo && key + 15 <= all_hi;
+  // Stores past the buffer (rows and keys that are not there) are dropped.
+  const uint32_t kept = kStore ? s.n_rows * a.key_cap * (uint32_t)sizeof(float) : 0;
+  const auto store = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(a.scores + (uint64_t)blockIdx.x * a.row_cap * a.key_cap), 0, (int)kept, 0x00027000);
+  WeightTile<F, D> bufA[ST], bufB[ST];
+  auto load = [&](WeightTile<F, D> (&buf)[ST], int32_t key) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const floatx4 acc = weight_dot<T, D>(k, q[t]);
-      float x[4];
+    for (int tt = 0; tt < ST; ++tt) weight_load<F, D>(buf[tt], a, s, key + 16 * tt, lane);
+  };
+  int32_t key = k0 + 16 * ST * wave;
+  auto step = [&](WeightTile<F, D> (&cur)[ST], WeightTile<F, D> (&next)[ST])
+      __attribute__((always_inline)) -> bool {
+    if (key > k1) return false;
+    load(next, key + 16 * ST * kWeightWaves);
+    float by[ST];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int32_t at = key + 4 * (int32_t)g + i;
-        x[i] = whole || (at >= lo[t] && at <= hi[t]) ? acc[i] * by : -INFINITY;
+    for (int tt = 0; tt < ST; ++tt) {
+      weight_stage<F, D>(stage[wave][tt], cur[tt], lane);
+      by[tt] = cur[tt].scale * a.scale_log2;
+    }
+    weight_fence();
+    const bool whole = key >= all_lo && key + 16 * ST - 1 <= all_hi;
+    float x[ST][MT][4], mx[MT];
+    bool grow = false;
+#pragma unroll
+    for (int tt = 0; tt < ST; ++tt) {
+      uint4 k[D / 32];
+      weight_operand<T, F, D>(stage[wave][tt], k, a.hd, col, g);
+      floatx4 acc[MT];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[t] = mfma16x16x32<T>(k[c], q[t][c], acc[t]);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[tt][t][i] = acc[t][i] * by[tt];
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int32_t at = key + 16 * tt + 4 * (int32_t)g + i;
+            if (!(at >= lo[t] && at <= hi[t])) x[tt][t][i] = -INFINITY;
+          }
+        }
+        const float top = max_nc(max_nc(x[tt][t][0], x[tt][t][1]), max_nc(x[tt][t][2], x[tt][t][3]));
+        mx[t] = tt == 0 ? top : max_nc(mx[t], top);
       }
-      const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-      if (__any(mx > m[t] + kRescaleSlack)) {
-        const float mn = fmaxf(m[t], mx);
+      if constexpr (kStore) {
+        const int32_t at = key + 16 * tt + 4 * (int32_t)g;
+        const uint32_t to = at <= k1 ? (col * a.key_cap + (uint32_t)at) * 4 : 0xFFFFFFF0u;
+        const floatx4 v = {x[tt][0][0], x[tt][0][1], x[tt][0][2], x[tt][0][3]};
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint32x4, v), store, (int)to, 0,
+                                               0);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) grow |= mx[t] > m[t] + kRescaleSlack;
+    if (__any(grow)) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        const float mn = max_nc(m[t], mx[t]);
         l[t] *= fast_exp2(m[t] - mn);
         m[t] = mn;
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) l[t] += fast_exp2(x[i] - m[t]);
     }
+#pragma unroll
+    for (int tt = 0; tt < ST; ++tt)
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+        l[t] += (fast_exp2(x[tt][t][0] - m[t]) + fast_exp2(x[tt][t][1] - m[t])) +
+                (fast_exp2(x[tt][t][2] - m[t]) + fast_exp2(x[tt][t][3] - m[t]));
+    weight_fence();
+    key += 16 * ST * kWeightWaves;
+    return true;
+  };
+  load(bufA, key);
+  while (step(bufA, bufB) && step(bufB, bufA)) {
   }
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
@@ -229,7 +330,7 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_lse(WeightArgs a) {
     for (int w = 0; w < kWeightWaves; ++w) mx = fmaxf(mx, part[w][r].x);
 #pragma unroll
     for (int w = 0; w < kWeightWaves; ++w) sum += part[w][r].y * fast_exp2(part[w][r].x - mx);
-    a.ml[((uint64_t)blockIdx.y * a.row_cap + row0 + r) * a.n_chunk + chunk] =
+    a.ml[((uint64_t)blockIdx.x * a.row_cap + row0 + r) * a.n_chunk + chunk] =
         make_float2(mx, sum);
   }
 }
@@ -237,90 +338,126 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_lse(WeightArgs a) {
 // ---- pass 2 --------------------------------------------------------------------
 
 // lse of a row from its chunks' (m, l); +infinity (weights of 0) where it saw
-// no key.
+// no key. Eight loads at a time.
 __device__ __forceinline__ float weight_join(const float2* ml, uint32_t n) {
   float mx = kNegBig, sum = 0.f;
-  for (uint32_t c = 0; c < n; ++c) {
-    const float2 x = ml[c];
-    const float mn = fmaxf(mx, x.x);
-    sum = sum * fast_exp2(mx - mn) + x.y * fast_exp2(x.x - mn);
+  for (uint32_t c0 = 0; c0 < n; c0 += 8) {
+    float2 x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = c0 + j < n ? ml[c0 + j] : make_float2(kNegBig, 0.f);
+    float mn = mx;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mn = fmaxf(mn, x[j].x);
+    sum *= fast_exp2(mx - mn);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum += x[j].y * fast_exp2(x[j].x - mn);
     mx = mn;
   }
   return sum > 0.f ? mx + __builtin_amdgcn_logf(sum) : INFINITY;
 }
 
 constexpr uint32_t kWeightJoinRows = 1024;  // rows whose lse a workgroup joins in LDS
+constexpr int kWeightKt = 4;                // 16-key tiles a wave of pass 2 holds
 
-// Grid: (key tiles of 16 KT x 4 waves, segments).
-template <typename T, int F, int D, int KT, bool kJoin>
+// Joins the segment's rows [r0, r1) into lds; every thread calls it.
+__device__ __forceinline__ void weight_lse_rows(float* lds, const WeightArgs& a, uint32_t seg,
+                                                uint32_t r0, uint32_t r1) {
+  const float2* ml = a.ml + (uint64_t)seg * a.row_cap * a.n_chunk;
+  for (uint32_t r = r0 + threadIdx.x; r < r1; r += 64 * kWeightWaves)
+    lds[r - r0] = weight_join(ml + (uint64_t)r * a.n_chunk, a.n_chunk);
+  __syncthreads();
+}
+
+__device__ __forceinline__ void weight_write(const WeightArgs& a, float* w, float x) {
+  *w = a.decay == 0.f ? x : *w * a.decay + x;
+}
+
+// Grid: (segments, key tiles of 16 KT x 4 waves, parts of the rows). With more
+// than one part the sums go to a.part, which weights_add adds up.
+template <typename T, int F, int D>
 __global__ __launch_bounds__(64 * kWeightWaves) void weights_sum(WeightArgs a) {
-  __shared__ float lse_lds[kJoin ? kWeightJoinRows : 1];
-  const WeightSeg s = weight_seg(a, blockIdx.y);
-  const int32_t wg0 = (int32_t)(blockIdx.x * 16 * KT * kWeightWaves);
+  constexpr int KT = kWeightKt;
+  __shared__ float lse_lds[kWeightJoinRows];
+  __shared__ uint32x4 stage[kWeightWaves][16 * WeightTile<F, D>::kPieces];
+  const WeightSeg s = weight_seg(a, blockIdx.x);
+  const int32_t wg0 = (int32_t)(blockIdx.y * 16 * KT * kWeightWaves);
   if (!s.ok || wg0 >= s.len_k) return;
-  const float2* ml = a.ml + (uint64_t)blockIdx.y * a.row_cap * a.n_chunk;
-  if constexpr (kJoin) {
-    for (uint32_t r = threadIdx.x; r < s.n_rows; r += 64 * kWeightWaves)
-      lse_lds[r] = weight_join(ml + (uint64_t)r * a.n_chunk, a.n_chunk);
-    __syncthreads();
+  // This part's rows, and of them those that see any key of the workgroup:
+  // pos >= first key - wr, pos <= last key + wl.
+  uint32_t r0 = blockIdx.z * a.part_rows, r1 = min(r0 + a.part_rows, s.n_rows);
+  const int32_t wg1 = min(wg0 + 16 * KT * kWeightWaves, s.len_k) - 1;
+  if (a.wr >= 0) {
+    const int64_t j = (int64_t)wg0 - a.wr - s.pos0;
+    if (j > 0) r0 = max(r0, (uint32_t)min(j * a.group.d, (int64_t)s.n_rows) & ~15u);
   }
+  if (a.wl >= 0) {
+    const int64_t j = (int64_t)wg1 + a.wl - s.pos0 + 1;
+    r1 = (uint32_t)max((int64_t)0, min((int64_t)r1, j * a.group.d));
+  }
+  r1 = max(r0, r1);
+  weight_lse_rows(lse_lds, a, blockIdx.x, r0, r1);
   const uint32_t lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int32_t wave = (int32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int32_t key0 = wg0 + 16 * KT * wave;
   if (key0 >= s.len_k) return;
   uint4 k[KT][D / 32];
   float by[KT], sum[KT][4];
+  {
+    WeightTile<F, D> raw[KT];
 #pragma unroll
-  for (int t = 0; t < KT; ++t) {
-    WeightTile<F, D> raw;
-    weight_load<F, D>(raw, a, s, key0 + 16 * t, col, g);
-    weight_operand<T, F, D>(raw, k[t]);
-    by[t] = raw.scale * a.scale_log2;
+    for (int t = 0; t < KT; ++t) weight_load<F, D>(raw[t], a, s, key0 + 16 * t, lane);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[t][i] = 0.f;
+    for (int t = 0; t < KT; ++t) {
+      weight_stage<F, D>(stage[wave], raw[t], lane);
+      weight_fence();
+      weight_operand<T, F, D>(stage[wave], k[t], a.hd, col, g);
+      weight_fence();
+      by[t] = raw[t].scale * a.scale_log2;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[t][i] = 0.f;
+    }
   }
-  // The queries that see any of these keys: pos >= key0 - wr, pos <= last + wl.
-  const int32_t key1 = min(key0 + 16 * KT, s.len_k) - 1;
-  const int32_t n_q = (int32_t)a.group.div(s.n_rows - 1) + 1;
-  const int32_t j0 = a.wr >= 0 ? (int32_t)max((int64_t)0, (int64_t)key0 - a.wr - s.pos0) : 0;
-  const int32_t j1 =
-      a.wl >= 0 ? (int32_t)min((int64_t)n_q - 1, (int64_t)key1 + a.wl - s.pos0) : n_q - 1;
-  if (j0 <= j1) {
-    const uint32_t r0 = ((uint32_t)j0 * a.group.d) & ~15u;
-    const uint32_t r1 = min(((uint32_t)j1 + 1) * a.group.d, s.n_rows);
+  if (r0 < r1) {
     uint4 next[D / 32];
     weight_q<T, F, D>(next, a, s, r0 + col, g);
     for (uint32_t r = r0; r < r1; r += 16) {
       uint4 q[D / 32];
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) q[c] = next[c];
-      const uint32_t row = min(r + col, s.n_rows - 1);
-      float lse;
-      if constexpr (kJoin) {
-        lse = lse_lds[row];
-      } else {
-        const float2 x = ml[row];
-        lse = x.y > 0.f ? x.x + __builtin_amdgcn_logf(x.y) : INFINITY;
-      }
-      if (r + col >= s.n_rows) lse = INFINITY;
       weight_q<T, F, D>(next, a, s, r + 16 + col, g);
+      const uint32_t row = min(r + col, r1 - 1);
+      const float lse = r + col < r1 ? lse_lds[row - r0] : INFINITY;
       const int32_t pos = s.pos0 + (int32_t)a.group.div(row);
       const int32_t lo = weight_lo(a, pos), hi = weight_hi(a, pos, s.len_k);
       const bool whole = __all(key0 >= lo && key0 + 16 * KT - 1 <= hi);
+      floatx4 acc[KT];
 #pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        const floatx4 acc = weight_dot<T, D>(k[t], q);
+      for (int t = 0; t < KT; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int32_t at = key0 + 16 * t + 4 * (int32_t)g + i;
-          const float x = __builtin_fmaf(acc[i], by[t], -lse);
-          sum[t][i] += fast_exp2(whole || (at >= lo && at <= hi) ? x : -INFINITY);
-        }
+      for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int t = 0; t < KT; ++t) acc[t] = mfma16x16x32<T>(k[t][c], q[c], acc[t]);
+      if (whole) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            sum[t][i] += fast_exp2(__builtin_fmaf(acc[t][i], by[t], -lse));
+      } else {
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int32_t at = key0 + 16 * t + 4 * (int32_t)g + i;
+            const float x = __builtin_fmaf(acc[t][i], by[t], -lse);
+            sum[t][i] += fast_exp2(at >= lo && at <= hi ? x : -INFINITY);
+          }
       }
     }
   }
   // Over the 16 rows of a lane group; lane col then writes key 4 g + col.
   float* w = a.w + s.state_row * a.row_stride + s.h * a.head_stride;
+  float* part = a.part + ((uint64_t)blockIdx.z * gridDim.x + blockIdx.x) * a.key_cap;
 #pragma unroll
   for (int t = 0; t < KT; ++t) {
 #pragma unroll
@@ -332,55 +469,113 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_sum(WeightArgs a) {
     }
     const float x = col == 0 ? sum[t][0] : col == 1 ? sum[t][1] : col == 2 ? sum[t][2] : sum[t][3];
     const int32_t at = key0 + 16 * t + 4 * (int32_t)g + (int32_t)col;
-    if (col < 4 && at < s.len_k) w[at] = a.decay == 0.f ? x : w[at] * a.decay + x;
+    if (col < 4 && at < s.len_k) {
+      if (gridDim.z > 1) part[at] = x;
+      else weight_write(a, w + at, x);
+    }
   }
+}
+
+// Grid: (segments, keys / 256): the parts' sums, in order.
+__global__ __launch_bounds__(256) void weights_add(WeightArgs a, uint32_t parts) {
+  const WeightSeg s = weight_seg(a, blockIdx.x);
+  const int32_t at = (int32_t)(blockIdx.y * 256 + threadIdx.x);
+  if (!s.ok || at >= s.len_k) return;
+  float x = 0.f;
+  for (uint32_t p = 0; p < parts; ++p)
+    x += a.part[((uint64_t)p * gridDim.x + blockIdx.x) * a.key_cap + at];
+  weight_write(a, a.w + s.state_row * a.row_stride + s.h * a.head_stride + at, x);
+}
+
+// Pass 2 over stored scores. Grid: (keys / 1,024, segments); a thread sums four
+// keys over the segment's rows (at most 16).
+__global__ __launch_bounds__(64 * kWeightWaves) void weights_stored(WeightArgs a) {
+  __shared__ float lse[16];
+  const WeightSeg s = weight_seg(a, blockIdx.x);
+  if (!s.ok || (int32_t)(blockIdx.y * 1024) >= s.len_k) return;
+  const int32_t at = (int32_t)(blockIdx.y * 1024 + 4 * threadIdx.x);
+  const float* scores = a.scores + (uint64_t)blockIdx.x * a.row_cap * a.key_cap + at;
+  weight_lse_rows(lse, a, blockIdx.x, 0, s.n_rows);
+  if (at >= s.len_k) return;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  // (Pass 1 visits the keys that some row sees, from a 16-key tile's first.)
+  const int32_t last = s.pos0 + (int32_t)a.group.div(s.n_rows - 1);
+  const bool seen = at >= (weight_lo(a, s.pos0) & ~15) && at <= weight_hi(a, last, s.len_k);
+  for (uint32_t r = 0; seen && r < s.n_rows; ++r) {
+    const float4 x = *(const float4*)(scores + (uint64_t)r * a.key_cap);
+    sum[0] += fast_exp2(x.x - lse[r]), sum[1] += fast_exp2(x.y - lse[r]);
+    sum[2] += fast_exp2(x.z - lse[r]), sum[3] += fast_exp2(x.w - lse[r]);
+  }
+  float* w = a.w + s.state_row * a.row_stride + s.h * a.head_stride + at;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (at + i < s.len_k) weight_write(a, w + i, sum[i]);
 }
 
 // ---- host ------------------------------------------------------------------------
 
 struct WeightPlan {
-  uint32_t row_cap, row_tiles, n_chunk, chunk_keys;
-  int mt, kt;
-  size_t bytes;
+  uint32_t row_cap, row_tiles, n_chunk, chunk_keys, key_cap, parts, part_rows;
+  int mt;
+  bool store;
+  size_t ml_bytes, bytes;
 };
 
-// Rows per workgroup of pass 1 (16 mt): enough to use a K tile many times where
-// there are many rows. Chunks of keys: as many as give pass 1 about kWeightWgs
-// workgroups, where the rows are few enough for pass 2 to join them.
-constexpr uint64_t kWeightWgs = 2048;
+// Rows a workgroup of pass 1 takes (16 mt): one tile for single tokens, else
+// enough to use each K tile many times. Chunks of keys give pass 1 about
+// kWeightWgs workgroups where the rows alone do not, parts of the rows pass 2.
+// Up to 16 rows and kStoreBytes the scores are kept between the passes: 8 bytes
+// a score moved instead of K read again (16 sequences of 256-8,192 keys, 32 q /
+// 8 kv heads, bf16: @STORED@).
+constexpr uint64_t kWeightWgs = 1024;
+constexpr uint64_t kStoreBytes = 256ull << 20;
 static WeightPlan weight_plan(uint32_t batch, uint32_t kvh, uint32_t group, uint32_t hd,
                               uint32_t max_q, uint32_t max_k, uint32_t last) {
   WeightPlan p;
+  const uint64_t segs = (uint64_t)batch * kvh;
   const uint64_t n_q = last ? std::min(max_q, last) : max_q;
   const uint64_t rows = n_q * group;
   p.row_cap = (uint32_t)std::min<uint64_t>(rows, 0x7FFFFFF0u);
-  const int most = hd > 128 ? 4 : 8;
-  p.mt = rows <= 16 ? 1 : rows <= 64 ? 4 : most;
+  p.mt = rows <= 16 ? 1 : hd > 128 ? 4 : 8;
   p.row_tiles = (p.row_cap + 16 * p.mt - 1) / (16 * p.mt);
-  p.kt = rows <= 64 ? 1 : 4;
-  const uint64_t wgs = std::max<uint64_t>((uint64_t)p.row_tiles * batch * kvh, 1);
-  uint64_t n = p.row_cap <= kWeightJoinRows ? std::max<uint64_t>(kWeightWgs / wgs, 1) : 1;
-  uint64_t keys = (((uint64_t)max_k + n - 1) / n + 63) & ~63ull;
-  keys = std::max<uint64_t>(keys, p.row_cap <= kWeightJoinRows ? 256 : 64);
-  p.chunk_keys = (uint32_t)keys;
-  p.n_chunk = (uint32_t)std::max<uint64_t>(((uint64_t)max_k + keys - 1) / keys, 1);
-  p.bytes = (size_t)batch * kvh * p.row_cap * p.n_chunk * sizeof(float2);
+  p.key_cap = (max_k + 63) & ~63u;
+  p.store = rows <= 16 && segs * rows * p.key_cap * sizeof(float) <= kStoreBytes;
+  auto up = [](uint64_t x, uint64_t y) { return (x + y - 1) / y; };
+  const uint64_t want = std::max<uint64_t>(up(kWeightWgs, p.row_tiles * segs), 1);
+  uint64_t keys = std::max<uint64_t>(up(max_k, want), 512);
+  p.chunk_keys = (uint32_t)(up(keys, 256) * 256);
+  p.n_chunk = (uint32_t)std::max<uint64_t>(up(max_k, p.chunk_keys), 1);
+  const uint64_t blocks = up(max_k, 16 * kWeightKt * kWeightWaves);
+  // (A part's rows are joined in LDS, so there are at least enough parts.)
+  uint64_t parts = std::max<uint64_t>(up(kWeightWgs, blocks * segs), 1);
+  parts = std::max(std::min<uint64_t>(parts, up(rows, 128)), up(rows, kWeightJoinRows));
+  p.part_rows = (uint32_t)(up(up(rows, parts), 16) * 16);
+  p.parts = p.store ? 1 : (uint32_t)up(rows, p.part_rows);
+  p.ml_bytes = (segs * p.row_cap * p.n_chunk * sizeof(float2) + 255) & ~(size_t)255;
+  p.bytes = p.ml_bytes;
+  if (p.store) p.bytes += segs * rows * p.key_cap * sizeof(float);
+  else if (p.parts > 1) p.bytes += p.parts * segs * p.key_cap * sizeof(float);
   return p;
 }
 
 template <typename T, int F, int D>
 static void launch_weights_d(const WeightArgs& a, const WeightPlan& p, uint32_t segs,
                              uint32_t max_k, hipStream_t s) {
-  const dim3 block(64 * kWeightWaves), g1(p.row_tiles * p.n_chunk, segs);
-  if (p.mt == 1) hipLaunchKernelGGL((weights_lse<T, F, D, 1>), g1, block, 0, s, a);
-  else if (p.mt == 4) hipLaunchKernelGGL((weights_lse<T, F, D, 4>), g1, block, 0, s, a);
-  else if constexpr (D <= 128) hipLaunchKernelGGL((weights_lse<T, F, D, 8>), g1, block, 0, s, a);
-  const uint32_t keys = 16 * p.kt * kWeightWaves;
-  const dim3 g2((max_k + keys - 1) / keys, segs);
-  const bool join = p.row_cap <= kWeightJoinRows;
-  if (p.kt == 1) hipLaunchKernelGGL((weights_sum<T, F, D, 1, true>), g2, block, 0, s, a);
-  else if (join) hipLaunchKernelGGL((weights_sum<T, F, D, 4, true>), g2, block, 0, s, a);
-  else hipLaunchKernelGGL((weights_sum<T, F, D, 4, false>), g2, block, 0, s, a);
+  const dim3 block(64 * kWeightWaves), g1(segs, p.row_tiles * p.n_chunk);
+  if (p.store) {
+    hipLaunchKernelGGL((weights_lse<T, F, D, 1, true>), g1, block, 0, s, a);
+    hipLaunchKernelGGL(weights_stored, dim3(segs, (max_k + 1023) / 1024), block, 0, s, a);
+    return;
+  }
+  if (p.mt == 1) hipLaunchKernelGGL((weights_lse<T, F, D, 1, false>), g1, block, 0, s, a);
+  else if constexpr (D == 256)
+    hipLaunchKernelGGL((weights_lse<T, F, D, 4, false>), g1, block, 0, s, a);
+  else hipLaunchKernelGGL((weights_lse<T, F, D, 8, false>), g1, block, 0, s, a);
+  const uint32_t keys = 16 * kWeightKt * kWeightWaves;
+  hipLaunchKernelGGL((weights_sum<T, F, D>), dim3(segs, (max_k + keys - 1) / keys, p.parts), block,
+                     0, s, a);
+  if (p.parts > 1)
+    hipLaunchKernelGGL(weights_add, dim3(segs, (max_k + 255) / 256), dim3(256), 0, s, a, p.parts);
 }
 template <typename T, int F>
 static void launch_weights(const WeightArgs& a, const WeightPlan& p, uint32_t segs, uint32_t max_k,
@@ -439,11 +634,12 @@ static int weight_checks(const WeightCall& c, uint32_t kvh, uint32_t hd, uint32_
   if (num_blocks == 0) VK_FAIL(VAPI_KV_EINVAL, "%s: keys in an empty pool", who);
   if (c.max_blocks == 0) VK_FAIL(VAPI_KV_EINVAL, "%s: block table width 0", who);
   const uint64_t segs = (uint64_t)c.batch * kvh, n_q = c.last ? std::min(c.max_q, c.last) : c.max_q;
-  if (segs > 65535 || n_q * (c.num_heads / kvh) > 0x3FFFFFFFu || c.max_k > 0x3FFFFFFFu)
+  // (Grids: segments up to 2^31, the rest up to 65,535 each.)
+  if (segs > 0x7FFFFFFFu || n_q * (c.num_heads / kvh) > 0x3FFFFFFFu || c.max_k > 65535u * 256u)
     VK_FAIL(VAPI_KV_EUNSUP, "%s: a batch of %u x %u kv heads with %u queries of %u heads", who,
             c.batch, kvh, c.max_q, c.num_heads);
   *plan = weight_plan(c.batch, kvh, c.num_heads / kvh, hd, c.max_q, c.max_k, c.last);
-  if ((uint64_t)plan->row_tiles * plan->n_chunk > 0x7FFFFFFFu)
+  if ((uint64_t)plan->row_tiles * plan->n_chunk > 65535 || plan->parts > 65535)
     VK_FAIL(VAPI_KV_EUNSUP, "%s: batch too large for one launch", who);
   if (c.ws_bytes < plan->bytes || !c.ws)
     VK_FAIL(VAPI_KV_ESPACE, "%s: workspace %zu bytes < %zu", who, c.ws_bytes, plan->bytes);
@@ -470,6 +666,8 @@ static WeightArgs weight_args(const WeightCall& c, const WeightPlan& p, uint32_t
   a.kvh = kvh, a.num_heads = c.num_heads, a.hd = hd, a.last_queries = c.last;
   a.group = FastDiv(c.num_heads / kvh);
   a.row_cap = p.row_cap, a.n_chunk = p.n_chunk, a.chunk_keys = p.chunk_keys;
+  a.key_cap = p.key_cap, a.part_rows = p.part_rows;
+  a.part = a.scores = (float*)((char*)c.ws + p.ml_bytes);
   a.scale_log2 = c.scale * kLog2e;
   a.decay = c.decay;
   a.wl = c.wl < 0 ? -1 : c.wl;

@@ -18,8 +18,7 @@ import torch
 
 from ._lib import Weights, check, lib
 from .attention import PreparedAttention
-from .cache import HybridKvCache, _is_quantised, _per_layer, stream_handle
-from .quant import check_on_device
+from .cache import HybridKvCache, _is_quantised, _per_layer, check_on_device, stream_handle
 
 
 def new_weights(rows: int, num_kv_heads: int, width: int, device="cuda") -> torch.Tensor:
@@ -92,8 +91,8 @@ def accumulate_attention_weights(q: torch.Tensor, cache, layer: int, prepared: P
     b = prepared.seqlens_q.shape[0] - 1
     index = _rows(rows, b, cache.device)
     state = _state(weights, cache, index, b, "weights")
-    on = [q, weights, prepared.block_table, prepared.seqlens_q, prepared.seqlens_k]
-    check_on_device(cache.device, *(on if index is None else on + [index]))
+    on = (weights, q, prepared.block_table, prepared.seqlens_q)
+    check_on_device(*(on if index is None else on + (index,)))
     q = q.contiguous()
     heads, max_q, max_k = q.shape[1], max(prepared.max_seqlen_q, 1), max(prepared.max_seqlen_k, 1)
     need = lib().vapi_kv_attention_weights_workspace_size(
@@ -203,16 +202,17 @@ def evict_kv(cache, layer: int, weights: torch.Tensor, plan: EvictionPlan,
         raise ValueError(f"block {plan.top_block} of {cache.num_blocks}")
     b = len(plan.new_lens)
     src = _state(weights, cache, plan.rows, b, "weights")
-    on = [weights, plan.lens, plan.src_table, plan.dst_table]
+    on = [weights, plan.lens, plan.src_table]
     dst = None
     if weights_out is not None:
         dst = _state(weights_out, cache, plan.rows, b, "weights_out")
         on.append(weights_out)
-        if weights_out.data_ptr() != weights.data_ptr() or weights_out.stride() != weights.stride():
+        if weights_out is not weights and (weights_out.data_ptr() != weights.data_ptr() or
+                                           weights_out.stride() != weights.stride()):
             (a0, a1), (b0, b1) = _extent(weights), _extent(weights_out)
             if a0 < b1 and b0 < a1:
                 raise ValueError("weights_out overlaps weights: give the same tensor or another")
-    check_on_device(cache.device, *on)
+    check_on_device(*on)
     kept = torch.empty((b, cache.num_kv_heads, plan.max_keep), dtype=torch.int32,
                        device=weights.device)
     quantised = _is_quantised(cache)

@@ -115,19 +115,6 @@ class QuantKvCache:
         return c * s[:, None, :, None]
 
 
-def check_on_device(device, *tensors) -> None:
-    """Every tensor on one GPU, and that the current one: the library launches
-    on the current device's stream."""
-    device = torch.device(device)
-    if device.type != "cuda":
-        raise ValueError(f"the cache is on {device}: the kernels run on a GPU")
-    now = torch.cuda.current_device()
-    for index in [device.index] + [t.device.index if t.is_cuda else -1 for t in tensors]:
-        if index is not None and index != now:
-            raise ValueError(f"the cache is on {device} and the tensors on "
-                             f"{[str(t.device) for t in tensors]}, the current device is cuda:{now}")
-
-
 def check_block_runs(slots: np.ndarray, block_size: int) -> None:
     """Raises ValueError unless each block's tokens follow one another in
     `slots` (skipped ones aside) and no slot comes twice, as the append into an
