@@ -82,6 +82,19 @@ __device__ __forceinline__ uint32_t weight_d(int c, uint32_t g) {
   return F == kK16 ? 32 * c + 8 * g : 64 * (c / 2) + 16 * g + 8 * (c % 2);
 }
 
+// Pieces past head_dim as zeros: one uniform branch around selects (a branch per
+// piece waits for its load before the next is issued).
+template <int F, int D>
+__device__ __forceinline__ void weight_zero(uint4 (&x)[D / 32], uint32_t hd, uint32_t g) {
+  if (hd < D) {
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      const uint32_t keep = weight_d<F>(c, g) < hd ? 0xFFFFFFFFu : 0u;
+      x[c] = make_uint4(x[c].x & keep, x[c].y & keep, x[c].z & keep, x[c].w & keep);
+    }
+  }
+}
+
 // Q operand of 16 rows from `first` (rows past the segment's repeat its last).
 template <typename T, int F, int D>
 __device__ __forceinline__ void weight_q(uint4 (&q)[D / 32], const WeightArgs& a,
@@ -94,8 +107,8 @@ __device__ __forceinline__ void weight_q(uint4 (&q)[D / 32], const WeightArgs& a
   for (int c2 = 0; c2 < D / 32; ++c2) {
     const uint32_t d = weight_d<F>(c2, g);
     q[c2] = *(const uint4*)(p + min(d, a.hd - 8));
-    if (d >= a.hd) q[c2] = make_uint4(0u, 0u, 0u, 0u);
   }
+  weight_zero<F, D>(q, a.hd, g);
 }
 
 // A 16-key tile as it is stored, and its scale, on its way to MFMA operands
@@ -119,7 +132,8 @@ struct WeightTile {
 // Keys past the last repeat it, pieces past head_dim the row's last (they meet
 // zeros of Q). Every load is unconditional: one under a branch makes the
 // compiler wait for all loads in flight.
-template <int F, int D>
+// kNt: streaming loads, where no other workgroup reads the tile.
+template <int F, int D, bool kNt>
 __device__ __forceinline__ void weight_load(WeightTile<F, D>& t, const WeightArgs& a,
                                             const WeightSeg& s, int32_t key, uint32_t lane) {
   using ConstU32 = const __attribute__((address_space(4))) uint32_t;
@@ -137,7 +151,8 @@ __device__ __forceinline__ void weight_load(WeightTile<F, D>& t, const WeightArg
 #pragma unroll
   for (int i = 0; i < Tile::N; ++i) {
     const uint32_t row = (64 * i + lane) / Tile::kPieces, piece = lane % Tile::kPieces;
-    t.w[i] = *(const uint32x4*)(p + min((int32_t)row, last - ts) * a.tok_b + min(16 * piece, end));
+    t.w[i] = load_kv<kNt>(
+        (const uint32x4*)(p + min((int32_t)row, last - ts) * a.tok_b + min(16 * piece, end)));
   }
 }
 template <int F, int D>
@@ -157,11 +172,7 @@ __device__ __forceinline__ void weight_operand(const uint32x4* lds, uint4 (&k)[D
   if constexpr (F == kK16) {
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) k[c] = __builtin_bit_cast(uint4, lds[Tile::place(col, 4 * c + g)]);
-    if (hd < D) {
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c)
-        if (32 * c + 8 * g >= hd) k[c] = make_uint4(0u, 0u, 0u, 0u);
-    }
+    weight_zero<F, D>(k, hd, g);
   } else {
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) {
@@ -189,12 +200,13 @@ __device__ __forceinline__ int32_t weight_hi(const WeightArgs& a, int32_t pos, i
 
 constexpr int kWeightWaves = 4;
 
-// Tiles a wave of pass 1 loads at a time: 8 KiB of K where few rows use them
-// (the load is the work), fewer where many rows do.
+// Tiles a wave of pass 1 loads at a time: 4 KiB of K where few rows use them
+// (with four workgroups a CU the next step's 4 KiB of 16 waves are in flight; 8
+// and 16 KiB a wave measured 1 and 3 us slower of 37), one where many rows do.
 template <int F, int D, int MT>
 constexpr int weight_step() {
-  const int n = MT == 1 ? 8192 / (16 * D * (F == kK16 ? 2 : 1)) : 1;
-  return n < 1 ? 1 : n > 4 ? 4 : n;
+  const int n = MT == 1 ? 4096 / (16 * D * (F == kK16 ? 2 : 1)) : 1;
+  return n < 1 ? 1 : n;
 }
 
 // ---- pass 1 --------------------------------------------------------------------
@@ -210,7 +222,10 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_lse(WeightArgs a) {
   constexpr int ST = weight_step<F, D, MT>();
   __shared__ float2 part[kWeightWaves][16 * MT];
   __shared__ uint32x4 stage[kWeightWaves][ST][16 * WeightTile<F, D>::kPieces];
-  const WeightSeg s = weight_seg(a, blockIdx.x);
+  // (Chunk by chunk the sequences are turned by five: otherwise all chunks of a
+  // long one land on the same CUs. 16 sequences of 256-8,192 keys 41.3 -> 37.3.)
+  const uint32_t seg = (blockIdx.x + 5 * a.kvh * blockIdx.y) % gridDim.x;
+  const WeightSeg s = weight_seg(a, seg);
   if (!s.ok) return;
   // The last rows see the most keys: their workgroups start first.
   const uint32_t back = blockIdx.y / a.n_chunk, chunk = blockIdx.y - back * a.n_chunk;
@@ -239,24 +254,25 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_lse(WeightArgs a) {
   // Stores past the buffer (rows and keys that are not there) are dropped.
   const uint32_t kept = kStore ? s.n_rows * a.key_cap * (uint32_t)sizeof(float) : 0;
   const auto store = __builtin_amdgcn_make_buffer_rsrc(
-      (void*)(a.scores + (uint64_t)blockIdx.x * a.row_cap * a.key_cap), 0, (int)kept, 0x00027000);
-  WeightTile<F, D> bufA[ST], bufB[ST];
-  auto load = [&](WeightTile<F, D> (&buf)[ST], int32_t key) __attribute__((always_inline)) {
-#pragma unroll
-    for (int tt = 0; tt < ST; ++tt) weight_load<F, D>(buf[tt], a, s, key + 16 * tt, lane);
-  };
+      (void*)(a.scores + (uint64_t)seg * a.row_cap * a.key_cap), 0, (int)kept, 0x00027000);
+  // The next step loads into the registers that staging has just freed, while
+  // this one is computed from LDS. (One loop body: a second one for a second set
+  // of registers doubles the code, which short walks fetch once.)
+  WeightTile<F, D> buf[ST];
   int32_t key = k0 + 16 * ST * wave;
-  auto step = [&](WeightTile<F, D> (&cur)[ST], WeightTile<F, D> (&next)[ST])
-      __attribute__((always_inline)) -> bool {
-    if (key > k1) return false;
-    load(next, key + 16 * ST * kWeightWaves);
+#pragma unroll
+  for (int tt = 0; tt < ST; ++tt) weight_load<F, D, kStore>(buf[tt], a, s, key + 16 * tt, lane);
+  while (key <= k1) {
     float by[ST];
 #pragma unroll
     for (int tt = 0; tt < ST; ++tt) {
-      weight_stage<F, D>(stage[wave][tt], cur[tt], lane);
-      by[tt] = cur[tt].scale * a.scale_log2;
+      weight_stage<F, D>(stage[wave][tt], buf[tt], lane);
+      by[tt] = buf[tt].scale * a.scale_log2;
     }
     weight_fence();
+#pragma unroll
+    for (int tt = 0; tt < ST; ++tt)
+      weight_load<F, D, kStore>(buf[tt], a, s, key + 16 * (ST * kWeightWaves + tt), lane);
     const bool whole = key >= all_lo && key + 16 * ST - 1 <= all_hi;
     float x[ST][MT][4], mx[MT];
     bool grow = false;
@@ -311,10 +327,6 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_lse(WeightArgs a) {
                 (fast_exp2(x[tt][t][2] - m[t]) + fast_exp2(x[tt][t][3] - m[t]));
     weight_fence();
     key += 16 * ST * kWeightWaves;
-    return true;
-  };
-  load(bufA, key);
-  while (step(bufA, bufB) && step(bufB, bufA)) {
   }
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
@@ -330,7 +342,7 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_lse(WeightArgs a) {
     for (int w = 0; w < kWeightWaves; ++w) mx = fmaxf(mx, part[w][r].x);
 #pragma unroll
     for (int w = 0; w < kWeightWaves; ++w) sum += part[w][r].y * fast_exp2(part[w][r].x - mx);
-    a.ml[((uint64_t)blockIdx.x * a.row_cap + row0 + r) * a.n_chunk + chunk] =
+    a.ml[((uint64_t)seg * a.row_cap + row0 + r) * a.n_chunk + chunk] =
         make_float2(mx, sum);
   }
 }
@@ -358,6 +370,7 @@ __device__ __forceinline__ float weight_join(const float2* ml, uint32_t n) {
 
 constexpr uint32_t kWeightJoinRows = 1024;  // rows whose lse a workgroup joins in LDS
 constexpr int kWeightKt = 4;                // 16-key tiles a wave of pass 2 holds
+constexpr uint32_t kWeightBlock = 64;       // rows whose Q a workgroup of pass 2 stages
 
 // Joins the segment's rows [r0, r1) into lds; every thread calls it.
 __device__ __forceinline__ void weight_lse_rows(float* lds, const WeightArgs& a, uint32_t seg,
@@ -376,9 +389,13 @@ __device__ __forceinline__ void weight_write(const WeightArgs& a, float* w, floa
 // than one part the sums go to a.part, which weights_add adds up.
 template <typename T, int F, int D>
 __global__ __launch_bounds__(64 * kWeightWaves) void weights_sum(WeightArgs a) {
-  constexpr int KT = kWeightKt;
+  constexpr int KT = kWeightKt, PR = D / 8;  // 16-byte pieces of a Q row
+  constexpr int N = kWeightBlock * PR / (64 * kWeightWaves);
   __shared__ float lse_lds[kWeightJoinRows];
-  __shared__ uint32x4 stage[kWeightWaves][16 * WeightTile<F, D>::kPieces];
+  // The rows' Q, a block of them for all four waves (two blocks in turn); before
+  // the first, each wave's K on its way to operands.
+  __shared__ uint32x4 lds[2][kWeightBlock * PR];
+  static_assert(kWeightWaves * 16 * WeightTile<F, D>::kPieces <= 2 * kWeightBlock * PR, "K's place");
   const WeightSeg s = weight_seg(a, blockIdx.x);
   const int32_t wg0 = (int32_t)(blockIdx.y * 16 * KT * kWeightWaves);
   if (!s.ok || wg0 >= s.len_k) return;
@@ -395,63 +412,94 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_sum(WeightArgs a) {
     r1 = (uint32_t)max((int64_t)0, min((int64_t)r1, j * a.group.d));
   }
   r1 = max(r0, r1);
-  weight_lse_rows(lse_lds, a, blockIdx.x, r0, r1);
   const uint32_t lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int32_t wave = (int32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int32_t key0 = wg0 + 16 * KT * wave;
-  if (key0 >= s.len_k) return;
   uint4 k[KT][D / 32];
   float by[KT], sum[KT][4];
   {
+    uint32x4* const place = &lds[0][0] + wave * 16 * WeightTile<F, D>::kPieces;
     WeightTile<F, D> raw[KT];
 #pragma unroll
-    for (int t = 0; t < KT; ++t) weight_load<F, D>(raw[t], a, s, key0 + 16 * t, lane);
+    for (int t = 0; t < KT; ++t) weight_load<F, D, false>(raw[t], a, s, key0 + 16 * t, lane);
+    weight_lse_rows(lse_lds, a, blockIdx.x, r0, r1);
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
-      weight_stage<F, D>(stage[wave], raw[t], lane);
+      weight_stage<F, D>(place, raw[t], lane);
       weight_fence();
-      weight_operand<T, F, D>(stage[wave], k[t], a.hd, col, g);
+      weight_operand<T, F, D>(place, k[t], a.hd, col, g);
       weight_fence();
       by[t] = raw[t].scale * a.scale_log2;
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[t][i] = 0.f;
     }
+    __syncthreads();
   }
-  if (r0 < r1) {
-    uint4 next[D / 32];
-    weight_q<T, F, D>(next, a, s, r0 + col, g);
-    for (uint32_t r = r0; r < r1; r += 16) {
-      uint4 q[D / 32];
+  // A block's Q pieces in registers: loaded a block ahead, then put in LDS.
+  uint32x4 held[N];
+  auto fetch = [&](uint32_t first) __attribute__((always_inline)) {
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) q[c] = next[c];
-      weight_q<T, F, D>(next, a, s, r + 16 + col, g);
-      const uint32_t row = min(r + col, r1 - 1);
-      const float lse = r + col < r1 ? lse_lds[row - r0] : INFINITY;
-      const int32_t pos = s.pos0 + (int32_t)a.group.div(row);
-      const int32_t lo = weight_lo(a, pos), hi = weight_hi(a, pos, s.len_k);
-      const bool whole = __all(key0 >= lo && key0 + 16 * KT - 1 <= hi);
-      floatx4 acc[KT];
+    for (int i = 0; i < N; ++i) {
+      const uint32_t at = 64 * kWeightWaves * i + threadIdx.x;
+      const uint32_t row = min(first + at / PR, s.n_rows - 1), piece = at % PR;
+      const uint32_t j = a.group.div(row), c = row - j * a.group.d;
+      const char* q = a.q + (((uint64_t)(s.q0 + j) * a.num_heads + s.h * a.group.d + c) * a.hd) * 2;
+      held[i] = *(const uint32x4*)(q + min(16 * piece, 2 * a.hd - 16));
+    }
+  };
+  uint32_t turn = 0;
+  if (r0 < r1) fetch(r0);
+  for (uint32_t first = r0; first < r1; first += kWeightBlock, turn ^= 1) {
 #pragma unroll
-      for (int t = 0; t < KT; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < N; ++i) {
+      const uint32_t at = 64 * kWeightWaves * i + threadIdx.x, row = at / PR, piece = at % PR;
+      lds[turn][row * PR + (piece ^ (row & 7))] = held[i] & (8 * piece < a.hd ? 0xFFFFFFFFu : 0u);
+    }
+    if (first + kWeightBlock < r1) fetch(first + kWeightBlock);
+    // (One barrier a block: a wave that writes a buffer again has passed the
+    // barrier that every wave reaches after reading it.)
+    lds_barrier();
+    if (key0 < s.len_k) {
+      const uint32_t end = min(first + kWeightBlock, r1);
+#pragma unroll 1
+      for (uint32_t r = first; r < end; r += 16) {
+        uint4 q[D / 32];
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c)
+        for (int c = 0; c < D / 32; ++c) {
+          const uint32_t row = r - first + col;
+          q[c] = __builtin_bit_cast(uint4,
+                                    lds[turn][row * PR + ((weight_d<F>(c, g) / 8) ^ (row & 7))]);
+        }
+        const uint32_t row = min(r + col, r1 - 1);
+        const float lse = r + col < r1 ? lse_lds[row - r0] : INFINITY;
+        const int32_t pos = s.pos0 + (int32_t)a.group.div(row);
+        const int32_t lo = weight_lo(a, pos), hi = weight_hi(a, pos, s.len_k);
+        const bool whole = __all(key0 >= lo && key0 + 16 * KT - 1 <= hi);
+        floatx4 acc[KT];
 #pragma unroll
-        for (int t = 0; t < KT; ++t) acc[t] = mfma16x16x32<T>(k[t][c], q[c], acc[t]);
-      if (whole) {
+        for (int t = 0; t < KT; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+          for (int t = 0; t < KT; ++t) acc[t] = mfma16x16x32<T>(k[t][c], q[c], acc[t]);
+        float x[KT][4];
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            sum[t][i] += fast_exp2(__builtin_fmaf(acc[t][i], by[t], -lse));
-      } else {
+          for (int i = 0; i < 4; ++i) x[t][i] = __builtin_fmaf(acc[t][i], by[t], -lse);
+        if (!whole) {
+#pragma unroll
+          for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int32_t at = key0 + 16 * t + 4 * (int32_t)g + i;
+              x[t][i] = at >= lo && at <= hi ? x[t][i] : -INFINITY;
+            }
+        }
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int32_t at = key0 + 16 * t + 4 * (int32_t)g + i;
-            const float x = __builtin_fmaf(acc[t][i], by[t], -lse);
-            sum[t][i] += fast_exp2(at >= lo && at <= hi ? x : -INFINITY);
-          }
+          for (int i = 0; i < 4; ++i) sum[t][i] += fast_exp2(x[t][i]);
       }
     }
   }
@@ -536,13 +584,13 @@ static WeightPlan weight_plan(uint32_t batch, uint32_t kvh, uint32_t group, uint
   const uint64_t n_q = last ? std::min(max_q, last) : max_q;
   const uint64_t rows = n_q * group;
   p.row_cap = (uint32_t)std::min<uint64_t>(rows, 0x7FFFFFF0u);
-  p.mt = rows <= 16 ? 1 : hd > 128 ? 4 : 8;
+  p.mt = rows <= 16 ? 1 : 4;
   p.row_tiles = (p.row_cap + 16 * p.mt - 1) / (16 * p.mt);
   p.key_cap = (max_k + 63) & ~63u;
   p.store = rows <= 16 && segs * rows * p.key_cap * sizeof(float) <= kStoreBytes;
   auto up = [](uint64_t x, uint64_t y) { return (x + y - 1) / y; };
   const uint64_t want = std::max<uint64_t>(up(kWeightWgs, p.row_tiles * segs), 1);
-  uint64_t keys = std::max<uint64_t>(up(max_k, want), 512);
+  uint64_t keys = std::max<uint64_t>(up(max_k, want), 256);
   p.chunk_keys = (uint32_t)(up(keys, 256) * 256);
   p.n_chunk = (uint32_t)std::max<uint64_t>(up(max_k, p.chunk_keys), 1);
   const uint64_t blocks = up(max_k, 16 * kWeightKt * kWeightWaves);
@@ -568,9 +616,7 @@ static void launch_weights_d(const WeightArgs& a, const WeightPlan& p, uint32_t 
     return;
   }
   if (p.mt == 1) hipLaunchKernelGGL((weights_lse<T, F, D, 1, false>), g1, block, 0, s, a);
-  else if constexpr (D == 256)
-    hipLaunchKernelGGL((weights_lse<T, F, D, 4, false>), g1, block, 0, s, a);
-  else hipLaunchKernelGGL((weights_lse<T, F, D, 8, false>), g1, block, 0, s, a);
+  else hipLaunchKernelGGL((weights_lse<T, F, D, 4, false>), g1, block, 0, s, a);
   const uint32_t keys = 16 * kWeightKt * kWeightWaves;
   hipLaunchKernelGGL((weights_sum<T, F, D>), dim3(segs, (max_k + keys - 1) / keys, p.parts), block,
                      0, s, a);
