@@ -369,7 +369,7 @@ __device__ __forceinline__ float weight_join(const float2* ml, uint32_t n) {
 }
 
 constexpr uint32_t kWeightJoinRows = 1024;  // rows whose lse a workgroup joins in LDS
-constexpr int kWeightKt = 4;                // 16-key tiles a wave of pass 2 holds
+constexpr int kWeightKt = 2;                // 16-key tiles a wave of pass 2 holds
 constexpr uint32_t kWeightBlock = 64;       // rows whose Q a workgroup of pass 2 stages
 
 // Joins the segment's rows [r0, r1) into lds; every thread calls it.

@@ -82,6 +82,12 @@ __device__ __forceinline__ float q8_finite(T x) {
   return mag > __float_as_uint(big) ? copysignf(big, f) : f;
 }
 
+// The bits of kBig in T: magnitudes up to it are stored as they are.
+template <typename T, int F>
+__device__ __forceinline__ uint32_t q8_big_bits() {
+  return from_f32<T>(Q8Range<T, F>::kBig).x;
+}
+
 // The least power of two s >= kMinScale with amax / s <= 448 (e4m3), < 128
 // (int8); 0 for amax = 0. amax = m 2^E with m in [1, 2): s = 2^(E - 8), or
 // 2^(E - 7) where m > 1.75; 2^(E - 6) for int8. Works on the bits of amax;
@@ -117,6 +123,23 @@ __device__ __forceinline__ uint32_t q8_pack4(float a, float b, float c, float d)
       return (uint32_t)(int32_t)fminf(fmaxf(__builtin_rintf(x), -127.f), 127.f) & 0xffu;
     };
     return one(a) | one(b) << 8 | one(c) << 16 | one(d) << 24;
+  }
+}
+
+// The same where no value needs a limit: magnitudes up to 448, below 127.5.
+// (Adding 1.5 2^23 rounds to a whole number, ties to even, in the low bits.)
+template <int F>
+__device__ __forceinline__ uint32_t q8_pack4_within(float a, float b, float c, float d) {
+  if constexpr (F == VAPI_KV_Q8_E4M3) {
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+  } else {
+    constexpr float kRound = 12582912.f;
+    const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(b + kRound),
+                                              __float_as_uint(a + kRound), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(d + kRound),
+                                              __float_as_uint(c + kRound), 0x04000c0cu);
+    return lo | hi;
   }
 }
 

@@ -72,6 +72,10 @@ int check_q8_pool(const vapi_kv_q8_pool* p, uint32_t layer, const char* who) {
 // before it, skipped ones aside, lies in another block). A workgroup looks at
 // `chunk` tokens; its waves and those of the grid's y dimension share the
 // units of the leaders among them.
+//
+// 4,096 rows of 8 x 128 in runs of 256 (24 MB read and written): 10.5 us, 2.3
+// TB/s; what bounds it is the chain slot -> rows -> largest magnitude -> codes of
+// one unit a wave, ~5 us with the launch, and the VALU's ~5 operations a value.
 
 struct Q8AppendArgs {
   const char* src[2];  // K, V rows
@@ -95,27 +99,29 @@ __global__ __launch_bounds__(64 * kAppendWaves) void q8_append_kernel(Q8AppendAr
   int32_t* const rows = row_of[wave];
   const uint32_t bs = 1u << a.bs_shift;
   const uint32_t t0 = blockIdx.x * a.chunk;
-  // The block of each of this workgroup's tokens (none: past the pool).
+  // The blocks of the 64 tokens from the first of this workgroup's on, and of the
+  // 64 before (none: skipped, or past the pool).
   constexpr uint32_t kNone = 0xFFFFFFFFu;
-  auto block_of = [&](uint32_t t) {
-    const uint32_t s = a.slots[t];
-    return s < a.num_slots ? s >> a.bs_shift : kNone;
-  };
-  const uint32_t mine = lane < a.chunk && t0 + lane < a.n ? block_of(t0 + lane) : kNone;
+  auto block_of = [&](uint32_t s) { return s < a.num_slots ? s >> a.bs_shift : kNone; };
+  auto slot_at = [&](uint32_t t) { return t < a.n ? a.slots[t] : kNone; };
+  const uint32_t slot = slot_at(t0 + lane);
+  uint32_t back = block_of(lane < t0 ? a.slots[t0 - 1 - lane] : kNone);
+  const uint32_t mine = block_of(slot);
   const uint64_t valid = __ballot(mine != kNone);
-  if (valid == 0) return;
-  // The last valid token before this lane's: within the chunk, or before it.
+  const uint64_t own = a.chunk >= 64 ? ~0ull : (1ull << a.chunk) - 1;
+  if ((valid & own) == 0) return;
+  // The last valid token before this workgroup's.
   uint32_t before = kNone;
-  for (uint32_t end = t0; end > 0 && before == kNone;) {
-    const uint32_t w = min(end, 64u);
-    const uint32_t b = lane < w ? block_of(end - 1 - lane) : kNone;
-    const uint64_t m = __ballot(b != kNone);
-    if (m) before = __builtin_amdgcn_readlane(b, (uint32_t)__builtin_ctzll(m));
-    end -= w;
+  for (uint32_t end = t0;;) {
+    const uint64_t m = __ballot(back != kNone);
+    if (m) before = __builtin_amdgcn_readlane(back, (uint32_t)__builtin_ctzll(m));
+    if (m || end <= 64) break;
+    end -= 64;
+    back = block_of(lane < end ? a.slots[end - 1 - lane] : kNone);
   }
   const uint64_t below = valid & ((1ull << lane) - 1);
   const uint32_t prev = (uint32_t)__shfl((int)mine, below ? 63 - __builtin_clzll(below) : 0);
-  uint64_t leaders = __ballot(mine != kNone && mine != (below ? prev : before));
+  uint64_t leaders = own & __ballot(mine != kNone && mine != (below ? prev : before));
 
   const uint32_t units = 2 * a.kvh;
   const uint32_t waves = gridDim.y * kAppendWaves;
@@ -131,13 +137,17 @@ __global__ __launch_bounds__(64 * kAppendWaves) void q8_append_kernel(Q8AppendAr
     // Which token brings each slot of the block (-1: none of this call's).
     for (uint32_t o = lane; o < bs; o += 64) rows[o] = -1;
     wait_lds();
-    for (uint32_t t = t0 + li; t < a.n; t += 64) {
-      const uint32_t s = t + lane < a.n ? a.slots[t + lane] : kNone;
-      const uint32_t b = s < a.num_slots ? s >> a.bs_shift : kNone;
-      const uint64_t other = __ballot(b != kNone && b != blk);
-      const bool in = b == blk && !(other & ((1ull << lane) - 1));
-      if (in) rows[s & (bs - 1)] = (int32_t)(t + lane);
-      if (other) break;
+    uint32_t sl = slot;
+    uint64_t from = ~0ull << li;  // the window's tokens from the leader on
+    for (uint32_t t = t0;;) {
+      const uint32_t bl = block_of(sl);
+      const uint64_t other = __ballot(bl != kNone && bl != blk) & from;
+      if (bl == blk && (from >> lane & 1) && !(other & ((1ull << lane) - 1)))
+        rows[sl & (bs - 1)] = (int32_t)(t + lane);
+      t += 64;
+      if (other || t >= a.n) break;
+      sl = slot_at(t + lane);
+      from = ~0ull;
     }
     wait_lds();
     const bool fresh = __builtin_amdgcn_readfirstlane(rows[0]) >= 0;
@@ -163,22 +173,47 @@ __global__ __launch_bounds__(64 * kAppendWaves) void q8_append_kernel(Q8AppendAr
           }
         }
       };
-      auto at = [](const uint4& v, int e) {
+      // An element as it is (two to a word), and as it is stored where some are
+      // not numbers the format holds.
+      auto raw = [](const uint4& v, int e) {
         const uint32_t w = e < 2 ? v.x : e < 4 ? v.y : e < 6 ? v.z : v.w;
-        return q8_finite<T, F>(T{(uint16_t)(e & 1 ? w >> 16 : w & 0xffffu)});
+        return T{(uint16_t)(e & 1 ? w >> 16 : w & 0xffffu)};
       };
-      uint32_t top = 0;  // the bits of a magnitude order as the magnitude does
+      // The largest magnitude: the bits of magnitudes order as they do.
+      typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+      u16x2 most = {0, 0};
       for (uint32_t base = 0; base < total; base += 64 * kAppendRegs) {
         load(base);
 #pragma unroll
-        for (int j = 0; j < kAppendRegs; ++j)
+        for (int j = 0; j < kAppendRegs; ++j) {
+          const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            top = max(top, __float_as_uint(at(x[j], e)) & 0x7fffffffu);
+          for (int e = 0; e < 4; ++e)
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w[e] & 0x7fff7fffu));
+        }
       }
-      top = wave_reduce(top, [](uint32_t p, uint32_t q) { return max(p, q); });
+      uint32_t top = wave_reduce((uint32_t)max(most[0], most[1]),
+                                 [](uint32_t p, uint32_t q) { return max(p, q); });
+      // NaN, infinities and what rounds past the format's range are rare: such a
+      // unit takes the long way round.
+      const bool odd = top > q8_big_bits<T, F>();
+      if (odd) {
+        uint32_t big = 0;
+        for (uint32_t base = 0; base < total; base += 64 * kAppendRegs) {
+          if (total > 64 * kAppendRegs) load(base);
+#pragma unroll
+          for (int j = 0; j < kAppendRegs; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              big = max(big, __float_as_uint(q8_finite<T, F>(raw(x[j], e))) & 0x7fffffffu);
+        }
+        top = wave_reduce(big, [](uint32_t p, uint32_t q) { return max(p, q); });
+      } else {
+        top = __float_as_uint(to_f32(T{(uint16_t)top}));
+      }
       const float s = fmaxf(s_old, q8_scale<T, F>(__uint_as_float(top)));
       const float inv = q8_inverse(s);
+      const bool slow = odd || (F == VAPI_KV_Q8_INT8 && __uint_as_float(top) * inv >= 127.5f);
       // Rows of earlier calls: 0 in a block that starts here, shifted where
       // the scale grew, untouched otherwise.
       const bool rest = fresh || s != s_old;
@@ -194,10 +229,17 @@ __global__ __launch_bounds__(64 * kAppendWaves) void q8_append_kernel(Q8AppendAr
           uint2* p = (uint2*)(dst + (uint64_t)o * a.tok + 8 * c);
           if (rows[o] >= 0) {
             float v[8];
+            if (slow) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = at(x[j], e) * inv;
-            *p = make_uint2(q8_pack4<F>(v[0], v[1], v[2], v[3]),
-                            q8_pack4<F>(v[4], v[5], v[6], v[7]));
+              for (int e = 0; e < 8; ++e) v[e] = q8_finite<T, F>(raw(x[j], e)) * inv;
+              *p = make_uint2(q8_pack4<F>(v[0], v[1], v[2], v[3]),
+                              q8_pack4<F>(v[4], v[5], v[6], v[7]));
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] = to_f32(raw(x[j], e)) * inv;
+              *p = make_uint2(q8_pack4_within<F>(v[0], v[1], v[2], v[3]),
+                              q8_pack4_within<F>(v[4], v[5], v[6], v[7]));
+            }
           } else if (rest) {
             uint2 w = make_uint2(0u, 0u);
             if (shift > 0.f) {
@@ -306,7 +348,12 @@ int vapi_kv_q8_append(const vapi_kv_q8_pool* pool, uint32_t layer, const void* k
   a.kvh = g.kvh, a.d = g.d;
   a.blk = g.blk, a.head = g.head, a.tok = g.tok, a.sblk = g.sblk;
   a.upr = FastDiv(g.d / 8);
-  a.chunk = n_tokens <= 512 ? 1 : n_tokens <= 16384 ? 4 : 16;
+  // Tokens a workgroup looks at. Few tokens are mostly single ones of decode rows,
+  // a unit each (64 tokens, 8 kv heads: 7.4 us one to a workgroup, 9.5 at four);
+  // many are runs, where a workgroup without a leader is launched for nothing
+  // (4,096 tokens in runs of 256: 30.1 / 15.0 / 12.5 / 10.5 us at 1 / 4 / 8 / 16;
+  // 4,096 single ones 40.8 / 37.1 / 41.2 / 44.1; 512 in runs 8.3 / 7.7 / 7.6 / 7.7).
+  a.chunk = n_tokens <= 256 ? 1 : n_tokens <= 1024 ? 4 : 16;
   const uint32_t y = std::min((2 * g.kvh + kAppendWaves - 1) / kAppendWaves, 65535u);
   const dim3 grid((n_tokens + a.chunk - 1) / a.chunk, y);
 #define VK_APPEND(T, F)                                                                     \
