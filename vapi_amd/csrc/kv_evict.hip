@@ -2,10 +2,10 @@
 // stay, and their rows moved into new blocks.
 //
 //  1. evict_select: a workgroup per (sequence, kv head) finds the weight of the
-//     last key that stays by a radix select on order-preserving keys (8 bits a
-//     pass, a histogram in LDS), then walks the positions in order and writes
-//     the kept ones with their weights. Ties go to the earlier position: the
-//     walk counts those equal to the threshold as it meets them.
+//     last key that stays by a radix select on order-preserving keys (a
+//     histogram of a digit in LDS), then writes the kept positions in order with
+//     their weights. Ties go to the earlier position: a prefix sum numbers those
+//     equal to the threshold.
 //  2. evict_copy (any pool): 16-byte pieces of K and V rows, from each head's
 //     own positions. evict_q8: a wave per (new block, kv head, K or V) takes
 //     the rows' codes and scales, finds the block's scale from their largest
@@ -15,8 +15,6 @@
 #include "q8.hpp"
 
 namespace vk {
-
-constexpr uint32_t kSelectThreads = 1024;
 
 struct EvictArgs {
   const float* in;
@@ -40,11 +38,55 @@ __device__ __forceinline__ uint32_t evict_key(float w) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-__global__ __launch_bounds__(kSelectThreads) void evict_select(EvictArgs a) {
-  constexpr uint32_t kWaves = kSelectThreads / 64;
-  __shared__ uint32_t hist[256], counts[2][kWaves], found[2];
+// The sum of x over the lanes up to this one.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+#define VK_SHIFT(CTRL, ROWS) \
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, false)
+  VK_SHIFT(0x111, 0xF);  // row_shr:1, 2, 4, 8: within rows of 16 lanes
+  VK_SHIFT(0x112, 0xF);
+  VK_SHIFT(0x114, 0xF);
+  VK_SHIFT(0x118, 0xF);
+  VK_SHIFT(0x142, 0xA);  // row_bcast:15 and :31: the rows before
+  VK_SHIFT(0x143, 0xC);
+#undef VK_SHIFT
+  return x;
+}
+
+// The sum of x over the threads before this one (in thread order), and over all
+// of them; `waves` is LDS of a word a wave. Every thread calls it.
+template <uint32_t NT>
+__device__ __forceinline__ uint32_t evict_scan(uint32_t x, uint32_t* waves, uint32_t* total) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t run = wave_scan(x);
+  __syncthreads();  // the words' last readers
+  if (lane == 63) waves[wave] = run;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+#pragma unroll
+  for (uint32_t v = 0; v < NT / 64; ++v) {
+    const uint32_t t = waves[v];
+    before += v < wave ? t : 0u;
+    all += t;
+  }
+  *total = all;
+  return before + run - x;
+}
+
+constexpr uint32_t kSelectBins = 1u << 11;
+constexpr uint32_t kSelectKeys = 12288;  // keys held in LDS (48 KiB)
+
+// Up to kSelectKeys keys are read once and held in LDS, longer sequences walked in
+// tiles of that many. Digits of 11, 11 and 10 bits from the top: three passes, and
+// bins that part weights of one magnitude (8-bit digits hold little but the
+// exponent, and a wave's adds to one bin queue up). NT threads: 256 for up to
+// 4,096 keys, where barriers are most of the time, else 1,024. (Keys in
+// registers, 16 a thread, unrolled: 16.8 against @B1@ us for 8 heads of 1,500
+// keys; the code is fetched once.)
+template <uint32_t NT>
+__global__ __launch_bounds__(NT) void evict_select(EvictArgs a) {
+  __shared__ uint32_t hist[kSelectBins], waves[NT / 64], found[2], keys[kSelectKeys];
   const uint32_t seq = blockIdx.x / a.kvh, h = blockIdx.x - seq * a.kvh;
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t tid = threadIdx.x;
   const uint32_t in_row = a.in_index ? a.in_index[seq] : seq;
   const uint32_t out_row = a.out ? (a.out_index ? a.out_index[seq] : seq) : 0;
   int32_t* kept = a.kept + (uint64_t)blockIdx.x * a.max_keep;
@@ -58,88 +100,113 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select(EvictArgs a) {
   // Always kept: [0, first) and [end, len); of [first, end) the `want` largest.
   const uint32_t first = min(a.sinks, len), end = len - min(a.recent, len - first);
   const uint32_t want = n - first - (len - end);
+  const bool once = len <= kSelectKeys;
+  auto load = [&](uint32_t base) {
+    const uint32_t count = min(len - base, kSelectKeys);
+#pragma unroll 4
+    for (uint32_t i = tid; i < count; i += NT) keys[i] = evict_key(w[base + i]);
+  };
+  if (once) load(0);
   uint32_t threshold = 0, equal = 0xFFFFFFFFu;  // all of them
-  if (want < end - first) {
+  if (want == 0) {
+    threshold = 0xFFFFFFFFu, equal = 0;
+  } else if (want < end - first) {
     // The want-th largest key: digit by digit, `equal` of the keys that share
     // the digits found so far are still wanted.
-    uint32_t prefix = 0;
+    uint32_t prefix = 0, mask = 0, shift = 32;
     equal = want;
-    for (int shift = 24; shift >= 0 && want > 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const uint32_t bits = pass < 2 ? 11 : 10, digit = (1u << bits) - 1;
+      shift -= bits;
+      for (uint32_t i = tid; i < kSelectBins; i += NT) hist[i] = 0;
       __syncthreads();
-      const uint32_t above = shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
-      for (uint32_t i = first + tid; i < end; i += kSelectThreads) {
-        const uint32_t key = evict_key(w[i]);
-        if ((key & above) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1u);
+      for (uint32_t base = 0; base < len; base += kSelectKeys) {
+        if (!once) {
+          __syncthreads();
+          load(base);
+        }
+        // (A thread reads the keys that it put there.)
+        const uint32_t count = min(len - base, kSelectKeys);
+#pragma unroll 2
+        for (uint32_t i = tid; i < count; i += NT) {
+          const uint32_t key = keys[i], at = base + i;
+          if (at >= first && at < end && (key & mask) == prefix)
+            atomicAdd(&hist[key >> shift & digit], 1u);
+        }
       }
       __syncthreads();
-      if (tid < 64) {
-        // Lane l holds digits 255 - 4 l .. 252 - 4 l, from the largest down.
-        uint32_t c[4], sum = 0;
+      // A thread's bins, from the largest down.
+      constexpr uint32_t kOwn = kSelectBins / NT;
+      uint32_t sum = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) c[j] = hist[255 - (4 * lane + j)], sum += c[j];
-        uint32_t run = sum;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const uint32_t y = __shfl_up(run, o);
-          if (lane >= (uint32_t)o) run += y;
-        }
-        run -= sum;  // keys with larger digits than this lane's
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (run < equal && equal <= run + c[j])
-            found[0] = 255 - (4 * lane + j), found[1] = equal - run;
-          run += c[j];
+      for (uint32_t j = 0; j < kOwn; ++j) sum += hist[kSelectBins - 1 - kOwn * tid - j];
+      uint32_t total;
+      uint32_t above = evict_scan<NT>(sum, waves, &total);
+      if (above < equal && equal <= above + sum) {
+        for (uint32_t j = 0; j < kOwn; ++j) {
+          const uint32_t bin = kSelectBins - 1 - kOwn * tid - j, c = hist[bin];
+          if (equal <= above + c) {
+            found[0] = bin, found[1] = equal - above;
+            break;
+          }
+          above += c;
         }
       }
       __syncthreads();
       prefix |= found[0] << shift;
+      mask |= digit << shift;
       equal = found[1];
-      __syncthreads();
     }
     threshold = prefix;
-    if (want == 0) threshold = 0xFFFFFFFFu, equal = 0;
   }
-  // In order of position: larger ones, and the first `equal` of the equal ones.
+  // In order of position: larger ones, and the first `equal` of the equal ones. A
+  // thread takes consecutive keys (an odd number, so that no two lanes meet in a
+  // bank more often than they must).
   uint32_t eq_before = 0, at = 0;
-  for (uint32_t base = 0; base < len; base += kSelectThreads) {
-    const uint32_t i = base + tid;
-    const bool mid = i >= first && i < end;
-    const float x = i < len ? w[i] : 0.f;
-    const uint32_t key = evict_key(x);
-    const uint64_t eq = __ballot(mid && key == threshold);
-    if (lane == 0) counts[0][wave] = (uint32_t)__popcll(eq);
+  for (uint32_t base = 0; base < len; base += kSelectKeys) {
     __syncthreads();
-    uint32_t rank = eq_before, total = eq_before;
-    for (uint32_t v = 0; v < kWaves; ++v) {
-      if (v < wave) rank += counts[0][v];
-      total += counts[0][v];
+    if (!once) {
+      load(base);
+      __syncthreads();
     }
-    eq_before = total;
-    rank += (uint32_t)__popcll(eq & ((1ull << lane) - 1));
-    const bool take = i < len && (!mid || key > threshold || (key == threshold && rank < equal));
-    const uint64_t taken = __ballot(take);
-    if (lane == 0) counts[1][wave] = (uint32_t)__popcll(taken);
-    __syncthreads();
-    uint32_t to = at;
-    total = at;
-    for (uint32_t v = 0; v < kWaves; ++v) {
-      if (v < wave) to += counts[1][v];
-      total += counts[1][v];
+    const uint32_t count = min(len - base, kSelectKeys);
+    const uint32_t per = (count + NT - 1) / NT | 1u;
+    const uint32_t i0 = min(tid * per, count), i1 = min(i0 + per, count);
+    uint32_t eq = 0, sure = 0;  // equal to the threshold; taken whatever their rank
+    for (uint32_t i = i0; i < i1; ++i) {
+      const uint32_t p = base + i;
+      const bool mid = p >= first && p < end;
+      eq += mid && keys[i] == threshold;
+      sure += !mid || keys[i] > threshold;
     }
-    at = total;
-    to += (uint32_t)__popcll(taken & ((1ull << lane) - 1));
-    // to <= i: with out the same row as in, what is overwritten has been read.
-    if (take && to < n) {
-      kept[to] = (int32_t)i;
-      if (out && to < a.out_width) out[to] = x;
+    uint32_t total, rank = eq_before + evict_scan<NT>(eq, waves, &total);
+    eq_before += total;
+    // Of this thread's equal ones, those whose rank is below `equal`.
+    const uint32_t of_eq = rank < equal ? min(eq, equal - rank) : 0u;
+    uint32_t to = at + evict_scan<NT>(sure + of_eq, waves, &total);
+    at += total;
+    for (uint32_t i = i0; i < i1; ++i) {
+      const uint32_t p = base + i, key = keys[i];
+      bool take = p < first || p >= end || key > threshold;
+      if (!take && key == threshold) take = rank++ < equal;
+      if (take && to < a.max_keep) kept[to] = (int32_t)p;
+      to += take;
     }
   }
-  for (uint32_t j = n + tid; j < a.max_keep; j += kSelectThreads) kept[j] = -1;
-  if (out && ok) {
+  for (uint32_t j = n + tid; j < a.max_keep; j += NT) kept[j] = -1;
+  if (!out || !ok) return;
+  // The kept ones' weights. j <= kept[j], so with out the same row as in a round
+  // of NT reads before it writes, and later rounds read past what it wrote.
+  __syncthreads();
+  for (uint32_t base = 0; base < n; base += NT) {
+    const uint32_t j = base + tid;
+    const float x = j < n ? w[kept[j]] : 0.f;
     __syncthreads();
-    for (uint32_t j = n + tid; j < a.out_width; j += kSelectThreads) out[j] = 0.f;
+    if (j < n) out[j] = x;
   }
+  __syncthreads();
+  for (uint32_t j = n + tid; j < a.out_width; j += NT) out[j] = 0.f;
 }
 
 // ---- rows into their new blocks ---------------------------------------------------
@@ -155,25 +222,47 @@ struct EvictMove {
   uint32_t row_bytes;
 };
 
-// Grid: (pieces of a head's kept rows, segments, K or V).
+// Grid: (groups of kCopyRows kept rows a thread, segments, K or V): a thread copies
+// one piece of kCopyRows rows, their addresses (kept position, table entry) and
+// loads in flight together.
+constexpr int kCopyRows = 4;
 template <int C>
 __global__ __launch_bounds__(256) void evict_copy(EvictMove a, FastDiv upr) {
   using V = typename Chunk<C>::T;
   const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-  const uint32_t j = upr.div(i), u = i - j * upr.d;
-  if (j >= a.max_keep) return;
+  const uint32_t r = upr.div(i), u = i - r * upr.d;
   const uint32_t seq = blockIdx.y / a.kvh, h = blockIdx.y - seq * a.kvh;
-  const int32_t from = a.kept[(uint64_t)blockIdx.y * a.max_keep + j];
-  if (from < 0) return;
-  const uint32_t sb = a.bs.div((uint32_t)from), db = a.bs.div(j);
-  const uint32_t src = min(a.src_table[(uint64_t)seq * a.src_blocks + min(sb, a.src_blocks - 1)],
-                           a.num_blocks - 1);
-  if (db >= a.dst_blocks) return;
-  const uint32_t dst = a.dst_table[(uint64_t)seq * a.dst_blocks + db];
-  if (dst >= a.num_blocks) return;
+  const int32_t* kept = a.kept + (uint64_t)blockIdx.y * a.max_keep;
+  const uint32_t* from = a.src_table + (uint64_t)seq * a.src_blocks;
+  const uint32_t* to = a.dst_table + (uint64_t)seq * a.dst_blocks;
   char* base = (blockIdx.z ? a.v : a.k) + h * a.head_b + (uint64_t)u * C;
-  const uint64_t so = ((uint32_t)from - sb * a.bs.d) * a.tok_b, d_o = (j - db * a.bs.d) * a.tok_b;
-  *(V*)(base + dst * a.blk_b + d_o) = load_stream((const V*)(base + src * a.blk_b + so));
+  // Row k of a thread lies `apart` rows from row k - 1.
+  const uint32_t apart = (a.max_keep + kCopyRows - 1) / kCopyRows;
+  if (r >= apart) return;
+  int32_t pos[kCopyRows];
+  uint32_t dst[kCopyRows];
+#pragma unroll
+  for (int k = 0; k < kCopyRows; ++k) {
+    const uint32_t j = r + k * apart, db = a.bs.div(j);
+    pos[k] = j < a.max_keep ? kept[j] : -1;
+    dst[k] = j < a.max_keep && db < a.dst_blocks ? to[db] : 0xFFFFFFFFu;
+  }
+  const char* src[kCopyRows];
+#pragma unroll
+  for (int k = 0; k < kCopyRows; ++k) {
+    const uint32_t p = (uint32_t)max(pos[k], 0), sb = a.bs.div(p);
+    src[k] = base + min(from[min(sb, a.src_blocks - 1)], a.num_blocks - 1) * a.blk_b +
+             (p - sb * a.bs.d) * a.tok_b;
+  }
+  V v[kCopyRows];
+#pragma unroll
+  for (int k = 0; k < kCopyRows; ++k) v[k] = load_stream((const V*)src[k]);
+#pragma unroll
+  for (int k = 0; k < kCopyRows; ++k) {
+    const uint32_t j = r + k * apart;
+    if (pos[k] >= 0 && dst[k] < a.num_blocks)
+      *(V*)(base + dst[k] * a.blk_b + (j - a.bs.div(j) * a.bs.d) * a.tok_b) = v[k];
+  }
 }
 
 constexpr int kMoveRegs = 4;  // 16-code pieces a lane holds: 4,096 codes a wave
@@ -239,17 +328,20 @@ __global__ __launch_bounds__(64 * kMoveWaves) void evict_q8(EvictMove a, FastDiv
 #pragma unroll
     for (int r = 0; r < kMoveRegs; ++r) {
       const uint32_t i = first + 64 * r + lane;
+      // A power of two, 1 where the scale stays. (Past 2^20 only rows of zeros
+      // have it: a value of theirs would have made the new scale larger.)
+      const float by = fminf(s[r] * inv, 0x1p20f);
+      uint32_t out[4] = {w[r].x, w[r].y, w[r].z, w[r].w};
+      if (__any(by != 1.f)) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x[4];
+          q8_unpack4<F>(out[e], x);
+          out[e] = q8_pack4_within<F>(x[0] * by, x[1] * by, x[2] * by, x[3] * by);
+        }
+      }
       if (i >= total) continue;
       const uint32_t o = upr.div(i), c = i - o * upr.d;
-      uint32_t out[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float x[4];
-        q8_unpack4<F>(word(w[r], e), x);
-        // (Two products: s times 1 / scale may not be a number of its own.)
-        out[e] = q8_pack4<F>(x[0] * s[r] * inv, x[1] * s[r] * inv, x[2] * s[r] * inv,
-                             x[3] * s[r] * inv);
-      }
       *(uint4*)(base + dst * a.blk_b + o * a.tok_b + 16 * c) =
           make_uint4(out[0], out[1], out[2], out[3]);
     }
@@ -308,7 +400,10 @@ static void launch_evict_select(const EvictCall& c, uint32_t kvh, hipStream_t s)
   a.lens = c.lens, a.kept = c.kept, a.kvh = kvh, a.max_len = c.max_len;
   a.max_keep = std::min(c.budget, c.max_len);
   a.budget = c.budget, a.sinks = c.sinks, a.recent = c.recent;
-  hipLaunchKernelGGL(evict_select, dim3(c.batch * kvh), dim3(kSelectThreads), 0, s, a);
+  if (c.max_len <= 4096)
+    hipLaunchKernelGGL((evict_select<256>), dim3(c.batch * kvh), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((evict_select<1024>), dim3(c.batch * kvh), dim3(1024), 0, s, a);
 }
 
 static EvictMove evict_move(const EvictCall& c, uint32_t kvh, uint32_t num_blocks,
@@ -353,7 +448,8 @@ int vapi_kv_evict(const vapi_kv_pool* pool, uint32_t layer, const vapi_kv_weight
   if ((uint64_t)m.max_keep * upr >= 0x7FFFFFFFull)
     VK_FAIL(VAPI_KV_EUNSUP, "%s: %u kept keys of %u bytes", who, m.max_keep, m.row_bytes);
   launch_evict_select(c, g.kvh, hs(stream));
-  const dim3 grid((m.max_keep * upr + 255) / 256, batch * g.kvh, pool->v ? 2 : 1);
+  const uint32_t rows = (m.max_keep + kCopyRows - 1) / kCopyRows;
+  const dim3 grid((rows * upr + 255) / 256, batch * g.kvh, pool->v ? 2 : 1);
 #define VK_EVICT(C)                                                                       \
   case C:                                                                                 \
     hipLaunchKernelGGL((evict_copy<C>), grid, dim3(256), 0, hs(stream), m, FastDiv(upr)); \

@@ -29,23 +29,26 @@ def new_weights(rows: int, num_kv_heads: int, width: int, device="cuda") -> torc
 
 def _state(weights: torch.Tensor, cache, index: torch.Tensor | None, batch: int, name: str):
     """vapi_kv_weights over a [rows, num_kv_heads, width] f32 tensor."""
-    if weights.dim() != 3 or weights.shape[1] != cache.num_kv_heads:
+    shape = weights.shape
+    if len(shape) != 3 or shape[1] != cache.num_kv_heads:
         raise ValueError(f"{name} must be (rows, {cache.num_kv_heads}, width), "
-                         f"got {tuple(weights.shape)}")
+                         f"got {tuple(shape)}")
     if weights.dtype != torch.float32:
         raise ValueError(f"{name} must be float32, not {weights.dtype}")
-    if weights.numel() == 0:
-        raise ValueError(f"{name} is empty: {tuple(weights.shape)}")
-    if weights.shape[2] > 1 and weights.stride(2) != 1:
+    rows, _, width = shape
+    if rows == 0 or width == 0:
+        raise ValueError(f"{name} is empty: {tuple(shape)}")
+    row_stride, head_stride, last = weights.stride()
+    if width > 1 and last != 1:
         raise ValueError(f"{name}'s last dimension must be contiguous")
-    if index is not None and (index.dtype not in (torch.int32, torch.uint32) or
-                              tuple(index.shape) != (batch,) or not index.is_contiguous()):
-        raise ValueError(f"rows must be {batch} contiguous 32-bit indices")
-    if index is None and batch > weights.shape[0]:
-        raise ValueError(f"{batch} sequences but {weights.shape[0]} rows of {name}")
-    return Weights(data=weights.data_ptr(), index=None if index is None else index.data_ptr(),
-                   row_stride=weights.stride(0), head_stride=weights.stride(1),
-                   rows=weights.shape[0], width=weights.shape[2])
+    if index is not None:
+        if (index.dtype is not torch.int32 and index.dtype is not torch.uint32) or \
+                index.dim() != 1 or index.shape[0] != batch or not index.is_contiguous():
+            raise ValueError(f"rows must be {batch} contiguous 32-bit indices")
+    elif batch > rows:
+        raise ValueError(f"{batch} sequences but {rows} rows of {name}")
+    return Weights(weights.data_ptr(), None if index is None else index.data_ptr(), row_stride,
+                   head_stride, rows, width)
 
 
 def _rows(rows, count: int, device) -> torch.Tensor | None:
@@ -177,8 +180,9 @@ class EvictionPlan:
 
 
 def _extent(t: torch.Tensor) -> tuple[int, int]:
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    (r, h, w), (sr, sh, sw) = t.shape, t.stride()
+    first = t.data_ptr()
+    return first, first + 4 * ((r - 1) * sr + (h - 1) * sh + (w - 1) * sw + 1)
 
 
 def evict_kv(cache, layer: int, weights: torch.Tensor, plan: EvictionPlan,
@@ -204,11 +208,12 @@ def evict_kv(cache, layer: int, weights: torch.Tensor, plan: EvictionPlan,
     src = _state(weights, cache, plan.rows, b, "weights")
     on = [weights, plan.lens, plan.src_table]
     dst = None
-    if weights_out is not None:
+    if weights_out is weights:
+        dst = src
+    elif weights_out is not None:
         dst = _state(weights_out, cache, plan.rows, b, "weights_out")
         on.append(weights_out)
-        if weights_out is not weights and (weights_out.data_ptr() != weights.data_ptr() or
-                                           weights_out.stride() != weights.stride()):
+        if dst.data != src.data or weights_out.stride() != weights.stride():
             (a0, a1), (b0, b1) = _extent(weights), _extent(weights_out)
             if a0 < b1 and b0 < a1:
                 raise ValueError("weights_out overlaps weights: give the same tensor or another")
