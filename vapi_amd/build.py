@@ -62,7 +62,7 @@ NO_SCRATCH = {"attn_prefill.hip": ("paged_prefill_tiled", "paged_mixed_stream"),
               "attn_decode.hip": ("paged_decode_stream",),
               "attn_decode_small.hip": ("paged_decode_small",),
               "attn_prefill_f32.hip": ("paged_prefill_f32",),
-              "attn_q8.hip": ("q8_decode_stream",),
+              "attn_q8.hip": ("q8_decode_stream", "q8_decode_small"),
               "kv_weights.hip": ("weights_lse", "weights_sum")}
 
 # Half of a CU's 160 KiB of LDS less the dynamic part (4 bytes for each of the

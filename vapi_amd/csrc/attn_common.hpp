@@ -786,6 +786,10 @@ SmallPlan decode_small_plan(uint32_t batch, uint32_t kvh, uint32_t group, uint32
 // `part`: the split's partials (16-byte aligned; unused without a split).
 void launch_decode_small(const AttnArgs& a, uint32_t head_dim, uint32_t dtype, SmallPlan plan,
                          void* part, hipStream_t s);
+// The merge of a split's partials alone (16-bit outputs), after a kernel that
+// wrote them as launch_decode_small's does.
+void launch_decode_small_merge(const AttnArgs& a, uint32_t head_dim, bool bf16, uint32_t n_split,
+                               hipStream_t s);
 // Prefill rows (len_q > 1); bf16/f16, head_dim 64, 128 or 256.
 // Workgroups of the prefill launch (query tiles x kv heads x sequences); a
 // launch needs it below 2^32.

@@ -443,6 +443,30 @@ SmallPlan decode_small_plan(uint32_t batch, uint32_t kvh, uint32_t group, uint32
   return {bytes <= n * kSmallMaxBytes, (uint32_t)n};
 }
 
+void launch_decode_small_merge(const AttnArgs& a, uint32_t head_dim, bool bf16, uint32_t n_split,
+                               hipStream_t s) {
+  const dim3 grid(a.batch * a.kvh), block(64 * kSmallWaves);
+#define VK_SMM(T, DD)                                                                             \
+  do {                                                                                            \
+    if (a.hd != DD)                                                                               \
+      hipLaunchKernelGGL((paged_decode_small_merge<T, DD, true>), grid, block, 0, s, a, a.cu_q,   \
+                         a.cu_k, n_split);                                                        \
+    else                                                                                          \
+      hipLaunchKernelGGL((paged_decode_small_merge<T, DD, false>), grid, block, 0, s, a, a.cu_q,  \
+                         a.cu_k, n_split);                                                        \
+  } while (0)
+  if (bf16) {
+    if (head_dim == 256) VK_SMM(bf16_t, 256);
+    else if (head_dim == 128) VK_SMM(bf16_t, 128);
+    else VK_SMM(bf16_t, 64);
+  } else {
+    if (head_dim == 256) VK_SMM(f16_t, 256);
+    else if (head_dim == 128) VK_SMM(f16_t, 128);
+    else VK_SMM(f16_t, 64);
+  }
+#undef VK_SMM
+}
+
 void launch_decode_small(const AttnArgs& a_in, uint32_t head_dim, uint32_t dtype, SmallPlan plan,
                          void* part, hipStream_t s) {
   AttnArgs a = a_in;

@@ -36,9 +36,9 @@ struct Q8Scales {
 template <int D>
 constexpr int q8_step_keys() { return D == 256 ? 32 : 64; }
 
-template <int D>
+template <int D, int kKeys = q8_step_keys<D>()>
 struct Q8Step {
-  static constexpr int KS = q8_step_keys<D>(), NT = KS / 16;
+  static constexpr int KS = kKeys, NT = KS / 16;
   uint4 k[NT][D / 64];
   uint32_t v[NT][4][D / 64];
   float ks[NT], vs[NT];
@@ -65,8 +65,8 @@ __device__ __forceinline__ void q8_load_q(uint4* qs, const AttnArgs& a, const De
 // Codes and scales of the step at p.key0. Every load stays inside a block the
 // table names: tiles past the row's last key re-read the tile that holds it and
 // keys past it read that key (masked out of the softmax).
-template <int D, bool kPad, bool kNt>
-__device__ __forceinline__ void q8_load(Q8Step<D>& st, const AttnArgs& a, const Q8Scales& sc,
+template <int D, bool kPad, bool kNt, int KS>
+__device__ __forceinline__ void q8_load(Q8Step<D, KS>& st, const AttnArgs& a, const Q8Scales& sc,
                                         const uint32_t* __restrict__ table, const DecodePos& p,
                                         uint32_t col, uint32_t g) {
   using ConstU32 = const __attribute__((address_space(4))) uint32_t;
@@ -75,7 +75,7 @@ __device__ __forceinline__ void q8_load(Q8Step<D>& st, const AttnArgs& a, const 
   const uint32_t kh = a.kv_parts.div(p.kh);
   const int32_t last = p.len_k - 1;
 #pragma unroll
-  for (int tt = 0; tt < Q8Step<D>::NT; ++tt) {
+  for (int tt = 0; tt < KS / 16; ++tt) {
     const int32_t ts = min(p.key0 + 16 * tt, last & ~15);
     const int32_t lim = last - ts;
     const uint32_t blk = min(tab[min((uint32_t)ts >> a.bs_shift, a.max_blocks - 1)], a.last_blk);
@@ -115,17 +115,14 @@ __device__ __forceinline__ void q8_load(Q8Step<D>& st, const AttnArgs& a, const 
 
 // One step of the online softmax for 16 query columns (attend_qk and attend_pv
 // of the 16-bit kernels, with the tiles' scales).
-template <typename T, int F, int D>
-__device__ __forceinline__ void q8_attend(const Q8Step<D>& st, const uint4* qs, uint32_t lane,
+template <typename T, int F, int D, int KS>
+__device__ __forceinline__ void q8_attend(const Q8Step<D, KS>& st, const uint4 (&qf)[D / 32],
                                           floatx4 (&o)[D / 16], float& m_run, float& l_run,
                                           float scale_log2, int32_t key0, int32_t lo,
                                           int32_t len_k, uint32_t g) {
-  constexpr int NT = Q8Step<D>::NT, DPL = D / 16;
+  constexpr int NT = KS / 16, DPL = D / 16;
   float s[4 * NT];
   float mx = -INFINITY;
-  uint4 qf[D / 32];
-#pragma unroll
-  for (int c = 0; c < D / 32; ++c) qf[c] = qs[c * 64 + lane];
 #pragma unroll
   for (int tt = 0; tt < NT; ++tt) {
     floatx4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -243,7 +240,7 @@ __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void q8_de
 #pragma unroll
   for (int k = 0; k < DPL; ++k) o[k] = floatx4{0.f, 0.f, 0.f, 0.f};
   Q8Step<D> stA, stB;
-  q8_load<D, kPad, kNt>(stA, a, sc, table, pos, col, g);
+  q8_load<D, kPad, kNt, KS>(stA, a, sc, table, pos, col, g);
 
   auto step = [&](Q8Step<D>& cur, Q8Step<D>& next) -> bool {
     const bool more = t + 1 < t_end;
@@ -261,9 +258,11 @@ __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void q8_de
       nxt.key0 = 0;
       nxt.len_k = 1;
     }
-    q8_load<D, kPad, kNt>(next, a, sc, table, nxt, col, g);
-    q8_attend<T, F, D>(cur, qs, lane, o, m_run, l_run, a.scale_log2, pos.key0, pos.lo, pos.len_k,
-                       g);
+    q8_load<D, kPad, kNt, KS>(next, a, sc, table, nxt, col, g);
+    uint4 qf[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) qf[c] = qs[c * 64 + lane];
+    q8_attend<T, F, D>(cur, qf, o, m_run, l_run, a.scale_log2, pos.key0, pos.lo, pos.len_k, g);
     if (!same_piece) {
       const uint32_t seg = pos.seq * a.kvh + pos.kh;
       if (lane == 0) {
@@ -288,6 +287,115 @@ __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void q8_de
   }
   const uint32_t t_done = (uint32_t)__builtin_amdgcn_s_memrealtime();
   if (lane == 0) *(uint4*)stat = make_uint4(t_end - t_begin, t_entry, t_done, 0u);
+}
+
+// ---- short contexts ------------------------------------------------------------
+
+// Few short rows: paged_decode_small's scheme (a workgroup of 8 waves, 4 at
+// head_dim 256, per (sequence, kv head), or n_split of them; steps of 32 keys in
+// turn; (m, l, o) joined through LDS in wave order; a split's partials merged by
+// the second launch of the 16-bit kernel) over 8-bit steps.
+template <int D>
+constexpr int q8_small_waves() { return D == 256 ? 4 : 8; }
+constexpr uint32_t kQ8SmallPad = 4;  // floats between rows of O in LDS (bank conflicts)
+
+template <typename T, int F, int D, bool kPad, bool kSplit>
+__global__ __launch_bounds__(64 * q8_small_waves<D>(), 1) void q8_decode_small(
+    AttnArgs a, Q8Scales sc, const uint32_t* __restrict__ cu_q, const uint32_t* __restrict__ cu_k,
+    const uint32_t* __restrict__ table, uint32_t n_split_arg) {
+  constexpr int W = q8_small_waves<D>(), DPL = D / 16, KS = 32;
+  const uint32_t n_split = kSplit ? n_split_arg : 1u;
+  extern __shared__ __attribute__((aligned(16))) float o_lds[];  // [W][group][D + pad]
+  __shared__ float2 ml_lds[W][16];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
+  const int32_t wave = (int32_t)__builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t seg = blockIdx.x / n_split, split = blockIdx.x - seg * n_split;
+  DecodePos p;
+  p.seq = seg / a.kvh;
+  p.kh = seg - p.seq * a.kvh;
+  p.q0 = cu_q[p.seq];
+  p.len_k = (int32_t)(cu_k[p.seq + 1] - cu_k[p.seq]);
+  if (cu_q[p.seq + 1] - p.q0 != 1 || p.len_k <= 0) return;
+  p.lo = a.wl >= 0 ? max(0, p.len_k - 1 - a.wl) : 0;
+  p.fuse = 0, p.seg_first = 0;
+  const int32_t first = p.lo & ~(KS - 1);
+  int32_t key_end = p.len_k;
+  p.key0 = first;
+  if constexpr (kSplit) {
+    const uint32_t steps = (uint32_t)(p.len_k - first + KS - 1) / KS;
+    p.key0 = first + KS * (int32_t)(split * steps / n_split);
+    key_end = min(p.len_k, first + KS * (int32_t)((split + 1) * steps / n_split));
+  }
+  p.key0 += KS * wave;
+  float m_run = kNegBig, l_run = 0.f;
+  floatx4 o[DPL];
+#pragma unroll
+  for (int k = 0; k < DPL; ++k) o[k] = floatx4{0.f, 0.f, 0.f, 0.f};
+  const uint32_t count = vhead_count(a, p.kh), h0 = vhead_base(a, p.kh);
+  const uint32_t hd = kPad ? a.hd : (uint32_t)D;
+  if (p.key0 < key_end) {
+    Q8Step<D, KS> stA, stB;
+    q8_load<D, kPad, true, KS>(stA, a, sc, table, p, col, g);
+    const T* qrow =
+        (const T*)a.q + ((uint64_t)p.q0 * a.num_heads + h0 + (col < count ? col : 0)) * hd;
+    uint4 qf[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      const uint32_t d = 64 * (c / 2) + 16 * g + 8 * (c % 2);
+      const uint32_t keep = !kPad || d < hd ? 0xFFFFFFFFu : 0u;
+      const uint4 x = *(const uint4*)(qrow + (kPad ? min(d, hd - 8) : d));
+      qf[c] = make_uint4((x.x ^ a.q_sign) & keep, (x.y ^ a.q_sign) & keep,
+                         (x.z ^ a.q_sign) & keep, (x.w ^ a.q_sign) & keep);
+    }
+    // The next step on its way while one is computed (a wave's last repeats it).
+    auto step = [&](Q8Step<D, KS>& cur, Q8Step<D, KS>& next) __attribute__((always_inline)) {
+      const int32_t s0 = p.key0;
+      const bool more = s0 + KS * W < key_end;
+      if (more) p.key0 += KS * W;
+      q8_load<D, kPad, true, KS>(next, a, sc, table, p, col, g);
+      q8_attend<T, F, D, KS>(cur, qf, o, m_run, l_run, a.scale_log2, s0, p.lo, p.len_k, g);
+      return more;
+    };
+    while (step(stA, stB) && step(stB, stA)) {
+    }
+  }
+  constexpr uint32_t S = D + kQ8SmallPad;
+  const float l_tot = wave_sum_g(l_run);
+  if (g == 0) ml_lds[wave][col] = make_float2(m_run, l_tot);
+  if (col < count) {
+    float* row = o_lds + ((uint32_t)wave * a.group + col) * S;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < DPL; k += 4)
+        *(float4*)(row + v_d<D>(4 * g + i, k)) =
+            make_float4(o[k][i], o[k + 1][i], o[k + 2][i], o[k + 3][i]);
+  }
+  __syncthreads();
+  for (uint32_t e = 4 * tid; e < count * D; e += 4 * 64 * W) {
+    const uint32_t c = e / D, d = e % D;
+    if (kPad && d >= hd) continue;
+    float M = kNegBig, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) M = fmaxf(M, ml_lds[w][c].x);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float f = fast_exp2(ml_lds[w][c].x - M);
+      const float4 y = *(const float4*)(o_lds + ((uint32_t)w * a.group + c) * S + d);
+      L += ml_lds[w][c].y * f;
+      x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
+    }
+    if constexpr (kSplit) {
+      const uint64_t slot = (uint64_t)blockIdx.x * a.group + c;
+      *(float4*)(a.ws_o + slot * D + d) = x;
+      if (d == 0) *(float2*)(a.ws_ml + slot * 2) = make_float2(M, L);
+    } else {
+      const float inv = L > 0.f ? 1.f / L : 0.f;
+      T* dst = (T*)a.out + ((uint64_t)p.q0 * a.num_heads + h0 + c) * hd + d;
+      *(uint2*)dst = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+    }
+  }
 }
 
 // ---- prefill: codes expanded into the workspace ----------------------------------
@@ -402,6 +510,65 @@ static void launch_q8_decode(const AttnArgs& a, const Q8Scales& sc, void* worksp
     launch_decode_merge(c, nwg, D, std::is_same_v<T, bf16_t>, s,
                         decode_merge_slices(c.group, D));
   }
+}
+
+// Whether a call takes the short-context kernel, and into how many workgroups a
+// row's keys go, by the bytes of K codes a row has (the host's bound). Measured, 32
+// q / 8 kv heads, e4m3, us a call, stream / one workgroup / shares of 32 KiB: 1 x
+// 100 keys 12.6 / 9.3 / 9.1, 1 x 700 13.8 / 9.6 / 11.4, 1 x 1,337 14.2 / 13.4 /
+// 11.4, 1 x 8,191 17.5 / 60.1 / 12.5, 4 x 2,000 15.0 / 19.6 / 12.6, 16 x 700 16.9 /
+// 11.5 / 13.1, 16 x 2,000 23.2 / 22.3 / 19.6, 32 x 300 17.2 / 9.6 / 9.2, 32 x 700
+// 20.9 / 13.3 / 13.3 (the first two columns of short rows are the host's time for
+// one launch, 9 us, and two, 11). Only the longest row is known here and a share
+// of a long one ends after the balanced stream does, hence the largest share.
+constexpr uint64_t kQ8SmallWgs = 256;              // workgroups at once, one per CU
+constexpr uint64_t kQ8SmallUnsplit = 112ull << 10;  // whole rows up to this
+constexpr uint64_t kQ8SmallShare = 32ull << 10;     // else into shares of at least this
+constexpr uint64_t kQ8SmallMaxBytes = 128ull << 10;
+static size_t q8_small_lds(uint32_t group, uint32_t D) {
+  return (size_t)(D == 256 ? 4 : 8) * group * (D + kQ8SmallPad) * sizeof(float);
+}
+static SmallPlan q8_small_plan(const AttnArgs& a, uint32_t D, uint32_t max_k, size_t part_bytes) {
+  const uint64_t seg = (uint64_t)a.batch * a.kvh;
+  if (seg > kQ8SmallWgs || q8_small_lds(a.group, D) > 56 * 1024) return {false, 1};
+  const uint64_t span = a.wl >= 0 ? std::min<uint64_t>(max_k, (uint64_t)a.wl + 32) : max_k;
+  const uint64_t bytes = span * D;
+  uint64_t n = 1;
+  if (bytes > kQ8SmallUnsplit)
+    n = std::max<uint64_t>(
+        std::min<uint64_t>(kQ8SmallWgs / seg, (bytes + kQ8SmallShare - 1) / kQ8SmallShare), 1);
+  n = std::min<uint64_t>(n, 32);
+  while (n > 1 && seg * n * a.group * (D + 2) * sizeof(float) > part_bytes) --n;
+  return {bytes <= n * kQ8SmallMaxBytes, (uint32_t)n};
+}
+
+template <typename T, int F, int D, bool kPad>
+static void launch_q8_small_d(const AttnArgs& a, const Q8Scales& sc, uint32_t n_split,
+                              hipStream_t s) {
+  const dim3 grid(a.batch * a.kvh * n_split), block(64 * q8_small_waves<D>());
+  const size_t lds = q8_small_lds(a.group, D);
+  if (n_split > 1)
+    hipLaunchKernelGGL((q8_decode_small<T, F, D, kPad, true>), grid, block, lds, s, a, sc, a.cu_q,
+                       a.cu_k, a.table, n_split);
+  else
+    hipLaunchKernelGGL((q8_decode_small<T, F, D, kPad, false>), grid, block, lds, s, a, sc,
+                       a.cu_q, a.cu_k, a.table, 1u);
+}
+template <typename T, int F>
+static void launch_q8_small(const AttnArgs& a_in, const Q8Scales& sc, uint32_t D, uint32_t n_split,
+                            void* part, hipStream_t s) {
+  AttnArgs a = a_in;
+  a.ws_o = (float*)part;
+  a.ws_ml = (float*)part + (uint64_t)a.batch * a.kvh * n_split * a.group * D;
+  const bool pad = a.hd != D;
+  if (D == 256 && pad) launch_q8_small_d<T, F, 256, true>(a, sc, n_split, s);
+  else if (D == 256) launch_q8_small_d<T, F, 256, false>(a, sc, n_split, s);
+  else if (D == 128 && pad) launch_q8_small_d<T, F, 128, true>(a, sc, n_split, s);
+  else if (D == 128) launch_q8_small_d<T, F, 128, false>(a, sc, n_split, s);
+  else if (pad) launch_q8_small_d<T, F, 64, true>(a, sc, n_split, s);
+  else launch_q8_small_d<T, F, 64, false>(a, sc, n_split, s);
+  if (n_split > 1)
+    launch_decode_small_merge(a, D, std::is_same_v<T, bf16_t>, n_split, s);
 }
 
 template <typename T, int F>
@@ -530,7 +697,12 @@ int vapi_kv_q8_attention(const vapi_kv_q8_pool* pool, uint32_t layer, const void
       dec.group = (G + parts - 1) / parts;
       dec.kv_parts = FastDiv(parts);
     }
-    VK_Q8(launch_q8_decode, dec, sc, workspace, D, s);
+    // (The partials of a split lie past the balance block, as the stream's.)
+    const SmallPlan small = q8_small_plan(dec, D, max_seqlen_k, dec_ws - kDecodeBalanceBytes);
+    if (small.ok)
+      VK_Q8(launch_q8_small, dec, sc, D, small.n_split, (char*)workspace + kDecodeBalanceBytes, s);
+    else
+      VK_Q8(launch_q8_decode, dec, sc, workspace, D, s);
   }
   if (pf_n && mb) {
     char* ws = (char*)workspace + off;
