@@ -225,6 +225,21 @@ def test_decode(fmt, dtype, heads, kvh, d, bs, layout):
                     layout)
 
 
+@pytest.mark.parametrize("fmt,dtype", [("e4m3", BF16), ("e4m3", F16), ("int8", BF16),
+                                       ("int8", F16)])
+@pytest.mark.parametrize("heads,kvh,d,bs,layout,left", [
+    (4, 2, 128, 16, "HND", None), (4, 4, 64, 32, "NHD", 50), (3, 1, 256, 16, "HND", None),
+    (2, 2, 80, 16, "NHD", 70), (4, 4, 96, 64, "HND", 129), (3, 3, 16, 16, "HND", None),
+    (34, 2, 128, 16, "HND", None), (71, 1, 64, 16, "HND", 40), (40, 1, 208, 128, "NHD", None)])
+def test_decode_of_many_rows(fmt, dtype, heads, kvh, d, bs, layout, left):
+    """More (sequence, kv head) pairs than the short-context kernel takes, rows of
+    other lengths among them (the persistent stream)."""
+    n = 260 // kvh + 3
+    lens = [1 + (7 * i) % 150 + (400 if i % 41 == 7 else 0) for i in range(n)]
+    check_attention([1 + 2 * (i == 5) for i in range(n)], [max(k, 3) for k in lens], heads, kvh,
+                    d, bs, fmt, dtype, layout, left)
+
+
 @pytest.mark.parametrize("fmt,dtype", [("e4m3", BF16), ("int8", F16), ("int8", BF16)])
 @pytest.mark.parametrize("left", [0, 1, 15, 63, 64, 100, 5000])
 def test_decode_window(fmt, dtype, left):

@@ -80,7 +80,7 @@ constexpr uint32_t kSelectKeys = 12288;  // keys held in LDS (48 KiB)
 // bins that part weights of one magnitude (8-bit digits hold little but the
 // exponent, and a wave's adds to one bin queue up). NT threads: 256 for up to
 // 4,096 keys, where barriers are most of the time, else 1,024. (Keys in
-// registers, 16 a thread, unrolled: 16.8 against @B1@ us for 8 heads of 1,500
+// registers, 16 a thread, unrolled: 16.8 against 10.9 us for 8 heads of 1,500
 // keys; the code is fetched once.)
 template <uint32_t NT>
 __global__ __launch_bounds__(NT) void evict_select(EvictArgs a) {

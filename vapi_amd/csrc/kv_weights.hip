@@ -11,12 +11,20 @@
 //     sum of its own over the keys it sees, joined across lanes and waves at
 //     the end: (m, l) per row and chunk.
 //  2. weights_sum: a wave holds KT 16-key tiles of K in registers, walks the
-//     rows that see them and adds up exp2(s - lse) per key; the 16 lanes of a
-//     key are added at the end. Each weight has one owner: no atomics, a fixed
-//     order.
-// S^T = K Q^T as in the attention kernels (lane (col, g) holds keys 4 g .. +3
-// of row col), straight from HBM/L2 into MFMA operands. Pass 2 reads K again:
-// from L2 or the last-level cache where a call's K fits them.
+//     rows that see them (Q staged in LDS for the workgroup's four waves) and
+//     adds up exp2(s - lse) per key; the 16 lanes of a key are added at the end.
+//     Many rows go in parts, whose sums weights_add adds in order. Each weight has
+//     one owner: no atomics, a fixed order.
+// S^T = K Q^T as in the attention kernels: lane (col, g) holds keys 4 g .. +3 of
+// row col. Up to 16 rows (single tokens) the scores themselves are kept and pass 2
+// is a sum over them (weights_stored).
+//
+// What bounds it. Single tokens: HBM, K once (129 MB in 31 us, 4.2 TB/s, of 37 us
+// with pass 2). Many rows: VALU, an exponential and ~6 operations a score in each
+// pass beside 1/16 of an MFMA: three fresh prompts of 700-2,000 tokens (32 q / 8 kv
+// heads, f16; 30 GFLOP of scores) 56 + 69 + 5 us. Few rows over long contexts:
+// latency, ~4 us of dependent loads before a workgroup's first product in each
+// pass (a prompt's last 32 queries over 6,500 keys, 28 q / 4 kv heads: 16 + 13 us).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -213,8 +221,8 @@ constexpr int weight_step() {
 
 // Every grid has the segments fastest, so that the round-robin dealing over the
 // XCDs gives each of them work of every sequence (with the chunks fastest, eight
-// chunks put the ends of all long sequences on one XCD: 16 sequences of
-// 256-8,192 keys 47.9 us against @ORDER@).
+// chunks put the ends of all long sequences on one XCD; the three fresh prompts
+// 285 -> 207 us).
 // Grid: (segments, row tiles x chunks). kStore: the scores are kept (then one
 // row tile, MT = 1).
 template <typename T, int F, int D, int MT, bool kStore>
@@ -368,8 +376,11 @@ __device__ __forceinline__ float weight_join(const float2* ml, uint32_t n) {
   return sum > 0.f ? mx + __builtin_amdgcn_logf(sum) : INFINITY;
 }
 
-constexpr uint32_t kWeightJoinRows = 1024;  // rows whose lse a workgroup joins in LDS
-constexpr int kWeightKt = 2;                // 16-key tiles a wave of pass 2 holds
+constexpr uint32_t kWeightJoinRows = 512;  // rows whose lse a workgroup joins in LDS
+// 16-key tiles a wave of pass 2 holds. More of them read Q less often, fewer leave
+// registers for more waves: three fresh prompts (below) 73.2 / 69.2 / 84.6 us at 2 /
+// 3 / 4, a prompt's last 32 queries 15.5 / 13.5 / 18.6.
+constexpr int kWeightKt = 3;
 constexpr uint32_t kWeightBlock = 64;       // rows whose Q a workgroup of pass 2 stages
 
 // Joins the segment's rows [r0, r1) into lds; every thread calls it.
@@ -472,9 +483,11 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_sum(WeightArgs a) {
         }
         const uint32_t row = min(r + col, r1 - 1);
         const float lse = r + col < r1 ? lse_lds[row - r0] : INFINITY;
-        const int32_t pos = s.pos0 + (int32_t)a.group.div(row);
-        const int32_t lo = weight_lo(a, pos), hi = weight_hi(a, pos, s.len_k);
-        const bool whole = __all(key0 >= lo && key0 + 16 * KT - 1 <= hi);
+        // (Uniform: the first row's last key and the last row's first one.)
+        const int32_t p0 = s.pos0 + (int32_t)a.group.div(r);
+        const int32_t p1 = s.pos0 + (int32_t)a.group.div(min(r + 15, r1 - 1));
+        const bool whole =
+            key0 >= weight_lo(a, p1) && key0 + 16 * KT - 1 <= weight_hi(a, p0, s.len_k);
         floatx4 acc[KT];
 #pragma unroll
         for (int t = 0; t < KT; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -488,6 +501,8 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_sum(WeightArgs a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[t][i] = __builtin_fmaf(acc[t][i], by[t], -lse);
         if (!whole) {
+          const int32_t pos = s.pos0 + (int32_t)a.group.div(row);
+          const int32_t lo = weight_lo(a, pos), hi = weight_hi(a, pos, s.len_k);
 #pragma unroll
           for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -574,7 +589,7 @@ struct WeightPlan {
 // kWeightWgs workgroups where the rows alone do not, parts of the rows pass 2.
 // Up to 16 rows and kStoreBytes the scores are kept between the passes: 8 bytes
 // a score moved instead of K read again (16 sequences of 256-8,192 keys, 32 q /
-// 8 kv heads, bf16: @STORED@).
+// 8 kv heads, bf16: pass 2 53.6 -> 7.1 us).
 constexpr uint64_t kWeightWgs = 1024;
 constexpr uint64_t kStoreBytes = 256ull << 20;
 static WeightPlan weight_plan(uint32_t batch, uint32_t kvh, uint32_t group, uint32_t hd,
