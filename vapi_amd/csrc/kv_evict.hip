@@ -38,6 +38,11 @@ __device__ __forceinline__ uint32_t evict_key(float w) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
+// The weight of a key (a NaN for a NaN, +0 for either zero).
+__device__ __forceinline__ float evict_weight(uint32_t key) {
+  return __uint_as_float(key >> 31 ? key ^ 0x80000000u : ~key);
+}
+
 // The sum of x over the lanes up to this one.
 __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 #define VK_SHIFT(CTRL, ROWS) \
@@ -190,21 +195,17 @@ __global__ __launch_bounds__(NT) void evict_select(EvictArgs a) {
       const uint32_t p = base + i, key = keys[i];
       bool take = p < first || p >= end || key > threshold;
       if (!take && key == threshold) take = rank++ < equal;
-      if (take && to < a.max_keep) kept[to] = (int32_t)p;
+      // to <= p: with out the same row as in, what is overwritten has been read (the
+      // keys in LDS hold the weights).
+      if (take && to < a.max_keep) {
+        kept[to] = (int32_t)p;
+        if (out) out[to] = evict_weight(key);
+      }
       to += take;
     }
   }
   for (uint32_t j = n + tid; j < a.max_keep; j += NT) kept[j] = -1;
   if (!out || !ok) return;
-  // The kept ones' weights. j <= kept[j], so with out the same row as in a round
-  // of NT reads before it writes, and later rounds read past what it wrote.
-  __syncthreads();
-  for (uint32_t base = 0; base < n; base += NT) {
-    const uint32_t j = base + tid;
-    const float x = j < n ? w[kept[j]] : 0.f;
-    __syncthreads();
-    if (j < n) out[j] = x;
-  }
   __syncthreads();
   for (uint32_t j = n + tid; j < a.out_width; j += NT) out[j] = 0.f;
 }
