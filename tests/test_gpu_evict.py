@@ -368,6 +368,53 @@ def test_prompt_eviction_and_generation(fmt):
     assert not state[0].any() and kept.shape == (2, kvh, 80)
 
 
+def test_another_stream():
+    """Everything made for a call on a side stream outlives it: host rows, a query
+    that has to be made contiguous, outputs dropped at once."""
+    cache, tables, free = filled([300, 90], 2, 64, 16, "int8", BF16, "HND", 3, spare=20)
+    dst = [[free.pop() for _ in range(4)] for _ in range(2)]
+    plan = EvictionPlan.from_tables([300, 90], tables, dst, 60, 4, 10, 16, "cuda", [3, 1])
+    prep = PreparedAttention.from_batch(batch_of([20, 1], [300, 90], tables), "cuda")
+    wide = torch.randn(21, 4, 128, device="cuda").to(BF16)
+    q = wide[:, :, ::2]
+    want = accumulate_attention_weights(q, cache, 0, prep, 0.1, new_weights(4, 2, 300),
+                                        rows=[3, 1])
+    kept = evict_kv(cache, 0, want, plan)
+    codes = cache._codes.clone()
+    side = torch.cuda.Stream()
+    w = new_weights(4, 2, 300)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(10_000_000)  # the current stream is behind
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        accumulate_attention_weights(q, cache, 0, prep, 0.1, w, rows=[3, 1], decay=0.0,
+                                     stream=side)
+        got = evict_kv(cache, 0, w, plan, stream=side)
+        junk = [torch.full((n,), -1, dtype=torch.int32, device="cuda") for n in (2, 21 * 256, 240)]
+        del junk
+    side.synchronize()
+    assert torch.equal(w, want) and torch.equal(got, kept) and torch.equal(cache._codes, codes)
+
+
+def test_states_of_two_sizes_share_a_step():
+    """A call that needs a larger workspace leaves a captured one's alone."""
+    cache, tables, _ = filled([300], 2, 64, 16, "none", BF16, "HND", 3)
+    prep = PreparedAttention.from_batch(batch_of([200], [300], tables), "cuda")
+    q = torch.randn(200, 4, 64, device="cuda").to(BF16)
+    w, big = new_weights(1, 2, 300), new_weights(1, 2, 300)
+    accumulate_attention_weights(q, cache, 0, prep, 0.1, w, last_queries=3, decay=0.0)
+    want = w.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        accumulate_attention_weights(q, cache, 0, prep, 0.1, w, last_queries=3, decay=0.0)
+    accumulate_attention_weights(q, cache, 0, prep, 0.1, big)
+    for _ in range(3):
+        w.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(w, want)
+
+
 def test_captured_weights_and_eviction_replay():
     cache, tables, free = filled([300, 90], 2, 64, 16, "e4m3", BF16, "HND", 3, spare=20)
     dst = [[free.pop() for _ in range(4)] for _ in range(2)]

@@ -15,8 +15,8 @@ import numpy as np
 import torch
 
 from ._lib import ESPACE, check, lib
-from .cache import (PagedKvCache, _is_quantised, _per_layer, check_on_device, stream_handle,
-                    write_rows_indexed)
+from .cache import (PagedKvCache, _is_quantised, _per_layer, check_on_device, keep_for,
+                    stream_handle, write_rows_indexed)
 
 _u32p = ctypes.POINTER(ctypes.c_uint32)
 
@@ -116,6 +116,7 @@ class PreparedAttention:
     prefill_seqs: torch.Tensor | None = None
     n_prefill: int = 0
     weights_workspace: torch.Tensor | None = None  # accumulate_attention_weights
+    weights_workspaces: list = field(default_factory=list)  # earlier, smaller ones
 
     @classmethod
     def from_batch(cls, batch: ForwardBatch, device, cache=None, num_heads: int | None = None,
@@ -246,6 +247,8 @@ def paged_attention_prepared(q: torch.Tensor, cache: PagedKvCache, layer: int,
         args += (prepared.prefill_seqs.data_ptr(), prepared.n_prefill)
     _run(lambda ptr, size: fn(*args, ptr, size, handle), cache, prepared, b, num_heads, max_q,
          max_k, q.device)
+    if _is_quantised(cache):
+        keep_for(stream, q, out)
     return out
 
 

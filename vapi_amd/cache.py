@@ -240,6 +240,20 @@ def check_on_device(*tensors) -> None:
                      "kernels run on the current GPU")
 
 
+def keep_for(stream, *tensors) -> None:
+    """Keeps the memory of tensors that a call on `stream` uses (None: the
+    current one) from reuse before it has run: they belong to the stream they
+    were made on."""
+    if stream is None:
+        return
+    handle = stream.cuda_stream
+    device = tensors[0].device
+    on = (torch.cuda.default_stream(device) if handle == 0 else
+          torch.cuda.ExternalStream(handle, device=device))
+    for t in tensors:
+        t.record_stream(on)
+
+
 def _is_quantised(cache) -> bool:
     """Whether `cache` is a QuantKvCache (its per-layer calls are the 8-bit ones)."""
     return getattr(cache, "q8", None) is not None
@@ -260,6 +274,7 @@ def _write_quantised(cache, layer: int, k: torch.Tensor, v: torch.Tensor, idx: t
     k, v, idx = k.contiguous(), v.contiguous(), idx.contiguous()
     check(lib().vapi_kv_q8_append(cache.q8, layer, k.data_ptr(), v.data_ptr(), idx.data_ptr(),
                                   k.shape[0], stream_handle(stream)))
+    keep_for(stream, k, v, idx)
 
 
 def _k_only(cache, which: str = "k"):
@@ -449,6 +464,7 @@ def gather_kv(cache: PagedKvCache, layer: int, block_table, len_k: int,
         check_on_device(cache.k[0], table)
         check(lib().vapi_kv_q8_gather(cache.q8, layer, table.data_ptr(), table.shape[0], len_k,
                                       kp, vp, stream_handle(stream)))
+        keep_for(stream, table, out)
         return out
     check(lib().vapi_kv_gather(cache.pool, layer, table.data_ptr(), table.shape[0],
                                len_k, kp, vp, stream_handle(stream)))

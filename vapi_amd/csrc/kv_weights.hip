@@ -232,7 +232,8 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_lse(WeightArgs a) {
   __shared__ uint32x4 stage[kWeightWaves][ST][16 * WeightTile<F, D>::kPieces];
   // (Chunk by chunk the sequences are turned by five: otherwise all chunks of a
   // long one land on the same CUs. 16 sequences of 256-8,192 keys 41.3 -> 37.3.)
-  const uint32_t seg = (blockIdx.x + 5 * a.kvh * blockIdx.y) % gridDim.x;
+  const uint32_t turn = (uint32_t)((uint64_t)(5 * a.kvh) * blockIdx.y % gridDim.x);
+  const uint32_t seg = (blockIdx.x + turn) % gridDim.x;
   const WeightSeg s = weight_seg(a, seg);
   if (!s.ok) return;
   // The last rows see the most keys: their workgroups start first.

@@ -18,7 +18,8 @@ import torch
 
 from ._lib import Weights, check, lib
 from .attention import PreparedAttention
-from .cache import HybridKvCache, _is_quantised, _per_layer, check_on_device, stream_handle
+from .cache import (HybridKvCache, _is_quantised, _per_layer, check_on_device, keep_for,
+                    stream_handle)
 
 
 def new_weights(rows: int, num_kv_heads: int, width: int, device="cuda") -> torch.Tensor:
@@ -82,6 +83,7 @@ def accumulate_attention_weights(q: torch.Tensor, cache, layer: int, prepared: P
     sequence count (0: all); with decay 0 that is the observation window at the
     end of a prompt, with decay 1 and single tokens the running sum of a
     generation. Returns weights."""
+    held = cache.k[0]
     cache, layer = _per_layer(cache, layer)
     if getattr(cache, "has_v", True) is False:
         raise ValueError("a rows layer has no attention")
@@ -94,7 +96,7 @@ def accumulate_attention_weights(q: torch.Tensor, cache, layer: int, prepared: P
     b = prepared.seqlens_q.shape[0] - 1
     index = _rows(rows, b, cache.device)
     state = _state(weights, cache, index, b, "weights")
-    on = (weights, q, prepared.block_table, prepared.seqlens_q)
+    on = (weights, held, q, prepared.block_table, prepared.seqlens_q)
     check_on_device(*(on if index is None else on + (index,)))
     q = q.contiguous()
     heads, max_q, max_k = q.shape[1], max(prepared.max_seqlen_q, 1), max(prepared.max_seqlen_k, 1)
@@ -102,7 +104,9 @@ def accumulate_attention_weights(q: torch.Tensor, cache, layer: int, prepared: P
         b, cache.num_kv_heads, heads, cache.head_dim, max_q, max_k, last_queries)
     ws = prepared.weights_workspace
     if need and (ws is None or ws.numel() < need):
-        # Kept for the step's other layers, as the attention's.
+        # Kept for the step's other layers, as the attention's; a smaller one stays
+        # too (a captured graph may hold it).
+        prepared.weights_workspaces.append(ws)
         ws = prepared.weights_workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     quantised = _is_quantised(cache)
     fn = lib().vapi_kv_q8_attention_weights if quantised else lib().vapi_kv_attention_weights
@@ -112,6 +116,8 @@ def accumulate_attention_weights(q: torch.Tensor, cache, layer: int, prepared: P
              heads, float(softmax_scale), -1 if window_size_left is None else int(window_size_left),
              -1 if window_size_right is None else int(window_size_right), int(last_queries),
              float(decay), state, ws.data_ptr() if need else None, need, stream_handle(stream)))
+    if stream is not None:
+        keep_for(stream, q, weights, *([] if index is None else [index]), *([ws] if need else []))
     return weights
 
 
@@ -196,6 +202,7 @@ def evict_kv(cache, layer: int, weights: torch.Tensor, plan: EvictionPlan,
     weights_out: a state whose rows plan.rows become the kept keys' weights,
     zeros after them; `weights` itself updates it in place. An 8-bit cache's
     kept codes get the scales of their new blocks."""
+    held = cache.k[0]
     if isinstance(cache, HybridKvCache):
         if cache.layouts[layer][0] != "kv":
             raise ValueError("a rows layer has no attention weights to evict by")
@@ -206,7 +213,7 @@ def evict_kv(cache, layer: int, weights: torch.Tensor, plan: EvictionPlan,
         raise ValueError(f"block {plan.top_block} of {cache.num_blocks}")
     b = len(plan.new_lens)
     src = _state(weights, cache, plan.rows, b, "weights")
-    on = [weights, plan.lens, plan.src_table]
+    on = [weights, held, plan.lens, plan.src_table]
     dst = None
     if weights_out is weights:
         dst = src
@@ -227,4 +234,7 @@ def evict_kv(cache, layer: int, weights: torch.Tensor, plan: EvictionPlan,
              plan.src_table.data_ptr(), plan.src_table.shape[1], plan.dst_table.data_ptr(),
              plan.dst_table.shape[1], b, plan.max_len, plan.budget, plan.sinks, plan.recent,
              kept.data_ptr(), stream_handle(stream)))
+    if stream is not None:
+        keep_for(stream, kept, weights, plan.lens, plan.src_table, plan.dst_table,
+                 *([] if plan.rows is None else [plan.rows]))
     return kept
