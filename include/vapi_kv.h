@@ -601,7 +601,8 @@ int vapi_kv_q8_gather(const vapi_kv_q8_pool* pool, uint32_t layer, const uint32_
  * max_seqlen_q > 1 covers every sequence, and that a call with prefill rows
  * needs the whole size that _workspace_size returns: their codes are
  * expanded there once, n_prefill * max_seqlen_k keys of the layer in the
- * pool's dtype. n_prefill is the list's length, or batch without a list.
+ * pool's dtype. n_prefill is the list's length, or batch where every sequence
+ * is covered: without a list, and with VAPI_ATTN_NO_DECODE_ROWS, which ignores it.
  * Groups of up to 256 query heads per kv head.
  */
 size_t vapi_kv_q8_attention_workspace_size(const vapi_kv_q8_pool* pool, uint32_t batch,
@@ -647,9 +648,11 @@ typedef struct vapi_kv_weights {
  * (max_seqlen_k past it is refused). The sums run in f32, in an order fixed
  * by the sizes: equal calls give equal bits.
  *
- * The pool's K alone is read: f16 or bf16, head_dim a multiple of 8 up to
- * 256, block_size a power of two from 16 (else VAPI_KV_EUNSUP), or an 8-bit
- * pool. q: 16-byte aligned. workspace: device scratch of
+ * The pool's K alone is read (a K-only pool, which attention does not take, is
+ * refused): f16 or bf16, head_dim a multiple of 8 up to 256, block_size a power
+ * of two from 16 (else VAPI_KV_EUNSUP), or an 8-bit pool. A NaN or an infinity
+ * in K or q reaches the weights of its own key, or of the keys its query sees,
+ * alone. q: 16-byte aligned. workspace: device scratch of
  * vapi_kv_attention_weights_workspace_size bytes, 16-byte aligned, nothing in
  * it kept between calls; calls sharing one must not overlap. No counterpart
  * in the reference.
@@ -695,7 +698,8 @@ int vapi_kv_q8_attention_weights(const vapi_kv_q8_pool* pool, uint32_t layer, co
  * other sequences may share) stay as they were. out may be the same rows as
  * in, or must not overlap it. A dst entry past the pool is not written, a src
  * entry past it reads its last block. Any pool dtype, with or without V.
- * No counterpart in the reference.
+ * At most 65,535 heads of sequences a call (batch x num_kv_heads, else
+ * VAPI_KV_EUNSUP). No counterpart in the reference.
  */
 int vapi_kv_evict(const vapi_kv_pool* pool, uint32_t layer, const vapi_kv_weights* in,
                   const vapi_kv_weights* out, const uint32_t* lens, const uint32_t* src_table,

@@ -176,6 +176,59 @@ def test_nan_behind_the_mask_counts_for_nothing():
     assert torch.equal(call(), want)
 
 
+@pytest.mark.parametrize("fmt,dtype", [("none", BF16), ("none", F16), ("e4m3", BF16)])
+@pytest.mark.parametrize("lens_q,heads,left,bad", [
+    (400, 3, 20, (212, 213, 300)), (400, 4, 50, (243, 399)), (4, 4, None, (1, 2)),
+    (5, 3, 7, (0, 4)), (1, 16, 30, (0,))])
+def test_a_nan_query_reaches_only_the_keys_it_sees(fmt, dtype, lens_q, heads, left, bad):
+    n = 400
+    cache, tables, _ = filled([n], 1, 64, 16, fmt, dtype, "HND", 8)
+    q = torch.randn(lens_q, heads, 64, generator=torch.Generator().manual_seed(9)).to(dtype).cuda()
+    prep = PreparedAttention.from_batch(batch_of([lens_q], [n], tables), "cuda")
+
+    def call():
+        return accumulate_attention_weights(q, cache, 0, prep, 0.1, new_weights(1, 1, n),
+                                            window_size_left=left)[0, 0].cpu()
+
+    want = call()
+    for j in bad:
+        q[j, 0] = float("nan")
+        got, pos = call(), n - lens_q + j
+        seen = torch.zeros(n, dtype=torch.bool)
+        seen[0 if left is None else max(pos - left, 0):pos + 1] = True
+        assert torch.equal(got[~seen], want[~seen])
+        q[j, 0] = 1.0
+        want = call()
+
+
+def test_a_query_made_contiguous_waits_for_the_call_s_stream_alone():
+    """A strided query or row is copied on the stream that the call is given."""
+    cache, tables, _ = filled([200], 2, 64, 16, "e4m3", BF16, "HND", 5)
+    prep = PreparedAttention.from_batch(batch_of([40], [200], tables), "cuda", cache, 4)
+    wide = torch.randn(40, 4, 128, device="cuda").to(BF16)
+    q, k = wide[:, :, ::2], wide[:, ::2, ::2]
+    idx = scatter_index(ref.slots_of(tables[0], 200, 16)[160:], "cuda")
+
+    def step(w, stream=None):
+        write_rows_indexed(cache, 0, k, k, idx, stream=stream)
+        out = paged_attention_prepared(q, cache, 0, prep, 0.1, stream=stream)
+        accumulate_attention_weights(q, cache, 0, prep, 0.1, w, stream=stream)
+        return out
+
+    w = new_weights(1, 2, 200)
+    step(new_weights(1, 2, 200))
+    want = new_weights(1, 2, 200)
+    first = step(want)
+    junk = [torch.full((40, 4, 64), float("nan"), device="cuda", dtype=BF16) for _ in range(8)]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    del junk
+    torch.cuda._sleep(20_000_000)  # the current stream is behind, and not waited for
+    out = step(w, side)
+    side.synchronize()
+    assert torch.equal(w, want) and torch.equal(out, first)
+
+
 def test_rows_past_the_state_are_left_out_and_strided_states():
     cache, tables, _ = filled([30, 40], 2, 64, 16, "none", F16, "HND", 5)
     prep = PreparedAttention.from_batch(batch_of([1, 1], [30, 40], tables), "cuda")

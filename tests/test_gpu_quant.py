@@ -442,3 +442,19 @@ def test_bad_tables_and_small_workspaces():
     assert torch.equal(out, want)
     with pytest.raises(VapiKvError):
         paged_attention_prepared(q, cache, 3, prep, 0.1)
+
+
+def test_prefill_rows_without_any_key_are_written():
+    """max_seqlen_k 0: zeros, as with a larger bound."""
+    cache, tables = filled([40], 2, 64, 16, "e4m3", BF16, "HND", 6)
+    q = torch.randn(3, 4, 64, device="cuda").to(BF16)
+    prep = PreparedAttention.from_batch(batch_of([3], [40], tables), "cuda")
+    out, none = torch.full_like(q, 5.0), torch.zeros_like(prep.seqlens_k)
+    need = lib().vapi_kv_q8_attention_workspace_size(cache.q8, 1, 1, 4, 3, 0)
+    ws = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    assert lib().vapi_kv_q8_attention(
+        cache.q8, 0, q.data_ptr(), out.data_ptr(), prep.seqlens_q.data_ptr(), none.data_ptr(),
+        prep.block_table.data_ptr(), 1, 3, 3, 0, 4, 0.1, -1, 0, 0, None, 0, ws.data_ptr(), need,
+        torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert not out.any()

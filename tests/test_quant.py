@@ -171,6 +171,21 @@ def test_bad_evictions_are_refused(pool):
     assert evict(pool, state(rows=40000), batch=40000) == EUNSUP
 
 
+def test_calls_past_a_grid_s_reach_are_refused():
+    wide = state(head_stride=1 << 25, row_stride=1 << 27, width=1 << 25)
+    most = 65535 * 192  # workgroups of 192 keys
+    for pool in (pool16(), q8_pool()):
+        assert weigh(pool, wide, max_k=most + 1) == EUNSUP
+        assert weigh(pool, wide, max_k=most, ws_bytes=64) == ESPACE
+        assert weigh(pool, state(index=BASE), batch=1 << 23) == EUNSUP
+    pool = q8_pool()
+    assert append(pool, n=1 << 28) == EUNSUP
+    assert attend(pool, max_q=2, max_k=1 << 28) == EUNSUP
+    # (A size for no keys is that for one.)
+    size = lib().vapi_kv_q8_attention_workspace_size
+    assert size(pool, 2, 2, 4, 8, 0) == size(pool, 2, 2, 4, 8, 1)
+
+
 # ---- the Python side --------------------------------------------------------------
 
 

@@ -15,8 +15,8 @@ import numpy as np
 import torch
 
 from ._lib import ESPACE, check, lib
-from .cache import (PagedKvCache, _is_quantised, _per_layer, check_on_device, keep_for,
-                    stream_handle, write_rows_indexed)
+from .cache import (PagedKvCache, _is_quantised, _per_layer, check_on_device, contiguous_on,
+                    keep_for, on_stream, stream_handle, write_rows_indexed)
 
 _u32p = ctypes.POINTER(ctypes.c_uint32)
 
@@ -178,7 +178,7 @@ def workspace_bytes(cache: PagedKvCache, batch: int, num_heads: int, max_q: int,
 
 
 def _workspace(cache, prepared: PreparedAttention, b: int, num_heads: int, max_q: int,
-               max_k: int, device):
+               max_k: int, device, stream=None):
     need = workspace_bytes(cache, b, num_heads, max_q, max_k, prepared.n_prefill_arg(cache))
     ws = prepared.workspace
     if need and (ws is None or ws.numel() < need):
@@ -186,13 +186,14 @@ def _workspace(cache, prepared: PreparedAttention, b: int, num_heads: int, max_q
         # per-XCD shares; later calls carry the shares over. (A step whose
         # layers differ in geometry sizes it up front with reserve(), so that
         # no layer allocates mid-step or inside a captured graph.)
-        ws = torch.zeros(need, dtype=torch.uint8, device=device)
+        with on_stream(stream, device):
+            ws = torch.zeros(need, dtype=torch.uint8, device=device)
         prepared.workspace = ws
     return need, ws
 
 
 def _run(call, cache, prepared: PreparedAttention, b: int, num_heads: int, max_q: int,
-         max_k: int, device) -> None:
+         max_k: int, device, stream=None) -> None:
     """call(workspace pointer, bytes) with the step's workspace, grown first
     if it is too small. A decode's workspace has no optional part, so the
     library, which refuses a small one before it launches anything, is asked
@@ -203,7 +204,7 @@ def _run(call, cache, prepared: PreparedAttention, b: int, num_heads: int, max_q
         if rc != ESPACE:
             check(rc)
             return
-    need, ws = _workspace(cache, prepared, b, num_heads, max_q, max_k, device)
+    need, ws = _workspace(cache, prepared, b, num_heads, max_q, max_k, device, stream)
     check(call(ws.data_ptr() if need else None, need))
 
 
@@ -221,7 +222,7 @@ def paged_attention_prepared(q: torch.Tensor, cache: PagedKvCache, layer: int,
         raise ValueError(f"q must be (tokens, heads, {cache.head_dim}), got {tuple(q.shape)}")
     if q.dtype != cache.dtype:
         raise ValueError(f"q is {q.dtype} but the cache is {cache.dtype}")
-    q = q.contiguous()
+    q = contiguous_on(stream, q)
     if out is None:
         out = torch.empty_like(q)
     b = prepared.seqlens_q.shape[0] - 1
@@ -246,7 +247,7 @@ def paged_attention_prepared(q: torch.Tensor, cache: PagedKvCache, layer: int,
         fn = lib().vapi_paged_attention_prepared
         args += (prepared.prefill_seqs.data_ptr(), prepared.n_prefill)
     _run(lambda ptr, size: fn(*args, ptr, size, handle), cache, prepared, b, num_heads, max_q,
-         max_k, q.device)
+         max_k, q.device, stream)
     if _is_quantised(cache):
         keep_for(stream, q, out)
     return out
@@ -296,7 +297,7 @@ def paged_attention_append_prepared(q: torch.Tensor, k: torch.Tensor, v: torch.T
                          f"got {tuple(k.shape)} and {tuple(v.shape)}")
     if slot_mapping.numel() != k.shape[0] or slot_mapping.element_size() != 4:
         raise ValueError("slot_mapping must hold one 32-bit slot per row")
-    q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    q, k, v = (contiguous_on(stream, t) for t in (q, k, v))
     if out is None:
         out = torch.empty_like(q)
     b = prepared.seqlens_q.shape[0] - 1
@@ -330,5 +331,5 @@ def paged_attention_append_prepared(q: torch.Tensor, k: torch.Tensor, v: torch.T
             -1 if window_size_right is None else int(window_size_right), prepared.flags)
     handle, fn = stream_handle(stream), lib().vapi_paged_attention_append_ex
     _run(lambda ptr, size: fn(*args, ptr, size, handle), cache, prepared, b, num_heads, max_q,
-         max_k, q.device)
+         max_k, q.device, stream)
     return out

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 from typing import Sequence
 
+import contextlib
 import ctypes
 
 import numpy as np
@@ -246,12 +247,32 @@ def keep_for(stream, *tensors) -> None:
     were made on."""
     if stream is None:
         return
-    handle = stream.cuda_stream
-    device = tensors[0].device
-    on = (torch.cuda.default_stream(device) if handle == 0 else
-          torch.cuda.ExternalStream(handle, device=device))
+    on = _torch_stream(stream, tensors[0].device)
     for t in tensors:
         t.record_stream(on)
+
+
+def _torch_stream(stream, device):
+    handle = stream.cuda_stream
+    return (torch.cuda.default_stream(device) if handle == 0 else
+            torch.cuda.ExternalStream(handle, device=device))
+
+
+def on_stream(stream, device):
+    """The context for what a call on `stream` (None: the current one) does
+    besides its kernels, copies and fills: in their order."""
+    return (contextlib.nullcontext() if stream is None else
+            torch.cuda.stream(_torch_stream(stream, device)))
+
+
+def contiguous_on(stream, t: torch.Tensor) -> torch.Tensor:
+    """t, or a contiguous copy of it made on `stream`."""
+    if t.is_contiguous():
+        return t
+    with on_stream(stream, t.device):
+        copy = t.contiguous()
+    keep_for(stream, t)
+    return copy
 
 
 def _is_quantised(cache) -> bool:
@@ -271,7 +292,7 @@ def _write_quantised(cache, layer: int, k: torch.Tensor, v: torch.Tensor, idx: t
     if k.dtype != cache.dtype or v.dtype != cache.dtype:
         raise ValueError(f"cache is {cache.dtype} but the rows are {k.dtype} and {v.dtype}")
     check_on_device(cache.k[0], k, v, idx)
-    k, v, idx = k.contiguous(), v.contiguous(), idx.contiguous()
+    k, v, idx = (contiguous_on(stream, t) for t in (k, v, idx))
     check(lib().vapi_kv_q8_append(cache.q8, layer, k.data_ptr(), v.data_ptr(), idx.data_ptr(),
                                   k.shape[0], stream_handle(stream)))
     keep_for(stream, k, v, idx)

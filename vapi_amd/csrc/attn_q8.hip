@@ -590,6 +590,7 @@ size_t vapi_kv_q8_attention_workspace_size(const vapi_kv_q8_pool* pool, uint32_t
   if (check_q8_pool(pool, 0, "vapi_kv_q8_attention_workspace_size") || batch == 0 ||
       num_heads == 0 || num_heads % pool->num_kv_heads)
     return 0;
+  max_seqlen_k = std::max(max_seqlen_k, 1u);
   size_t need = std::max(up256(q8_decode_ws(pool, batch, num_heads)), (size_t)256);
   n_prefill = std::min(n_prefill, batch);
   if (max_seqlen_q > 1 && n_prefill)
@@ -617,6 +618,7 @@ int vapi_kv_q8_attention(const vapi_kv_q8_pool* pool, uint32_t layer, const void
   if (flags & ~(uint32_t)(VAPI_ATTN_DETERMINISTIC | VAPI_ATTN_NO_DECODE_ROWS))
     VK_FAIL(VAPI_KV_EINVAL, "%s: unknown flags 0x%x", who, flags);
   if (batch == 0 || max_seqlen_q == 0) return 0;
+  max_seqlen_k = std::max(max_seqlen_k, 1u);  // rows without keys are written all the same
   if (!q || !out || !cu_seqlens_q || !cu_seqlens_k || !block_table)
     VK_FAIL(VAPI_KV_EINVAL, "%s: null device pointer", who);
   if (((uintptr_t)q | (uintptr_t)out) & 15)
@@ -635,7 +637,7 @@ int vapi_kv_q8_attention(const vapi_kv_q8_pool* pool, uint32_t layer, const void
   const uint32_t pf_n = !prefill ? 0 : listed ? n_prefill : batch;
   const uint64_t mb = ((uint64_t)max_seqlen_k + pool->block_size - 1) / pool->block_size;
   if (pf_n && (pf_n > 65535 || prefill_grid(pf_n, pool->num_kv_heads, G, max_seqlen_q, D) >
-                                   0xFFFFFFFFull || pf_n * mb > 0x7FFFFFFFull))
+                                   0xFFFFFFFFull || pf_n * mb > 0xFFFFFFull))
     VK_FAIL(VAPI_KV_EUNSUP, "%s: prefill batch too large for one launch", who);
   const size_t dec_ws = skip_decode ? 0 : q8_decode_ws(pool, batch, num_heads);
   const size_t off = std::max(up256(dec_ws), (size_t)256);
@@ -704,7 +706,7 @@ int vapi_kv_q8_attention(const vapi_kv_q8_pool* pool, uint32_t layer, const void
     else
       VK_Q8(launch_q8_decode, dec, sc, workspace, D, s);
   }
-  if (pf_n && mb) {
+  if (pf_n) {
     char* ws = (char*)workspace + off;
     VK_Q8(launch_q8_expand, a, sc, ws, w, (uint32_t)mb, g.kvh, s);
     AttnArgs f = a;  // the expanded pool: HND blocks of the same size, its own table

@@ -359,7 +359,8 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_lse(WeightArgs a) {
 // ---- pass 2 --------------------------------------------------------------------
 
 // lse of a row from its chunks' (m, l); +infinity (weights of 0) where it saw
-// no key. Eight loads at a time.
+// no key, or NaN (a test of the bits: the compiler takes NaN as absent). Eight
+// loads at a time.
 __device__ __forceinline__ float weight_join(const float2* ml, uint32_t n) {
   float mx = kNegBig, sum = 0.f;
   for (uint32_t c0 = 0; c0 < n; c0 += 8) {
@@ -374,7 +375,7 @@ __device__ __forceinline__ float weight_join(const float2* ml, uint32_t n) {
     for (int j = 0; j < 8; ++j) sum += x[j].y * fast_exp2(x[j].x - mn);
     mx = mn;
   }
-  return sum > 0.f ? mx + __builtin_amdgcn_logf(sum) : INFINITY;
+  return __float_as_uint(sum) - 1u < 0x7f7fffffu ? mx + __builtin_amdgcn_logf(sum) : INFINITY;
 }
 
 constexpr uint32_t kWeightJoinRows = 512;  // rows whose lse a workgroup joins in LDS
@@ -483,12 +484,13 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_sum(WeightArgs a) {
                                     lds[turn][row * PR + ((weight_d<F>(c, g) / 8) ^ (row & 7))]);
         }
         const uint32_t row = min(r + col, r1 - 1);
-        const float lse = r + col < r1 ? lse_lds[row - r0] : INFINITY;
-        // (Uniform: the first row's last key and the last row's first one.)
+        const float lse = lse_lds[row - r0];
+        // (Uniform: no row past the last, the first row's last key and the last
+        // row's first one. Rows past the last see nothing here, whatever they hold.)
         const int32_t p0 = s.pos0 + (int32_t)a.group.div(r);
         const int32_t p1 = s.pos0 + (int32_t)a.group.div(min(r + 15, r1 - 1));
         const bool whole =
-            key0 >= weight_lo(a, p1) && key0 + 16 * KT - 1 <= weight_hi(a, p0, s.len_k);
+            r + 16 <= r1 && key0 >= weight_lo(a, p1) && key0 + 16 * KT - 1 <= weight_hi(a, p0, s.len_k);
         floatx4 acc[KT];
 #pragma unroll
         for (int t = 0; t < KT; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -503,7 +505,8 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_sum(WeightArgs a) {
           for (int i = 0; i < 4; ++i) x[t][i] = __builtin_fmaf(acc[t][i], by[t], -lse);
         if (!whole) {
           const int32_t pos = s.pos0 + (int32_t)a.group.div(row);
-          const int32_t lo = weight_lo(a, pos), hi = weight_hi(a, pos, s.len_k);
+          const int32_t lo = weight_lo(a, pos);
+          const int32_t hi = r + col < r1 ? weight_hi(a, pos, s.len_k) : -1;
 #pragma unroll
           for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -696,10 +699,11 @@ static int weight_checks(const WeightCall& c, uint32_t kvh, uint32_t hd, uint32_
   if (num_blocks == 0) VK_FAIL(VAPI_KV_EINVAL, "%s: keys in an empty pool", who);
   if (c.max_blocks == 0) VK_FAIL(VAPI_KV_EINVAL, "%s: block table width 0", who);
   const uint64_t segs = (uint64_t)c.batch * kvh, n_q = c.last ? std::min(c.max_q, c.last) : c.max_q;
-  // (Grids: segments up to 2^31, the rest up to 65,535 each.)
-  if (segs > 0x7FFFFFFFu || n_q * (c.num_heads / kvh) > 0x3FFFFFFFu || c.max_k > 65535u * 256u)
-    VK_FAIL(VAPI_KV_EUNSUP, "%s: a batch of %u x %u kv heads with %u queries of %u heads", who,
-            c.batch, kvh, c.max_q, c.num_heads);
+  // (Grids: 2^32 threads in x, 65,535 workgroups of the fewest keys, pass 2's, in y.)
+  if (segs > 0xFFFFFFu || n_q * (c.num_heads / kvh) > 0x3FFFFFFFu ||
+      c.max_k > 65535u * 16 * kWeightKt * kWeightWaves)
+    VK_FAIL(VAPI_KV_EUNSUP, "%s: a batch of %u x %u kv heads with %u queries of %u heads, %u keys",
+            who, c.batch, kvh, c.max_q, c.num_heads, c.max_k);
   *plan = weight_plan(c.batch, kvh, c.num_heads / kvh, hd, c.max_q, c.max_k, c.last);
   if ((uint64_t)plan->row_tiles * plan->n_chunk > 65535 || plan->parts > 65535)
     VK_FAIL(VAPI_KV_EUNSUP, "%s: batch too large for one launch", who);
@@ -732,8 +736,9 @@ static WeightArgs weight_args(const WeightCall& c, const WeightPlan& p, uint32_t
   a.part = a.scores = (float*)((char*)c.ws + p.ml_bytes);
   a.scale_log2 = c.scale * kLog2e;
   a.decay = c.decay;
-  a.wl = c.wl < 0 ? -1 : c.wl;
-  a.wr = c.wr < 0 ? -1 : c.wr;
+  // (No position lies further than 2^30 from another: differences stay in 32 bits.)
+  a.wl = c.wl < 0 ? -1 : std::min(c.wl, 1 << 30);
+  a.wr = c.wr < 0 ? -1 : std::min(c.wr, 1 << 30);
   return a;
 }
 

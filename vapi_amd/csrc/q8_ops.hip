@@ -333,7 +333,7 @@ int vapi_kv_q8_append(const vapi_kv_q8_pool* pool, uint32_t layer, const void* k
     VK_FAIL(VAPI_KV_EINVAL, "vapi_kv_q8_append: null source or slot_mapping");
   if (((uintptr_t)k_src | (uintptr_t)v_src) & 15)
     VK_FAIL(VAPI_KV_EINVAL, "vapi_kv_q8_append: k_src and v_src must be 16-byte aligned");
-  if (n_tokens > 0x7FFFFFFFu)
+  if (n_tokens > 0xFFFFFFFu)  // 2^32 threads in a grid
     VK_FAIL(VAPI_KV_EUNSUP, "vapi_kv_q8_append: %u tokens in one call", n_tokens);
   const Q8Geom g = q8_geom(pool);
   const Q8Ptrs p = q8_ptrs(pool, layer);

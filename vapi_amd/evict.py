@@ -18,8 +18,8 @@ import torch
 
 from ._lib import Weights, check, lib
 from .attention import PreparedAttention
-from .cache import (HybridKvCache, _is_quantised, _per_layer, check_on_device, keep_for,
-                    stream_handle)
+from .cache import (HybridKvCache, _is_quantised, _per_layer, check_on_device, contiguous_on,
+                    keep_for, on_stream, stream_handle)
 
 
 def new_weights(rows: int, num_kv_heads: int, width: int, device="cuda") -> torch.Tensor:
@@ -98,7 +98,7 @@ def accumulate_attention_weights(q: torch.Tensor, cache, layer: int, prepared: P
     state = _state(weights, cache, index, b, "weights")
     on = (weights, held, q, prepared.block_table, prepared.seqlens_q)
     check_on_device(*(on if index is None else on + (index,)))
-    q = q.contiguous()
+    q = contiguous_on(stream, q)
     heads, max_q, max_k = q.shape[1], max(prepared.max_seqlen_q, 1), max(prepared.max_seqlen_k, 1)
     need = lib().vapi_kv_attention_weights_workspace_size(
         b, cache.num_kv_heads, heads, cache.head_dim, max_q, max_k, last_queries)
@@ -107,7 +107,9 @@ def accumulate_attention_weights(q: torch.Tensor, cache, layer: int, prepared: P
         # Kept for the step's other layers, as the attention's; a smaller one stays
         # too (a captured graph may hold it).
         prepared.weights_workspaces.append(ws)
-        ws = prepared.weights_workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        with on_stream(stream, q.device):
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        prepared.weights_workspace = ws
     quantised = _is_quantised(cache)
     fn = lib().vapi_kv_q8_attention_weights if quantised else lib().vapi_kv_attention_weights
     check(fn(cache.q8 if quantised else cache.pool, layer, q.data_ptr(),
@@ -236,5 +238,6 @@ def evict_kv(cache, layer: int, weights: torch.Tensor, plan: EvictionPlan,
              kept.data_ptr(), stream_handle(stream)))
     if stream is not None:
         keep_for(stream, kept, weights, plan.lens, plan.src_table, plan.dst_table,
-                 *([] if plan.rows is None else [plan.rows]))
+                 *([] if plan.rows is None else [plan.rows]),
+                 *([] if weights_out is None else [weights_out]))
     return kept
