@@ -51,7 +51,10 @@ EXTRA_FLAGS = {"attn_decode.hip": ["-fno-honor-nans", "-Rpass-analysis=kernel-re
                "attn_prefill_f32.hip": ["-fno-honor-nans",
                                         "-Rpass-analysis=kernel-resource-usage"],
                "attn_q8.hip": ["-fno-honor-nans", "-Rpass-analysis=kernel-resource-usage"],
-               "kv_weights.hip": ["-fno-honor-nans", "-Rpass-analysis=kernel-resource-usage"]}
+               # (-amdgpu-mfma-vgpr-form: products into the registers that the vector
+               # unit reads; through the others each score is copied once.)
+               "kv_weights.hip": ["-fno-honor-nans", "-mllvm", "-amdgpu-mfma-vgpr-form=1",
+                                  "-Rpass-analysis=kernel-resource-usage"]}
 
 # The prefill kernel's step barrier counts its own vector-memory operations
 # (the direct loads into LDS) with an explicit vmcnt wait, and the decode

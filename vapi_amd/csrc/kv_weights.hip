@@ -20,11 +20,12 @@
 // is a sum over them (weights_stored).
 //
 // What bounds it. Single tokens: HBM, K once (129 MB in 31 us, 4.2 TB/s, of 37 us
-// with pass 2). Many rows: VALU, an exponential and ~6 operations a score in each
-// pass beside 1/16 of an MFMA: three fresh prompts of 700-2,000 tokens (32 q / 8 kv
-// heads, f16; 30 GFLOP of scores) 56 + 69 + 5 us. Few rows over long contexts:
-// latency, ~4 us of dependent loads before a workgroup's first product in each
-// pass (a prompt's last 32 queries over 6,500 keys, 28 q / 4 kv heads: 16 + 13 us).
+// with pass 2). Many rows: issue, an exponential and ~5 operations a score in each
+// pass beside 1/16 of an MFMA, from two to three waves a SIMD: three fresh prompts
+// of 700-2,000 tokens (32 q / 8 kv heads, f16; 30 GFLOP of scores) 56 + 54 + 6 us.
+// Few rows over long contexts: latency, ~4 us of dependent loads before a workgroup's
+// first product in each pass (a prompt's last 32 queries over 6,500 keys, 28 q / 4
+// kv heads: 16 + 12 + 4 us).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -54,7 +55,9 @@ struct WeightArgs {
   uint32_t row_cap, n_chunk, chunk_keys, key_cap, part_rows;
   float* part;    // [part][segment][key_cap] sums of pass 2
   float* scores;  // [segment][row_cap][key_cap] (kept scores)
-  float scale_log2, decay;
+  float scale_log2;  // of the absolute scale; a negative one flips Q's signs
+  uint32_t q_sign;
+  float decay;
   int32_t wl, wr;
 };
 
@@ -103,18 +106,39 @@ __device__ __forceinline__ void weight_zero(uint4 (&x)[D / 32], uint32_t hd, uin
   }
 }
 
-// Q operand of 16 rows from `first` (rows past the segment's repeat its last).
-template <typename T, int F, int D>
-__device__ __forceinline__ void weight_q(uint4 (&q)[D / 32], const WeightArgs& a,
-                                         const WeightSeg& s, uint32_t row, uint32_t g) {
+// Rows of Q by their distance from `first`, a uniform row of the segment: row
+// (query j, head c of the group) lies row + j (heads - group) rows of Q further.
+struct WeightQ {
+  const char* base;
+  uint32_t first, j0, skip, row_b;
+};
+__device__ __forceinline__ WeightQ weight_q_from(const WeightArgs& a, const WeightSeg& s,
+                                                 uint32_t first) {
+  WeightQ w;
+  w.first = first, w.j0 = a.group.div(first);
+  w.skip = a.num_heads - a.group.d, w.row_b = 2 * a.hd;
+  w.base = a.q + ((uint64_t)(s.q0 + w.j0) * a.num_heads + s.h * a.group.d +
+                  (first - w.j0 * a.group.d)) * w.row_b;
+  return w;
+}
+// Bytes from the base (at most 64 rows on: the heads, up to 65,535, keep it in 32
+// bits), of the segment's last row for rows past it.
+__device__ __forceinline__ uint32_t weight_q_row(const WeightQ& w, const WeightArgs& a,
+                                                 const WeightSeg& s, uint32_t row) {
   row = min(row, s.n_rows - 1);
-  const uint32_t j = a.group.div(row), c = row - j * a.group.d;
-  const T* p = (const T*)a.q +
-               ((uint64_t)(s.q0 + j) * a.num_heads + s.h * a.group.d + c) * a.hd;
+  return (row - w.first + (a.group.div(row) - w.j0) * w.skip) * w.row_b;
+}
+
+// Q operand of a row (rows past the segment's repeat its last).
+template <int F, int D>
+__device__ __forceinline__ void weight_q(uint4 (&q)[D / 32], const WeightQ& w, const WeightArgs& a,
+                                         const WeightSeg& s, uint32_t row, uint32_t g) {
+  const uint32_t at = weight_q_row(w, a, s, row);
 #pragma unroll
   for (int c2 = 0; c2 < D / 32; ++c2) {
-    const uint32_t d = weight_d<F>(c2, g);
-    q[c2] = *(const uint4*)(p + min(d, a.hd - 8));
+    const uint4 x =
+        *(const uint4*)(w.base + (at + min(2 * weight_d<F>(c2, g), w.row_b - 16)));
+    q[c2] = make_uint4(x.x ^ a.q_sign, x.y ^ a.q_sign, x.z ^ a.q_sign, x.w ^ a.q_sign);
   }
   weight_zero<F, D>(q, a.hd, g);
 }
@@ -141,16 +165,22 @@ struct WeightTile {
 // zeros of Q). Every load is unconditional: one under a branch makes the
 // compiler wait for all loads in flight.
 // kNt: streaming loads, where no other workgroup reads the tile.
+__device__ __forceinline__ int32_t weight_tile(const WeightSeg& s, int32_t key) {
+  return __builtin_amdgcn_readfirstlane(min(key, (s.len_k - 1) & ~15));
+}
+__device__ __forceinline__ uint32_t weight_block(const WeightArgs& a, const WeightSeg& s,
+                                                 int32_t key) {
+  using ConstU32 = const __attribute__((address_space(4))) uint32_t;
+  ConstU32* tab = (ConstU32*)(a.table + (uint64_t)s.seq * a.max_blocks);
+  return min(tab[min((uint32_t)weight_tile(s, key) >> a.bs_shift, a.max_blocks - 1)], a.last_blk);
+}
 template <int F, int D, bool kNt>
 __device__ __forceinline__ void weight_load(WeightTile<F, D>& t, const WeightArgs& a,
-                                            const WeightSeg& s, int32_t key, uint32_t lane) {
-  using ConstU32 = const __attribute__((address_space(4))) uint32_t;
+                                            const WeightSeg& s, int32_t key, uint32_t blk,
+                                            uint32_t lane) {
   using ConstF32 = const __attribute__((address_space(4))) float;
   using Tile = WeightTile<F, D>;
-  const int32_t last = s.len_k - 1;
-  const int32_t ts = __builtin_amdgcn_readfirstlane(min(key, last & ~15));
-  ConstU32* tab = (ConstU32*)(a.table + (uint64_t)s.seq * a.max_blocks);
-  const uint32_t blk = min(tab[min((uint32_t)ts >> a.bs_shift, a.max_blocks - 1)], a.last_blk);
+  const int32_t last = s.len_k - 1, ts = weight_tile(s, key);
   const uint32_t off = (uint32_t)ts & ((1u << a.bs_shift) - 1);
   const char* p = a.k + blk * a.blk_b + s.h * a.head_b + (uint64_t)off * a.tok_b;
   t.scale = 1.f;
@@ -170,6 +200,12 @@ __device__ __forceinline__ void weight_stage(uint32x4* lds, const WeightTile<F, 
 #pragma unroll
   for (int i = 0; i < Tile::N; ++i)
     lds[Tile::place((64 * i + lane) / Tile::kPieces, lane % Tile::kPieces)] = t.w[i];
+}
+// Log2 units per unit of a tile's products. Positive even where a block's scale is
+// 0 (its codes are): a masked score, -infinity, stays one.
+template <int F, int D>
+__device__ __forceinline__ float weight_unit(const WeightTile<F, D>& t, const WeightArgs& a) {
+  return F == kK16 ? a.scale_log2 : fmaxf(t.scale * a.scale_log2, 1e-37f);
 }
 // The staged tile as MFMA operands (codes unscaled). A 16-bit pool's pieces past
 // head_dim are zeroed: they may repeat an infinity (codes are finite).
@@ -203,7 +239,7 @@ __device__ __forceinline__ int32_t weight_lo(const WeightArgs& a, int32_t pos) {
   return a.wl >= 0 ? max(0, pos - a.wl) : 0;
 }
 __device__ __forceinline__ int32_t weight_hi(const WeightArgs& a, int32_t pos, int32_t len_k) {
-  return a.wr >= 0 ? (int32_t)min((int64_t)len_k - 1, (int64_t)pos + a.wr) : len_k - 1;
+  return a.wr >= 0 ? min(len_k - 1, pos + a.wr) : len_k - 1;
 }
 
 constexpr int kWeightWaves = 4;
@@ -245,10 +281,11 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_lse(WeightArgs a) {
   uint4 q[MT][D / 32];
   int32_t lo[MT], hi[MT];
   float m[MT], l[MT];
+  const WeightQ rows = weight_q_from(a, s, row0);
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     const uint32_t row = row0 + 16 * t + col;
-    weight_q<T, F, D>(q[t], a, s, row, g);
+    weight_q<F, D>(q[t], rows, a, s, row, g);
     const int32_t pos = s.pos0 + (int32_t)a.group.div(min(row, s.n_rows - 1));
     lo[t] = weight_lo(a, pos), hi[t] = weight_hi(a, pos, s.len_k);
     m[t] = kNegBig, l[t] = 0.f;
@@ -269,37 +306,41 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_lse(WeightArgs a) {
   // of registers doubles the code, which short walks fetch once.)
   WeightTile<F, D> buf[ST];
   int32_t key = k0 + 16 * ST * wave;
+  uint32_t blk[ST];  // the next step's table entries: their loads come before the tiles'
 #pragma unroll
-  for (int tt = 0; tt < ST; ++tt) weight_load<F, D, kStore>(buf[tt], a, s, key + 16 * tt, lane);
+  for (int tt = 0; tt < ST; ++tt) {
+    weight_load<F, D, kStore>(buf[tt], a, s, key + 16 * tt, weight_block(a, s, key + 16 * tt), lane);
+    blk[tt] = weight_block(a, s, key + 16 * (ST * kWeightWaves + tt));
+  }
   while (key <= k1) {
     float by[ST];
 #pragma unroll
     for (int tt = 0; tt < ST; ++tt) {
       weight_stage<F, D>(stage[wave][tt], buf[tt], lane);
-      by[tt] = buf[tt].scale * a.scale_log2;
+      by[tt] = weight_unit(buf[tt], a);
     }
     weight_fence();
 #pragma unroll
-    for (int tt = 0; tt < ST; ++tt)
-      weight_load<F, D, kStore>(buf[tt], a, s, key + 16 * (ST * kWeightWaves + tt), lane);
+    for (int tt = 0; tt < ST; ++tt) {
+      weight_load<F, D, kStore>(buf[tt], a, s, key + 16 * (ST * kWeightWaves + tt), blk[tt], lane);
+      blk[tt] = weight_block(a, s, key + 16 * (2 * ST * kWeightWaves + tt));
+    }
     const bool whole = key >= all_lo && key + 16 * ST - 1 <= all_hi;
-    float x[ST][MT][4], mx[MT];
+    floatx4 x[ST][MT];  // products; times by[tt] the scores
+    float mx[MT];
     bool grow = false;
 #pragma unroll
     for (int tt = 0; tt < ST; ++tt) {
       uint4 k[D / 32];
       weight_operand<T, F, D>(stage[wave][tt], k, a.hd, col, g);
-      floatx4 acc[MT];
 #pragma unroll
-      for (int t = 0; t < MT; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < MT; ++t) x[tt][t] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < D / 32; ++c)
 #pragma unroll
-        for (int t = 0; t < MT; ++t) acc[t] = mfma16x16x32<T>(k[c], q[t][c], acc[t]);
+        for (int t = 0; t < MT; ++t) x[tt][t] = mfma16x16x32<T>(k[c], q[t][c], x[tt][t]);
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[tt][t][i] = acc[t][i] * by[tt];
         if (!whole) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -307,13 +348,14 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_lse(WeightArgs a) {
             if (!(at >= lo[t] && at <= hi[t])) x[tt][t][i] = -INFINITY;
           }
         }
-        const float top = max_nc(max_nc(x[tt][t][0], x[tt][t][1]), max_nc(x[tt][t][2], x[tt][t][3]));
+        const float top =
+            by[tt] * max_nc(max3_nc(x[tt][t][0], x[tt][t][1], x[tt][t][2]), x[tt][t][3]);
         mx[t] = tt == 0 ? top : max_nc(mx[t], top);
       }
       if constexpr (kStore) {
         const int32_t at = key + 16 * tt + 4 * (int32_t)g;
         const uint32_t to = at <= k1 ? (col * a.key_cap + (uint32_t)at) * 4 : 0xFFFFFFF0u;
-        const floatx4 v = {x[tt][0][0], x[tt][0][1], x[tt][0][2], x[tt][0][3]};
+        const floatx4 v = x[tt][0] * by[tt];
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint32x4, v), store, (int)to, 0,
                                                0);
       }
@@ -331,9 +373,12 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_lse(WeightArgs a) {
 #pragma unroll
     for (int tt = 0; tt < ST; ++tt)
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
-        l[t] += (fast_exp2(x[tt][t][0] - m[t]) + fast_exp2(x[tt][t][1] - m[t])) +
-                (fast_exp2(x[tt][t][2] - m[t]) + fast_exp2(x[tt][t][3] - m[t]));
+      for (int t = 0; t < MT; ++t) {
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = fast_exp2(__builtin_fmaf(x[tt][t][i], by[tt], -m[t]));
+        l[t] += (p[0] + p[1]) + (p[2] + p[3]);
+      }
     weight_fence();
     key += 16 * ST * kWeightWaves;
   }
@@ -380,8 +425,8 @@ __device__ __forceinline__ float weight_join(const float2* ml, uint32_t n) {
 
 constexpr uint32_t kWeightJoinRows = 512;  // rows whose lse a workgroup joins in LDS
 // 16-key tiles a wave of pass 2 holds. More of them read Q less often, fewer leave
-// registers for more waves: three fresh prompts (below) 73.2 / 69.2 / 84.6 us at 2 /
-// 3 / 4, a prompt's last 32 queries 15.5 / 13.5 / 18.6.
+// registers for more waves: three fresh prompts (above) 55.8 / 53.5 / 66.9 us at 2 /
+// 3 / 4, a prompt's last 32 queries 13.8 / 12.0 / 16.2.
 constexpr int kWeightKt = 3;
 constexpr uint32_t kWeightBlock = 64;       // rows whose Q a workgroup of pass 2 stages
 
@@ -396,6 +441,19 @@ __device__ __forceinline__ void weight_lse_rows(float* lds, const WeightArgs& a,
 
 __device__ __forceinline__ void weight_write(const WeightArgs& a, float* w, float x) {
   *w = a.decay == 0.f ? x : *w * a.decay + x;
+}
+
+// The sum over each 16 lanes, in all of them.
+__device__ __forceinline__ float row_sum(float x) {
+#define VK_ROTATE(N)                                                                       \
+  x += __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), \
+                                                             0x120 + N, 0xF, 0xF, true))
+  VK_ROTATE(8);
+  VK_ROTATE(4);
+  VK_ROTATE(2);
+  VK_ROTATE(1);
+#undef VK_ROTATE
+  return x;
 }
 
 // Grid: (segments, key tiles of 16 KT x 4 waves, parts of the rows). With more
@@ -424,6 +482,11 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_sum(WeightArgs a) {
     const int64_t j = (int64_t)wg1 + a.wl - s.pos0 + 1;
     r1 = (uint32_t)max((int64_t)0, min((int64_t)r1, j * a.group.d));
   }
+  float* part = a.part + ((uint64_t)blockIdx.z * gridDim.x + blockIdx.x) * a.key_cap;
+  if (r0 >= r1 && gridDim.z > 1) {  // nothing sees them (of a causal prompt, half)
+    if (wg0 + (int32_t)threadIdx.x <= wg1) part[wg0 + threadIdx.x] = 0.f;
+    return;
+  }
   r1 = max(r0, r1);
   const uint32_t lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int32_t wave = (int32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -434,7 +497,8 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_sum(WeightArgs a) {
     uint32x4* const place = &lds[0][0] + wave * 16 * WeightTile<F, D>::kPieces;
     WeightTile<F, D> raw[KT];
 #pragma unroll
-    for (int t = 0; t < KT; ++t) weight_load<F, D, false>(raw[t], a, s, key0 + 16 * t, lane);
+    for (int t = 0; t < KT; ++t)
+      weight_load<F, D, false>(raw[t], a, s, key0 + 16 * t, weight_block(a, s, key0 + 16 * t), lane);
     weight_lse_rows(lse_lds, a, blockIdx.x, r0, r1);
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
@@ -442,55 +506,62 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_sum(WeightArgs a) {
       weight_fence();
       weight_operand<T, F, D>(place, k[t], a.hd, col, g);
       weight_fence();
-      by[t] = raw[t].scale * a.scale_log2;
+      by[t] = __uint_as_float(__float_as_uint(weight_unit(raw[t], a)) ^ (a.q_sign << 16));
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[t][i] = 0.f;
     }
     __syncthreads();
   }
+  uint32_t q_at[D / 32];  // this lane's pieces among a tile of 16 rows
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) q_at[c] = col * PR + ((weight_d<F>(c, g) / 8) ^ (col & 7));
   // A block's Q pieces in registers: loaded a block ahead, then put in LDS.
   uint32x4 held[N];
+  const uint32_t in_row = min(16 * (threadIdx.x % PR), 2 * a.hd - 16);
   auto fetch = [&](uint32_t first) __attribute__((always_inline)) {
+    const WeightQ rows = weight_q_from(a, s, first);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const uint32_t at = 64 * kWeightWaves * i + threadIdx.x;
-      const uint32_t row = min(first + at / PR, s.n_rows - 1), piece = at % PR;
-      const uint32_t j = a.group.div(row), c = row - j * a.group.d;
-      const char* q = a.q + (((uint64_t)(s.q0 + j) * a.num_heads + s.h * a.group.d + c) * a.hd) * 2;
-      held[i] = *(const uint32x4*)(q + min(16 * piece, 2 * a.hd - 16));
+      const uint32_t row = first + (64 * kWeightWaves * i + threadIdx.x) / PR;
+      held[i] = *(const uint32x4*)(rows.base + (weight_q_row(rows, a, s, row) + in_row));
     }
   };
+  // Of this wave's keys: rows [some0, some1) see any, [all0, all1) all of them
+  // (pos >= key - wr, pos <= key + wl). Worked out here once: per tile of rows they
+  // were most of the loop's scalar instructions.
+  auto row_at = [&](int64_t pos) {
+    return (uint32_t)min(max((pos - s.pos0) * a.group.d, (int64_t)r0), (int64_t)r1);
+  };
+  const int32_t key1 = key0 + 16 * KT - 1;
+  const bool held_all = key1 < s.len_k;  // (else never whole)
+  const uint32_t some0 = a.wr >= 0 ? row_at((int64_t)key0 - a.wr) & ~15u : r0;
+  const uint32_t some1 = key0 >= s.len_k ? r0 : a.wl >= 0 ? row_at((int64_t)key1 + a.wl + 1) : r1;
+  const uint32_t all0 = a.wr >= 0 ? row_at((int64_t)key1 - a.wr) : r0;
+  const uint32_t all1 = !held_all ? r0 : a.wl >= 0 ? row_at((int64_t)key0 + a.wl + 1) : r1;
   uint32_t turn = 0;
   if (r0 < r1) fetch(r0);
   for (uint32_t first = r0; first < r1; first += kWeightBlock, turn ^= 1) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const uint32_t at = 64 * kWeightWaves * i + threadIdx.x, row = at / PR, piece = at % PR;
-      lds[turn][row * PR + (piece ^ (row & 7))] = held[i] & (8 * piece < a.hd ? 0xFFFFFFFFu : 0u);
+      if (a.hd < D) held[i] &= 8 * piece < a.hd ? 0xFFFFFFFFu : 0u;
+      lds[turn][row * PR + (piece ^ (row & 7))] = held[i];
     }
     if (first + kWeightBlock < r1) fetch(first + kWeightBlock);
     // (One barrier a block: a wave that writes a buffer again has passed the
     // barrier that every wave reaches after reading it.)
     lds_barrier();
-    if (key0 < s.len_k) {
-      const uint32_t end = min(first + kWeightBlock, r1);
+    {
+      const uint32_t end = min(first + kWeightBlock, some1);
 #pragma unroll 1
-      for (uint32_t r = first; r < end; r += 16) {
+      for (uint32_t r = max(first, some0); r < end; r += 16) {
+        // (Rows past r1 see nothing here, whatever they hold.)
+        const bool whole = r >= all0 && r + 16 <= all1;
         uint4 q[D / 32];
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          const uint32_t row = r - first + col;
-          q[c] = __builtin_bit_cast(uint4,
-                                    lds[turn][row * PR + ((weight_d<F>(c, g) / 8) ^ (row & 7))]);
-        }
-        const uint32_t row = min(r + col, r1 - 1);
-        const float lse = lse_lds[row - r0];
-        // (Uniform: no row past the last, the first row's last key and the last
-        // row's first one. Rows past the last see nothing here, whatever they hold.)
-        const int32_t p0 = s.pos0 + (int32_t)a.group.div(r);
-        const int32_t p1 = s.pos0 + (int32_t)a.group.div(min(r + 15, r1 - 1));
-        const bool whole =
-            r + 16 <= r1 && key0 >= weight_lo(a, p1) && key0 + 16 * KT - 1 <= weight_hi(a, p0, s.len_k);
+        for (int c = 0; c < D / 32; ++c)
+          q[c] = __builtin_bit_cast(uint4, lds[turn][(r - first) * PR + q_at[c]]);
+        const float lse = lse_lds[r - r0 + col];  // (a part is whole tiles)
         floatx4 acc[KT];
 #pragma unroll
         for (int t = 0; t < KT; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -504,7 +575,7 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_sum(WeightArgs a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[t][i] = __builtin_fmaf(acc[t][i], by[t], -lse);
         if (!whole) {
-          const int32_t pos = s.pos0 + (int32_t)a.group.div(row);
+          const int32_t pos = s.pos0 + (int32_t)a.group.div(r + col);
           const int32_t lo = weight_lo(a, pos);
           const int32_t hi = r + col < r1 ? weight_hi(a, pos, s.len_k) : -1;
 #pragma unroll
@@ -524,15 +595,11 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_sum(WeightArgs a) {
   }
   // Over the 16 rows of a lane group; lane col then writes key 4 g + col.
   float* w = a.w + s.state_row * a.row_stride + s.h * a.head_stride;
-  float* part = a.part + ((uint64_t)blockIdx.z * gridDim.x + blockIdx.x) * a.key_cap;
 #pragma unroll
   for (int t = 0; t < KT; ++t) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float x = sum[t][i];
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) x += __shfl_xor(x, o);
-      sum[t][i] = x;
+      sum[t][i] = row_sum(sum[t][i]);
     }
     const float x = col == 0 ? sum[t][0] : col == 1 ? sum[t][1] : col == 2 ? sum[t][2] : sum[t][3];
     const int32_t at = key0 + 16 * t + 4 * (int32_t)g + (int32_t)col;
@@ -700,7 +767,7 @@ static int weight_checks(const WeightCall& c, uint32_t kvh, uint32_t hd, uint32_
   if (c.max_blocks == 0) VK_FAIL(VAPI_KV_EINVAL, "%s: block table width 0", who);
   const uint64_t segs = (uint64_t)c.batch * kvh, n_q = c.last ? std::min(c.max_q, c.last) : c.max_q;
   // (Grids: 2^32 threads in x, 65,535 workgroups of the fewest keys, pass 2's, in y.)
-  if (segs > 0xFFFFFFu || n_q * (c.num_heads / kvh) > 0x3FFFFFFFu ||
+  if (segs > 0xFFFFFFu || c.num_heads > 65535 || n_q * (c.num_heads / kvh) > 0x3FFFFFFFu ||
       c.max_k > 65535u * 16 * kWeightKt * kWeightWaves)
     VK_FAIL(VAPI_KV_EUNSUP, "%s: a batch of %u x %u kv heads with %u queries of %u heads, %u keys",
             who, c.batch, kvh, c.max_q, c.num_heads, c.max_k);
@@ -734,7 +801,8 @@ static WeightArgs weight_args(const WeightCall& c, const WeightPlan& p, uint32_t
   a.row_cap = p.row_cap, a.n_chunk = p.n_chunk, a.chunk_keys = p.chunk_keys;
   a.key_cap = p.key_cap, a.part_rows = p.part_rows;
   a.part = a.scores = (float*)((char*)c.ws + p.ml_bytes);
-  a.scale_log2 = c.scale * kLog2e;
+  a.scale_log2 = fmaxf(fabsf(c.scale) * kLog2e, 1e-30f);
+  a.q_sign = c.scale < 0.f ? 0x80008000u : 0u;
   a.decay = c.decay;
   // (No position lies further than 2^30 from another: differences stay in 32 bits.)
   a.wl = c.wl < 0 ? -1 : std::min(c.wl, 1 << 30);
