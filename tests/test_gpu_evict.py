@@ -136,6 +136,17 @@ def test_weights_of_long_prompts(fmt, dtype):
     check_weights([1], [20000], 4, 1, 64, 16, fmt, dtype, "HND")
 
 
+@pytest.mark.parametrize("fmt,dtype,heads,kvh,d", [
+    ("none", BF16, 4, 1, 128), ("int8", F16, 3, 1, 64), ("e4m3", BF16, 12, 4, 256)])
+@pytest.mark.parametrize("left,right", [
+    (0, 0), (50, 0), (333, 0), (50, 5), (None, 100), (20, None), (0, None), (1 << 30, 1 << 30),
+    (2 ** 31 - 1, 2 ** 31 - 1)])
+def test_weights_of_long_prompts_in_windows(fmt, dtype, heads, kvh, d, left, right):
+    """Workgroups and waves whose keys no row, some rows or all rows see."""
+    check_weights([700, 1, 90, 333], [900, 600, 1000, 333], heads, kvh, d, 16, fmt, dtype, "HND",
+                  left, right, seed=2)
+
+
 def test_weights_with_odd_scales_and_wide_batches():
     check_weights([1, 20], [50, 60], 4, 2, 64, 16, "none", BF16, "HND", scale=-0.2)
     check_weights([1, 20], [50, 60], 4, 2, 64, 16, "int8", F16, "HND", scale=0.0)

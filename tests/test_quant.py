@@ -178,6 +178,7 @@ def test_calls_past_a_grid_s_reach_are_refused():
         assert weigh(pool, wide, max_k=most + 1) == EUNSUP
         assert weigh(pool, wide, max_k=most, ws_bytes=64) == ESPACE
         assert weigh(pool, state(index=BASE), batch=1 << 23) == EUNSUP
+        assert weigh(pool, state(), heads=65538) == EUNSUP
     pool = q8_pool()
     assert append(pool, n=1 << 28) == EUNSUP
     assert attend(pool, max_q=2, max_k=1 << 28) == EUNSUP
