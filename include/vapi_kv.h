@@ -651,12 +651,11 @@ typedef struct vapi_kv_weights {
  * The pool's K alone is read (a K-only pool, which attention does not take, is
  * refused): f16 or bf16, head_dim a multiple of 8 up to 256, block_size a power
  * of two from 16, up to 65,535 query heads (else VAPI_KV_EUNSUP), or an 8-bit
- * pool. A NaN or an infinity
- * in K or q reaches the weights of its own key, or of the keys its query sees,
- * alone. q: 16-byte aligned. workspace: device scratch of
- * vapi_kv_attention_weights_workspace_size bytes, 16-byte aligned, nothing in
- * it kept between calls; calls sharing one must not overlap. No counterpart
- * in the reference.
+ * pool. A NaN or an infinity in K or q reaches the weights of its own key, or
+ * of the keys its query sees, alone. q: 16-byte aligned. workspace: device
+ * scratch of vapi_kv_attention_weights_workspace_size bytes, 16-byte aligned,
+ * nothing in it kept between calls; calls sharing one must not overlap. No
+ * counterpart in the reference.
  */
 size_t vapi_kv_attention_weights_workspace_size(uint32_t batch, uint32_t num_kv_heads,
                                                 uint32_t num_heads, uint32_t head_dim,
