@@ -243,6 +243,7 @@ __device__ __forceinline__ int32_t weight_hi(const WeightArgs& a, int32_t pos, i
 }
 
 constexpr int kWeightWaves = 4;
+constexpr uint32_t kWeightChunk = 256;  // pass 1's chunks of keys are multiples of this
 
 // Tiles a wave of pass 1 loads at a time: 4 KiB of K where few rows use them
 // (with four workgroups a CU the next step's 4 KiB of 16 waves are in flight; 8
@@ -296,7 +297,12 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_lse(WeightArgs a) {
   const int32_t all_lo = weight_lo(a, p1), all_hi = weight_hi(a, p0, s.len_k);
   const int32_t c0 = (int32_t)(chunk * a.chunk_keys);
   const int32_t c1 = (int32_t)min((int64_t)c0 + a.chunk_keys, (int64_t)s.len_k) - 1;
-  const int32_t k0 = max(c0, weight_lo(a, p0) & ~15), k1 = min(c1, weight_hi(a, p1, s.len_k));
+  // (From a whole step of the chunk's, which is a multiple of every step: the walk
+  // then ends at the chunk's end. From any other tile its last step would take keys
+  // of the next chunk, which counts them too.)
+  static_assert(kWeightChunk % (16 * ST) == 0, "chunks are whole steps");
+  const int32_t k0 = max(c0, weight_lo(a, p0) & ~(16 * ST - 1));
+  const int32_t k1 = min(c1, weight_hi(a, p1, s.len_k));
   // Stores past the buffer (rows and keys that are not there) are dropped.
   const uint32_t kept = kStore ? s.n_rows * a.key_cap * (uint32_t)sizeof(float) : 0;
   const auto store = __builtin_amdgcn_make_buffer_rsrc(
@@ -632,7 +638,7 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_stored(WeightArgs a
   weight_lse_rows(lse, a, blockIdx.x, 0, s.n_rows);
   if (at >= s.len_k) return;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  // (Pass 1 visits the keys that some row sees, from a 16-key tile's first.)
+  // (Pass 1 visits every key from the 16-key tile of the first that some row sees.)
   const int32_t last = s.pos0 + (int32_t)a.group.div(s.n_rows - 1);
   const bool seen = at >= (weight_lo(a, s.pos0) & ~15) && at <= weight_hi(a, last, s.len_k);
   for (uint32_t r = 0; seen && r < s.n_rows; ++r) {
@@ -676,8 +682,8 @@ static WeightPlan weight_plan(uint32_t batch, uint32_t kvh, uint32_t group, uint
   p.store = rows <= 16 && segs * rows * p.key_cap * sizeof(float) <= kStoreBytes;
   auto up = [](uint64_t x, uint64_t y) { return (x + y - 1) / y; };
   const uint64_t want = std::max<uint64_t>(up(kWeightWgs, p.row_tiles * segs), 1);
-  uint64_t keys = std::max<uint64_t>(up(max_k, want), 256);
-  p.chunk_keys = (uint32_t)(up(keys, 256) * 256);
+  const uint64_t keys = std::max<uint64_t>(up(max_k, want), 1);
+  p.chunk_keys = (uint32_t)(up(keys, kWeightChunk) * kWeightChunk);
   p.n_chunk = (uint32_t)std::max<uint64_t>(up(max_k, p.chunk_keys), 1);
   const uint64_t blocks = up(max_k, 16 * kWeightKt * kWeightWaves);
   // (A part's rows are joined in LDS, so there are at least enough parts.)
