@@ -16,7 +16,7 @@ import torch
 
 from ._lib import ESPACE, check, lib
 from .cache import (PagedKvCache, _is_quantised, _per_layer, check_on_device, contiguous_on,
-                    keep_for, on_stream, stream_handle, write_rows_indexed)
+                    empty_on, keep_for, on_stream, stream_handle, write_rows_indexed)
 
 _u32p = ctypes.POINTER(ctypes.c_uint32)
 
@@ -224,7 +224,7 @@ def paged_attention_prepared(q: torch.Tensor, cache: PagedKvCache, layer: int,
         raise ValueError(f"q is {q.dtype} but the cache is {cache.dtype}")
     q = contiguous_on(stream, q)
     if out is None:
-        out = torch.empty_like(q)
+        out = empty_on(stream, q)
     b = prepared.seqlens_q.shape[0] - 1
     num_heads = q.shape[1]
     max_q = max(int(prepared.max_seqlen_q), 1)
@@ -299,7 +299,7 @@ def paged_attention_append_prepared(q: torch.Tensor, k: torch.Tensor, v: torch.T
         raise ValueError("slot_mapping must hold one 32-bit slot per row")
     q, k, v = (contiguous_on(stream, t) for t in (q, k, v))
     if out is None:
-        out = torch.empty_like(q)
+        out = empty_on(stream, q)
     b = prepared.seqlens_q.shape[0] - 1
     num_heads = q.shape[1]
     max_q = max(int(prepared.max_seqlen_q), 1)

@@ -265,6 +265,19 @@ def on_stream(stream, device):
             torch.cuda.stream(_torch_stream(stream, device)))
 
 
+def empty_on(stream, like: torch.Tensor, shape=None, dtype=None) -> torch.Tensor:
+    """An output of a call on `stream` (None: the current one), like a tensor or
+    of a shape and dtype of its own: memory of that stream, since the current
+    one's may still be written by work queued there before it was freed."""
+    if stream is None or stream.cuda_stream == stream_handle():
+        return (torch.empty_like(like) if shape is None else
+                torch.empty(shape, dtype=dtype, device=like.device))
+    with on_stream(stream, like.device):
+        out = empty_on(None, like, shape, dtype)  # (`stream` is the current one here)
+    out.record_stream(torch.cuda.current_stream(like.device))
+    return out
+
+
 def contiguous_on(stream, t: torch.Tensor) -> torch.Tensor:
     """t, or a contiguous copy of it made on `stream`."""
     if t.is_contiguous():

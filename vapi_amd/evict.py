@@ -19,7 +19,7 @@ import torch
 from ._lib import Weights, check, lib
 from .attention import PreparedAttention
 from .cache import (HybridKvCache, _is_quantised, _per_layer, check_on_device, contiguous_on,
-                    keep_for, on_stream, stream_handle)
+                    empty_on, keep_for, stream_handle)
 
 
 def new_weights(rows: int, num_kv_heads: int, width: int, device="cuda") -> torch.Tensor:
@@ -107,8 +107,7 @@ def accumulate_attention_weights(q: torch.Tensor, cache, layer: int, prepared: P
         # Kept for the step's other layers, as the attention's; a smaller one stays
         # too (a captured graph may hold it).
         prepared.weights_workspaces.append(ws)
-        with on_stream(stream, q.device):
-            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws = empty_on(stream, q, need, torch.uint8)
         prepared.weights_workspace = ws
     quantised = _is_quantised(cache)
     fn = lib().vapi_kv_q8_attention_weights if quantised else lib().vapi_kv_attention_weights
@@ -227,8 +226,7 @@ def evict_kv(cache, layer: int, weights: torch.Tensor, plan: EvictionPlan,
             if a0 < b1 and b0 < a1:
                 raise ValueError("weights_out overlaps weights: give the same tensor or another")
     check_on_device(*on)
-    kept = torch.empty((b, cache.num_kv_heads, plan.max_keep), dtype=torch.int32,
-                       device=weights.device)
+    kept = empty_on(stream, weights, (b, cache.num_kv_heads, plan.max_keep), torch.int32)
     quantised = _is_quantised(cache)
     fn = lib().vapi_kv_q8_evict if quantised else lib().vapi_kv_evict
     check(fn(cache.q8 if quantised else cache.pool, layer, src,
