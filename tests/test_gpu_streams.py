@@ -9,7 +9,8 @@ from test_gpu_quant import batch_of
 from vapi_amd.attention import (PreparedAttention, paged_attention_append_prepared,
                                 paged_attention_prepared)
 from vapi_amd.cache import scatter_index
-from vapi_amd.evict import EvictionPlan, evict_kv
+from vapi_amd.evict import (EvictionPlan, accumulate_attention_weights, evict_kv,
+                            new_weights)
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +67,35 @@ def test_a_captured_call_names_its_stream():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, paged_attention_prepared(q, cache, 0, prep, 0.1))
+
+
+@pytest.mark.parametrize("fmt", ["none", "e4m3"])
+@pytest.mark.parametrize("lens_q", [[1, 1], [30, 1]])
+def test_a_step_dropped_before_its_call_has_run(fmt, lens_q):
+    """Its device arrays and workspace are not handed out while the call, on
+    another stream, waits. (Zeros in their place would leave rows unwritten.)"""
+    lens_k, heads, kvh, d = [300, 90], 4, 2, 64
+    cache, tables, _ = filled(lens_k, kvh, d, 16, fmt, BF16, "HND", 3)
+    q = torch.randn(sum(lens_q), heads, d, device="cuda").to(BF16)
+
+    def step():
+        return PreparedAttention.from_batch(batch_of(lens_q, lens_k, tables), "cuda", cache,
+                                            heads, deterministic=True)
+
+    w, want_w = new_weights(2, kvh, 300), new_weights(2, kvh, 300)
+    prep = step()
+    want = paged_attention_prepared(q, cache, 0, prep, 0.1)
+    accumulate_attention_weights(q, cache, 0, prep, 0.1, want_w)
+    prep, side = step(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(40_000_000)
+    got = paged_attention_prepared(q, cache, 0, prep, 0.1, stream=side)
+    accumulate_attention_weights(q, cache, 0, prep, 0.1, w, stream=side)
+    sizes = [t.numel() * t.element_size() for t in
+             (prep.block_table, prep.seqlens_q, prep.seqlens_k, prep.prefill_seqs, prep.workspace,
+              prep.weights_workspace)]
+    del prep
+    junk = [torch.zeros(n, dtype=torch.uint8, device="cuda") for n in sizes for _ in range(4)]
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and torch.equal(w, want_w) and junk

@@ -12,7 +12,8 @@ import torch
 import quant_ref as ref
 from vapi_amd import _lib
 from vapi_amd._lib import BF16, EINVAL, ESPACE, EUNSUP, F16, F32, Pool, Q8Pool, Weights, lib
-from vapi_amd.attention import ForwardBatch, PreparedAttention, workspace_bytes
+from vapi_amd.attention import (ForwardBatch, PreparedAttention, _workspace,
+                                workspace_bytes)
 from vapi_amd.cache import (PagedKvCache, gather_kv, scatter_index, write_k_to_cache,
                             write_kv_to_cache, write_kv_to_cache_layers, write_rows_indexed,
                             write_v_rows_indexed)
@@ -258,6 +259,23 @@ def test_the_workspace_of_a_step():
                          block_tables=[[0], [1]], max_seqlen_q=3, max_seqlen_k=11)
     prep = PreparedAttention.from_batch(batch, "cpu")
     assert prep.n_prefill_arg() == 1 and prep.n_prefill_arg(cache) is None
+
+
+def test_a_larger_workspace_leaves_the_smaller_one_alone():
+    """A captured graph, or a call on another stream, may still use it."""
+    small, large = cpu_cache(), PagedKvCache(1, 6, 16, 2, 128, torch.bfloat16, "HND", "cpu")
+    batch = ForwardBatch(cu_seqlens_q=[0, 1, 2], cu_seqlens_k=[0, 9, 20],
+                         block_tables=[[0], [1]], max_seqlen_q=1, max_seqlen_k=11)
+    prep = PreparedAttention.from_batch(batch, "cpu", small, 4)
+    first = prep.workspace
+    _workspace(large, prep, 2, 4, 1, 11, "cpu")
+    second = prep.workspace
+    assert second.numel() > first.numel()
+    prep.reserve(cpu_cache(num_kv_heads=4, head_dim=256), 16, "cpu")
+    assert prep.workspace.numel() > second.numel()
+    assert prep.workspaces[0] is first and prep.workspaces[1] is second
+    _workspace(small, prep, 2, 4, 1, 11, "cpu")
+    assert len(prep.workspaces) == 2
 
 
 def test_weights_states_that_do_not_fit_are_refused():

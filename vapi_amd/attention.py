@@ -117,6 +117,8 @@ class PreparedAttention:
     n_prefill: int = 0
     weights_workspace: torch.Tensor | None = None  # accumulate_attention_weights
     weights_workspaces: list = field(default_factory=list)  # earlier, smaller ones
+    workspaces: list = field(default_factory=list)  # the attention's earlier ones
+    streams: set = field(default_factory=set)  # handles keep_for has seen
 
     @classmethod
     def from_batch(cls, batch: ForwardBatch, device, cache=None, num_heads: int | None = None,
@@ -151,8 +153,33 @@ class PreparedAttention:
                   if isinstance(cache, HybridKvCache) else [cache])
         need = max(workspace_bytes(c, b, num_heads, max_q, max_k, self.n_prefill_arg(c))
                    for c in layers)
-        if need and (self.workspace is None or self.workspace.numel() < need):
-            self.workspace = torch.zeros(need, dtype=torch.uint8, device=device)
+        self.grow(need, device)
+
+    def grow(self, need: int, device, stream=None) -> torch.Tensor | None:
+        """The workspace, replaced by a zeroed one of `need` bytes if it is
+        smaller. The smaller one stays: a captured graph may hold its address, or
+        a call on another stream be using it."""
+        ws = self.workspace
+        if need and (ws is None or ws.numel() < need):
+            if ws is not None:
+                self.workspaces.append(ws)
+            with on_stream(stream, device):
+                ws = torch.zeros(need, dtype=torch.uint8, device=device)
+            if stream is not None:
+                ws.record_stream(torch.cuda.current_stream(ws.device))
+            self.workspace = ws
+            self.streams.clear()
+        return ws
+
+    def keep_for(self, stream) -> None:
+        """Keeps the step's device arrays and workspace from reuse before a call on
+        `stream` (None: the current one) has run, whenever the step is dropped.
+        (Memory once marked for a stream stays marked.)"""
+        if stream is None or stream.cuda_stream in self.streams:
+            return
+        keep_for(stream, *(t for t in (self.block_table, self.seqlens_q, self.seqlens_k,
+                                       self.prefill_seqs, self.workspace) if t is not None))
+        self.streams.add(stream.cuda_stream)
 
     def n_prefill_arg(self, cache=None) -> int | None:
         """The prefill sequence count the calls pass (None: no list). Over an
@@ -180,15 +207,11 @@ def workspace_bytes(cache: PagedKvCache, batch: int, num_heads: int, max_q: int,
 def _workspace(cache, prepared: PreparedAttention, b: int, num_heads: int, max_q: int,
                max_k: int, device, stream=None):
     need = workspace_bytes(cache, b, num_heads, max_q, max_k, prepared.n_prefill_arg(cache))
-    ws = prepared.workspace
-    if need and (ws is None or ws.numel() < need):
-        # Zero-filled once: a zeroed workspace starts the decode from equal
-        # per-XCD shares; later calls carry the shares over. (A step whose
-        # layers differ in geometry sizes it up front with reserve(), so that
-        # no layer allocates mid-step or inside a captured graph.)
-        with on_stream(stream, device):
-            ws = torch.zeros(need, dtype=torch.uint8, device=device)
-        prepared.workspace = ws
+    # Zero-filled once: a zeroed workspace starts the decode from equal per-XCD
+    # shares; later calls carry the shares over. (A step whose layers differ in
+    # geometry sizes it up front with reserve(), so that no layer allocates
+    # mid-step or inside a captured graph.)
+    ws = prepared.grow(need, device, stream)
     return need, ws
 
 
@@ -198,14 +221,14 @@ def _run(call, cache, prepared: PreparedAttention, b: int, num_heads: int, max_q
     if it is too small. A decode's workspace has no optional part, so the
     library, which refuses a small one before it launches anything, is asked
     first (the size query is ~1 us of a call's ~8)."""
-    ws = prepared.workspace
+    ws, rc = prepared.workspace, ESPACE
     if max_q == 1 and ws is not None:
         rc = call(ws.data_ptr(), ws.numel())
-        if rc != ESPACE:
-            check(rc)
-            return
-    need, ws = _workspace(cache, prepared, b, num_heads, max_q, max_k, device, stream)
-    check(call(ws.data_ptr() if need else None, need))
+    if rc == ESPACE:
+        need, ws = _workspace(cache, prepared, b, num_heads, max_q, max_k, device, stream)
+        rc = call(ws.data_ptr() if need else None, need)
+    check(rc)
+    prepared.keep_for(stream)
 
 
 def paged_attention_prepared(q: torch.Tensor, cache: PagedKvCache, layer: int,

@@ -106,7 +106,8 @@ def accumulate_attention_weights(q: torch.Tensor, cache, layer: int, prepared: P
     if need and (ws is None or ws.numel() < need):
         # Kept for the step's other layers, as the attention's; a smaller one stays
         # too (a captured graph may hold it).
-        prepared.weights_workspaces.append(ws)
+        if ws is not None:
+            prepared.weights_workspaces.append(ws)
         ws = empty_on(stream, q, need, torch.uint8)
         prepared.weights_workspace = ws
     quantised = _is_quantised(cache)
@@ -118,6 +119,7 @@ def accumulate_attention_weights(q: torch.Tensor, cache, layer: int, prepared: P
              -1 if window_size_right is None else int(window_size_right), int(last_queries),
              float(decay), state, ws.data_ptr() if need else None, need, stream_handle(stream)))
     if stream is not None:
+        prepared.keep_for(stream)
         keep_for(stream, q, weights, *([] if index is None else [index]), *([ws] if need else []))
     return weights
 
