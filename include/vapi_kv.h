@@ -603,7 +603,8 @@ int vapi_kv_q8_gather(const vapi_kv_q8_pool* pool, uint32_t layer, const uint32_
  * expanded there once, n_prefill * max_seqlen_k keys of the layer in the
  * pool's dtype. n_prefill is the list's length, or batch where every sequence
  * is covered: without a list, and with VAPI_ATTN_NO_DECODE_ROWS, which ignores it.
- * Groups of up to 256 query heads per kv head.
+ * Groups of up to 256 query heads per kv head. _workspace_size is 0 where the call
+ * would be refused for its pool, heads or lengths (vapi_kv_last_error says why).
  */
 size_t vapi_kv_q8_attention_workspace_size(const vapi_kv_q8_pool* pool, uint32_t batch,
                                            uint32_t n_prefill, uint32_t num_heads,

@@ -458,3 +458,34 @@ def test_prefill_rows_without_any_key_are_written():
         torch.cuda.current_stream().cuda_stream) == 0
     torch.cuda.synchronize()
     assert not out.any()
+
+
+def test_a_refused_step_writes_nothing():
+    """Whatever the attention of an append-and-attend call would refuse is refused
+    before the rows are written."""
+    cache, tables = filled([40], 2, 64, 16, "e4m3", BF16, "HND", 6)
+    codes, scales = cache._codes.clone(), cache._scales.clone()
+    k = torch.randn(3, 2, 64, device="cuda").to(BF16)
+    slots = scatter_index(ref.slots_of(tables[0], 40, 16)[37:], "cuda")
+    flat = torch.randn(3 * 4 * 64 + 8, device="cuda").to(BF16)
+    q = flat[:3 * 4 * 64].view(3, 4, 64)
+
+    def step(q=q, out=None, lens_q=(3,), heads=4, **fields):
+        prep = PreparedAttention.from_batch(batch_of(lens_q, [40], tables), "cuda")
+        for name, value in fields.items():
+            setattr(prep, name, value)
+        return paged_attention_append_prepared(q, k, k, slots, cache, 0, prep, 0.1, out=out)
+
+    odd = flat[4:4 + 3 * 4 * 64].view(3, 4, 64)
+    calls = [dict(q=odd), dict(out=odd), dict(q=q.cpu()), dict(out=q.cpu()),
+             dict(q=q[:, :3].contiguous()), dict(q=q[:, :0].contiguous()),
+             dict(max_seqlen_k=1 << 29), dict(flags=0x10),
+             dict(block_table=torch.zeros(1, 0, dtype=torch.int32, device="cuda"))]
+    for kw in calls:
+        with pytest.raises((ValueError, VapiKvError)):
+            step(**kw)
+        torch.cuda.synchronize()
+        assert torch.equal(cache._codes, codes) and torch.equal(cache._scales, scales), kw
+    step()
+    torch.cuda.synchronize()
+    assert not torch.equal(cache._codes, codes)

@@ -188,6 +188,14 @@ def test_calls_past_a_grid_s_reach_are_refused():
     assert size(pool, 2, 2, 4, 8, 0) == size(pool, 2, 2, 4, 8, 1)
 
 
+def test_sizes_that_are_refused_need_no_workspace():
+    size, pool = lib().vapi_kv_q8_attention_workspace_size, q8_pool()
+    for args in ((2, 2, 0, 1, 64), (2, 2, 3, 1, 64), (2, 2, 2 * 257, 1, 64),
+                 (2, 2, 4, 2, 1 << 28), (70000, 66000, 4, 2, 64)):
+        assert size(pool, *args) == 0 and lib().vapi_kv_last_error()
+    assert size(pool, 70000, 66000, 4, 1, 64) > 0  # no prefill rows: the list counts for nothing
+
+
 # ---- the Python side --------------------------------------------------------------
 
 

@@ -328,9 +328,17 @@ def paged_attention_append_prepared(q: torch.Tensor, k: torch.Tensor, v: torch.T
     max_q = max(int(prepared.max_seqlen_q), 1)
     max_k = max(int(prepared.max_seqlen_k), 1)
     if _is_quantised(cache):
-        # Two calls; what the second would refuse is refused before the first.
-        if num_heads % cache.num_kv_heads or num_heads > 256 * cache.num_kv_heads:
-            raise ValueError(f"{num_heads} query heads over {cache.num_kv_heads} kv heads")
+        # Two calls; what the second would refuse is refused before the first, and
+        # its workspace is there before rows are written.
+        check_on_device(cache.k[0], q, out, prepared.block_table, prepared.seqlens_q)
+        if (q.data_ptr() | out.data_ptr()) & 15:
+            raise ValueError("q and out must be 16-byte aligned")
+        if prepared.block_table.shape[1] == 0 or prepared.flags & ~(ATTN_DETERMINISTIC |
+                                                                    ATTN_NO_DECODE_ROWS):
+            raise ValueError(f"a block table of no columns, or unknown flags {prepared.flags:#x}")
+        if b and not _workspace(cache, prepared, b, num_heads, max_q, max_k, q.device,
+                                stream)[0]:
+            raise ValueError(lib().vapi_kv_last_error().decode())
         write_rows_indexed(cache, layer, k, v, slot_mapping, stream=stream)
         return paged_attention_prepared(q, cache, layer, prepared, softmax_scale,
                                         window_size_left, window_size_right, out=out,

@@ -471,6 +471,24 @@ static size_t q8_decode_ws(const vapi_kv_q8_pool* p, uint32_t batch, uint32_t nu
            : 0;
 }
 
+// What a call refuses for its sizes alone: 0 or an error code with a message.
+// pf_n: sequences that the prefill covers.
+static int q8_check_sizes(const vapi_kv_q8_pool* p, uint32_t num_heads, uint32_t pf_n,
+                          uint32_t max_q, uint32_t max_k, const char* who) {
+  if (num_heads == 0 || num_heads % p->num_kv_heads)
+    VK_FAIL(VAPI_KV_EINVAL, "%s: %u query heads is not a multiple of %u kv heads", who, num_heads,
+            p->num_kv_heads);
+  const uint32_t G = num_heads / p->num_kv_heads;
+  if (!q8_parts(G) || num_heads > 65535)
+    VK_FAIL(VAPI_KV_EUNSUP, "%s: %u query heads for %u kv heads", who, num_heads, p->num_kv_heads);
+  const uint64_t mb = ((uint64_t)max_k + p->block_size - 1) / p->block_size;
+  if (pf_n && (pf_n > 65535 || prefill_grid(pf_n, p->num_kv_heads, G, max_q,
+                                            q8_dim(p->head_dim)) > 0xFFFFFFFFull ||
+               pf_n * mb > 0xFFFFFFull))
+    VK_FAIL(VAPI_KV_EUNSUP, "%s: prefill batch too large for one launch", who);
+  return 0;
+}
+
 template <typename T, int F, int D>
 static void launch_q8_stream_d(const AttnArgs& c, const Q8Scales& sc, uint32_t nwg, size_t lds,
                                hipStream_t s) {
@@ -587,13 +605,14 @@ extern "C" {
 size_t vapi_kv_q8_attention_workspace_size(const vapi_kv_q8_pool* pool, uint32_t batch,
                                            uint32_t n_prefill, uint32_t num_heads,
                                            uint32_t max_seqlen_q, uint32_t max_seqlen_k) {
-  if (check_q8_pool(pool, 0, "vapi_kv_q8_attention_workspace_size") || batch == 0 ||
-      num_heads == 0 || num_heads % pool->num_kv_heads)
-    return 0;
+  const char* who = "vapi_kv_q8_attention_workspace_size";
+  n_prefill = max_seqlen_q > 1 ? std::min(n_prefill, batch) : 0;
   max_seqlen_k = std::max(max_seqlen_k, 1u);
+  if (check_q8_pool(pool, 0, who) || batch == 0 ||
+      q8_check_sizes(pool, num_heads, n_prefill, max_seqlen_q, max_seqlen_k, who))
+    return 0;
   size_t need = std::max(up256(q8_decode_ws(pool, batch, num_heads)), (size_t)256);
-  n_prefill = std::min(n_prefill, batch);
-  if (max_seqlen_q > 1 && n_prefill)
+  if (n_prefill)
     need += q8_expand_ws(pool, batch, n_prefill, max_seqlen_k).total +
             prefill_split_bytes(n_prefill, pool->num_kv_heads, num_heads / pool->num_kv_heads,
                                 q8_dim(pool->head_dim), max_seqlen_q, max_seqlen_k);
@@ -627,18 +646,13 @@ int vapi_kv_q8_attention(const vapi_kv_q8_pool* pool, uint32_t layer, const void
     VK_FAIL(VAPI_KV_EINVAL, "%s: keys to attend over in an empty pool", who);
   if (max_blocks == 0) VK_FAIL(VAPI_KV_EINVAL, "%s: block table width 0", who);
   const uint32_t G = num_heads / pool->num_kv_heads, parts = q8_parts(G);
-  if (!parts || num_heads > 65535)
-    VK_FAIL(VAPI_KV_EUNSUP, "%s: %u query heads for %u kv heads", who, num_heads,
-            pool->num_kv_heads);
   const uint32_t D = q8_dim(pool->head_dim);
   const bool prefill = max_seqlen_q > 1;
   const bool skip_decode = prefill && (flags & VAPI_ATTN_NO_DECODE_ROWS);
   const bool listed = prefill_seqs && !skip_decode;
   const uint32_t pf_n = !prefill ? 0 : listed ? n_prefill : batch;
+  if (int rc = q8_check_sizes(pool, num_heads, pf_n, max_seqlen_q, max_seqlen_k, who)) return rc;
   const uint64_t mb = ((uint64_t)max_seqlen_k + pool->block_size - 1) / pool->block_size;
-  if (pf_n && (pf_n > 65535 || prefill_grid(pf_n, pool->num_kv_heads, G, max_seqlen_q, D) >
-                                   0xFFFFFFFFull || pf_n * mb > 0xFFFFFFull))
-    VK_FAIL(VAPI_KV_EUNSUP, "%s: prefill batch too large for one launch", who);
   const size_t dec_ws = skip_decode ? 0 : q8_decode_ws(pool, batch, num_heads);
   const size_t off = std::max(up256(dec_ws), (size_t)256);
   const Q8ExpandWs w = pf_n ? q8_expand_ws(pool, batch, pf_n, max_seqlen_k) : Q8ExpandWs{0, 0, 0, 0};
