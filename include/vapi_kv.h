@@ -655,8 +655,10 @@ typedef struct vapi_kv_weights {
  * pool. A NaN or an infinity in K or q reaches the weights of its own key, or
  * of the keys its query sees, alone. q: 16-byte aligned. workspace: device
  * scratch of vapi_kv_attention_weights_workspace_size bytes, 16-byte aligned,
- * nothing in it kept between calls; calls sharing one must not overlap. No
- * counterpart in the reference.
+ * nothing in it kept between calls; calls sharing one must not overlap. Its size:
+ * 8 bytes a (query, query head) and chunk of keys, one chunk where the rows fill
+ * the GPU, and up to 64 MiB of partial sums, or for at most 16 such rows a kv
+ * head up to 256 MiB of scores. No counterpart in the reference.
  */
 size_t vapi_kv_attention_weights_workspace_size(uint32_t batch, uint32_t num_kv_heads,
                                                 uint32_t num_heads, uint32_t head_dim,

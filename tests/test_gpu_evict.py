@@ -510,3 +510,24 @@ def test_captured_weights_and_eviction_replay():
         k2 = step()
         assert all(torch.equal(a, b) for a, b in zip(got, (w, out, k2, cache._codes,
                                                            cache._scales)))
+
+
+@pytest.mark.parametrize("fmt,dtype", [("none", BF16), ("e4m3", F16)])
+@pytest.mark.parametrize("left,max_k", [(None, 1 << 20), (None, 1 << 22), (300, 1 << 22)])
+def test_weights_of_more_rows_than_a_workgroup_holds(fmt, dtype, left, max_k):
+    """A bound on the keys that leaves room for few parts of the rows, or for one:
+    each walks 512 rows at a time."""
+    lens_q, lens_k, heads, kvh, d = [1300, 900], [1300, 1100], 4, 2, 64
+    cache, tables, _ = filled(lens_k, kvh, d, 16, fmt, dtype, "HND", 12)
+    q = torch.randn(sum(lens_q), heads, d, generator=torch.Generator().manual_seed(1)).to(dtype)
+    prep = PreparedAttention.from_batch(batch_of(lens_q, lens_k, tables), "cuda")
+    prep.max_seqlen_k = max_k
+    w = torch.zeros(2, kvh, max_k, device="cuda")
+    accumulate_attention_weights(q.cuda(), cache, 0, prep, 0.125, w, window_size_left=left)
+    n = max(lens_k) + 3
+    assert not w[:, :, n:].any()
+    old = torch.zeros(2, kvh, n)
+    want, bound = weights_ref(q, ref.values(cache, 0, "k"), lens_q, lens_k, tables, 16, 0.125,
+                              left, 0, 0, 1.0, old, [0, 1])
+    err = (w[:, :, :n].cpu().double() - want).abs()
+    assert torch.all(err <= bound), f"{float((err / bound.clamp_min(1e-300)).max()):.3g} bounds"

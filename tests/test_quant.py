@@ -188,6 +188,16 @@ def test_calls_past_a_grid_s_reach_are_refused():
     assert size(pool, 2, 2, 4, 8, 0) == size(pool, 2, 2, 4, 8, 1)
 
 
+def test_the_weights_workspace_of_long_prompts():
+    """8 bytes a row and chunk, and at most 64 MiB of sums: not a sum for every key
+    and 512 rows."""
+    size = lib().vapi_kv_attention_weights_workspace_size
+    for batch, kvh, heads, n in ((1, 8, 32, 32768), (4, 8, 32, 32768), (1, 8, 32, 131072),
+                                 (1, 1, 16, 1 << 20), (64, 8, 32, 131072)):
+        rows = batch * heads * n * 8
+        assert rows <= size(batch, kvh, heads, 128, n, n, 0) <= rows + (64 << 20) + 4096
+
+
 def test_sizes_that_are_refused_need_no_workspace():
     size, pool = lib().vapi_kv_q8_attention_workspace_size, q8_pool()
     for args in ((2, 2, 0, 1, 64), (2, 2, 3, 1, 64), (2, 2, 2 * 257, 1, 64),

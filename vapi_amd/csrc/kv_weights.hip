@@ -429,7 +429,7 @@ __device__ __forceinline__ float weight_join(const float2* ml, uint32_t n) {
   return __float_as_uint(sum) - 1u < 0x7f7fffffu ? mx + __builtin_amdgcn_logf(sum) : INFINITY;
 }
 
-constexpr uint32_t kWeightJoinRows = 512;  // rows whose lse a workgroup joins in LDS
+constexpr uint32_t kWeightJoinRows = 512;  // rows whose lse a workgroup holds in LDS
 // 16-key tiles a wave of pass 2 holds. More of them read Q less often, fewer leave
 // registers for more waves: three fresh prompts (above) 55.8 / 53.5 / 66.9 us at 2 /
 // 3 / 4, a prompt's last 32 queries 13.8 / 12.0 / 16.2.
@@ -505,7 +505,7 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_sum(WeightArgs a) {
 #pragma unroll
     for (int t = 0; t < KT; ++t)
       weight_load<F, D, false>(raw[t], a, s, key0 + 16 * t, weight_block(a, s, key0 + 16 * t), lane);
-    weight_lse_rows(lse_lds, a, blockIdx.x, r0, r1);
+    weight_lse_rows(lse_lds, a, blockIdx.x, r0, min(r0 + kWeightJoinRows, r1));
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
       weight_stage<F, D>(place, raw[t], lane);
@@ -544,9 +544,15 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_sum(WeightArgs a) {
   const uint32_t some1 = key0 >= s.len_k ? r0 : a.wl >= 0 ? row_at((int64_t)key1 + a.wl + 1) : r1;
   const uint32_t all0 = a.wr >= 0 ? row_at((int64_t)key1 - a.wr) : r0;
   const uint32_t all1 = !held_all ? r0 : a.wl >= 0 ? row_at((int64_t)key0 + a.wl + 1) : r1;
-  uint32_t turn = 0;
+  uint32_t turn = 0, lse0 = r0;  // lse0: the row of lse_lds's first
+  static_assert(kWeightJoinRows % kWeightBlock == 0, "lse_lds holds whole blocks");
   if (r0 < r1) fetch(r0);
   for (uint32_t first = r0; first < r1; first += kWeightBlock, turn ^= 1) {
+    if (first - lse0 == kWeightJoinRows) {
+      lse0 = first;
+      __syncthreads();  // the last rows' readers
+      weight_lse_rows(lse_lds, a, blockIdx.x, lse0, min(lse0 + kWeightJoinRows, r1));
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const uint32_t at = 64 * kWeightWaves * i + threadIdx.x, row = at / PR, piece = at % PR;
@@ -567,7 +573,7 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_sum(WeightArgs a) {
 #pragma unroll
         for (int c = 0; c < D / 32; ++c)
           q[c] = __builtin_bit_cast(uint4, lds[turn][(r - first) * PR + q_at[c]]);
-        const float lse = lse_lds[r - r0 + col];  // (a part is whole tiles)
+        const float lse = lse_lds[r - lse0 + col];  // (a part is whole tiles)
         floatx4 acc[KT];
 #pragma unroll
         for (int t = 0; t < KT; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -669,6 +675,10 @@ struct WeightPlan {
 // 8 kv heads, bf16: pass 2 53.6 -> 7.1 us).
 constexpr uint64_t kWeightWgs = 1024;
 constexpr uint64_t kStoreBytes = 256ull << 20;
+// Each part holds a sum a key: at most this much of them. Where it binds, pass 2
+// has at least 43,000 workgroups of 192 keys (half of it, 8 M sums), enough without
+// more parts.
+constexpr uint64_t kPartBytes = 64ull << 20;
 static WeightPlan weight_plan(uint32_t batch, uint32_t kvh, uint32_t group, uint32_t hd,
                               uint32_t max_q, uint32_t max_k, uint32_t last) {
   WeightPlan p;
@@ -686,9 +696,11 @@ static WeightPlan weight_plan(uint32_t batch, uint32_t kvh, uint32_t group, uint
   p.chunk_keys = (uint32_t)(up(keys, kWeightChunk) * kWeightChunk);
   p.n_chunk = (uint32_t)std::max<uint64_t>(up(max_k, p.chunk_keys), 1);
   const uint64_t blocks = up(max_k, 16 * kWeightKt * kWeightWaves);
-  // (A part's rows are joined in LDS, so there are at least enough parts.)
+  // (Parts of at most kWeightJoinRows rows where kPartBytes takes them: the rows
+  // of a causal prompt's late parts are many, of its early ones few.)
   uint64_t parts = std::max<uint64_t>(up(kWeightWgs, blocks * segs), 1);
   parts = std::max(std::min<uint64_t>(parts, up(rows, 128)), up(rows, kWeightJoinRows));
+  parts = std::min(parts, std::max<uint64_t>(kPartBytes / (segs * p.key_cap * sizeof(float)), 1));
   p.part_rows = (uint32_t)(up(up(rows, parts), 16) * 16);
   p.parts = p.store ? 1 : (uint32_t)up(rows, p.part_rows);
   p.ml_bytes = (segs * p.row_cap * p.n_chunk * sizeof(float2) + 255) & ~(size_t)255;
