@@ -531,3 +531,25 @@ def test_weights_of_more_rows_than_a_workgroup_holds(fmt, dtype, left, max_k):
                               left, 0, 0, 1.0, old, [0, 1])
     err = (w[:, :, :n].cpu().double() - want).abs()
     assert torch.all(err <= bound), f"{float((err / bound.clamp_min(1e-300)).max()):.3g} bounds"
+
+
+@pytest.mark.parametrize("fmt", ["none", "int8"])
+@pytest.mark.parametrize("lens", [[0, 0], [0, 40]])
+def test_sequences_without_keys_leave_zeros(fmt, lens):
+    """The rows of a state that an eviction writes are zeros from a sequence's kept
+    keys on, also where no sequence of the batch has any."""
+    cache, tables, free = filled([40], 2, 64, 16, fmt, BF16, "HND", 3, spare=8)
+    before = cache.k[0].clone()
+    w = torch.rand(4, 2, 50, device="cuda")
+    rows, held = [2, 0], w.clone()
+    dst = [[], [free.pop(), free.pop()] if lens[1] else []]
+    plan = EvictionPlan.from_tables(lens, [[], tables[0] if lens[1] else []], dst, 20, 2, 4, 16,
+                                    "cuda", rows)
+    out = torch.full_like(w, 9.0)
+    for target in (out, w):
+        kept = evict_kv(cache, 0, w, plan, weights_out=target)
+        assert kept.shape == (2, 2, min(max(lens), 20)) and torch.all(kept[0] == -1)
+        assert not target[2].any() and not target[0, :, min(lens[1], 20):].any()
+    assert torch.all(out[[1, 3]] == 9.0) and torch.equal(w[[1, 3]], held[[1, 3]])
+    assert evict_kv(cache, 0, held, plan).shape == kept.shape
+    assert lens[1] or torch.equal(cache.k[0].view(torch.uint8), before.view(torch.uint8))

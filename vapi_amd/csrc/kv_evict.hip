@@ -27,7 +27,7 @@ struct EvictArgs {
 };
 
 __device__ __forceinline__ uint32_t evict_len(const EvictArgs& a, uint32_t seq) {
-  return min(a.lens[seq], a.max_len);
+  return a.max_len ? min(a.lens[seq], a.max_len) : 0u;
 }
 
 // Weights as unsigned numbers in the same order: NaN lowest, both zeros alike.
@@ -375,11 +375,12 @@ static int evict_checks(const EvictCall& c, uint32_t kvh, uint32_t num_blocks, c
   if (c.out && keep > c.out->width)
     VK_FAIL(VAPI_KV_EINVAL, "%s: %u kept keys exceed the weights' width %u", who, keep,
             c.out->width);
-  if (c.batch == 0 || c.max_len == 0) return 0;
-  if (!c.lens || !c.src_table || !c.dst_table || !c.kept)
+  if (c.batch == 0 || (c.max_len == 0 && !c.out)) return 0;
+  // (Without keys nothing is read, kept or moved, but rows of `out` become zeros.)
+  if (c.max_len && (!c.lens || !c.src_table || !c.dst_table || !c.kept))
     VK_FAIL(VAPI_KV_EINVAL, "%s: null device pointer", who);
-  if (num_blocks == 0) VK_FAIL(VAPI_KV_EINVAL, "%s: keys in an empty pool", who);
-  if (c.src_blocks == 0 || c.dst_blocks == 0)
+  if (c.max_len && num_blocks == 0) VK_FAIL(VAPI_KV_EINVAL, "%s: keys in an empty pool", who);
+  if (c.max_len && (c.src_blocks == 0 || c.dst_blocks == 0))
     VK_FAIL(VAPI_KV_EINVAL, "%s: block table width 0", who);
   if ((uint64_t)c.batch * kvh > 65535 || c.max_len > 0x3FFFFFFFu)
     VK_FAIL(VAPI_KV_EUNSUP, "%s: a batch of %u x %u kv heads of up to %u keys", who, c.batch, kvh,
@@ -449,6 +450,10 @@ int vapi_kv_evict(const vapi_kv_pool* pool, uint32_t layer, const vapi_kv_weight
   if ((uint64_t)m.max_keep * upr >= 0x7FFFFFFFull)
     VK_FAIL(VAPI_KV_EUNSUP, "%s: %u kept keys of %u bytes", who, m.max_keep, m.row_bytes);
   launch_evict_select(c, g.kvh, hs(stream));
+  if (c.max_len == 0) {
+    VK_LAUNCHED(who);
+    return 0;
+  }
   const uint32_t rows = (m.max_keep + kCopyRows - 1) / kCopyRows;
   const dim3 grid((rows * upr + 255) / 256, batch * g.kvh, pool->v ? 2 : 1);
 #define VK_EVICT(C)                                                                       \
@@ -484,6 +489,10 @@ int vapi_kv_q8_evict(const vapi_kv_q8_pool* pool, uint32_t layer, const vapi_kv_
   m.k = p.k, m.v = p.v;
   m.blk_b = g.blk, m.head_b = g.head, m.tok_b = g.tok, m.row_bytes = g.d;
   launch_evict_select(c, g.kvh, hs(stream));
+  if (c.max_len == 0) {
+    VK_LAUNCHED(who);
+    return 0;
+  }
   const uint32_t nb = (m.max_keep + g.block_size - 1) / g.block_size;
   const dim3 grid((nb + kMoveWaves - 1) / kMoveWaves, batch * g.kvh, 2);
   const FastDiv upr(g.d / 16);
