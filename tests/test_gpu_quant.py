@@ -8,7 +8,8 @@ from vapi_amd._lib import SLOT_SKIP, VapiKvError, lib
 from vapi_amd.attention import (ForwardBatch, PreparedAttention, paged_attention,
                                 paged_attention_append_prepared, paged_attention_prepared)
 from vapi_amd.backend import KvBlockBackend
-from vapi_amd.cache import gather_kv, scatter_index, write_kv_to_cache, write_rows_indexed
+from vapi_amd.cache import (PagedKvCache, gather_kv, scatter_index, write_kv_to_cache,
+                            write_rows_indexed)
 from vapi_amd.quant import QuantKvCache
 
 pytestmark = pytest.mark.gpu
@@ -489,3 +490,33 @@ def test_a_refused_step_writes_nothing():
     step()
     torch.cuda.synchronize()
     assert not torch.equal(cache._codes, codes)
+
+
+@pytest.mark.parametrize("fmt", ["none", "f32", "valu", "e4m3", "int8"])
+@pytest.mark.parametrize("lens_q", [[40, 1, 130], [300]])
+def test_windows_near_2_to_the_31(fmt, lens_q):
+    """They hide nothing, like no window: over 16-bit and 8-bit caches, f32 ones and
+    head sizes that the vector unit serves."""
+    lens_k = [n + 70 for n in lens_q]
+    gen = torch.Generator().manual_seed(4)
+    d, dtype = (72 if fmt == "valu" else 64), (torch.float32 if fmt in ("f32", "valu") else BF16)
+    if fmt in ("e4m3", "int8"):
+        cache, tables = filled(lens_k, 2, d, 16, fmt, dtype, "HND", 5)
+    else:
+        bs = 16 if fmt != "valu" else 8
+        need = [-(-n // bs) for n in lens_k]
+        cache = PagedKvCache(1, sum(need), bs, 2, d, dtype, "HND", "cuda")
+        ends = np.cumsum(need)
+        tables = [list(range(e - n, e)) for e, n in zip(ends, need)]
+        slots = np.concatenate([ref.slots_of(t, n, bs) for t, n in zip(tables, lens_k)])
+        k, v = (torch.randn(len(slots), 2, d, generator=gen).to(dtype).cuda() for _ in range(2))
+        write_kv_to_cache(cache, 0, k, v, slots)
+    q = torch.randn(sum(lens_q), 4, d, generator=gen).to(dtype).cuda()
+    prep = PreparedAttention.from_batch(batch_of(lens_q, lens_k, tables), "cuda", cache, 4,
+                                        deterministic=True)
+    far = 2 ** 31 - 1
+    for near, left, right in ((0, far, 0), (None, None, far), (None, far, far), (0, far - 60, 0),
+                              (None, far, far - 60)):
+        want = paged_attention_prepared(q, cache, 0, prep, 0.1, None, near)
+        got = paged_attention_prepared(q, cache, 0, prep, 0.1, left, right)
+        assert torch.equal(got, want), (left, right)

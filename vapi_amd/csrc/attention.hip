@@ -475,8 +475,8 @@ static int paged_attention_impl(const vapi_kv_pool* pool, uint32_t layer, const 
   // A zero scale is kept positive so that masked scores (-inf) times it stay -inf.
   a.scale_log2 = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
   a.q_sign = scale < 0.f ? 0x80008000u : 0u;
-  a.wl = window_left < 0 ? -1 : window_left;
-  a.wr = window_right < 0 ? -1 : window_right;
+  a.wl = window_arg(window_left);
+  a.wr = window_arg(window_right);
   a.deterministic = (flags & VAPI_ATTN_DETERMINISTIC) ? 1u : 0u;
   a.pf_min_q = 2;
   a.pf_seqs = listed ? pf->seqs : nullptr;

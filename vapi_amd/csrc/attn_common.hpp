@@ -35,6 +35,10 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2e = 1.4426950408889634f;
+
+// A window as the kernels take it: -1 (unlimited), or up to 2^30, further than any
+// position lies from another (position + window stays in 32 bits).
+inline int32_t window_arg(int32_t w) { return w < 0 ? -1 : w < (1 << 30) ? w : 1 << 30; }
 constexpr float kNegBig = -1e30f;  // running-max start: finite, so exp2 never sees inf-inf
 constexpr float kRescaleSlack = 8.0f;  // log2 units the running max may lag by
 

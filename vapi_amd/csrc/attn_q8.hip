@@ -686,8 +686,8 @@ int vapi_kv_q8_attention(const vapi_kv_q8_pool* pool, uint32_t layer, const void
   a.scale = scale;
   a.scale_log2 = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
   a.q_sign = scale < 0.f ? 0x80008000u : 0u;
-  a.wl = window_left < 0 ? -1 : window_left;
-  a.wr = window_right < 0 ? -1 : window_right;
+  a.wl = window_arg(window_left);
+  a.wr = window_arg(window_right);
   a.deterministic = (flags & VAPI_ATTN_DETERMINISTIC) ? 1u : 0u;
   a.pf_min_q = skip_decode ? 1 : 2;
   a.pf_seqs = listed ? prefill_seqs : nullptr;

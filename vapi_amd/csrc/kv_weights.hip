@@ -822,9 +822,8 @@ static WeightArgs weight_args(const WeightCall& c, const WeightPlan& p, uint32_t
   a.scale_log2 = fmaxf(fabsf(c.scale) * kLog2e, 1e-30f);
   a.q_sign = c.scale < 0.f ? 0x80008000u : 0u;
   a.decay = c.decay;
-  // (No position lies further than 2^30 from another: differences stay in 32 bits.)
-  a.wl = c.wl < 0 ? -1 : std::min(c.wl, 1 << 30);
-  a.wr = c.wr < 0 ? -1 : std::min(c.wr, 1 << 30);
+  a.wl = window_arg(c.wl);
+  a.wr = window_arg(c.wr);
   return a;
 }
 
