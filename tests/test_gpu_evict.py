@@ -553,3 +553,55 @@ def test_sequences_without_keys_leave_zeros(fmt, lens):
     assert torch.all(out[[1, 3]] == 9.0) and torch.equal(w[[1, 3]], held[[1, 3]])
     assert evict_kv(cache, 0, held, plan).shape == kept.shape
     assert lens[1] or torch.equal(cache.k[0].view(torch.uint8), before.view(torch.uint8))
+
+
+def tied_across(n_rows, kvh, width):
+    """Few distinct weights, so the last kept ones are ties spread over the row."""
+    return (plain_weights(n_rows, kvh, width) * 3).floor() / 4
+
+
+@pytest.mark.parametrize("weights", [plain_weights, tied_across])
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("lens", [[4097, 7], [12288, 300], [12289, 4096, 0], [30011, 12290, 100]])
+def test_evict_long_sequences(lens, in_place, weights):
+    """Past the keys that 256 threads take, and past those held in LDS at once, where
+    a row is walked in tiles and what it keeps is written while later ones are read."""
+    check_evict(lens, 1, 16, 16, "none", BF16, "HND", 2000, 4, 100, weights, in_place)
+    check_evict(lens, 1, 16, 16, "none", BF16, "HND", lens[0] * 2 // 3, 0, 0, weights, in_place)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_evict_long_8_bit_sequences(fmt):
+    check_evict([12289, 4100], 2, 32, 32, fmt, BF16, "NHD", 900, 4, 64, tied_across, True)
+    check_evict([12289 + 4096], 1, 16, 16, fmt, F16, "HND", 13000, 4, 64, plain_weights)
+
+
+def test_evict_long_sequences_of_one_weight():
+    """Every key ties with every other, over three tiles."""
+    check_evict([26000], 1, 16, 16, "none", F16, "HND", 13000, 10, 300,
+                lambda r, h, w: torch.full((r, h, w), 0.5), True)
+
+
+@pytest.mark.parametrize("lens_q", [[0, 3, 1], [2, 0, 40]])
+def test_decay_0_replaces_nan_and_nothing_else(lens_q):
+    """NaN in the rows of sequences with queries goes; other rows, and columns past a
+    sequence's keys, keep theirs."""
+    lens_k = [50, 64, 90]
+    cache, tables, _ = filled(lens_k, 2, 64, 16, "none", BF16, "HND", 7)
+    q = torch.randn(sum(lens_q), 4, 64, generator=torch.Generator().manual_seed(2)).to(BF16)
+    prep = PreparedAttention.from_batch(batch_of(lens_q, lens_k, tables), "cuda")
+    old = torch.rand(5, 2, 100)
+    old[:, :, ::7] = float("nan")
+    rows = [4, 0, 2]
+    w = old.cuda()
+    accumulate_attention_weights(q.cuda(), cache, 0, prep, 0.125, w, rows=rows, decay=0.0)
+    fresh = torch.zeros(5, 2, 100)
+    want, bound = weights_ref(q, ref.values(cache, 0, "k"), lens_q, lens_k, tables, 16, 0.125,
+                              None, 0, 0, 0.0, fresh, rows)
+    written = torch.zeros(5, 2, 100, dtype=torch.bool)
+    for r, lq, lk in zip(rows, lens_q, lens_k):
+        written[r, :, :lk] = lq > 0
+    got = w.cpu()
+    assert torch.equal(got.isnan(), old.isnan() & ~written)
+    assert torch.equal(torch.nan_to_num(got[~written], 5.0), torch.nan_to_num(old[~written], 5.0))
+    assert torch.all((got.double() - want).abs()[written] <= bound[written])
