@@ -209,9 +209,10 @@ int vapi_kv_gather(const vapi_kv_pool* pool, uint32_t layer,
  *   first use. Keep one workspace per stream across calls and layers: each
  *   call measures how fast each XCD streamed and moves the shares the next
  *   call on that workspace uses (a fresh workspace starts from equal
- *   shares). Results do not depend on the shares beyond f32 rounding of the
- *   split merge. Calls sharing one workspace must not overlap (same stream,
- *   or ordered streams).
+ *   shares). Where a row's keys are divided changes the f32 order of its sums
+ *   and, in 16-bit pools, the rounding of its probabilities to 16 bits (an
+ *   output by about its last bit): VAPI_ATTN_DETERMINISTIC below. Calls
+ *   sharing one workspace must not overlap (same stream, or ordered streams).
  * max_seqlen_q/k must bound every sequence's len_q/len_k (as in
  *   flash-attention); max_seqlen_q sizes the prefill grid. On the MFMA path
  *   (bf16/f16, head_dim 64, 128 or 256, or any other multiple of 8 below 256,
@@ -594,8 +595,9 @@ int vapi_kv_q8_gather(const vapi_kv_q8_pool* pool, uint32_t layer, const uint32_
 /*
  * vapi_paged_attention_prepared over an 8-bit pool: the attention of the
  * values the codes stand for, computed in the pool's dtype on matrix cores
- * with f32 sums as for a 16-bit pool. Same arguments (q and out of the
- * pool's dtype), same flags, same meaning of prefill_seqs, same rules for
+ * with f32 sums and probabilities rounded to that dtype as for a 16-bit pool (the
+ * same rounding whatever the decode's shares, which change f32 sums only). Same
+ * arguments (q and out of the pool's dtype), same flags, same meaning of prefill_seqs, same rules for
  * the workspace (zero-fill it once; one per stream; calls sharing one must
  * not overlap), except that prefill_seqs == NULL with n_prefill == 0 and
  * max_seqlen_q > 1 covers every sequence, and that a call with prefill rows

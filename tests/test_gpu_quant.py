@@ -520,3 +520,27 @@ def test_windows_near_2_to_the_31(fmt, lens_q):
         want = paged_attention_prepared(q, cache, 0, prep, 0.1, None, near)
         got = paged_attention_prepared(q, cache, 0, prep, 0.1, left, right)
         assert torch.equal(got, want), (left, right)
+
+
+@pytest.mark.parametrize("fmt,dtype", [("e4m3", BF16), ("int8", BF16), ("int8", F16)])
+def test_shares_change_no_more_than_f32_sums(fmt, dtype):
+    """Calls whose work is split at other keys, as the shares they measure move.
+
+    P is rounded alike wherever a range of keys begins, so two calls add the same
+    products in f32 in another order: sums of n ~ 1,000 terms, off by some 2^-22 of
+    sum p |v|, which is about n ** 0.5 = 30 of the output here. An output's step is
+    2^-8 (bf16) or 2^-11 of it, so some 30 * 2^-14 or 2^-11 of the outputs, 0.2 and
+    1.5%, land on another side of a rounding border; rounding P anew moves 45%."""
+    lens = [300 + 61 * i % 3000 for i in range(64)]
+    cache, tables = filled(lens, 8, 128, 16, fmt, dtype, "HND", 3)
+    q = torch.randn(64, 32, 128, generator=torch.Generator().manual_seed(3)).to(dtype).cuda()
+    prep = PreparedAttention.from_batch(batch_of([1] * 64, lens, tables), "cuda", cache, 32)
+    # (Element by element the definition's bound: a p next to a rounding border goes
+    # either way with the last bit of its exponent's f32 sum, by a step of its own.)
+    want, bound = ref.attention(q, ref.values(cache, 0, "k"), ref.values(cache, 0, "v"), [1] * 64,
+                                lens, tables, 16, 0.05)
+    first = paged_attention_prepared(q, cache, 0, prep, 0.05)
+    for _ in range(12):
+        again = paged_attention_prepared(q, cache, 0, prep, 0.05)
+        assert float((again != first).double().mean()) < 0.05
+        assert torch.all((again.cpu().double() - want).abs() <= bound)

@@ -515,11 +515,15 @@ __device__ __forceinline__ void qk_scores(const KTile<D>& kt, const uint4 (&qf)[
 // max across the four lane groups and rescale O and l to it.
 // DPL: the 16-column d tiles of O that are live (fewer than D / 16 when the
 // rest are padding).
-template <int D, int DPL = D / 16>
+// kWhole: maxima are rounded up to whole numbers, so that every factor between
+// maxima is a power of two and P keeps its 16-bit rounding whichever keys came
+// before.
+template <int D, int DPL = D / 16, bool kWhole = false>
 __device__ __forceinline__ void rescale_rows(float mx, floatx4 (&o)[D / 16], float& m_run,
                                              float& l_run) {
   if (__any(mx > m_run + kRescaleSlack)) {
-    const float m_new = fmaxf(m_run, wave_max_g(mx));
+    const float top = wave_max_g(mx);
+    const float m_new = fmaxf(m_run, kWhole ? __builtin_ceilf(top) : top);
     const float alpha = fast_exp2(m_run - m_new);
     m_run = m_new;
     l_run *= alpha;

@@ -114,8 +114,14 @@ __device__ __forceinline__ void q8_load(Q8Step<D, KS>& st, const AttnArgs& a, co
 }
 
 // One step of the online softmax for 16 query columns (attend_qk and attend_pv
-// of the 16-bit kernels, with the tiles' scales).
-template <typename T, int F, int D, int KS>
+// of the 16-bit kernels, with the tiles' scales). P is rounded to T, whose matrix
+// cores multiply it: off by at most half a step, 2^-8 of itself in bf16 and 2^-11
+// in f16, which is what V and the output have too; sums and maxima are f32.
+// kWhole: maxima are whole numbers, so that where a range of keys begins, which the
+// stream's measured shares move from call to call, changes no rounding of P (of
+// 64 x 256-8,192 keys 0.03% of the outputs differed between calls, 45% without;
+// 74.5 us either way).
+template <typename T, int F, int D, int KS, bool kWhole>
 __device__ __forceinline__ void q8_attend(const Q8Step<D, KS>& st, const uint4 (&qf)[D / 32],
                                           floatx4 (&o)[D / 16], float& m_run, float& l_run,
                                           float scale_log2, int32_t key0, int32_t lo,
@@ -142,7 +148,7 @@ __device__ __forceinline__ void q8_attend(const Q8Step<D, KS>& st, const uint4 (
     }
     mx = max_nc(mx, max_nc(max_nc(s[4 * tt], s[4 * tt + 1]), max_nc(s[4 * tt + 2], s[4 * tt + 3])));
   }
-  rescale_rows<D>(mx, o, m_run, l_run);
+  rescale_rows<D, DPL, kWhole>(mx, o, m_run, l_run);
   // int8 codes in bf16: the V scale on P (exact: bf16 has f32's exponents).
   constexpr bool kScaleP = F == VAPI_KV_Q8_INT8 && std::is_same_v<T, bf16_t>;
 #pragma unroll
@@ -262,7 +268,8 @@ __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void q8_de
     uint4 qf[D / 32];
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) qf[c] = qs[c * 64 + lane];
-    q8_attend<T, F, D>(cur, qf, o, m_run, l_run, a.scale_log2, pos.key0, pos.lo, pos.len_k, g);
+    q8_attend<T, F, D, KS, true>(cur, qf, o, m_run, l_run, a.scale_log2, pos.key0, pos.lo,
+                                 pos.len_k, g);
     if (!same_piece) {
       const uint32_t seg = pos.seq * a.kvh + pos.kh;
       if (lane == 0) {
@@ -353,7 +360,7 @@ __global__ __launch_bounds__(64 * q8_small_waves<D>(), 1) void q8_decode_small(
       const bool more = s0 + KS * W < key_end;
       if (more) p.key0 += KS * W;
       q8_load<D, kPad, true, KS>(next, a, sc, table, p, col, g);
-      q8_attend<T, F, D, KS>(cur, qf, o, m_run, l_run, a.scale_log2, s0, p.lo, p.len_k, g);
+      q8_attend<T, F, D, KS, false>(cur, qf, o, m_run, l_run, a.scale_log2, s0, p.lo, p.len_k, g);
       return more;
     };
     while (step(stA, stB) && step(stB, stA)) {
