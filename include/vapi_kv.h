@@ -597,14 +597,16 @@ int vapi_kv_q8_gather(const vapi_kv_q8_pool* pool, uint32_t layer, const uint32_
  * values the codes stand for, computed in the pool's dtype on matrix cores
  * with f32 sums and probabilities rounded to that dtype as for a 16-bit pool (the
  * same rounding whatever the decode's shares, which change f32 sums only). Same
- * arguments (q and out of the pool's dtype), same flags, same meaning of prefill_seqs, same rules for
- * the workspace (zero-fill it once; one per stream; calls sharing one must
- * not overlap), except that prefill_seqs == NULL with n_prefill == 0 and
- * max_seqlen_q > 1 covers every sequence, and that a call with prefill rows
- * needs the whole size that _workspace_size returns: their codes are
- * expanded there once, n_prefill * max_seqlen_k keys of the layer in the
- * pool's dtype. n_prefill is the list's length, or batch where every sequence
- * is covered: without a list, and with VAPI_ATTN_NO_DECODE_ROWS, which ignores it.
+ * arguments (q and out of the pool's dtype), same flags, same meaning of
+ * prefill_seqs, same rules for the workspace (zero-fill it once; one per stream;
+ * calls sharing one must not overlap), except that prefill_seqs == NULL with
+ * n_prefill == 0 and max_seqlen_q > 1 covers every sequence, and that a call with
+ * prefill rows needs the whole size that _workspace_size returns: their codes are
+ * expanded there once, n_prefill * max_seqlen_k keys of the layer in the pool's
+ * dtype (134 MB a listed sequence of 8 kv heads of 128 where the longest has 32,768
+ * keys, however short it is itself). n_prefill is the list's length, or batch where
+ * every sequence is covered: without a list, and with VAPI_ATTN_NO_DECODE_ROWS,
+ * which ignores it.
  * Groups of up to 256 query heads per kv head. _workspace_size is 0 where the call
  * would be refused for its pool, heads or lengths (vapi_kv_last_error says why).
  */

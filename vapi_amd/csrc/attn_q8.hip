@@ -176,7 +176,8 @@ __device__ __forceinline__ void q8_attend(const Q8Step<D, KS>& st, const uint4 (
   }
 }
 
-// The stream: decode_stream_body's plan and pieces over 8-bit steps.
+// The stream: decode_stream_body's plan and pieces over 8-bit steps. (The plan is
+// written out here, without the fused append: what changes there changes here.)
 template <typename T, int F, int D, bool kPad, bool kNt>
 __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void q8_decode_stream(
     AttnArgs a, Q8Scales sc, const uint32_t* __restrict__ cu_q, const uint32_t* __restrict__ cu_k,

@@ -21,7 +21,7 @@ struct EvictArgs {
   float* out;  // null: weights are not wanted
   const uint32_t *in_index, *out_index, *lens;
   uint64_t in_row, in_head, out_row, out_head;
-  uint32_t in_rows, out_rows, in_width, out_width;
+  uint32_t in_rows, out_rows, out_width;
   int32_t* kept;
   uint32_t kvh, max_len, max_keep, budget, sinks, recent;
 };
@@ -393,7 +393,7 @@ static void launch_evict_select(const EvictCall& c, uint32_t kvh, hipStream_t s)
   EvictArgs a{};
   a.in = c.in->data, a.in_index = c.in->index;
   a.in_row = c.in->row_stride, a.in_head = c.in->head_stride;
-  a.in_rows = c.in->rows, a.in_width = c.in->width;
+  a.in_rows = c.in->rows;
   if (c.out) {
     a.out = c.out->data, a.out_index = c.out->index;
     a.out_row = c.out->row_stride, a.out_head = c.out->head_stride;

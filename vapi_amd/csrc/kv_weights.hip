@@ -20,9 +20,13 @@
 // is a sum over them (weights_stored).
 //
 // What bounds it. Single tokens: HBM, K once (129 MB in 31 us, 4.2 TB/s, of 37 us
-// with pass 2). Many rows: issue, an exponential and ~5 operations a score in each
-// pass beside 1/16 of an MFMA, from two to three waves a SIMD: three fresh prompts
-// of 700-2,000 tokens (32 q / 8 kv heads, f16; 30 GFLOP of scores) 56 + 54 + 6 us.
+// with pass 2). Many rows: three fresh prompts of 700-2,000 tokens (32 q / 8 kv
+// heads, f16; 30 GFLOP of scores) take 56 + 54 + 6 us. By the counters the vector
+// units issue in 59% of a SIMD's busy time in pass 1 and 62% in pass 2 (about 7
+// instructions a score, an exponential among them) and the matrix cores are busy in
+// 25% and 29%; a wave issues in 38 and 40% of its life and waits for results in 36
+// and 34%, which the 2.7 and 2.5 waves a SIMD do not cover. So half is vector work,
+// and the rest waits that more waves would hide, had they registers.
 // Few rows over long contexts: latency, ~4 us of dependent loads before a workgroup's
 // first product in each pass (a prompt's last 32 queries over 6,500 keys, 28 q / 4
 // kv heads: 16 + 12 + 4 us).
@@ -267,8 +271,9 @@ __global__ __launch_bounds__(64 * kWeightWaves) void weights_lse(WeightArgs a) {
   constexpr int ST = weight_step<F, D, MT>();
   __shared__ float2 part[kWeightWaves][16 * MT];
   __shared__ uint32x4 stage[kWeightWaves][ST][16 * WeightTile<F, D>::kPieces];
-  // (Chunk by chunk the sequences are turned by five: otherwise all chunks of a
-  // long one land on the same CUs. 16 sequences of 256-8,192 keys 41.3 -> 37.3.)
+  // (Chunk by chunk the sequences are turned by five, which has no factor in common
+  // with the usual batches: otherwise all chunks of a long one land on the same CUs.
+  // 16 sequences of 256-8,192 keys 41.3 -> 37.3, the one batch measured.)
   const uint32_t turn = (uint32_t)((uint64_t)(5 * a.kvh) * blockIdx.y % gridDim.x);
   const uint32_t seg = (blockIdx.x + turn) % gridDim.x;
   const WeightSeg s = weight_seg(a, seg);
@@ -432,7 +437,8 @@ __device__ __forceinline__ float weight_join(const float2* ml, uint32_t n) {
 constexpr uint32_t kWeightJoinRows = 512;  // rows whose lse a workgroup holds in LDS
 // 16-key tiles a wave of pass 2 holds. More of them read Q less often, fewer leave
 // registers for more waves: three fresh prompts (above) 55.8 / 53.5 / 66.9 us at 2 /
-// 3 / 4, a prompt's last 32 queries 13.8 / 12.0 / 16.2.
+// 3 / 4, a prompt's last 32 queries 13.8 / 12.0 / 16.2. (Measured at head_dim 128;
+// the other sizes take the same.)
 constexpr int kWeightKt = 3;
 constexpr uint32_t kWeightBlock = 64;       // rows whose Q a workgroup of pass 2 stages
 
@@ -633,7 +639,7 @@ __global__ __launch_bounds__(256) void weights_add(WeightArgs a, uint32_t parts)
   weight_write(a, a.w + s.state_row * a.row_stride + s.h * a.head_stride + at, x);
 }
 
-// Pass 2 over stored scores. Grid: (keys / 1,024, segments); a thread sums four
+// Pass 2 over stored scores. Grid: (segments, keys / 1,024); a thread sums four
 // keys over the segment's rows (at most 16).
 __global__ __launch_bounds__(64 * kWeightWaves) void weights_stored(WeightArgs a) {
   __shared__ float lse[16];
