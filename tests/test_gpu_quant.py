@@ -11,6 +11,7 @@ from vapi_amd.backend import KvBlockBackend
 from vapi_amd.cache import (PagedKvCache, gather_kv, scatter_index, write_kv_to_cache,
                             write_rows_indexed)
 from vapi_amd.quant import QuantKvCache
+from vapi_amd.spill import SpillStore, pinned_buffer, promote, spill_evicted
 
 pytestmark = pytest.mark.gpu
 
@@ -544,3 +545,37 @@ def test_shares_change_no_more_than_f32_sums(fmt, dtype):
         again = paged_attention_prepared(q, cache, 0, prep, 0.05)
         assert float((again != first).double().mean()) < 0.05
         assert torch.all((again.cpu().double() - want).abs() <= bound)
+
+
+@pytest.mark.parametrize("layout,fmt,kvh", [("HND", "e4m3", 3), ("NHD", "int8", 20)])
+def test_blocks_swap_and_come_back_from_the_store(layout, fmt, kvh):
+    """Codes and scales through pinned host memory and through the spill tier."""
+    cache, tables = filled([100], kvh, 64, 16, fmt, BF16, layout, 2, layers=2, spare=20)
+    be, table = KvBlockBackend(cache), tables[0]
+    free = [b for b in range(cache.num_blocks) if b not in table]
+    q = torch.randn(1, kvh * 2, 64, device="cuda").to(BF16)
+    want = paged_attention(q, cache, 1, batch_of([1], [100], tables), 0.1)
+
+    def dev(ids):
+        return torch.tensor(ids, dtype=torch.int32, device="cuda")
+
+    def same_over(ids):
+        assert torch.equal(paged_attention(q, cache, 1, batch_of([1], [100], [ids]), 0.1), want)
+
+    n = len(table)
+    size, back = n * cache.block_bytes(), free[:n]
+    host = torch.empty(size, dtype=torch.uint8, pin_memory=True)
+    staging = torch.empty(size, dtype=torch.uint8, device="cuda")
+    be.swap_out(dev(table), host, staging)
+    be.swap_in(dev(back), host, staging)
+    same_over(back)
+    store, pinned = SpillStore(None, 1 << 24, 0), pinned_buffer(cache, 3)
+    hashes = [bytes([i]) * 32 for i in range(n)]
+    assert spill_evicted(store, cache, zip(hashes, table), pinned) == n
+    cache._codes.fill_(0x11)  # the blocks' next users
+    cache._scales.fill_(3.0)
+    back = free[n:2 * n]
+    assert promote(store, cache, hashes, back, pinned) == n
+    torch.cuda.synchronize()
+    same_over(back)
+    store.close()
