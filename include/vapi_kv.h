@@ -309,6 +309,39 @@ int vapi_paged_attention_prepared(const vapi_kv_pool* pool, uint32_t layer, cons
                                   vapi_stream_t stream);
 
 /*
+ * vapi_paged_attention_prepared with sinks: the first `sinks` keys of a sequence
+ * stay visible behind its left window. Key k is visible to the query at position p
+ * iff (window_right < 0 or k <= p + window_right) and (window_left < 0 or
+ * k >= p - window_left or k < sinks); sinks = 0 is vapi_paged_attention_prepared,
+ * and without a left window sinks change nothing. Any pool that
+ * vapi_paged_attention takes, the same workspace, the same flags; prefill_seqs ==
+ * NULL with n_prefill == 0 covers every sequence. Keys between the sinks and the
+ * windows of a step's queries are not read (up to the 31 next to either), so their
+ * blocks may be given to others (the table's entries then name any block), and what
+ * V holds where no query of a sequence looks does not reach the output. No counterpart in the
+ * reference, whose windows hide all that lies before them (attention.rs:179-194).
+ */
+int vapi_paged_attention_sinks(const vapi_kv_pool* pool, uint32_t layer, const void* q, void* out,
+                               const uint32_t* cu_seqlens_q, const uint32_t* cu_seqlens_k,
+                               const uint32_t* block_table, uint32_t batch, uint32_t max_blocks,
+                               uint32_t max_seqlen_q, uint32_t max_seqlen_k, uint32_t num_heads,
+                               float scale, int32_t window_left, int32_t window_right,
+                               uint32_t sinks, uint32_t flags, const uint32_t* prefill_seqs,
+                               uint32_t n_prefill, void* workspace, size_t workspace_bytes,
+                               vapi_stream_t stream);
+
+/* vapi_kv_append and then vapi_paged_attention_sinks; a call that either refuses
+ * writes nothing. */
+int vapi_paged_attention_append_sinks(
+    const vapi_kv_pool* pool, uint32_t layer, const void* k_src, const void* v_src,
+    const uint32_t* slot_mapping, uint32_t n_tokens, const void* q, void* out,
+    const uint32_t* cu_seqlens_q, const uint32_t* cu_seqlens_k, const uint32_t* block_table,
+    uint32_t batch, uint32_t max_blocks, uint32_t max_seqlen_q, uint32_t max_seqlen_k,
+    uint32_t num_heads, float scale, int32_t window_left, int32_t window_right, uint32_t sinks,
+    uint32_t flags, const uint32_t* prefill_seqs, uint32_t n_prefill, void* workspace,
+    size_t workspace_bytes, vapi_stream_t stream);
+
+/*
  * vapi_paged_attention_ex without a workspace argument, for callers that
  * cannot allocate device memory (code under HIP graph capture, tight
  * serving loops, harnesses that forbid hipMalloc). No counterpart in the
@@ -620,6 +653,16 @@ int vapi_kv_q8_attention(const vapi_kv_q8_pool* pool, uint32_t layer, const void
                          float scale, int32_t window_left, int32_t window_right, uint32_t flags,
                          const uint32_t* prefill_seqs, uint32_t n_prefill, void* workspace,
                          size_t workspace_bytes, vapi_stream_t stream);
+
+/* vapi_kv_q8_attention with sinks (see vapi_paged_attention_sinks). */
+int vapi_kv_q8_attention_sinks(const vapi_kv_q8_pool* pool, uint32_t layer, const void* q,
+                               void* out, const uint32_t* cu_seqlens_q,
+                               const uint32_t* cu_seqlens_k, const uint32_t* block_table,
+                               uint32_t batch, uint32_t max_blocks, uint32_t max_seqlen_q,
+                               uint32_t max_seqlen_k, uint32_t num_heads, float scale,
+                               int32_t window_left, int32_t window_right, uint32_t sinks,
+                               uint32_t flags, const uint32_t* prefill_seqs, uint32_t n_prefill,
+                               void* workspace, size_t workspace_bytes, vapi_stream_t stream);
 
 /* ---- attention weights and eviction ---------------------------------------- */
 

@@ -41,6 +41,8 @@ EXPORTS = (
     "vapi_paged_attention_prepared", "vapi_paged_attention_prepared_workspace_size",
     "vapi_kv_q8_append", "vapi_kv_q8_gather", "vapi_kv_q8_attention",
     "vapi_kv_q8_attention_workspace_size",
+    "vapi_paged_attention_sinks", "vapi_paged_attention_append_sinks",
+    "vapi_kv_q8_attention_sinks",
     "vapi_kv_attention_weights", "vapi_kv_attention_weights_workspace_size",
     "vapi_kv_q8_attention_weights", "vapi_kv_evict", "vapi_kv_q8_evict",
 )
@@ -193,6 +195,11 @@ def lib():
     L.vapi_kv_q8_attention.argtypes = [
         _q8p, _u32, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32,
         ctypes.c_float, _i32, _i32, _u32, _vp, _u32, _vp, _sz, _vp]
+    sinks = [_u32, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, ctypes.c_float, _i32,
+             _i32, _u32, _u32, _vp, _u32, _vp, _sz, _vp]
+    L.vapi_paged_attention_sinks.argtypes = [_poolp] + sinks
+    L.vapi_kv_q8_attention_sinks.argtypes = [_q8p] + sinks
+    L.vapi_paged_attention_append_sinks.argtypes = [_poolp, _u32, _vp, _vp, _vp] + sinks
     L.vapi_kv_attention_weights_workspace_size.argtypes = [_u32] * 7
     L.vapi_kv_attention_weights_workspace_size.restype = _sz
     weights = [_u32, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, ctypes.c_float, _i32,

@@ -235,16 +235,19 @@ def paged_attention_prepared(q: torch.Tensor, cache: PagedKvCache, layer: int,
                              prepared: PreparedAttention, softmax_scale: float,
                              window_size_left: int | None = None,
                              window_size_right: int | None = 0,
-                             out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+                             out: torch.Tensor | None = None, stream=None,
+                             sinks: int = 0) -> torch.Tensor:
     """attention.rs:262-288 on libvapi_kv.so. None for a window side means
     unlimited (flash convention); the default right window 0 is causal.
-    `cache` may be a HybridKvCache (`layer` then names one of its K/V layers)
+    `sinks`: a sequence's first keys that stay visible behind its left window
+    (vapi_paged_attention_sinks). `cache` may be a HybridKvCache (`layer` then names one of its K/V layers)
     or a QuantKvCache."""
     cache, layer = _per_layer(cache, layer)
     if q.dim() != 3 or q.shape[2] != cache.head_dim:
         raise ValueError(f"q must be (tokens, heads, {cache.head_dim}), got {tuple(q.shape)}")
     if q.dtype != cache.dtype:
         raise ValueError(f"q is {q.dtype} but the cache is {cache.dtype}")
+    sinks = sinks_arg(sinks)
     q = contiguous_on(stream, q)
     if out is None:
         out = empty_on(stream, q)
@@ -252,18 +255,23 @@ def paged_attention_prepared(q: torch.Tensor, cache: PagedKvCache, layer: int,
     num_heads = q.shape[1]
     max_q = max(int(prepared.max_seqlen_q), 1)
     max_k = max(int(prepared.max_seqlen_k), 1)
+    mask = (float(softmax_scale), -1 if window_size_left is None else int(window_size_left),
+            -1 if window_size_right is None else int(window_size_right))
+    mask += (sinks, prepared.flags) if sinks else (prepared.flags,)
     args = (cache.pool, layer, q.data_ptr(), out.data_ptr(), prepared.seqlens_q.data_ptr(),
             prepared.seqlens_k.data_ptr(), prepared.block_table.data_ptr(), b,
-            prepared.block_table.shape[1], max_q, max_k, num_heads, float(softmax_scale),
-            -1 if window_size_left is None else int(window_size_left),
-            -1 if window_size_right is None else int(window_size_right), prepared.flags)
+            prepared.block_table.shape[1], max_q, max_k, num_heads) + mask
     handle = stream_handle(stream)
+    if _is_quantised(cache) or sinks:
+        listed = prepared.prefill_seqs is not None
+        args += (prepared.prefill_seqs.data_ptr() if listed else None,
+                 prepared.n_prefill if listed else 0)
     if _is_quantised(cache):
         check_on_device(cache.k[0], q, out, prepared.block_table, prepared.seqlens_q)
-        listed = prepared.prefill_seqs is not None
-        args = (cache.q8,) + args[1:] + (prepared.prefill_seqs.data_ptr() if listed else None,
-                                         prepared.n_prefill if listed else 0)
-        fn = lib().vapi_kv_q8_attention
+        args = (cache.q8,) + args[1:]
+        fn = lib().vapi_kv_q8_attention_sinks if sinks else lib().vapi_kv_q8_attention
+    elif sinks:
+        fn = lib().vapi_paged_attention_sinks
     elif prepared.prefill_seqs is None:
         fn = lib().vapi_paged_attention_ex
     else:
@@ -276,21 +284,31 @@ def paged_attention_prepared(q: torch.Tensor, cache: PagedKvCache, layer: int,
     return out
 
 
+def sinks_arg(sinks) -> int:
+    """`sinks` as the library takes it (more than any position counts the same)."""
+    if int(sinks) < 0:
+        raise ValueError(f"{sinks} sinks")
+    return min(int(sinks), 1 << 30)
+
+
 def paged_attention_windowed(q, cache, layer, batch: ForwardBatch, softmax_scale,
-                             window_size_left=None, window_size_right=0, stream=None):
+                             window_size_left=None, window_size_right=0, stream=None,
+                             sinks: int = 0):
     """attention.rs:201-232."""
     prepared = PreparedAttention.from_batch(batch, q.device)
     return paged_attention_prepared(q, cache, layer, prepared, softmax_scale,
-                                    window_size_left, window_size_right, stream=stream)
+                                    window_size_left, window_size_right, stream=stream,
+                                    sinks=sinks)
 
 
 def paged_attention(q, cache, layer, batch: ForwardBatch, softmax_scale,
-                    sliding_window: int | None = None, stream=None):
+                    sliding_window: int | None = None, stream=None, sinks: int = 0):
     """paged_attention_cuda (attention.rs:170-195): causal, with an optional
-    sliding window w mapped to window_size_left = w - 1 (saturating)."""
+    sliding window w mapped to window_size_left = w - 1 (saturating), and the
+    first `sinks` keys visible behind it."""
     wl = None if sliding_window is None else max(int(sliding_window) - 1, 0)
     return paged_attention_windowed(q, cache, layer, batch, softmax_scale, wl, 0,
-                                    stream=stream)
+                                    stream=stream, sinks=sinks)
 
 
 def paged_attention_append_prepared(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -300,11 +318,11 @@ def paged_attention_append_prepared(q: torch.Tensor, k: torch.Tensor, v: torch.T
                                     window_size_left: int | None = None,
                                     window_size_right: int | None = 0,
                                     out: torch.Tensor | None = None,
-                                    stream=None) -> torch.Tensor:
+                                    stream=None, sinks: int = 0) -> torch.Tensor:
     """One layer's cache write and attention in one call (the pair of
     models/qwen.rs:371-391 and models/llama.rs:157-165): the same result as
     write_kv_to_cache(k, v, slot_mapping) then paged_attention_prepared(q),
-    in one launch pair fewer for decode batches.
+    in one launch pair fewer for decode batches without sinks.
 
     k, v: [n, num_kv_heads, head_dim] in the cache dtype; slot_mapping: a
     device u32 (int32 view) tensor of n slots.
@@ -320,6 +338,7 @@ def paged_attention_append_prepared(q: torch.Tensor, k: torch.Tensor, v: torch.T
                          f"got {tuple(k.shape)} and {tuple(v.shape)}")
     if slot_mapping.numel() != k.shape[0] or slot_mapping.element_size() != 4:
         raise ValueError("slot_mapping must hold one 32-bit slot per row")
+    sinks = sinks_arg(sinks)
     q, k, v = (contiguous_on(stream, t) for t in (q, k, v))
     if out is None:
         out = empty_on(stream, q)
@@ -342,8 +361,8 @@ def paged_attention_append_prepared(q: torch.Tensor, k: torch.Tensor, v: torch.T
         write_rows_indexed(cache, layer, k, v, slot_mapping, stream=stream)
         return paged_attention_prepared(q, cache, layer, prepared, softmax_scale,
                                         window_size_left, window_size_right, out=out,
-                                        stream=stream)
-    if max_q > 1 and prepared.prefill_seqs is not None and cache.pool.v:
+                                        stream=stream, sinks=sinks)
+    if max_q > 1 and prepared.prefill_seqs is not None and cache.pool.v and not sinks:
         # (A K-only pool goes to the library call below, which refuses it
         # before writing anything.)
         # A step with prefill rows is not fused (the library runs the append
@@ -359,8 +378,15 @@ def paged_attention_append_prepared(q: torch.Tensor, k: torch.Tensor, v: torch.T
             prepared.seqlens_k.data_ptr(), prepared.block_table.data_ptr(), b,
             prepared.block_table.shape[1], max_q, max_k, num_heads, float(softmax_scale),
             -1 if window_size_left is None else int(window_size_left),
-            -1 if window_size_right is None else int(window_size_right), prepared.flags)
+            -1 if window_size_right is None else int(window_size_right))
     handle, fn = stream_handle(stream), lib().vapi_paged_attention_append_ex
+    if sinks:
+        listed = prepared.prefill_seqs is not None
+        fn = lib().vapi_paged_attention_append_sinks
+        args += (sinks, prepared.flags, prepared.prefill_seqs.data_ptr() if listed else None,
+                 prepared.n_prefill if listed else 0)
+    else:
+        args += (prepared.flags,)
     _run(lambda ptr, size: fn(*args, ptr, size, handle), cache, prepared, b, num_heads, max_q,
          max_k, q.device, stream)
     return out

@@ -136,7 +136,7 @@ def build(verbose: bool = False) -> Path:
     libvapi_probe.so). Always rebuilds."""
     OBJ_DIR.mkdir(exist_ok=True)
     jobs = [(CSRC / n, OBJ_DIR / (Path(n).stem + ".o")) for n in SOURCES + PROBE_SOURCES]
-    with ThreadPoolExecutor(max_workers=min(len(jobs), 4)) as ex:
+    with ThreadPoolExecutor(max_workers=min(len(jobs), 6)) as ex:
         list(ex.map(lambda j: _compile(*j), jobs))
     _link([o for s, o in jobs if s.name in SOURCES], LIB)
     _link([o for s, o in jobs if s.name in PROBE_SOURCES], PROBE_LIB)

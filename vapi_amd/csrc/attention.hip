@@ -178,7 +178,8 @@ static int paged_attention_impl(const vapi_kv_pool* pool, uint32_t layer, const 
                                 int32_t window_left, int32_t window_right, void* workspace,
                                 size_t workspace_bytes, vapi_stream_t stream,
                                 const NewRows* fuse, uint32_t flags,
-                                const PrefillSeqs* pf = nullptr);
+                                const PrefillSeqs* pf = nullptr, uint32_t sinks = 0,
+                                bool checks_only = false);
 
 // The workspace a call cannot run without: the decode's (unless the call
 // launches no decode kernel) or the VALU kernel's split partials.
@@ -264,6 +265,53 @@ int vapi_paged_attention_prepared(const vapi_kv_pool* pool, uint32_t layer, cons
                               batch, max_blocks, max_seqlen_q, max_seqlen_k, num_heads, scale,
                               window_left, window_right, workspace, workspace_bytes, stream,
                               nullptr, flags, &pf);
+}
+
+int vapi_paged_attention_sinks(const vapi_kv_pool* pool, uint32_t layer, const void* q, void* out,
+                               const uint32_t* cu_seqlens_q, const uint32_t* cu_seqlens_k,
+                               const uint32_t* block_table, uint32_t batch, uint32_t max_blocks,
+                               uint32_t max_seqlen_q, uint32_t max_seqlen_k, uint32_t num_heads,
+                               float scale, int32_t window_left, int32_t window_right,
+                               uint32_t sinks, uint32_t flags, const uint32_t* prefill_seqs,
+                               uint32_t n_prefill, void* workspace, size_t workspace_bytes,
+                               vapi_stream_t stream) {
+  if (n_prefill > batch)
+    VK_FAIL(VAPI_KV_EINVAL, "vapi_paged_attention_sinks: %u prefill sequences in a batch of %u",
+            n_prefill, batch);
+  if (n_prefill && !prefill_seqs)
+    VK_FAIL(VAPI_KV_EINVAL, "vapi_paged_attention_sinks: null prefill_seqs");
+  const PrefillSeqs pf{prefill_seqs, n_prefill};
+  return paged_attention_impl(pool, layer, q, out, cu_seqlens_q, cu_seqlens_k, block_table, batch,
+                              max_blocks, max_seqlen_q, max_seqlen_k, num_heads, scale,
+                              window_left, window_right, workspace, workspace_bytes, stream,
+                              nullptr, flags, prefill_seqs ? &pf : nullptr, sinks);
+}
+
+int vapi_paged_attention_append_sinks(
+    const vapi_kv_pool* pool, uint32_t layer, const void* k_src, const void* v_src,
+    const uint32_t* slot_mapping, uint32_t n_tokens, const void* q, void* out,
+    const uint32_t* cu_seqlens_q, const uint32_t* cu_seqlens_k, const uint32_t* block_table,
+    uint32_t batch, uint32_t max_blocks, uint32_t max_seqlen_q, uint32_t max_seqlen_k,
+    uint32_t num_heads, float scale, int32_t window_left, int32_t window_right, uint32_t sinks,
+    uint32_t flags, const uint32_t* prefill_seqs, uint32_t n_prefill, void* workspace,
+    size_t workspace_bytes, vapi_stream_t stream) {
+  const char* who = "vapi_paged_attention_append_sinks";
+  if (n_prefill > batch)
+    VK_FAIL(VAPI_KV_EINVAL, "%s: %u prefill sequences in a batch of %u", who, n_prefill, batch);
+  if (n_prefill && !prefill_seqs) VK_FAIL(VAPI_KV_EINVAL, "%s: null prefill_seqs", who);
+  // What the attention refuses is refused before the append is launched.
+  const PrefillSeqs pf{prefill_seqs, n_prefill};
+  if (int rc = paged_attention_impl(pool, layer, q, out, cu_seqlens_q, cu_seqlens_k, block_table,
+                                    batch, max_blocks, max_seqlen_q, max_seqlen_k, num_heads,
+                                    scale, window_left, window_right, workspace, workspace_bytes,
+                                    stream, nullptr, flags, prefill_seqs ? &pf : nullptr, sinks,
+                                    true))
+    return rc;
+  if (int rc = vapi_kv_append(pool, layer, k_src, v_src, slot_mapping, n_tokens, stream)) return rc;
+  return vapi_paged_attention_sinks(pool, layer, q, out, cu_seqlens_q, cu_seqlens_k, block_table,
+                                    batch, max_blocks, max_seqlen_q, max_seqlen_k, num_heads,
+                                    scale, window_left, window_right, sinks, flags, prefill_seqs,
+                                    n_prefill, workspace, workspace_bytes, stream);
 }
 
 int vapi_paged_attention(const vapi_kv_pool* pool, uint32_t layer,
@@ -388,7 +436,8 @@ static int paged_attention_impl(const vapi_kv_pool* pool, uint32_t layer, const 
                                 uint32_t max_seqlen_k, uint32_t num_heads, float scale,
                                 int32_t window_left, int32_t window_right, void* workspace,
                                 size_t workspace_bytes, vapi_stream_t stream,
-                                const NewRows* fuse, uint32_t flags, const PrefillSeqs* pf) {
+                                const NewRows* fuse, uint32_t flags, const PrefillSeqs* pf,
+                                uint32_t sinks, bool checks_only) {
   if (int rc = check_pool(pool, "vapi_paged_attention")) return rc;
   if (!pool->v) VK_FAIL(VAPI_KV_EINVAL, "vapi_paged_attention: a K-only pool has no V to attend over");
   if (layer >= pool->num_layers)
@@ -431,13 +480,24 @@ static int paged_attention_impl(const vapi_kv_pool* pool, uint32_t layer, const 
     VK_FAIL(VAPI_KV_EUNSUP, "vapi_paged_attention: prefill batch too large for one launch");
   if (f32_mfma_ok(pool, num_heads, max_seqlen_q, max_seqlen_k, batch) && max_seqlen_q > 1 &&
       prefill_f32_items(pf_n, pool->num_kv_heads, num_heads / pool->num_kv_heads,
-                        max_seqlen_q) > 0xFFFFFFFFull)
+                        max_seqlen_q) > (sinks ? 0x7FFFFFFFull : 0xFFFFFFFFull))
     VK_FAIL(VAPI_KV_EUNSUP, "vapi_paged_attention: prefill batch too large for one launch");
   const size_t need =
       required_workspace(pool, batch, num_heads, max_seqlen_q, max_seqlen_k, skip_decode);
   if (workspace_bytes < need || (need && !workspace))
     VK_FAIL(VAPI_KV_ESPACE, "vapi_paged_attention: workspace %zu bytes < %zu",
             workspace_bytes, need);
+  if (checks_only) {
+    if (mfma16_ok(pool, num_heads) ||
+        f32_mfma_ok(pool, num_heads, max_seqlen_q, max_seqlen_k, batch))
+      return 0;
+    if (pool->head_dim > 256 ||
+        generic_grid(batch, pool->num_kv_heads, num_heads / pool->num_kv_heads, max_seqlen_q,
+                     max_seqlen_k) > 0xFFFFFFFFull)
+      VK_FAIL(VAPI_KV_EUNSUP, "vapi_paged_attention: head_dim %u or batch %u too large",
+              pool->head_dim, batch);
+    return 0;
+  }
 
   const Geom g = make_geom(pool);
   LayerPtrs lp = layer_ptrs(pool, layer);
@@ -477,6 +537,7 @@ static int paged_attention_impl(const vapi_kv_pool* pool, uint32_t layer, const 
   a.q_sign = scale < 0.f ? 0x80008000u : 0u;
   a.wl = window_arg(window_left);
   a.wr = window_arg(window_right);
+  a.sinks = sinks_arg(sinks, a.wl);
   a.deterministic = (flags & VAPI_ATTN_DETERMINISTIC) ? 1u : 0u;
   a.pf_min_q = 2;
   a.pf_seqs = listed ? pf->seqs : nullptr;
@@ -526,7 +587,8 @@ static int paged_attention_impl(const vapi_kv_pool* pool, uint32_t layer, const 
       dec.num_waves = a.num_waves;
       // (The partials lie past the balance block, as the stream's.)
       const SmallPlan small =
-          decode_small_plan(batch, dec.kvh, dec.group, D, pool->dtype, max_seqlen_k, a.wl,
+          decode_small_plan(batch, dec.kvh, dec.group, D, pool->dtype, max_seqlen_k,
+                            row_window(a.wl, a.sinks),
                             need - kDecodeBalanceBytes);
       if (small.ok)
         launch_decode_small(dec, D, pool->dtype, small, (char*)workspace + kDecodeBalanceBytes, s);
@@ -547,7 +609,7 @@ static int paged_attention_impl(const vapi_kv_pool* pool, uint32_t layer, const 
       dec.num_waves = decode_num_waves();
       const SmallPlan small =
           decode_small_plan(batch, dec.kvh, dec.group, decode_dim(g.d), pool->dtype, max_seqlen_k,
-                            a.wl, need - kDecodeBalanceBytes);
+                            row_window(a.wl, a.sinks), need - kDecodeBalanceBytes);
       if (small.ok)
         launch_decode_small(dec, decode_dim(g.d), pool->dtype, small,
                             (char*)workspace + kDecodeBalanceBytes, s);
@@ -568,7 +630,7 @@ static int paged_attention_impl(const vapi_kv_pool* pool, uint32_t layer, const 
     SmallPlan small{false, 1};
     if (max_seqlen_q <= 1 && f32_shape_ok(pool, num_heads))
       small = decode_small_plan(batch, dec.kvh, dec.group, decode_dim(g.d), pool->dtype,
-                                max_seqlen_k, a.wl,
+                                max_seqlen_k, row_window(a.wl, a.sinks),
                                 need > kDecodeBalanceBytes ? need - kDecodeBalanceBytes : 0);
     if (small.ok) {
       launch_decode_small(dec, decode_dim(g.d), pool->dtype, small,

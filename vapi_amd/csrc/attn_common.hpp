@@ -9,7 +9,7 @@
 // to the input dtype. Masking follows the flash convention the reference's
 // CUDA path passes (attention.rs:179-194): key k is visible iff
 //   (window_right < 0 || k <= p + window_right) &&
-//   (window_left  < 0 || k >= p - window_left).
+//   (window_left  < 0 || k >= p - window_left || k < sinks).
 //
 // MFMA scheme (v_mfma_f32_16x16x32_{bf16,f16}; lane l: row/col = l%16,
 // k-group g = l/16 holding 8 consecutive k):
@@ -39,6 +39,14 @@ constexpr float kLog2e = 1.4426950408889634f;
 // A window as the kernels take it: -1 (unlimited), or up to 2^30, further than any
 // position lies from another (position + window stays in 32 bits).
 inline int32_t window_arg(int32_t w) { return w < 0 ? -1 : w < (1 << 30) ? w : 1 << 30; }
+// The first keys that a left window does not hide (none without one: all are visible).
+inline int32_t sinks_arg(uint32_t sinks, int32_t wl) {
+  return wl < 0 ? 0 : (int32_t)std::min(sinks, 1u << 30);
+}
+// A window as wide as what a decode row sees of it and of the sinks (whole steps).
+inline int32_t row_window(int32_t wl, int32_t sinks) {
+  return wl < 0 || !sinks ? wl : std::min<int32_t>(wl + std::min(sinks, 1 << 29) + 64, 1 << 30);
+}
 constexpr float kNegBig = -1e30f;  // running-max start: finite, so exp2 never sees inf-inf
 constexpr float kRescaleSlack = 8.0f;  // log2 units the running max may lag by
 
@@ -69,6 +77,7 @@ struct AttnArgs {
   float scale;
   uint32_t q_sign;     // 0x80008000 when scale < 0: XOR into packed 16-bit Q words
   int32_t wl, wr;
+  int32_t sinks;  // first keys that wl does not hide (0 without a left window)
   uint32_t deterministic;  // decode: fixed equal XCD shares, no share update
   uint32_t pf_min_q;       // prefill: rows with len_q >= this (2, or 1 when no decode launch)
   // prefill: the sequences its grid covers, u32[pf_seqs_n] (null: 0 ..
@@ -686,20 +695,53 @@ __device__ __forceinline__ floatx4 mfma16x16x4f32(float a, float b, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// K and V of the 16-key tile at s0 + 16 tt (keys past `last` re-read it).
+// What a tile of rows reads of its steps: keys hidden from all of them re-read one
+// that is visible (their zero weights then meet values that count anyway). Sinks'
+// steps (positions before ks.hop) hold keys [0, sinks), the window's [klo, khi];
+// `hole` is klo where sinks end in the window's first step, else 0.
+struct KeyReads {
+  int32_t first, last, hole, sinks;
+  __device__ __forceinline__ KeyReads(const KeySteps<true>& ks, int32_t at, int32_t klo, int32_t khi,
+                                      int32_t sinks_)
+      : sinks(sinks_) {
+    const bool sink = at < ks.hop, mid = sinks > (klo & ~31);
+    first = sink || mid ? 0 : klo;
+    last = sink ? min(sinks - 1, khi) : khi;
+    hole = mid ? klo : 0;
+  }
+  // The 16-key tile read for the one at s, and the row of it for row r.
+  __device__ __forceinline__ int32_t tile(int32_t s) const {
+    return max(min(s, last & ~15), first & ~15);
+  }
+  __device__ __forceinline__ uint32_t row(int32_t r, int32_t ts) const {
+    int32_t k = max(min(r, last - ts), first - ts);
+    if (hole && ts + k >= sinks && ts + k < hole) k = (ts < sinks ? sinks - 1 : hole) - ts;
+    return (uint32_t)k;
+  }
+};
+// The same for one row's decode, which masks hidden keys' V itself.
+struct RowReads {
+  int32_t last;
+  __device__ __forceinline__ int32_t tile(int32_t s) const { return min(s, last & ~15); }
+  __device__ __forceinline__ uint32_t row(int32_t r, int32_t ts) const {
+    return (uint32_t)min(r, last - ts);
+  }
+};
+
+// K and V of the 16-key tile at s0 + 16 tt (`rd`: what is read for hidden keys).
 // kStream: streaming loads (the decode reads each byte once); the prefill's
 // waves share a kv head's K/V through L2 and load them the ordinary way.
 // CL: the 16-column chunks of K that are loaded (fewer than D / 16 when the
 // rest are padding; those stay as they were).
-template <int D, bool kStream = true, bool kPad = false, int CL = D / 16>
+template <int D, bool kStream = true, bool kPad = false, int CL = D / 16, typename Reads>
 __device__ __forceinline__ void load_half_f32(KHalfF32<D>& kt, VHalfF32<D>& vt,
                                               const uint32_t* __restrict__ tab, const float* kb,
                                               const float* vb, const AttnArgs& a, int32_t s0,
-                                              int tt, int32_t last, uint32_t col, uint32_t g) {
-  const int32_t ts = min(s0 + 16 * tt, last & ~15);
-  const int32_t lim = last - ts;
-  const char* kp = tile_base(tab, kb, a, ts) +
-                   ((uint32_t)min((int32_t)col, lim) * a.tok_e + 4 * g) * sizeof(float);
+                                              int tt, const Reads& rd, uint32_t col,
+                                              uint32_t g) {
+  const int32_t ts = rd.tile(s0 + 16 * tt);
+  const char* kp =
+      tile_base(tab, kb, a, ts) + (rd.row((int32_t)col, ts) * a.tok_e + 4 * g) * sizeof(float);
   const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
   for (int c = 0; c < CL; ++c)
@@ -710,7 +752,7 @@ __device__ __forceinline__ void load_half_f32(KHalfF32<D>& kt, VHalfF32<D>& vt,
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const char* row =
-        vp + ((uint32_t)min((int32_t)(4 * g + i), lim) * a.tok_e + 4 * col) * sizeof(float);
+        vp + (rd.row((int32_t)(4 * g + i), ts) * a.tok_e + 4 * col) * sizeof(float);
 #pragma unroll
     for (int h = 0; h < D / 64; ++h)
       vt.v[i][h] = kPad && 64 * h + 4 * col >= a.hd ? z

@@ -3,12 +3,13 @@
 
 namespace vk {
 
-template <typename T, int D, bool kFuse, bool kPad = false, int DL = D / 16, bool kNt = true>
+template <typename T, int D, bool kFuse, bool kPad = false, int DL = D / 16, bool kNt = true,
+          bool kSinks = false>
 __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void paged_decode_stream(
     AttnArgs a, const uint32_t* __restrict__ cu_q, const uint32_t* __restrict__ cu_k,
     const uint32_t* __restrict__ table) {
   extern __shared__ uint32_t P[];
-  decode_stream_body<T, D, kFuse, kPad, DL, kNt>(a, cu_q, cu_k, table, P, blockIdx.x,
+  decode_stream_body<T, D, kFuse, kPad, DL, kNt, kSinks>(a, cu_q, cu_k, table, P, blockIdx.x,
                                                  gridDim.x);
 }
 
@@ -19,6 +20,16 @@ __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void paged
 // and 74.0 us); every other call with streaming loads.
 template <typename T, int D, bool F, bool PAD, int DL>
 static void launch_stream(const AttnArgs& c, uint32_t nwg, size_t lds, hipStream_t s) {
+  // Sinks (no fused append): all d tiles live.
+  if constexpr (!F) {
+    if (c.sinks) {
+      constexpr auto once = paged_decode_stream<T, D, false, PAD, D / 16, true, true>;
+      constexpr auto shared = paged_decode_stream<T, D, false, PAD, D / 16, false, true>;
+      hipLaunchKernelGGL(c.kv_parts.d > 1 ? shared : once, dim3(nwg),
+                         dim3(64 * kDecodeWavesPerWG), lds, s, c, c.cu_q, c.cu_k, c.table);
+      return;
+    }
+  }
   if constexpr (!F && DL == D / 16) {
     if (c.kv_parts.d > 1) {
       hipLaunchKernelGGL((paged_decode_stream<T, D, F, PAD, DL, false>), dim3(nwg),

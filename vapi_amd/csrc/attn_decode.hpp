@@ -62,7 +62,7 @@ constexpr uint32_t kStatWords = 4;
 
 // Steps of sequence s (0 for rows that are not decode rows). KS: keys per step
 // (a power of two; 32 but for the streams of 8-bit pools).
-template <int KS = 32>
+template <int KS = 32, bool kSinks = false>
 __device__ __forceinline__ uint32_t decode_steps(const AttnArgs& a,
                                                  const uint32_t* __restrict__ cu_q,
                                                  const uint32_t* __restrict__ cu_k, uint32_t s) {
@@ -70,7 +70,23 @@ __device__ __forceinline__ uint32_t decode_steps(const AttnArgs& a,
   const int32_t len_k = (int32_t)(cu_k[s + 1] - cu_k[s]);
   if (len_k <= 0) return 0;
   const int32_t lo = a.wl >= 0 ? max(0, len_k - 1 - a.wl) : 0;
-  return (uint32_t)(len_k - (lo & ~(KS - 1)) + KS - 1) / KS;
+  const KeySteps<kSinks> ks(lo, len_k - 1, a.sinks, KS);
+  return (uint32_t)(ks.last - ks.start) / KS + 1;
+}
+
+// Whether a row with window start lo and len_k keys sees `key`: [sinks, lo) is the
+// hole between its sinks and its window.
+template <bool kSinks>
+__device__ __forceinline__ bool row_sees(int32_t key, int32_t lo, int32_t len_k, int32_t sinks) {
+  if constexpr (!kSinks) return key >= lo && key < len_k;
+  return (uint32_t)(key - sinks) >= (uint32_t)max(lo - sinks, 0) && key < len_k;
+}
+
+// The step after the one at key0: from the sinks' last on to the window's first.
+template <bool kSinks, int KS = 32>
+__device__ __forceinline__ int32_t next_step(int32_t key0, int32_t lo, int32_t sinks) {
+  const int32_t k = key0 + KS;
+  return kSinks && k >= sinks ? max(k, lo & ~(KS - 1)) : k;
 }
 
 // Fused append: whether decode row s's new key (position len_k - 1) comes
@@ -136,7 +152,7 @@ struct DecodePos {
 // kvh_plan: the kv heads the step order counts (a.kvh, or with a split
 // group's parts side by side the pool heads: then the position is part
 // `part` of pool head kp, virtual head kp * n + part).
-template <int KS = 32>
+template <int KS = 32, bool kSinks = false>
 __device__ __forceinline__ DecodePos locate(const AttnArgs& a, const uint32_t* __restrict__ cu_q,
                                             const uint32_t* __restrict__ cu_k, const uint32_t* P,
                                             const uint32_t* FZ, uint32_t t,
@@ -158,7 +174,8 @@ __device__ __forceinline__ DecodePos locate(const AttnArgs& a, const uint32_t* _
   p.q0 = cu_q[p.seq];
   p.len_k = (int32_t)(cu_k[p.seq + 1] - cu_k[p.seq]);
   p.lo = a.wl >= 0 ? max(0, p.len_k - 1 - a.wl) : 0;
-  p.key0 = (p.lo & ~(KS - 1)) + KS * (int32_t)ks;
+  const KeySteps<kSinks> steps(p.lo, p.len_k - 1, a.sinks, KS);
+  p.key0 = steps.key(steps.start + KS * (int32_t)ks);
   p.seg_first = ks == 0;
   p.fuse = FZ ? FZ[lo_i] : 0u;
   return p;
@@ -168,7 +185,7 @@ __device__ __forceinline__ DecodePos locate(const AttnArgs& a, const uint32_t* _
 // or kv head 0 of the next sequence that has decode steps. A wave's slice
 // is contiguous, so the step after a segment's last is always this one,
 // and a wave that moves on from a finished segment needs no search.
-template <int KS = 32>
+template <int KS = 32, bool kSinks = false>
 __device__ __forceinline__ DecodePos next_segment(const AttnArgs& a,
                                                   const uint32_t* __restrict__ cu_q,
                                                   const uint32_t* __restrict__ cu_k,
@@ -190,7 +207,7 @@ __device__ __forceinline__ DecodePos next_segment(const AttnArgs& a,
     p.lo = a.wl >= 0 ? max(0, p.len_k - 1 - a.wl) : 0;
     p.fuse = FZ ? FZ[s] : 0u;
   }
-  p.key0 = p.lo & ~(KS - 1);
+  p.key0 = kSinks ? 0 : p.lo & ~(KS - 1);
   p.seg_first = 1u;
   return p;
 }
@@ -314,7 +331,9 @@ __device__ __forceinline__ void flush_piece(const AttnArgs& a, const DecodePos& 
 // loads; ordinary ones for a group split into virtual kv heads, whose
 // parts read the same tiles at about the same time on one XCD (the plan
 // puts a pool head's parts side by side), so all but the first hit in L2.
-template <typename T, int D, bool kFuse, bool kPad = false, int DL = D / 16, bool kNt = true>
+// kSinks: a.sinks keys (at least one) before the left window.
+template <typename T, int D, bool kFuse, bool kPad = false, int DL = D / 16, bool kNt = true,
+          bool kSinks = false>
 __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
                                                    const uint32_t* __restrict__ cu_q,
                                                    const uint32_t* __restrict__ cu_k,
@@ -342,7 +361,7 @@ __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
     const uint32_t per = (B + NT - 1) / NT;
     const uint32_t b0 = min(tid * per, B), b1 = min(b0 + per, B);
     uint32_t sum = 0;
-    for (uint32_t s = b0; s < b1; ++s) sum += decode_steps(a, cu_q, cu_k, s) * kvh_plan;
+    for (uint32_t s = b0; s < b1; ++s) sum += decode_steps<32, kSinks>(a, cu_q, cu_k, s) * kvh_plan;
     uint32_t inc = sum;  // inclusive scan within the wave
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -355,7 +374,7 @@ __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
     for (uint32_t w = 0; w < wave; ++w) run += wave_tot[w];
     for (uint32_t s = b0; s < b1; ++s) {
       P[s] = run;
-      const uint32_t ns = decode_steps(a, cu_q, cu_k, s);
+      const uint32_t ns = decode_steps<32, kSinks>(a, cu_q, cu_k, s);
       run += ns * kvh_plan;
       if (kFuse) FZ[s] = ns ? fused_row(a, cu_q, cu_k, table, s) : 0u;
     }
@@ -397,7 +416,7 @@ __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
 
   uint32_t t = t_begin;
   const uint32_t col = lane & 15, g = lane >> 4;
-  DecodePos pos = locate(a, cu_q, cu_k, P, FZ, t, kvh_plan, n_parts, part);
+  DecodePos pos = locate<32, kSinks>(a, cu_q, cu_k, P, FZ, t, kvh_plan, n_parts, part);
   // The Q^T operand of the current segment lives in LDS (read back every
   // step) to keep the K/V buffers in registers.
   constexpr bool kF32 = sizeof(T) == 4;
@@ -424,8 +443,7 @@ __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
       __attribute__((always_inline)) {
     load_half_f32<D, kNt, kPad, DL>(kt.h[tt], vt.h[tt], table + (uint64_t)p.seq * a.max_blocks,
                      kbf + a.kv_parts.div(p.kh) * a.head_e, vbf + a.kv_parts.div(p.kh) * a.head_e,
-                     a, p.key0, tt, p.len_k - 1,
-                     col, g);
+                     a, p.key0, tt, RowReads{p.len_k - 1}, col, g);
   };
   if constexpr (kF32) {
     load_halves(kA, vA, pos, 0);
@@ -451,10 +469,10 @@ __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
     // and hold the wave's end for a memory round trip.
     DecodePos nxt = pos;
     if (same_piece) {
-      nxt.key0 += 32;
+      nxt.key0 = next_step<kSinks>(pos.key0, pos.lo, a.sinks);
       nxt.seg_first = false;
     } else if (more) {
-      nxt = next_segment(a, cu_q, cu_k, P, FZ, pos, n_parts);
+      nxt = next_segment<32, kSinks>(a, cu_q, cu_k, P, FZ, pos, n_parts);
     } else {
       nxt.seq = 0;
       nxt.key0 = 0;
@@ -474,9 +492,17 @@ __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
       }
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt) {
+        if (kSinks && key0 < lo) {  // (see below)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!row_sees<kSinks>(key0 + 16 * tt + 4 * (int32_t)g + i, lo, len_k, a.sinks))
+#pragma unroll
+              for (int h = 0; h < D / 64; ++h)
+                vc.h[tt].v[i][h] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
         attend_half_f32<D, DL>(kc.h[tt], vc.h[tt], qf, o, m_run, l_run, a.scale_log2, [&](int i) {
           const int32_t key = key0 + 16 * tt + 4 * (int32_t)g + i;
-          return key >= lo && key < len_k;
+          return row_sees<kSinks>(key, lo, len_k, a.sinks);
         });
         load_halves(kn, vn, nxt, tt);
       }
@@ -488,8 +514,17 @@ __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
       for (int c = 0; c < D / 32; ++c) qf[c] = qs[c * 64 + lane];
       const uint4 pf = attend_qk<T, D, KCL>(kc, qf, o, m_run, l_run, a.scale_log2, g, [&](int tt, int i) {
         const int32_t key = key0 + 16 * tt + 4 * (int32_t)g + i;
-        return key >= lo && key < len_k;
+        return row_sees<kSinks>(key, lo, len_k, a.sinks);
       });
+      // Between the sinks and the window keys weigh 0, whatever their V holds
+      // (infinities too).
+      if (kSinks && key0 < lo) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (!row_sees<kSinks>(key0 + 16 * (j >> 2) + 4 * (int32_t)g + (j & 3), lo, len_k, a.sinks))
+#pragma unroll
+            for (int w = 0; w < DPL / 2; ++w) vc.v[j].w[w] = 0u;
+      }
       attend_pv<T, D>(vc, pf, o);
     }
     if (!same_piece) {

@@ -90,7 +90,8 @@ __device__ __forceinline__ void attend_half_v2(const KHalfF32<D>& kt, const VHal
 // where f32 MFMAs would spend 14 of their 16 columns on padding (4,096 cycles
 // a step against ~1,300): 8 sequences of 82-401 keys, 16 q / 8 kv heads, with
 // their cache write 16.8 -> 13.5 us.
-template <typename T, int D, bool kFuse, bool kPad, bool kSplit, bool kV2 = false>
+template <typename T, int D, bool kFuse, bool kPad, bool kSplit, bool kV2 = false,
+          bool kSinks = false>
 __global__ __launch_bounds__(64 * kSmallWaves, 1) void paged_decode_small(
     AttnArgs a, const uint32_t* __restrict__ cu_q, const uint32_t* __restrict__ cu_k,
     const uint32_t* __restrict__ table, uint32_t n_wg, uint32_t n_split_arg) {
@@ -117,16 +118,16 @@ __global__ __launch_bounds__(64 * kSmallWaves, 1) void paged_decode_small(
   if (cu_q[p.seq + 1] - p.q0 != 1 || p.len_k <= 0) return;
   const int32_t lo = a.wl >= 0 ? max(0, p.len_k - 1 - a.wl) : 0, len_k = p.len_k;
   p.lo = lo;
-  // This workgroup's keys: all of the row's, or its split's whole steps.
-  const int32_t first = lo & ~31;
-  int32_t key_end = len_k;
-  p.key0 = first;
+  // This workgroup's steps: all of the row's, or its split's, by position.
+  const KeySteps<kSinks> ks(lo, len_k - 1, a.sinks, 32);
+  int32_t at = ks.start, end = ks.last + 32;
   if constexpr (kSplit) {
-    const uint32_t steps = (uint32_t)(len_k - first + 31) >> 5;
-    p.key0 = first + 32 * (int32_t)(split * steps / n_split);
-    key_end = min(len_k, first + 32 * (int32_t)((split + 1) * steps / n_split));
+    const uint32_t steps = (uint32_t)(end - at) >> 5;
+    end = at + 32 * (int32_t)((split + 1) * steps / n_split);
+    at += 32 * (int32_t)(split * steps / n_split);
   }
-  p.key0 += 32 * wave;
+  at += 32 * wave;
+  p.key0 = ks.key(at);
   p.fuse = 0;
   if constexpr (kFuse) {
     p.fuse = fused_row(a, cu_q, cu_k, table, p.seq);
@@ -154,8 +155,8 @@ __global__ __launch_bounds__(64 * kSmallWaves, 1) void paged_decode_small(
     }
     __syncthreads();
   }
-  if (p.key0 < key_end) {
-    auto visible = [&](int32_t key) { return key >= lo && key < len_k; };
+  if (at < end) {
+    auto visible = [&](int32_t key) { return row_sees<kSinks>(key, lo, len_k, a.sinks); };
     if constexpr (kF32) {
       const float* kb = (const float*)a.k + a.kv_parts.div(p.kh) * a.head_e;
       const float* vb = (const float*)a.v + a.kv_parts.div(p.kh) * a.head_e;
@@ -163,7 +164,8 @@ __global__ __launch_bounds__(64 * kSmallWaves, 1) void paged_decode_small(
       KTileF32<D> kt;
       VTileF32<D> vt;
       auto load = [&](int tt, int32_t s0) __attribute__((always_inline)) {
-        load_half_f32<D, true, kPad>(kt.h[tt], vt.h[tt], tab, kb, vb, a, s0, tt, len_k - 1, col, g);
+        load_half_f32<D, true, kPad>(kt.h[tt], vt.h[tt], tab, kb, vb, a, s0, tt,
+                                      RowReads{len_k - 1}, col, g);
       };
       load(0, p.key0);
       load(1, p.key0);
@@ -194,11 +196,13 @@ __global__ __launch_bounds__(64 * kSmallWaves, 1) void paged_decode_small(
                              [&](int i) { return visible(k0 + i); });
       };
       int32_t s0 = p.key0;
-      for (; s0 + 32 * W < key_end; s0 += 32 * W) {
+      for (; at + 32 * W < end; at += 32 * W) {
+        const int32_t next = ks.key(at + 32 * W);
         attend(0, s0);
-        load(0, s0 + 32 * W);
+        load(0, next);
         attend(1, s0);
-        load(1, s0 + 32 * W);
+        load(1, next);
+        s0 = next;
       }
       attend(0, s0);
       attend(1, s0);
@@ -240,8 +244,9 @@ __global__ __launch_bounds__(64 * kSmallWaves, 1) void paged_decode_small(
       // have read them; the last step of a wave loads nothing.
       while (true) {
         const int32_t s0 = p.key0;
-        if (s0 + 32 * W >= key_end) break;
-        p.key0 += 32 * W;
+        if (at + 32 * W >= end) break;
+        at += 32 * W;
+        p.key0 = ks.key(at);
         const uint4 pf = scores(s0);
         load_kt();
         values(pf, s0);
@@ -484,14 +489,19 @@ void launch_decode_small(const AttnArgs& a_in, uint32_t head_dim, uint32_t dtype
 #define VK_SM(T, DD, F, PAD) VK_SM2(T, DD, F, PAD, false)
 #define VK_SM2(T, DD, F, PAD, V2)                                                                 \
   do {                                                                                            \
+    if (!F && a.sinks) VK_SM3(T, DD, false, PAD, V2, true);                                       \
+    else VK_SM3(T, DD, F, PAD, V2, false);                                                        \
+  } while (0)
+#define VK_SM3(T, DD, F, PAD, V2, SK)                                                             \
+  do {                                                                                            \
     if (n_split > 1) {                                                                            \
-      hipLaunchKernelGGL((paged_decode_small<T, DD, F, PAD, true, V2>), grid, block, lds, s, a,   \
-                         a.cu_q, a.cu_k, a.table, n_wg, n_split);                                 \
+      hipLaunchKernelGGL((paged_decode_small<T, DD, F, PAD, true, V2, SK>), grid, block, lds, s,  \
+                         a, a.cu_q, a.cu_k, a.table, n_wg, n_split);                              \
       hipLaunchKernelGGL((paged_decode_small_merge<T, DD, PAD>), dim3(n_seg), block, 0, s, a,     \
                          a.cu_q, a.cu_k, n_split);                                                \
     } else {                                                                                      \
-      hipLaunchKernelGGL((paged_decode_small<T, DD, F, PAD, false, V2>), grid, block, lds, s, a,  \
-                         a.cu_q, a.cu_k, a.table, n_wg, 1u);                                      \
+      hipLaunchKernelGGL((paged_decode_small<T, DD, F, PAD, false, V2, SK>), grid, block, lds, s, \
+                         a, a.cu_q, a.cu_k, a.table, n_wg, 1u);                                   \
     }                                                                                             \
   } while (0)
   // Fused appends run on a kernel's own head dims only.
@@ -522,6 +532,7 @@ void launch_decode_small(const AttnArgs& a_in, uint32_t head_dim, uint32_t dtype
   }
 #undef VK_SM_F
 #undef VK_SM_D
+#undef VK_SM3
 #undef VK_SM2
 #undef VK_SM
 }

@@ -59,6 +59,12 @@ __device__ __forceinline__ void tile_chunks(int32_t klo, int32_t khi, uint32_t c
   c_last = min(khi / (int32_t)chunk, (int32_t)n_chunks - 1);
 }
 
+// Whether any of keys [c0, c1) is one of the sinks, or of [klo, khi].
+__device__ __forceinline__ bool keys_seen(int32_t c0, int32_t c1, int32_t klo, int32_t khi,
+                                          int32_t sinks) {
+  return c0 <= khi && (c1 > klo || c0 < sinks);
+}
+
 // Four consecutive elements as f32 (16 bytes of f32, 8 of bf16 / f16).
 template <typename T>
 __device__ __forceinline__ float4 load4(const T* p);
@@ -112,11 +118,16 @@ __global__ __launch_bounds__(kGenThreads) void paged_attn_generic(AttnArgs a, ui
   key_range(offset + (int32_t)(row0 / G), len_k, a.wl, a.wr, klo, unused);
   key_range(offset + (int32_t)((row0 + rows - 1) / G), len_k, a.wl, a.wr, unused, khi);
   int32_t c_first, c_last;
-  tile_chunks(klo, khi, chunk_keys, n_chunks, c_first, c_last);
-  if (khi < klo || (int32_t)chunk < c_first || (int32_t)chunk > c_last) return;
+  tile_chunks(a.sinks ? 0 : klo, khi, chunk_keys, n_chunks, c_first, c_last);
+  if (khi < klo || (int32_t)chunk < c_first || (int32_t)chunk > c_last ||
+      !keys_seen((int32_t)(chunk * chunk_keys), (int32_t)((chunk + 1) * chunk_keys), klo, khi,
+                 a.sinks))
+    return;
   const bool split = c_last > c_first;
-  klo = max(klo, (int32_t)(chunk * chunk_keys));
+  const int32_t w_first = klo;  // keys from the sinks' end to here are not read
+  klo = max(a.sinks ? 0 : klo, (int32_t)(chunk * chunk_keys));
   khi = min(khi, (int32_t)((chunk + 1) * chunk_keys) - 1);
+  auto seen = [&](int32_t key) { return key <= khi && (key >= w_first || key < a.sinks); };
 
   for (uint32_t i = tid; i < kGenRows * D; i += kGenThreads) {
     const uint32_t r = i / D, d = i - r * D;
@@ -172,7 +183,7 @@ __global__ __launch_bounds__(kGenThreads) void paged_attn_generic(AttnArgs a, ui
       const uint32_t c = tid + u * kGenThreads;
       kx[u] = vx[u] = make_float4(0.f, 0.f, 0.f, 0.f);
       const int32_t key = cs + (int32_t)(c * 4 / D);
-      if (c < kC4 && key <= khi) {
+      if (c < kC4 && seen(key)) {
         const uint32_t d = c * 4 % D;
         const uint64_t off = (uint64_t)blk_ids[(uint32_t)key / a.block_size - col0] * a.blk_e +
                              (uint64_t)((uint32_t)key % a.block_size) * a.tok_e;
@@ -203,7 +214,7 @@ __global__ __launch_bounds__(kGenThreads) void paged_attn_generic(AttnArgs a, ui
     } else {
       if (tid < kGenKeys) {
         const int32_t key = c0 + (int32_t)tid;
-        key_off[tid] = key <= khi ? (uint64_t)blk_ids[(uint32_t)key / a.block_size - col0] * a.blk_e +
+        key_off[tid] = seen(key) ? (uint64_t)blk_ids[(uint32_t)key / a.block_size - col0] * a.blk_e +
                                         (uint64_t)((uint32_t)key % a.block_size) * a.tok_e
                                   : ~0ull;
       }
@@ -253,7 +264,7 @@ __global__ __launch_bounds__(kGenThreads) void paged_attn_generic(AttnArgs a, ui
         key_range(offset + (int32_t)((row0 + r) / G), len_k, a.wl, a.wr, lo, hi);
         // Keys past this chunk (khi) are staged as zeros and belong to the
         // next chunk's workgroup, whatever the row's own range says.
-        if (key >= lo && key <= min(hi, khi)) {
+        if ((key >= lo || key < a.sinks) && key <= min(hi, khi)) {
           const float* qr = qs + r * D;
           const float* kr = ks + sk * KS;
           float dot;
@@ -365,8 +376,11 @@ __global__ __launch_bounds__(kGenThreads) void paged_attn_generic_merge(
   int32_t klo, khi, unused, c_first, c_last;
   key_range(offset + (int32_t)(row0 / G), len_k, a.wl, a.wr, klo, unused);
   key_range(offset + (int32_t)((row0 + rows - 1) / G), len_k, a.wl, a.wr, unused, khi);
-  tile_chunks(klo, khi, chunk_keys, n_chunks, c_first, c_last);
+  tile_chunks(a.sinks ? 0 : klo, khi, chunk_keys, n_chunks, c_first, c_last);
   if (khi < klo || c_last <= c_first) return;
+  auto skipped = [&](int32_t c) {  // chunks between the sinks and the window
+    return !keys_seen(c * (int32_t)chunk_keys, (c + 1) * (int32_t)chunk_keys, klo, khi, a.sinks);
+  };
   const uint32_t pr = tid >> 4, pd = tid & 15;
   if (pr >= rows) return;
   const uint64_t base = (uint64_t)blockIdx.x * n_chunks;
@@ -385,8 +399,8 @@ __global__ __launch_bounds__(kGenThreads) void paged_attn_generic_merge(
     float m[kB], l[kB], x[kB][kMaxDPer];
 #pragma unroll
     for (int u = 0; u < kB; ++u) {
-      const bool in = c0 + u <= c_last;
-      const float* pc = part + (base + (in ? c0 + u : c0)) * stride;
+      const bool in = c0 + u <= c_last && !skipped(c0 + u);
+      const float* pc = part + (base + (in ? c0 + u : c_first)) * stride;
       m[u] = pc[2 * pr];
       l[u] = in ? pc[2 * pr + 1] : 0.f;
 #pragma unroll

@@ -40,17 +40,18 @@ namespace vk {
 // V (D = 128, 256), or with 8 waves one of K or V (D = 64: waves 0-3 K,
 // waves 4-7 V), with 4 waves one of each. LDS slot t of a tensor holds the chunk its swizzled
 // position names; a wave's 64 slots are contiguous, as the load writes them.
+// rd: what is read for keys hidden from every row.
 // kPad (a head_dim a.hd below D, a multiple of 8): a chunk at or past a.hd
 // lies outside the key's row, so its slot is filled from the row's chunk 0
 // instead (the K fragment reads zero those chunks; the V columns past a.hd
 // only reach output columns that are never stored).
-template <typename T, int D, int W, bool kPad = false>
+template <typename T, int D, int W, bool kPad, typename Reads>
 __device__ __forceinline__ void pf_dma(uint16_t* kdst, uint16_t* vdst, const uint32_t* __restrict__ tab,
                                        const T* kb, const T* vb, const AttnArgs& a, int32_t s0,
-                                       int32_t last, uint32_t tid, uint32_t wave) {
+                                       const Reads& rd, uint32_t tid, uint32_t wave) {
   constexpr uint32_t CPR = D / 8;
   using ConstU32 = const __attribute__((address_space(4))) uint32_t;
-  const int32_t ts0 = min(s0, last & ~15), ts1 = min(s0 + 16, last & ~15);
+  const int32_t ts0 = rd.tile(s0), ts1 = rd.tile(s0 + 16);
   const uint32_t c0 = min((uint32_t)ts0 >> a.bs_shift, a.max_blocks - 1);
   const uint32_t c1 = min((uint32_t)ts1 >> a.bs_shift, a.max_blocks - 1);
   const uint32_t blk0 = min(((ConstU32*)tab)[c0], a.last_blk);
@@ -65,8 +66,7 @@ __device__ __forceinline__ void pf_dma(uint16_t* kdst, uint16_t* vdst, const uin
     // A wave's slots cover 64 / CPR whole rows of one 16-key tile.
     const bool second = __builtin_amdgcn_readfirstlane(r) >= 16;
     const T* base = base_t + (second ? off1 : off0);
-    const int32_t lim = last - (second ? ts1 : ts0);
-    const uint32_t kk = (uint32_t)min((int32_t)(r & 15), lim);
+    const uint32_t kk = rd.row((int32_t)(r & 15), second ? ts1 : ts0);
     __builtin_amdgcn_global_load_lds((const void*)(base + kk * a.tok_e + 8 * p),
                                      (LdsVoid*)(buf + wslot0 * 8), 16, 0, 0);
   };
@@ -115,8 +115,9 @@ __device__ __forceinline__ void lgkm_wait(uint2 (&r)[4]) {
 // same, or to the output if pb is null (all of the item: u0 = 0, u1 = c).
 // DL: the 16-column d tiles that hold head_dim (kPad; D / 16 otherwise):
 // the score MFMAs, V^T reads, PV MFMAs and stores of the tiles past them
-// are left out.
-template <typename T, int D, int RT, int W, int kSplit, bool kPad = false, int DL = D / 16>
+// are left out. kSinks: a.sinks keys (at least one) before the left window.
+template <typename T, int D, int RT, int W, int kSplit, bool kPad = false, int DL = D / 16,
+          bool kSinks = false>
 __device__ __forceinline__ void prefill_piece(const AttnArgs& a, const uint32_t* __restrict__ table,
                                               const PfItem& it, uint32_t u0, uint32_t u1,
                                               uint32_t c, char* pb) {
@@ -147,21 +148,20 @@ __device__ __forceinline__ void prefill_piece(const AttnArgs& a, const uint32_t*
   const uint32_t col = lane & 15, g = lane >> 4;
   const int32_t len_k = it.len_k;
   const int32_t offset = len_k - (int32_t)len_q;
-  const int32_t last = len_k - 1;
-
   const uint32_t wg_last = min(row_base + kPfRows, nrows) - 1;
   const int32_t wg_pmin = offset + (int32_t)(row_base / G);
   const int32_t wg_pmax = offset + (int32_t)(wg_last / G);
   const int32_t klo_wg = a.wl >= 0 ? max(0, wg_pmin - a.wl) : 0;
-  const int32_t khi_wg = a.wr >= 0 ? min(last, wg_pmax + a.wr) : last;
-  // This workgroup's run of 32-key steps: all of them, or its share.
-  int32_t klo = klo_wg, khi = khi_wg;
+  const int32_t khi_wg = a.wr >= 0 ? min(len_k - 1, wg_pmax + a.wr) : len_k - 1;
+  // This workgroup's run of 32-key steps, by position: all of them, or its share
+  // (s_last < s0_ when that is empty).
+  const KeySteps<kSinks> ks(klo_wg, khi_wg, a.sinks, 32);
+  int32_t s0_ = ks.start, s_last = khi_wg >= klo_wg ? ks.last : ks.start - 32;
   if (kSplit) {
-    const int32_t first = klo_wg & ~31;
-    const uint32_t steps = khi_wg >= klo_wg ? (uint32_t)(((khi_wg & ~31) - first) / 32 + 1) : 0u;
+    const uint32_t steps = (uint32_t)(s_last + 32 - s0_) / 32;
     const uint32_t a0 = pf_step_at(u0, c, steps), a1 = pf_step_at(u1, c, steps);
-    klo = max(klo_wg, first + 32 * (int32_t)a0);
-    khi = min(khi_wg, first + 32 * (int32_t)a1 - 1);  // < klo when the share is empty
+    s_last = s0_ + 32 * (int32_t)a1 - 32;
+    s0_ += 32 * (int32_t)a0;
   }
 
   const uint32_t row0 = row_base + wave * 16 * kPfRT;
@@ -220,11 +220,16 @@ __device__ __forceinline__ void prefill_piece(const AttnArgs& a, const uint32_t*
     for (int h = 0; h < 2; ++h)
       v_off[t][h] = pf_chunk<D>(16 * h + 4 * g + vj, 2 * t + (vq >> 1)) + 4 * (vq & 1);
 
-  int32_t s0_ = klo & ~31;
-  const int32_t s_last = khi & ~31;
-  if (!kSplit || s0_ <= khi) {  // (uniform) an empty key split issues no loads
-    pf_dma<T, D, W, kPad>(k0, v0, tab, kb, vb, a, s0_, last, tid, wave);
-    pf_dma<T, D, W, kPad>(k1, v1, tab, kb, vb, a, min(s0_ + 32, s_last), last, tid, wave);
+  auto load = [&](uint16_t* kd, uint16_t* vd, int32_t at) __attribute__((always_inline)) {
+    if constexpr (kSinks)
+      pf_dma<T, D, W, kPad>(kd, vd, tab, kb, vb, a, ks.key(at),
+                            KeyReads(ks, at, klo_wg, khi_wg, a.sinks), tid, wave);
+    else
+      pf_dma<T, D, W, kPad>(kd, vd, tab, kb, vb, a, at, RowReads{len_k - 1}, tid, wave);
+  };
+  if (!kSplit || s0_ <= s_last) {  // (uniform) an empty key split issues no loads
+    load(k0, v0, s0_);
+    load(k1, v1, min(s0_ + 32, s_last));
     wait_vmcnt<kLoadsPerStep>();
     ring_barrier();
   }
@@ -235,8 +240,8 @@ __device__ __forceinline__ void prefill_piece(const AttnArgs& a, const uint32_t*
     uint16_t* const vbuf = B == 0 ? v0 : B == 1 ? v1 : v2;
     uint16_t* const knext = B == 0 ? k2 : B == 1 ? k0 : k1;
     uint16_t* const vnext = B == 0 ? v2 : B == 1 ? v0 : v1;
-    const int32_t s0 = __builtin_amdgcn_readfirstlane(s0_);
-    pf_dma<T, D, W, kPad>(knext, vnext, tab, kb, vb, a, min(s0 + 64, s_last), last, tid, wave);
+    const int32_t at = __builtin_amdgcn_readfirstlane(s0_), s0 = ks.key(at);
+    load(knext, vnext, min(at + 64, s_last));
     // Steps inside [full_lo, full_hi] need no mask (a uniform branch).
     const bool masked = !(s0 >= full_lo && s0 + 31 <= full_hi);
     // V^T fragments in batches of two d tiles (four transposing reads): batch
@@ -274,11 +279,14 @@ __device__ __forceinline__ void prefill_piece(const AttnArgs& a, const uint32_t*
 #pragma unroll
           for (int i = 0; i < 4; ++i) sc[t][4 * tt + i] = acc[t][tt][i];
         if (masked) {
+          const int32_t key = s0 + 4 * (int32_t)g;
+          const int32_t top = kSinks ? min(a.sinks, lo[t] + cnt[t]) : 0;
 #pragma unroll
           for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (!(base + 16 * tt + i < n)) sc[t][4 * tt + i] = -INFINITY;
+              if (!(base + 16 * tt + i < n || (kSinks && key + 16 * tt + i < top)))
+                sc[t][4 * tt + i] = -INFINITY;
         }
       }
     }
@@ -330,11 +338,11 @@ __device__ __forceinline__ void prefill_piece(const AttnArgs& a, const uint32_t*
     s0_ += 32;
   };
   while (true) {
-    if (s0_ > khi) break;
+    if (s0_ > s_last) break;
     step(std::integral_constant<int, 0>{});
-    if (s0_ > khi) break;
+    if (s0_ > s_last) break;
     step(std::integral_constant<int, 1>{});
-    if (s0_ > khi) break;
+    if (s0_ > s_last) break;
     step(std::integral_constant<int, 2>{});
   }
   wait_vmcnt<0>();  // no load may land in LDS after the workgroup ends
@@ -379,7 +387,8 @@ __device__ __forceinline__ void prefill_piece(const AttnArgs& a, const uint32_t*
 // item are cut into n_split equal runs, one workgroup each, and
 // paged_prefill_merge combines their partials. Item order: kv head fastest,
 // then key split, then query tile (the items of one tile stay together).
-template <typename T, int D, int RT, int W, bool kSplit, bool kPad = false, int DL = D / 16>
+template <typename T, int D, int RT, int W, bool kSplit, bool kPad = false, int DL = D / 16,
+          bool kSinks = false>
 __device__ __forceinline__ void prefill_body(
     const AttnArgs& a, const uint32_t* __restrict__ cu_q, const uint32_t* __restrict__ cu_k,
     const uint32_t* __restrict__ table, uint32_t qtiles, uint32_t n_split_arg,
@@ -395,32 +404,33 @@ __device__ __forceinline__ void prefill_body(
   if (kSplit)
     pb = (char*)part + ((uint64_t)((it.li * a.kvh + it.kh) * qtiles + it.qt) * n_split + split) *
                            pf_part_bytes(kRows, D);
-  prefill_piece<T, D, RT, W, kSplit ? 1 : 0, kPad, DL>(a, table, it, split, split + 1, n_split, pb);
+  prefill_piece<T, D, RT, W, kSplit ? 1 : 0, kPad, DL, kSinks>(a, table, it, split, split + 1, n_split, pb);
 }
 
-template <typename T, int D, int RT, int OCC, bool kSplit, bool kPad, int DL = D / 16>
+template <typename T, int D, int RT, int OCC, bool kSplit, bool kPad, int DL = D / 16,
+          bool kSinks = false>
 __global__ __launch_bounds__(kPfThreads, OCC) void paged_prefill_tiled(
     AttnArgs a, const uint32_t* __restrict__ cu_q, const uint32_t* __restrict__ cu_k,
     const uint32_t* __restrict__ table, uint32_t qtiles, uint32_t n_split_arg,
     float* __restrict__ part) {
   __shared__ uint32_t order[64 * kPfWaves];
-  prefill_body<T, D, RT, kPfWaves, kSplit, kPad, DL>(a, cu_q, cu_k, table, qtiles, n_split_arg, part,
+  prefill_body<T, D, RT, kPfWaves, kSplit, kPad, DL, kSinks>(a, cu_q, cu_k, table, qtiles, n_split_arg, part,
                                            blockIdx.x, order);
 }
 
 // The same over ranges of equal work (see attn_prefill.hpp).
 // (One workgroup per CU at every head_dim: at 64 the walk takes the kernel past
 // the 128 registers of two, which are worth 1%.)
-template <typename T, int D, int RT, bool kPad, int DL = D / 16>
+template <typename T, int D, int RT, bool kPad, int DL = D / 16, bool kSinks = false>
 __global__ __launch_bounds__(kPfThreads, 1) void paged_prefill_tiled_ranges(
     AttnArgs a, const uint32_t* __restrict__ cu_q, const uint32_t* __restrict__ cu_k,
     const uint32_t* __restrict__ table, uint32_t qtiles, uint32_t ranges,
     PfSplitTile* __restrict__ tiles, char* __restrict__ part) {
   constexpr uint32_t kRows = 16 * RT * kPfWaves;
-  pf_walk_range<kPfWaves>(a, cu_q, cu_k, qtiles, kRows, ranges, tiles, blockIdx.x,
+  pf_walk_range<kPfWaves, kSinks>(a, cu_q, cu_k, qtiles, kRows, ranges, tiles, blockIdx.x,
                 [&](const PfItem& it, uint32_t u0, uint32_t u1, uint32_t c, uint32_t slot)
                     __attribute__((always_inline)) {
-                  prefill_piece<T, D, RT, kPfWaves, 2, kPad, DL>(
+                  prefill_piece<T, D, RT, kPfWaves, 2, kPad, DL, kSinks>(
                       a, table, it, u0, u1, c,
                       slot == ~0u ? nullptr : part + (uint64_t)slot * pf_part_bytes(kRows, D));
                 });
@@ -578,17 +588,18 @@ constexpr int kMixRowTiles = 2;
 constexpr int kMixPfWaves = 4;
 constexpr uint32_t kMixRows = 16 * kMixRowTiles * kMixPfWaves;
 
-template <typename T, int D, bool kSplit, bool kPad>
+template <typename T, int D, bool kSplit, bool kPad, bool kSinks>
 __global__ __launch_bounds__(256, 2) void paged_mixed_stream(AttnArgs a, uint32_t nwg,
                                                              uint32_t qtiles, uint32_t n_split,
                                                              float* __restrict__ part) {
   static_assert(64 * kDecodeWavesPerWG == 256 && 64 * kMixPfWaves == 256, "256 threads");
   extern __shared__ uint32_t P[];
   if (blockIdx.x < nwg)
-    decode_stream_body<T, D, false, kPad>(a, a.cu_q, a.cu_k, a.table, P, blockIdx.x, nwg);
+    decode_stream_body<T, D, false, kPad, D / 16, true, kSinks>(a, a.cu_q, a.cu_k, a.table, P,
+                                                                blockIdx.x, nwg);
   else {
-    prefill_body<T, D, kMixRowTiles, kMixPfWaves, kSplit, kPad>(a, a.cu_q, a.cu_k, a.table, qtiles,
-                                                          n_split, part, blockIdx.x - nwg, P);
+    prefill_body<T, D, kMixRowTiles, kMixPfWaves, kSplit, kPad, D / 16, kSinks>(
+        a, a.cu_q, a.cu_k, a.table, qtiles, n_split, part, blockIdx.x - nwg, P);
   }
 }
 
@@ -631,7 +642,8 @@ void launch_mixed(const AttnArgs& a_in, void* workspace, uint32_t max_q, uint32_
       --n_split;
   }
   c.pf_order = prefill_order(c.pf_seqs_n, c.kvh, qtiles, base, n_split,
-                             prefill_keys(max_q, max_k, c.wl), c.hd * sizeof(uint16_t), nwg,
+                             prefill_keys(max_q, max_k, c.wl, c.sinks), c.hd * sizeof(uint16_t),
+                             nwg,
                              false);
   float* part = n_split > 1 ? (float*)split_ws : nullptr;
   const dim3 grid((uint32_t)(nwg + base * n_split)), block(256);
@@ -642,11 +654,13 @@ void launch_mixed(const AttnArgs& a_in, void* workspace, uint32_t max_q, uint32_
 #define VK_MIX(T, DD, PAD)                                                                    \
   do {                                                                                        \
     if (n_split > 1)                                                                          \
-      hipLaunchKernelGGL((paged_mixed_stream<T, DD, true, PAD>), grid, block, lds, s, c, nwg, \
-                         qtiles, n_split, part);                                              \
+      hipLaunchKernelGGL((c.sinks ? paged_mixed_stream<T, DD, true, PAD, true>                \
+                                  : paged_mixed_stream<T, DD, true, PAD, false>),             \
+                         grid, block, lds, s, c, nwg, qtiles, n_split, part);                 \
     else                                                                                      \
-      hipLaunchKernelGGL((paged_mixed_stream<T, DD, false, PAD>), grid, block, lds, s, c,     \
-                         nwg, qtiles, 1u, nullptr);                                           \
+      hipLaunchKernelGGL((c.sinks ? paged_mixed_stream<T, DD, false, PAD, true>               \
+                                  : paged_mixed_stream<T, DD, false, PAD, false>),            \
+                         grid, block, lds, s, c, nwg, qtiles, 1u, nullptr);                   \
     if (n_split == 1) {                                                                       \
       launch_decode_merge(c, nwg, DD, bf16, s);                                               \
     } else {                                                                                  \
@@ -708,30 +722,36 @@ void launch_prefill(const AttnArgs& a_in, uint32_t max_q, uint32_t max_k, uint32
   const uint64_t base = route.items;
   const PfRangePlan rp = route.ranges;
   a.pf_order = prefill_order(a.pf_seqs_n, a.kvh, qtiles, base, n_split,
-                             prefill_keys(max_q, max_k, a.wl), a.hd * sizeof(uint16_t),
+                             prefill_keys(max_q, max_k, a.wl, a.sinks), a.hd * sizeof(uint16_t),
                              pf_slots(head_dim), false);
   float* part = n_split > 1 ? (float*)split_ws : nullptr;
   const dim3 grid((uint32_t)(base * n_split)), block(kPfThreads);
-#define VK_PF(T, DD, PAD, DL)                                                                    \
+  // Sinks: all d tiles live.
+#define VK_PF(T, DD, PAD, DL)                               \
+  do {                                                      \
+    if (a.sinks) VK_PFS(T, DD, PAD, DD / 16, true);         \
+    else VK_PFS(T, DD, PAD, DL, false);                     \
+  } while (0)
+#define VK_PFS(T, DD, PAD, DL, SK)                                                               \
   do {                                                                                           \
     constexpr int occ = DD == 64 ? kPfOcc64 : kPfOcc;                                            \
     constexpr int rt = DD == 256 ? kPfRowTiles256 : kPfRowTiles;                                 \
     if (rp.ranges) {                                                                             \
       if constexpr (DD <= 128)                                                                   \
-        hipLaunchKernelGGL((paged_prefill_tiled_ranges<T, DD, rt, PAD, DL>),                \
+        hipLaunchKernelGGL((paged_prefill_tiled_ranges<T, DD, rt, PAD, DL, SK>),                \
                            dim3(rp.ranges), block, 0, s, a, a.cu_q, a.cu_k, a.table, qtiles,     \
                            rp.ranges, (PfSplitTile*)split_ws,                                    \
                            (char*)split_ws + kPfRangeHead);                                      \
       launch_prefill_range_merge(a, rp.ranges, rows, bf16 ? VAPI_KV_BF16 : VAPI_KV_F16, DD,      \
                                  split_ws, s);                                                   \
     } else if (n_split > 1) {                                                                    \
-      hipLaunchKernelGGL((paged_prefill_tiled<T, DD, rt, occ, true, PAD, DL>), grid, block, 0,   \
+      hipLaunchKernelGGL((paged_prefill_tiled<T, DD, rt, occ, true, PAD, DL, SK>), grid, block, 0, \
                          s, a, a.cu_q, a.cu_k, a.table, qtiles, n_split, part);                  \
       hipLaunchKernelGGL((paged_prefill_merge<T, DD>),                                           \
                          dim3((uint32_t)(base * (rows / (256 / (DD / 4))))), dim3(256), 0, s, a, \
                          qtiles, rows, n_split, part);                                           \
     } else {                                                                                     \
-      hipLaunchKernelGGL((paged_prefill_tiled<T, DD, rt, occ, false, PAD, DL>), grid, block, 0,  \
+      hipLaunchKernelGGL((paged_prefill_tiled<T, DD, rt, occ, false, PAD, DL, SK>), grid, block, 0, \
                          s, a, a.cu_q, a.cu_k, a.table, qtiles, 1u, nullptr);                    \
     }                                                                                            \
   } while (0)
@@ -761,6 +781,7 @@ void launch_prefill(const AttnArgs& a_in, uint32_t max_q, uint32_t max_k, uint32
     else VK_PF_D(f16_t, 64);
   }
 #undef VK_PF_D
+#undef VK_PFS
 #undef VK_PF
 }
 

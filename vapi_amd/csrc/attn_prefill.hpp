@@ -76,6 +76,7 @@ struct PfWalk {
   uint32_t li, m, kh, c, f, n;  // (uniform) c: the count of the entry's last tile
   uint32_t seq, q0, len_q, len_k;
 
+  template <bool kSinks>
   __device__ __forceinline__ void init(const AttnArgs& a, const uint32_t* __restrict__ cu_q,
                                        const uint32_t* __restrict__ cu_k, uint32_t qtiles,
                                        uint32_t rows, PfEntry* entries) {
@@ -88,7 +89,7 @@ struct PfWalk {
         e.len_k = cu_k[e.seq + 1] - cu_k[e.seq];
         if (e.len_q >= a.pf_min_q && e.len_q > 0)
           pf_entry_tiles(e, a.group, qtiles, rows, a.wl, a.wr,
-                         pf_count_cap(qtiles * a.kvh * a.pf_seqs_n));
+                         pf_count_cap(qtiles * a.kvh * a.pf_seqs_n), kSinks ? a.sinks : 0);
       }
     }
     mine = e;
@@ -152,7 +153,7 @@ struct PfWalk {
 // Workgroup `bid`'s range of at most `ranges`: piece(item, u0, u1, c, slot)
 // for each of its pieces, counts [u0, u1) of the tile's c (slot: its partial,
 // or ~0u for a whole tile), the workgroup's LDS free again between them.
-template <int W, typename Piece>
+template <int W, bool kSinks, typename Piece>
 __device__ __forceinline__ void pf_walk_range(const AttnArgs& a, const uint32_t* __restrict__ cu_q,
                                               const uint32_t* __restrict__ cu_k, uint32_t qtiles,
                                               uint32_t rows, uint32_t ranges,
@@ -160,7 +161,7 @@ __device__ __forceinline__ void pf_walk_range(const AttnArgs& a, const uint32_t*
                                               Piece piece) {
   __shared__ PfEntry entries[64 * W];
   PfWalk w;
-  w.init(a, cu_q, cu_k, qtiles, rows, entries);
+  w.init<kSinks>(a, cu_q, cu_k, qtiles, rows, entries);
   const uint32_t S = w.total * a.kvh, nr = pf_range_count(S, ranges);
   if (bid >= nr || !w.some) {
     if (threadIdx.x == 0) tiles[bid].valid = 0;

@@ -128,15 +128,16 @@ __device__ __forceinline__ void lgkm_wait(uint2 (&r)[6]) {
                    : "memory");
 }
 
-// RT row tiles of one wave in f32 MFMAs, straight from the pool over keys
-// [klo, khi]: rows row0 .. of a sequence (its len_q * G rows are nrows). `pb`:
+// RT row tiles of one wave in f32 MFMAs, straight from the pool over the steps at
+// positions s0 .. s_last of ks (none if s_last < s0): rows row0 .. of a sequence (its len_q * G rows are nrows). `pb`:
 // the wave's item's partials of a key split ((m, l), then o / l per row,
 // prow0 the wave's first row in the item's part_rows), or null for the output.
-template <int D, int RT, bool kPad, int CL, bool kAhead>
+template <int D, int RT, bool kPad, int CL, bool kAhead, bool kSinks>
 __device__ __forceinline__ void f32_rows(const AttnArgs& a, const uint32_t* __restrict__ tab,
                                          uint32_t kh, uint32_t q0, uint32_t nrows, uint32_t row0,
-                                         int32_t offset, int32_t len_k, int32_t klo, int32_t khi,
-                                         char* pb, uint32_t prow0, uint32_t part_rows) {
+                                         int32_t offset, int32_t len_k, const KeySteps<kSinks>& ks,
+                                         int32_t s0, int32_t s_last, int32_t klo,
+                                         int32_t khi, char* pb, uint32_t prow0, uint32_t part_rows) {
   const uint32_t lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const uint32_t G = a.group;
   // This wave's rows: Q^T operands and visible key ranges.
@@ -173,23 +174,28 @@ __device__ __forceinline__ void f32_rows(const AttnArgs& a, const uint32_t* __re
     for (int k = 0; k < D / 16; ++k) o[t][k] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
 
-  if (khi >= klo) {
+  if (s0 <= s_last) {
     const float* kb = (const float*)a.k + kh * a.head_e;
     const float* vb = (const float*)a.v + kh * a.head_e;
-    const int32_t s_last = khi & ~31;
-    int32_t s0 = klo & ~31;
+    auto reads = [&](int32_t at) __attribute__((always_inline)) {
+      if constexpr (kSinks) return KeyReads(ks, at, klo, khi, a.sinks);
+      else return RowReads{khi};
+    };
+    auto sink_end = [&](int t) { return kSinks ? min(a.sinks, lo[t] + (int32_t)cnt[t]) : 0; };
     if constexpr (!kAhead) {
       // One half at a time, nothing in flight beside it (few registers).
 #pragma unroll 1
-      for (int32_t h0 = s0; h0 <= khi; h0 += 16) {
+      for (int32_t at = s0; at < s_last + 32; at += 16) {
+        const int32_t h0 = ks.key(at);
         KHalfF32<D> kt;
         VHalfF32<D> vt;
-        load_half_f32<D, false, kPad, CL>(kt, vt, tab, kb, vb, a, h0, 0, khi, col, g);
+        load_half_f32<D, false, kPad, CL>(kt, vt, tab, kb, vb, a, h0, 0, reads(at), col, g);
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-          const uint32_t base = (uint32_t)(h0 + 4 * (int32_t)g - lo[t]), n = cnt[t];
+          const int32_t key = h0 + 4 * (int32_t)g, top = sink_end(t);
+          const uint32_t base = (uint32_t)(key - lo[t]), n = cnt[t];
           attend_half_f32<D, CL>(kt, vt, qf[t], o[t], m_run[t], l_run[t], a.scale_log2,
-                                 [&](int i) { return base + (uint32_t)i < n; });
+                                 [&](int i) { return base + (uint32_t)i < n || (kSinks && key + i < top); });
         }
       }
     } else {
@@ -197,22 +203,25 @@ __device__ __forceinline__ void f32_rows(const AttnArgs& a, const uint32_t* __re
       VTileF32<D> vt;
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
-        load_half_f32<D, false, kPad, CL>(kt.h[tt], vt.h[tt], tab, kb, vb, a, s0, tt, khi, col, g);
+        load_half_f32<D, false, kPad, CL>(kt.h[tt], vt.h[tt], tab, kb, vb, a, ks.key(s0), tt,
+                                          reads(s0), col, g);
       while (true) {
         // The next step's halves are loaded unconditionally (the last step
         // re-reads its own keys, from L2): a load inside a branch would make
         // the compiler wait for it before this step's MFMAs.
-        const int32_t s_next = min(s0 + 32, s_last);
+        const int32_t s_next = min(s0 + 32, s_last), key0 = ks.key(s0), key_next = ks.key(s_next);
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
 #pragma unroll
           for (int t = 0; t < RT; ++t) {
-            const uint32_t base = (uint32_t)(s0 + 16 * tt + 4 * (int32_t)g - lo[t]);
-            const uint32_t n = cnt[t];
+            const int32_t key = key0 + 16 * tt + 4 * (int32_t)g;
+            const int32_t top = sink_end(t);
+            const uint32_t base = (uint32_t)(key - lo[t]), n = cnt[t];
             attend_half_f32<D, CL>(kt.h[tt], vt.h[tt], qf[t], o[t], m_run[t], l_run[t], a.scale_log2,
-                               [&](int i) { return base + (uint32_t)i < n; });
+                               [&](int i) { return base + (uint32_t)i < n || (kSinks && key + i < top); });
           }
-          load_half_f32<D, false, kPad, CL>(kt.h[tt], vt.h[tt], tab, kb, vb, a, s_next, tt, khi, col, g);
+          load_half_f32<D, false, kPad, CL>(kt.h[tt], vt.h[tt], tab, kb, vb, a, key_next, tt,
+                                            reads(s_next), col, g);
         }
         if (s0 >= s_last) break;
         s0 += 32;
@@ -241,7 +250,7 @@ __device__ __forceinline__ void f32_rows(const AttnArgs& a, const uint32_t* __re
 // One item: query tile it.qt of a sequence and kv head. kSplit, u0, u1, c,
 // pb: as prefill_piece's. DL: the 16-column d tiles that hold head_dim (kPad;
 // D / 16 otherwise): the MFMAs and reads of the tiles past them are left out.
-template <int D, int RT, int kSplit, bool kPad, int DL>
+template <int D, int RT, int kSplit, bool kPad, int DL, bool kSinks>
 __device__ __forceinline__ void x3_piece(const AttnArgs& a, const uint32_t* __restrict__ table,
                                          const PfItem& it, uint32_t u0, uint32_t u1, uint32_t c_all,
                                          char* pb) {
@@ -261,7 +270,7 @@ __device__ __forceinline__ void x3_piece(const AttnArgs& a, const uint32_t* __re
   const uint32_t tid = threadIdx.x, lane = tid & 63;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t col = lane & 15, g = lane >> 4;
-  const int32_t len_k = it.len_k, offset = len_k - (int32_t)it.len_q, last = len_k - 1;
+  const int32_t len_k = it.len_k, offset = len_k - (int32_t)it.len_q;
 
   // The keys any row of the workgroup sees, and this split's share of them.
   const uint32_t wg_last = min(row_base + kPf32Rows, nrows) - 1;
@@ -269,13 +278,15 @@ __device__ __forceinline__ void x3_piece(const AttnArgs& a, const uint32_t* __re
   int32_t klo, khi, unused;
   key_range(pmin, len_k, a.wl, a.wr, klo, unused);
   key_range(pmax, len_k, a.wl, a.wr, unused, khi);
+  const KeySteps<kSinks> ks(klo, khi, a.sinks, 32);
+  int32_t s0_ = ks.start, s_last = khi >= klo ? ks.last : ks.start - 32;  // positions of steps
   if (kSplit) {
-    const int32_t first = klo & ~31;
-    const uint32_t steps = khi >= klo ? (uint32_t)(((khi & ~31) - first) / 32 + 1) : 0u;
+    const uint32_t steps = (uint32_t)(s_last + 32 - s0_) / 32;
     const uint32_t a0 = pf_step_at(u0, c_all, steps), a1 = pf_step_at(u1, c_all, steps);
-    klo = max(klo, first + 32 * (int32_t)a0);
-    khi = min(khi, first + 32 * (int32_t)a1 - 1);
+    s_last = s0_ + 32 * (int32_t)a1 - 32;
+    s0_ += 32 * (int32_t)a0;
   }
+  const int32_t s_first = s0_;
   // Steps inside [full_lo, full_hi] need no mask.
   int32_t full_lo, full_hi;
   key_range(pmax, len_k, a.wl, a.wr, full_lo, unused);
@@ -292,7 +303,11 @@ __device__ __forceinline__ void x3_piece(const AttnArgs& a, const uint32_t* __re
   const uint32_t wr0 = __builtin_amdgcn_readfirstlane(ur0);
   const uint32_t d0 = kPad && 8 * up >= a.hd ? 0 : 8 * up;
   const uint32_t d1 = kPad && 8 * up + 4 >= a.hd ? 0 : 8 * up + 4;
-  auto dma = [&](int32_t s0) __attribute__((always_inline)) {
+  auto dma = [&](int32_t at) __attribute__((always_inline)) {
+    // (Hidden keys are read as they are: if one holds what P = 0 does not take
+    // out, f32_rows below computes the rows again.)
+    const RowReads rd{khi};
+    const int32_t s0 = ks.key(at);
     using ConstU32 = const __attribute__((address_space(4))) uint32_t;
     uint32_t row0_ = ur0, c0 = d0, c1 = d1;  // opaque: see attend
     asm volatile("" : "+v"(row0_), "+v"(c0), "+v"(c1));
@@ -300,7 +315,7 @@ __device__ __forceinline__ void x3_piece(const AttnArgs& a, const uint32_t* __re
     int32_t ts[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      ts[h] = min(s0 + 16 * h, last & ~15);
+      ts[h] = rd.tile(s0 + 16 * h);
       const uint32_t blk =
           min(((ConstU32*)tab)[min((uint32_t)ts[h] >> a.bs_shift, a.max_blocks - 1)], a.last_blk);
       tile[h] = (uint64_t)blk * a.blk_e + (uint64_t)((uint32_t)ts[h] & (a.block_size - 1)) * a.tok_e;
@@ -311,7 +326,7 @@ __device__ __forceinline__ void x3_piece(const AttnArgs& a, const uint32_t* __re
       const bool is_v = wr >= 32, second = (wr & 16) != 0;
       const uint32_t r = (row0_ + kRowsPerJ * j) & 15;
       const float* row = (is_v ? vb : kb) + (second ? tile[1] : tile[0]) +
-                         (uint32_t)min((int32_t)r, last - (second ? ts[1] : ts[0])) * a.tok_e;
+                         rd.row((int32_t)r, second ? ts[1] : ts[0]) * a.tok_e;
       __builtin_amdgcn_global_load_lds((const void*)(row + c0), (LdsVoid*)&raw[j][0][64 * wave], 16, 0, 0);
       __builtin_amdgcn_global_load_lds((const void*)(row + c1), (LdsVoid*)&raw[j][1][64 * wave], 16, 0, 0);
     }
@@ -347,7 +362,7 @@ __device__ __forceinline__ void x3_piece(const AttnArgs& a, const uint32_t* __re
   Split8 qf[RT][KCL];
   int32_t lo[RT], cnt[RT];
   const uint32_t sg = a.q_sign ? 0x80000000u : 0u;
-  if (klo <= khi) dma(klo & ~31);
+  if (s0_ <= s_last) dma(s0_);
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const uint32_t r = row0 + 16 * t + col;
@@ -388,9 +403,7 @@ __device__ __forceinline__ void x3_piece(const AttnArgs& a, const uint32_t* __re
   const uint32_t vj = col >> 2, vq = col & 3;
   const uint32_t v_off = 2 * (pf_chunk<D>(4 * g + vj, vq >> 1) + 4 * (vq & 1));
 
-  int32_t s0_ = klo & ~31;
-  const int32_t s_last = khi & ~31;
-  if (klo <= khi) {
+  if (s0_ <= s_last) {
     wait_vmcnt<0>();
     fetch();
     convert(0);
@@ -434,11 +447,14 @@ __device__ __forceinline__ void x3_piece(const AttnArgs& a, const uint32_t* __re
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[4 * tt + i] = acc[t][tt][i];
       if (masked) {
+        const int32_t key = s0 + 4 * (int32_t)g;
+        const int32_t top = kSinks ? min(a.sinks, lo[t] + cnt[t]) : 0;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (!(base + 16 * tt + i < n)) s[4 * tt + i] = -INFINITY;
+            if (!(base + 16 * tt + i < n || (kSinks && key + 16 * tt + i < top)))
+              s[4 * tt + i] = -INFINITY;
       }
       const float mx = max3_nc(max3_nc(s[0], s[1], s[2]), max3_nc(s[3], s[4], s[5]),
                                max_nc(s[6], s[7])) * a.scale_log2;
@@ -471,22 +487,22 @@ __device__ __forceinline__ void x3_piece(const AttnArgs& a, const uint32_t* __re
   };
   auto step = [&](auto cur) __attribute__((always_inline)) {
     constexpr int B = decltype(cur)::value;
-    const int32_t s0 = __builtin_amdgcn_readfirstlane(s0_);
+    const int32_t at = __builtin_amdgcn_readfirstlane(s0_), s0 = ks.key(at);
     // The next step: its f32 chunks (loaded since the last step) into
     // registers, the one after it on its way, its planes written.
     wait_vmcnt<0>();
     fetch();
     wait_lds();
-    dma(min(s0 + 64, s_last));
+    dma(min(at + 64, s_last));
     convert(1 - B);
     if (active) attend(s0, std::integral_constant<int, B>{});
     lds_barrier();
     s0_ += 32;
   };
   while (true) {
-    if (s0_ > khi) break;
+    if (s0_ > s_last) break;
     step(std::integral_constant<int, 0>{});
-    if (s0_ > khi) break;
+    if (s0_ > s_last) break;
     step(std::integral_constant<int, 1>{});
   }
   wait_vmcnt<0>();  // no load may land in LDS after the workgroup ends
@@ -511,8 +527,9 @@ __device__ __forceinline__ void x3_piece(const AttnArgs& a, const uint32_t* __re
   if (__builtin_amdgcn_readfirstlane(outside_lds)) {
 #pragma unroll 1
     for (uint32_t t = 0; t < (uint32_t)RT; ++t)
-      f32_rows<D, 1, kPad, D / 16, false>(a, tab, kh, q0, nrows, row0 + 16 * t, offset, len_k, klo,
-                                          khi, kSplit ? pb : nullptr, wrow0 + 16 * t, kPf32Rows);
+      f32_rows<D, 1, kPad, D / 16, false, kSinks>(a, tab, kh, q0, nrows, row0 + 16 * t, offset, len_k, ks,
+                                          s_first, s_last, klo, khi, kSplit ? pb : nullptr,
+                                          wrow0 + 16 * t, kPf32Rows);
     return;
   }
 #pragma unroll
@@ -541,7 +558,7 @@ __device__ __forceinline__ void x3_piece(const AttnArgs& a, const uint32_t* __re
 // Workgroups of a launch: an item each, or (kSplit) one of n_split equal
 // shares of each item's steps, to be merged (a batch too small to fill the
 // GPU with query tiles alone).
-template <int D, int RT, bool kSplit, bool kPad, int DL = D / 16>
+template <int D, int RT, bool kSplit, bool kPad, int DL, bool kSinks>
 __global__ __launch_bounds__(kPf32Threads, 1) void paged_prefill_f32x3(
     AttnArgs a, const uint32_t* __restrict__ cu_q, const uint32_t* __restrict__ cu_k,
     const uint32_t* __restrict__ table, uint32_t qtiles, uint32_t n_split_arg,
@@ -558,20 +575,20 @@ __global__ __launch_bounds__(kPf32Threads, 1) void paged_prefill_f32x3(
   if (kSplit)
     pb = (char*)part + ((uint64_t)((it.li * a.kvh + it.kh) * qtiles + it.qt) * n_split + split) *
                            pf_part_bytes(kRows, D);
-  x3_piece<D, RT, kSplit ? 1 : 0, kPad, DL>(a, table, it, split, split + 1, n_split, pb);
+  x3_piece<D, RT, kSplit ? 1 : 0, kPad, DL, kSinks>(a, table, it, split, split + 1, n_split, pb);
 }
 
 // The same over ranges of equal work (see attn_prefill.hpp).
-template <int D, int RT, bool kPad, int DL = D / 16>
+template <int D, int RT, bool kPad, int DL, bool kSinks>
 __global__ __launch_bounds__(kPf32Threads, 1) void paged_prefill_f32x3_ranges(
     AttnArgs a, const uint32_t* __restrict__ cu_q, const uint32_t* __restrict__ cu_k,
     const uint32_t* __restrict__ table, uint32_t qtiles, uint32_t ranges,
     PfSplitTile* __restrict__ tiles, char* __restrict__ part) {
   constexpr uint32_t kRows = x3_rows(RT);
-  pf_walk_range<kPf32Waves>(a, cu_q, cu_k, qtiles, kRows, ranges, tiles, blockIdx.x,
+  pf_walk_range<kPf32Waves, kSinks>(a, cu_q, cu_k, qtiles, kRows, ranges, tiles, blockIdx.x,
                             [&](const PfItem& it, uint32_t u0, uint32_t u1, uint32_t c,
                                 uint32_t slot) __attribute__((always_inline)) {
-                              x3_piece<D, RT, 2, kPad, DL>(
+                              x3_piece<D, RT, 2, kPad, DL, kSinks>(
                                   a, table, it, u0, u1, c,
                                   slot == ~0u ? nullptr
                                               : part + (uint64_t)slot * pf_part_bytes(kRows, D));
@@ -584,7 +601,7 @@ __global__ __launch_bounds__(kPf32Threads, 1) void paged_prefill_f32x3_ranges(
 // (pf_part_bytes of 16 * RT rows per (item, split)) for the merge.
 // CL: the 16-column chunks of d that hold head_dim (kPad; D / 16
 // otherwise): K chunks past them are neither loaded nor multiplied.
-template <int D, int RT, bool kSplit, bool kPad, int CL = D / 16>
+template <int D, int RT, bool kSplit, bool kPad, int CL, bool kSinks>
 __global__ __launch_bounds__(64 * kPfF32Waves, 1) void paged_prefill_f32(
     AttnArgs a, uint32_t qtiles, uint32_t n_items, uint32_t n_split_arg,
     float* __restrict__ part) {
@@ -614,20 +631,20 @@ __global__ __launch_bounds__(64 * kPfF32Waves, 1) void paged_prefill_f32(
   int32_t klo, khi, unused;
   key_range(offset + (int32_t)(row0 / G), len_k, a.wl, a.wr, klo, unused);
   key_range(offset + (int32_t)(r_last / G), len_k, a.wl, a.wr, unused, khi);
+  const KeySteps<kSinks> ks(klo, khi, a.sinks, 32);
+  int32_t s0 = ks.start, s_last = khi >= klo ? ks.last : ks.start - 32;
   if (kSplit) {
-    // This split's share of the wave's 32-key steps (empty: khi < klo).
-    const int32_t first = klo & ~31;
-    const uint32_t steps = khi >= klo ? (uint32_t)(((khi & ~31) - first) / 32 + 1) : 0u;
-    const uint32_t a0 = split * steps / n_split, a1 = (split + 1) * steps / n_split;
-    klo = max(klo, first + 32 * (int32_t)a0);
-    khi = min(khi, first + 32 * (int32_t)a1 - 1);
+    // This split's share of the wave's 32-key steps (empty: s_last < s0).
+    const uint32_t steps = (uint32_t)(s_last + 32 - s0) / 32;
+    s_last = s0 + 32 * (int32_t)((split + 1) * steps / n_split) - 32;
+    s0 += 32 * (int32_t)(split * steps / n_split);
   }
 
   char* const pb = kSplit ? (char*)part + ((uint64_t)(rest * qtiles + qt) * n_split + split) *
                                               pf_part_bytes(16 * RT, D)
                           : nullptr;
-  f32_rows<D, RT, kPad, CL, true>(a, a.table + (uint64_t)seq * a.max_blocks, kh, q0, nrows, row0, offset,
-                            len_k, klo, khi, pb, 0, 16 * RT);
+  f32_rows<D, RT, kPad, CL, true, kSinks>(a, a.table + (uint64_t)seq * a.max_blocks, kh, q0, nrows, row0, offset,
+                            len_k, ks, s0, s_last, klo, khi, pb, 0, 16 * RT);
 }
 
 
@@ -652,41 +669,54 @@ void launch_prefill_f32(const AttnArgs& a_in, uint32_t max_q, uint32_t max_k, ui
   // must not depend on the workspace it is given).
   const F32Route route = f32_route(a.pf_seqs_n, a.kvh, a.group, max_q, max_k, head_dim,
                                    split_ws && !a.deterministic, split_ws_bytes);
-  const F32Plan& p = route.plan;
+  F32Plan p = route.plan;
+  // (Padded to 128 columns, two row tiles and the sinks' masks do not fit the registers.)
+  if (a.sinks && p.x3 && p.row_tiles == 2 && head_dim == 128 && a.hd != 128) {
+    p.row_tiles = 1;
+    p.rows = x3_rows(1);
+    p.qtiles = (uint32_t)(((uint64_t)max_q * a.group + p.rows - 1) / p.rows);
+    p.items = (uint64_t)p.qtiles * a.kvh * a.pf_seqs_n;
+  }
   const PfRangePlan rp = route.ranges;
   const uint32_t qtiles = p.qtiles, n_split = route.n_split;
   const uint64_t items = p.items * n_split;
   a.pf_order = prefill_order(a.pf_seqs_n, a.kvh, qtiles, p.items, n_split,
-                             prefill_keys(max_q, max_k, a.wl), a.hd * sizeof(float), 256,
+                             prefill_keys(max_q, max_k, a.wl, a.sinks), a.hd * sizeof(float), 256,
                              true);
   const uint32_t wgs = (uint32_t)((items + kPfF32Waves - 1) / kPfF32Waves);
   float* part = n_split > 1 ? (float*)split_ws : nullptr;
-#define VK_X3(DD, RT, SPLIT, PAD, CL)                                                            \
-  hipLaunchKernelGGL((paged_prefill_f32x3<DD, RT, SPLIT, PAD, CL>), dim3((uint32_t)items),       \
+#define VK_X3(DD, RT, SPLIT, PAD, CL, SK)                                                            \
+  hipLaunchKernelGGL((paged_prefill_f32x3<DD, RT, SPLIT, PAD, CL, SK>), dim3((uint32_t)items),       \
                      dim3(kPf32Threads), 0, s, a, a.cu_q, a.cu_k, a.table, qtiles, n_split, part)
-#define VK_X3R(DD, PAD, CL)                                                                      \
-  hipLaunchKernelGGL((paged_prefill_f32x3_ranges<DD, 1, PAD, CL>), dim3(rp.ranges),              \
+#define VK_X3R(DD, PAD, CL, SK)                                                                      \
+  hipLaunchKernelGGL((paged_prefill_f32x3_ranges<DD, 1, PAD, CL, SK>), dim3(rp.ranges),              \
                      dim3(kPf32Threads), 0, s, a, a.cu_q, a.cu_k, a.table, qtiles, rp.ranges,    \
                      (PfSplitTile*)split_ws, (char*)split_ws + kPfRangeHead)
-#define VK_PF32(DD, PAD, CL)                                                                     \
+  // Sinks: all d tiles live.
+#define VK_PF32(DD, PAD, CL)                            \
+  do {                                                  \
+    if (a.sinks) VK_PF32S(DD, PAD, DD / 16, true);      \
+    else VK_PF32S(DD, PAD, CL, false);                  \
+  } while (0)
+#define VK_PF32S(DD, PAD, CL, SK)                                                                     \
   do {                                                                                           \
     if (rp.ranges) {                                                                             \
-      VK_X3R(DD, PAD, CL);                                                                       \
+      VK_X3R(DD, PAD, CL, SK);                                                                       \
       launch_prefill_range_merge(a, rp.ranges, p.rows, VAPI_KV_F32, DD, split_ws, s);            \
     } else if (p.x3) {                                                                                  \
-      if (p.row_tiles == 2) {                                                                    \
-        VK_X3(DD, 2, false, PAD, CL); /* enough items: never split */                            \
+      if (p.row_tiles == 2) { /* enough items: never split */                                    \
+        if constexpr (!(SK && PAD && DD == 128)) VK_X3(DD, 2, false, PAD, CL, SK);               \
       } else if (n_split > 1) {                                                                  \
-        VK_X3(DD, 1, true, PAD, CL);                                                             \
+        VK_X3(DD, 1, true, PAD, CL, SK);                                                             \
       } else {                                                                                   \
-        VK_X3(DD, 1, false, PAD, CL);                                                            \
+        VK_X3(DD, 1, false, PAD, CL, SK);                                                            \
       }                                                                                          \
     } else if (n_split > 1) {                                                                    \
-      hipLaunchKernelGGL((paged_prefill_f32<DD, kPfF32RowTiles, true, PAD, CL>), dim3(wgs),      \
+      hipLaunchKernelGGL((paged_prefill_f32<DD, kPfF32RowTiles, true, PAD, CL, SK>), dim3(wgs),  \
                          dim3(64 * kPfF32Waves), 0, s, a, qtiles, (uint32_t)items, n_split,      \
                          part);                                                                  \
     } else {                                                                                     \
-      hipLaunchKernelGGL((paged_prefill_f32<DD, kPfF32RowTiles, false, PAD, CL>), dim3(wgs),     \
+      hipLaunchKernelGGL((paged_prefill_f32<DD, kPfF32RowTiles, false, PAD, CL, SK>), dim3(wgs), \
                          dim3(64 * kPfF32Waves), 0, s, a, qtiles, (uint32_t)items, 1u, nullptr); \
     }                                                                                            \
     if (n_split > 1)                                                                             \
@@ -706,6 +736,7 @@ void launch_prefill_f32(const AttnArgs& a_in, uint32_t max_q, uint32_t max_k, ui
     else if (live <= 2) VK_PF32(64, true, 2);
     else VK_PF32(64, true, 4);
   }
+#undef VK_PF32S
 #undef VK_PF32
 #undef VK_X3R
 #undef VK_X3

@@ -121,11 +121,11 @@ __device__ __forceinline__ void q8_load(Q8Step<D, KS>& st, const AttnArgs& a, co
 // stream's measured shares move from call to call, changes no rounding of P (of
 // 64 x 256-8,192 keys 0.03% of the outputs differed between calls, 45% without;
 // 74.5 us either way).
-template <typename T, int F, int D, int KS, bool kWhole>
+template <typename T, int F, int D, int KS, bool kWhole, bool kSinks>
 __device__ __forceinline__ void q8_attend(const Q8Step<D, KS>& st, const uint4 (&qf)[D / 32],
                                           floatx4 (&o)[D / 16], float& m_run, float& l_run,
                                           float scale_log2, int32_t key0, int32_t lo,
-                                          int32_t len_k, uint32_t g) {
+                                          int32_t len_k, int32_t sinks, uint32_t g) {
   constexpr int NT = KS / 16, DPL = D / 16;
   float s[4 * NT];
   float mx = -INFINITY;
@@ -144,7 +144,7 @@ __device__ __forceinline__ void q8_attend(const Q8Step<D, KS>& st, const uint4 (
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int32_t key = key0 + 16 * tt + 4 * (int32_t)g + i;
-      s[4 * tt + i] = key >= lo && key < len_k ? acc[i] * by : -INFINITY;
+      s[4 * tt + i] = row_sees<kSinks>(key, lo, len_k, sinks) ? acc[i] * by : -INFINITY;
     }
     mx = max_nc(mx, max_nc(max_nc(s[4 * tt], s[4 * tt + 1]), max_nc(s[4 * tt + 2], s[4 * tt + 3])));
   }
@@ -178,7 +178,7 @@ __device__ __forceinline__ void q8_attend(const Q8Step<D, KS>& st, const uint4 (
 
 // The stream: decode_stream_body's plan and pieces over 8-bit steps. (The plan is
 // written out here, without the fused append: what changes there changes here.)
-template <typename T, int F, int D, bool kPad, bool kNt>
+template <typename T, int F, int D, bool kPad, bool kNt, bool kSinks>
 __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void q8_decode_stream(
     AttnArgs a, Q8Scales sc, const uint32_t* __restrict__ cu_q, const uint32_t* __restrict__ cu_k,
     const uint32_t* __restrict__ table) {
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void q8_de
     const uint32_t per = (B + NT - 1) / NT;
     const uint32_t b0 = min(tid * per, B), b1 = min(b0 + per, B);
     uint32_t sum = 0;
-    for (uint32_t s = b0; s < b1; ++s) sum += decode_steps<KS>(a, cu_q, cu_k, s) * kvh_plan;
+    for (uint32_t s = b0; s < b1; ++s) sum += decode_steps<KS, kSinks>(a, cu_q, cu_k, s) * kvh_plan;
     uint32_t inc = sum;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void q8_de
     for (uint32_t w = 0; w < wave; ++w) run += wave_tot[w];
     for (uint32_t s = b0; s < b1; ++s) {
       P[s] = run;
-      run += decode_steps<KS>(a, cu_q, cu_k, s) * kvh_plan;
+      run += decode_steps<KS, kSinks>(a, cu_q, cu_k, s) * kvh_plan;
     }
     if (tid == NT - 1) P[B] = run;
     __syncthreads();
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void q8_de
   const uint32_t t_end = bounds[x] + (uint32_t)(((uint64_t)(jr + 1) * len) / nr);
 
   uint32_t t = t_begin;
-  DecodePos pos = locate<KS>(a, cu_q, cu_k, P, nullptr, t, kvh_plan, n_parts, part);
+  DecodePos pos = locate<KS, kSinks>(a, cu_q, cu_k, P, nullptr, t, kvh_plan, n_parts, part);
   uint4* qs = q_lds[wave];
   q8_load_q<T, D, kPad>(qs, a, pos, lane, col, g);
   bool piece_first = pos.seg_first;
@@ -256,10 +256,10 @@ __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void q8_de
     // (The last step's loads point at one cached row, as in the 16-bit stream.)
     DecodePos nxt = pos;
     if (same_piece) {
-      nxt.key0 += KS;
+      nxt.key0 = next_step<kSinks, KS>(pos.key0, pos.lo, a.sinks);
       nxt.seg_first = false;
     } else if (more) {
-      nxt = next_segment<KS>(a, cu_q, cu_k, P, nullptr, pos, n_parts);
+      nxt = next_segment<KS, kSinks>(a, cu_q, cu_k, P, nullptr, pos, n_parts);
     } else {
       nxt.seq = 0;
       nxt.key0 = 0;
@@ -269,8 +269,8 @@ __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void q8_de
     uint4 qf[D / 32];
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) qf[c] = qs[c * 64 + lane];
-    q8_attend<T, F, D, KS, true>(cur, qf, o, m_run, l_run, a.scale_log2, pos.key0, pos.lo,
-                                 pos.len_k, g);
+    q8_attend<T, F, D, KS, true, kSinks>(cur, qf, o, m_run, l_run, a.scale_log2, pos.key0, pos.lo,
+                                 pos.len_k, a.sinks, g);
     if (!same_piece) {
       const uint32_t seg = pos.seq * a.kvh + pos.kh;
       if (lane == 0) {
@@ -307,7 +307,7 @@ template <int D>
 constexpr int q8_small_waves() { return D == 256 ? 4 : 8; }
 constexpr uint32_t kQ8SmallPad = 4;  // floats between rows of O in LDS (bank conflicts)
 
-template <typename T, int F, int D, bool kPad, bool kSplit>
+template <typename T, int F, int D, bool kPad, bool kSplit, bool kSinks>
 __global__ __launch_bounds__(64 * q8_small_waves<D>(), 1) void q8_decode_small(
     AttnArgs a, Q8Scales sc, const uint32_t* __restrict__ cu_q, const uint32_t* __restrict__ cu_k,
     const uint32_t* __restrict__ table, uint32_t n_split_arg) {
@@ -326,22 +326,22 @@ __global__ __launch_bounds__(64 * q8_small_waves<D>(), 1) void q8_decode_small(
   if (cu_q[p.seq + 1] - p.q0 != 1 || p.len_k <= 0) return;
   p.lo = a.wl >= 0 ? max(0, p.len_k - 1 - a.wl) : 0;
   p.fuse = 0, p.seg_first = 0;
-  const int32_t first = p.lo & ~(KS - 1);
-  int32_t key_end = p.len_k;
-  p.key0 = first;
+  const KeySteps<kSinks> ks(p.lo, p.len_k - 1, a.sinks, KS);
+  int32_t at = ks.start, end = ks.last + KS;  // positions of steps
   if constexpr (kSplit) {
-    const uint32_t steps = (uint32_t)(p.len_k - first + KS - 1) / KS;
-    p.key0 = first + KS * (int32_t)(split * steps / n_split);
-    key_end = min(p.len_k, first + KS * (int32_t)((split + 1) * steps / n_split));
+    const uint32_t steps = (uint32_t)(end - at) / KS;
+    end = at + KS * (int32_t)((split + 1) * steps / n_split);
+    at += KS * (int32_t)(split * steps / n_split);
   }
-  p.key0 += KS * wave;
+  at += KS * wave;
+  p.key0 = ks.key(at);
   float m_run = kNegBig, l_run = 0.f;
   floatx4 o[DPL];
 #pragma unroll
   for (int k = 0; k < DPL; ++k) o[k] = floatx4{0.f, 0.f, 0.f, 0.f};
   const uint32_t count = vhead_count(a, p.kh), h0 = vhead_base(a, p.kh);
   const uint32_t hd = kPad ? a.hd : (uint32_t)D;
-  if (p.key0 < key_end) {
+  if (at < end) {
     Q8Step<D, KS> stA, stB;
     q8_load<D, kPad, true, KS>(stA, a, sc, table, p, col, g);
     const T* qrow =
@@ -358,10 +358,11 @@ __global__ __launch_bounds__(64 * q8_small_waves<D>(), 1) void q8_decode_small(
     // The next step on its way while one is computed (a wave's last repeats it).
     auto step = [&](Q8Step<D, KS>& cur, Q8Step<D, KS>& next) __attribute__((always_inline)) {
       const int32_t s0 = p.key0;
-      const bool more = s0 + KS * W < key_end;
-      if (more) p.key0 += KS * W;
+      const bool more = at + KS * W < end;
+      if (more) at += KS * W, p.key0 = ks.key(at);
       q8_load<D, kPad, true, KS>(next, a, sc, table, p, col, g);
-      q8_attend<T, F, D, KS, false>(cur, qf, o, m_run, l_run, a.scale_log2, s0, p.lo, p.len_k, g);
+      q8_attend<T, F, D, KS, false, kSinks>(cur, qf, o, m_run, l_run, a.scale_log2, s0, p.lo, p.len_k,
+                                      a.sinks, g);
       return more;
     };
     while (step(stA, stB) && step(stB, stA)) {
@@ -421,9 +422,9 @@ __global__ __launch_bounds__(256) void q8_expand_kernel(AttnArgs a, Q8Scales sc,
   const uint32_t len_k = a.cu_k[seq + 1] - a.cu_k[seq];
   if (len_q < a.pf_min_q || (int32_t)len_k <= 0 || j * a.block_size >= len_k) return;
   // Keys that a left window hides from every query: the prefill reads whole
-  // steps of 32 keys from the first visible one.
-  if (a.wl >= 0 && (int64_t)(j + 1) * a.block_size <=
-                       (((int64_t)len_k - len_q - a.wl) & ~(int64_t)63))
+  // steps of 32 keys, those of the sinks and from the first visible one.
+  if (a.wl >= 0 && j * a.block_size >= (((uint32_t)a.sinks + 63) & ~63u) &&
+      (int64_t)(j + 1) * a.block_size <= (((int64_t)len_k - len_q - a.wl) & ~(int64_t)63))
     return;
   const uint32_t to = li * mb + j;
   if (h == 0 && threadIdx.x == 0) table_out[(uint64_t)seq * mb + j] = to;
@@ -501,8 +502,10 @@ template <typename T, int F, int D>
 static void launch_q8_stream_d(const AttnArgs& c, const Q8Scales& sc, uint32_t nwg, size_t lds,
                                hipStream_t s) {
 #define VK_Q8S(PAD, NT)                                                                     \
-  hipLaunchKernelGGL((q8_decode_stream<T, F, D, PAD, NT>), dim3(nwg),                       \
-                     dim3(64 * kDecodeWavesPerWG), lds, s, c, sc, c.cu_q, c.cu_k, c.table)
+  hipLaunchKernelGGL((c.sinks ? q8_decode_stream<T, F, D, PAD, NT, true>                    \
+                              : q8_decode_stream<T, F, D, PAD, NT, false>),                 \
+                     dim3(nwg), dim3(64 * kDecodeWavesPerWG), lds, s, c, sc, c.cu_q,        \
+                     c.cu_k, c.table)
   // Streaming loads where a line is read by one wave only. Parts of one group
   // read the same codes side by side (as the 16-bit stream's), and rows of whole
   // tokens ([token, head, d]) that are not whole lines share them with the next
@@ -557,7 +560,8 @@ static size_t q8_small_lds(uint32_t group, uint32_t D) {
 static SmallPlan q8_small_plan(const AttnArgs& a, uint32_t D, uint32_t max_k, size_t part_bytes) {
   const uint64_t seg = (uint64_t)a.batch * a.kvh;
   if (seg > kQ8SmallWgs || q8_small_lds(a.group, D) > 56 * 1024) return {false, 1};
-  const uint64_t span = a.wl >= 0 ? std::min<uint64_t>(max_k, (uint64_t)a.wl + 32) : max_k;
+  const int32_t wl = row_window(a.wl, a.sinks);
+  const uint64_t span = wl >= 0 ? std::min<uint64_t>(max_k, (uint64_t)wl + 32) : max_k;
   const uint64_t bytes = span * D;
   uint64_t n = 1;
   if (bytes > kQ8SmallUnsplit)
@@ -574,11 +578,13 @@ static void launch_q8_small_d(const AttnArgs& a, const Q8Scales& sc, uint32_t n_
   const dim3 grid(a.batch * a.kvh * n_split), block(64 * q8_small_waves<D>());
   const size_t lds = q8_small_lds(a.group, D);
   if (n_split > 1)
-    hipLaunchKernelGGL((q8_decode_small<T, F, D, kPad, true>), grid, block, lds, s, a, sc, a.cu_q,
-                       a.cu_k, a.table, n_split);
+    hipLaunchKernelGGL((a.sinks ? q8_decode_small<T, F, D, kPad, true, true>
+                                : q8_decode_small<T, F, D, kPad, true, false>),
+                       grid, block, lds, s, a, sc, a.cu_q, a.cu_k, a.table, n_split);
   else
-    hipLaunchKernelGGL((q8_decode_small<T, F, D, kPad, false>), grid, block, lds, s, a, sc,
-                       a.cu_q, a.cu_k, a.table, 1u);
+    hipLaunchKernelGGL((a.sinks ? q8_decode_small<T, F, D, kPad, false, true>
+                                : q8_decode_small<T, F, D, kPad, false, false>),
+                       grid, block, lds, s, a, sc, a.cu_q, a.cu_k, a.table, 1u);
 }
 template <typename T, int F>
 static void launch_q8_small(const AttnArgs& a_in, const Q8Scales& sc, uint32_t D, uint32_t n_split,
@@ -634,6 +640,20 @@ int vapi_kv_q8_attention(const vapi_kv_q8_pool* pool, uint32_t layer, const void
                          float scale, int32_t window_left, int32_t window_right, uint32_t flags,
                          const uint32_t* prefill_seqs, uint32_t n_prefill, void* workspace,
                          size_t workspace_bytes, vapi_stream_t stream) {
+  return vapi_kv_q8_attention_sinks(pool, layer, q, out, cu_seqlens_q, cu_seqlens_k, block_table,
+                                    batch, max_blocks, max_seqlen_q, max_seqlen_k, num_heads,
+                                    scale, window_left, window_right, 0, flags, prefill_seqs,
+                                    n_prefill, workspace, workspace_bytes, stream);
+}
+
+int vapi_kv_q8_attention_sinks(const vapi_kv_q8_pool* pool, uint32_t layer, const void* q,
+                               void* out, const uint32_t* cu_seqlens_q,
+                               const uint32_t* cu_seqlens_k, const uint32_t* block_table,
+                               uint32_t batch, uint32_t max_blocks, uint32_t max_seqlen_q,
+                               uint32_t max_seqlen_k, uint32_t num_heads, float scale,
+                               int32_t window_left, int32_t window_right, uint32_t sinks,
+                               uint32_t flags, const uint32_t* prefill_seqs, uint32_t n_prefill,
+                               void* workspace, size_t workspace_bytes, vapi_stream_t stream) {
   const char* who = "vapi_kv_q8_attention";
   if (int rc = check_q8_pool(pool, layer, who)) return rc;
   if (num_heads == 0 || num_heads % pool->num_kv_heads)
@@ -696,6 +716,7 @@ int vapi_kv_q8_attention(const vapi_kv_q8_pool* pool, uint32_t layer, const void
   a.q_sign = scale < 0.f ? 0x80008000u : 0u;
   a.wl = window_arg(window_left);
   a.wr = window_arg(window_right);
+  a.sinks = sinks_arg(sinks, a.wl);
   a.deterministic = (flags & VAPI_ATTN_DETERMINISTIC) ? 1u : 0u;
   a.pf_min_q = skip_decode ? 1 : 2;
   a.pf_seqs = listed ? prefill_seqs : nullptr;

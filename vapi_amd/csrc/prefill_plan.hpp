@@ -26,6 +26,26 @@ VK_HD void key_range(int32_t p, int32_t len_k, int32_t wl, int32_t wr, int32_t& 
   hi = wr >= 0 ? pf_min(len_k - 1, p + wr) : len_k - 1;
 }
 
+// The steps of `step` keys of a range whose first visible key is klo and last khi,
+// with kSinks the first `sinks` keys visible too: the sinks' steps, then the
+// window's, as one run of positions start .. last, `step` apart. A position is a
+// key's own place up to `hop`, and `gap` keys before it from there.
+template <bool kSinks>
+struct KeySteps {
+  int32_t start, last;  // the first and the last step's position
+  int32_t hop, gap;
+  VK_HD KeySteps(int32_t klo, int32_t khi, int32_t sinks, int32_t step)
+      : start(klo & ~(step - 1)), last(khi & ~(step - 1)), hop(0), gap(0) {
+    if (kSinks) {
+      hop = pf_min((pf_min(sinks, khi + 1) + step - 1) & ~(step - 1), start);
+      gap = start - hop;
+      start = 0;
+      last -= gap;
+    }
+  }
+  VK_HD int32_t key(int32_t at) const { return kSinks && at >= hop ? at + gap : at; }
+};
+
 // How a launch's items are ordered (prefill_item says why).
 constexpr uint32_t kLine = 128;  // bytes of an L2 line
 constexpr uint32_t kPfSortSeqs = 64;
@@ -95,9 +115,9 @@ VK_HD void pf_list_part(uint32_t i, uint32_t n_seqs, uint32_t kvh, uint32_t qtil
 }
 
 // The most keys that an item walks, with at most max_q queries and max_k keys
-// per sequence and the left window wl.
-inline uint64_t prefill_keys(uint32_t max_q, uint32_t max_k, int32_t wl) {
-  return wl >= 0 ? std::min<uint64_t>(max_k, (uint64_t)wl + max_q) : max_k;
+// per sequence, the left window wl and sinks before it.
+inline uint64_t prefill_keys(uint32_t max_q, uint32_t max_k, int32_t wl, int32_t sinks = 0) {
+  return wl >= 0 ? std::min<uint64_t>(max_k, (uint64_t)wl + max_q + (uint64_t)sinks) : max_k;
 }
 
 // The order of a launch's tiles by classes of work (kPfByClass): classes, the
@@ -180,14 +200,17 @@ VK_HD uint32_t pf_count_cap(uint32_t tiles) {
   return (uint32_t)kPfMaxCount / pf_max(tiles, 1u);
 }
 VK_HD void pf_entry_tiles(PfEntry& e, uint32_t group, uint32_t qtiles, uint32_t rows, int32_t wl,
-                          int32_t wr, uint32_t cap) {
+                          int32_t wr, uint32_t cap, int32_t sinks = 0) {
   e.nt = (uint32_t)pf_min(((uint64_t)e.len_q * group + rows - 1) / rows, (uint64_t)qtiles);
   // Steps of the last tile, from its first row's window to its last key.
   const int32_t offset = (int32_t)(e.len_k - e.len_q);
   int32_t klo, khi, unused;
   key_range(offset + (int32_t)((e.nt - 1) * rows / group), (int32_t)e.len_k, wl, wr, klo, unused);
   key_range(offset + (int32_t)e.len_q - 1, (int32_t)e.len_k, wl, wr, unused, khi);
-  const uint32_t steps = khi >= klo ? (uint32_t)((khi >> 5) - (klo >> 5) + 1) : 1u;
+  const uint32_t steps =
+      khi < klo ? 1u
+      : sinks   ? (uint32_t)(KeySteps<true>(klo, khi, sinks, 32).last / 32 + 1)
+                : (uint32_t)((khi >> 5) - (klo >> 5) + 1);
   e.c_last = pf_min(16u * steps, cap);
   e.fall = wl < 0 && wr >= 0 && e.nt > 1
                ? pf_min(rows / (2 * group), (e.c_last - 16) / (e.nt - 1))
