@@ -342,6 +342,59 @@ int vapi_paged_attention_append_sinks(
     size_t workspace_bytes, vapi_stream_t stream);
 
 /*
+ * Sequences of a batch that share the blocks of a prefix (forks of one prompt, a
+ * system prompt found in the prefix cache): group i is the queries offsets[i] ..
+ * offsets[i + 1] of the lists `rows` and `seqs`, which name a row of q and the
+ * sequence it belongs to, and its sequences' tables agree in their first keys[i] keys.
+ * All queries of a member are listed, in one group; start[s] is the keys of sequence
+ * s that its group shares (0: s is in none). All in device memory; n_rows entries,
+ * max_keys the most of keys[].
+ */
+typedef struct vapi_kv_prefixes {
+  const uint32_t* offsets; /* u32[n_groups + 1] */
+  const uint32_t* rows;    /* u32[n_rows] */
+  const uint32_t* seqs;    /* u32[n_rows] */
+  const uint32_t* keys;    /* u32[n_groups] */
+  const uint32_t* start;   /* u32[batch] */
+  uint32_t n_groups;
+  uint32_t n_rows;
+  uint32_t max_keys;
+} vapi_kv_prefixes;
+
+/*
+ * vapi_paged_attention_sinks of a batch with shared prefixes: the same output, up to
+ * the order of f32 sums and the rounding of probabilities to the pool's dtype, with
+ * each group's shared keys read once for all of its queries instead of once for each
+ * sequence. Any lengths, windows and sinks; sequences in no group, decode rows and
+ * prefill rows as there. prefill_seqs lists the sequences with len_q > 1 (NULL with
+ * n_prefill == 0: all of them); a sequence with len_q > 1 that it leaves out gets no
+ * output, or one without its own keys. Like the block table the lists are trusted:
+ * entries that name no query of the batch are left out, and a group whose sequences'
+ * tables differ attends the first one's blocks.
+ *
+ * f16 and bf16 pools with head_dim a multiple of 8 up to 256 and block_size a power of
+ * two from 16, up to 256 query heads per kv head, 4,096 sequences and 4,096 groups and
+ * prefill sequences together (else VAPI_KV_EUNSUP: such a batch runs
+ * vapi_paged_attention_sinks). The workspace has no optional part: all that
+ * vapi_paged_attention_shared_workspace_size returns, by the same rules as
+ * vapi_paged_attention's and usable by its calls too; that size is 0 where the call
+ * would be refused (vapi_kv_last_error says why). No counterpart in the reference, which reads a shared
+ * prefix once for each sequence (attention.rs:90-163).
+ */
+size_t vapi_paged_attention_shared_workspace_size(const vapi_kv_pool* pool, uint32_t batch,
+                                                  uint32_t n_prefill, uint32_t num_heads,
+                                                  uint32_t max_seqlen_q, uint32_t max_seqlen_k,
+                                                  const vapi_kv_prefixes* prefixes);
+int vapi_paged_attention_shared(const vapi_kv_pool* pool, uint32_t layer, const void* q, void* out,
+                                const uint32_t* cu_seqlens_q, const uint32_t* cu_seqlens_k,
+                                const uint32_t* block_table, uint32_t batch, uint32_t max_blocks,
+                                uint32_t max_seqlen_q, uint32_t max_seqlen_k, uint32_t num_heads,
+                                float scale, int32_t window_left, int32_t window_right,
+                                uint32_t sinks, uint32_t flags, const uint32_t* prefill_seqs,
+                                uint32_t n_prefill, const vapi_kv_prefixes* prefixes,
+                                void* workspace, size_t workspace_bytes, vapi_stream_t stream);
+
+/*
  * vapi_paged_attention_ex without a workspace argument, for callers that
  * cannot allocate device memory (code under HIP graph capture, tight
  * serving loops, harnesses that forbid hipMalloc). No counterpart in the

@@ -41,6 +41,7 @@ EXPORTS = (
     "vapi_paged_attention_prepared", "vapi_paged_attention_prepared_workspace_size",
     "vapi_kv_q8_append", "vapi_kv_q8_gather", "vapi_kv_q8_attention",
     "vapi_kv_q8_attention_workspace_size",
+    "vapi_paged_attention_shared", "vapi_paged_attention_shared_workspace_size",
     "vapi_paged_attention_sinks", "vapi_paged_attention_append_sinks",
     "vapi_kv_q8_attention_sinks",
     "vapi_kv_attention_weights", "vapi_kv_attention_weights_workspace_size",
@@ -105,6 +106,20 @@ class Weights(ctypes.Structure):
     ]
 
 
+class Prefixes(ctypes.Structure):
+    """vapi_kv_prefixes."""
+    _fields_ = [
+        ("offsets", ctypes.c_void_p),
+        ("rows", ctypes.c_void_p),
+        ("seqs", ctypes.c_void_p),
+        ("keys", ctypes.c_void_p),
+        ("start", ctypes.c_void_p),
+        ("n_groups", ctypes.c_uint32),
+        ("n_rows", ctypes.c_uint32),
+        ("max_keys", ctypes.c_uint32),
+    ]
+
+
 _lib = None
 _vp = ctypes.c_void_p
 _u32 = ctypes.c_uint32
@@ -114,6 +129,7 @@ _u32p = ctypes.POINTER(ctypes.c_uint32)
 _poolp = ctypes.POINTER(Pool)
 _q8p = ctypes.POINTER(Q8Pool)
 _wp = ctypes.POINTER(Weights)
+_pp = ctypes.POINTER(Prefixes)
 
 
 class SpillStats(ctypes.Structure):
@@ -199,6 +215,9 @@ def lib():
              _i32, _u32, _u32, _vp, _u32, _vp, _sz, _vp]
     L.vapi_paged_attention_sinks.argtypes = [_poolp] + sinks
     L.vapi_kv_q8_attention_sinks.argtypes = [_q8p] + sinks
+    L.vapi_paged_attention_shared_workspace_size.argtypes = [_poolp] + [_u32] * 5 + [_pp]
+    L.vapi_paged_attention_shared_workspace_size.restype = _sz
+    L.vapi_paged_attention_shared.argtypes = [_poolp] + sinks[:-3] + [_pp] + sinks[-3:]
     L.vapi_paged_attention_append_sinks.argtypes = [_poolp, _u32, _vp, _vp, _vp] + sinks
     L.vapi_kv_attention_weights_workspace_size.argtypes = [_u32] * 7
     L.vapi_kv_attention_weights_workspace_size.restype = _sz

@@ -17,6 +17,7 @@ import torch
 from ._lib import ESPACE, check, lib
 from .cache import (PagedKvCache, _is_quantised, _per_layer, check_on_device, contiguous_on,
                     empty_on, keep_for, on_stream, stream_handle, write_rows_indexed)
+from .prefix import PrefixPlan
 
 _u32p = ctypes.POINTER(ctypes.c_uint32)
 
@@ -105,7 +106,8 @@ class PreparedAttention:
     freezes the decode's work split so repeated calls are bit-identical.
     `prefill_seqs` lists the sequences with len_q > 1 (device u32), so that
     the prefill grid of a mixed step covers its prefill chunks only
-    (vapi_paged_attention_prepared); None covers every sequence."""
+    (vapi_paged_attention_prepared); None covers every sequence. `prefixes`: the
+    prefixes that sequences of the step share, which attention then reads once."""
     block_table: torch.Tensor
     seqlens_q: torch.Tensor
     seqlens_k: torch.Tensor
@@ -119,13 +121,22 @@ class PreparedAttention:
     weights_workspaces: list = field(default_factory=list)  # earlier, smaller ones
     workspaces: list = field(default_factory=list)  # the attention's earlier ones
     streams: set = field(default_factory=set)  # handles keep_for has seen
+    prefixes: PrefixPlan | None = None
+    sharing: dict = field(default_factory=dict)  # shares()'s answers
 
     @classmethod
     def from_batch(cls, batch: ForwardBatch, device, cache=None, num_heads: int | None = None,
-                   deterministic: bool = False) -> "PreparedAttention":
+                   deterministic: bool = False,
+                   share_prefixes: bool = False) -> "PreparedAttention":
         """With `cache` and `num_heads`, the workspace is sized here for the
         largest attention layer of the cache (a HybridKvCache's layers may
-        differ in heads and head_dim), so no layer of the step allocates."""
+        differ in heads and head_dim), so no layer of the step allocates.
+        `share_prefixes`: sequences whose tables begin with the same blocks of
+        `cache` are attended over them together, where that saves reads (the
+        same outputs up to rounding; layers whose pool takes no shared prefixes
+        run as without)."""
+        if share_prefixes and cache is None:
+            raise ValueError("share_prefixes needs the cache that the block tables refer to")
         cq = np.asarray(batch.cu_seqlens_q, dtype=np.int64)
         lens_q = np.diff(cq) if cq.size > 1 else np.zeros(0, np.int64)
         flags = ATTN_DETERMINISTIC if deterministic else 0
@@ -139,6 +150,8 @@ class PreparedAttention:
                    max_seqlen_k=int(batch.max_seqlen_k), flags=flags,
                    prefill_seqs=cu_seqlens(pf if pf.size else [0], device),
                    n_prefill=int(pf.size))
+        if share_prefixes:
+            prep.prefixes = PrefixPlan.from_batch(batch, cache.block_size, device)
         if cache is not None and num_heads is not None:
             prep.reserve(cache, num_heads, device)
         return prep
@@ -153,6 +166,7 @@ class PreparedAttention:
                   if isinstance(cache, HybridKvCache) else [cache])
         need = max(workspace_bytes(c, b, num_heads, max_q, max_k, self.n_prefill_arg(c))
                    for c in layers)
+        need = max([need] + [self.shared_bytes(c, num_heads) for c in layers])
         self.grow(need, device)
 
     def grow(self, need: int, device, stream=None) -> torch.Tensor | None:
@@ -171,6 +185,22 @@ class PreparedAttention:
             self.streams.clear()
         return ws
 
+    def shared_bytes(self, cache, num_heads: int) -> int:
+        """The workspace of a layer's attention over the step's shared prefixes;
+        0 where it runs without them."""
+        if self.prefixes is None:
+            return 0
+        key = (cache.num_kv_heads, cache.head_dim, cache.block_size, cache.dtype, num_heads,
+               getattr(cache, "fmt", None))
+        if key not in self.sharing:
+            b = self.seqlens_q.shape[0] - 1
+            listed = self.prefill_seqs is not None and not self.flags & ATTN_NO_DECODE_ROWS
+            args = (b, self.n_prefill if listed else b, num_heads, max(self.max_seqlen_q, 1),
+                    max(self.max_seqlen_k, 1), self.prefixes.ptr)
+            self.sharing[key] = (0 if _is_quantised(cache) else
+                                 lib().vapi_paged_attention_shared_workspace_size(cache.pool, *args))
+        return self.sharing[key]
+
     def keep_for(self, stream) -> None:
         """Keeps the step's device arrays and workspace from reuse before a call on
         `stream` (None: the current one) has run, whenever the step is dropped.
@@ -178,7 +208,8 @@ class PreparedAttention:
         if stream is None or stream.cuda_stream in self.streams:
             return
         keep_for(stream, *(t for t in (self.block_table, self.seqlens_q, self.seqlens_k,
-                                       self.prefill_seqs, self.workspace) if t is not None))
+                                       self.prefill_seqs, self.workspace,
+                                       self.prefixes and self.prefixes.lists) if t is not None))
         self.streams.add(stream.cuda_stream)
 
     def n_prefill_arg(self, cache=None) -> int | None:
@@ -215,6 +246,13 @@ def _workspace(cache, prepared: PreparedAttention, b: int, num_heads: int, max_q
     return need, ws
 
 
+def _run_shared(call, prepared: PreparedAttention, need: int, device, stream=None) -> None:
+    """_run of a call with shared prefixes, whose workspace has no optional part."""
+    ws = prepared.grow(need, device, stream)
+    check(call(ws.data_ptr(), ws.numel()))
+    prepared.keep_for(stream)
+
+
 def _run(call, cache, prepared: PreparedAttention, b: int, num_heads: int, max_q: int,
          max_k: int, device, stream=None) -> None:
     """call(workspace pointer, bytes) with the step's workspace, grown first
@@ -240,7 +278,8 @@ def paged_attention_prepared(q: torch.Tensor, cache: PagedKvCache, layer: int,
     """attention.rs:262-288 on libvapi_kv.so. None for a window side means
     unlimited (flash convention); the default right window 0 is causal.
     `sinks`: a sequence's first keys that stay visible behind its left window
-    (vapi_paged_attention_sinks). `cache` may be a HybridKvCache (`layer` then names one of its K/V layers)
+    (vapi_paged_attention_sinks). A step prepared with share_prefixes reads
+    shared prefixes once (vapi_paged_attention_shared). `cache` may be a HybridKvCache (`layer` then names one of its K/V layers)
     or a QuantKvCache."""
     cache, layer = _per_layer(cache, layer)
     if q.dim() != 3 or q.shape[2] != cache.head_dim:
@@ -257,15 +296,24 @@ def paged_attention_prepared(q: torch.Tensor, cache: PagedKvCache, layer: int,
     max_k = max(int(prepared.max_seqlen_k), 1)
     mask = (float(softmax_scale), -1 if window_size_left is None else int(window_size_left),
             -1 if window_size_right is None else int(window_size_right))
-    mask += (sinks, prepared.flags) if sinks else (prepared.flags,)
+    shared = prepared.shared_bytes(cache, num_heads) if b else 0
+    mask += (sinks, prepared.flags) if sinks or shared else (prepared.flags,)
     args = (cache.pool, layer, q.data_ptr(), out.data_ptr(), prepared.seqlens_q.data_ptr(),
             prepared.seqlens_k.data_ptr(), prepared.block_table.data_ptr(), b,
             prepared.block_table.shape[1], max_q, max_k, num_heads) + mask
     handle = stream_handle(stream)
-    if _is_quantised(cache) or sinks:
+    if _is_quantised(cache) or sinks or shared:
         listed = prepared.prefill_seqs is not None
         args += (prepared.prefill_seqs.data_ptr() if listed else None,
                  prepared.n_prefill if listed else 0)
+    if shared:
+        check_on_device(q, out, prepared.block_table, prepared.seqlens_q)
+        fn = lib().vapi_paged_attention_shared
+        args += (prepared.prefixes.ptr,)
+        _run_shared(lambda ptr, size: fn(*args, ptr, size, handle), prepared, shared, q.device,
+                    stream)
+        keep_for(stream, q, out)
+        return out
     if _is_quantised(cache):
         check_on_device(cache.k[0], q, out, prepared.block_table, prepared.seqlens_q)
         args = (cache.q8,) + args[1:]
@@ -311,6 +359,17 @@ def paged_attention(q, cache, layer, batch: ForwardBatch, softmax_scale,
                                     stream=stream, sinks=sinks)
 
 
+def _check_second(cache, q, out, prepared: PreparedAttention) -> None:
+    """What an attention refuses that follows a write as a second call."""
+    check_on_device(q, out, prepared.block_table, prepared.seqlens_q,
+                    *(cache.k[:1] if _is_quantised(cache) else ()))
+    if (q.data_ptr() | out.data_ptr()) & 15:
+        raise ValueError("q and out must be 16-byte aligned")
+    if prepared.block_table.shape[1] == 0 or prepared.flags & ~(ATTN_DETERMINISTIC |
+                                                                ATTN_NO_DECODE_ROWS):
+        raise ValueError(f"a block table of no columns, or unknown flags {prepared.flags:#x}")
+
+
 def paged_attention_append_prepared(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                                     slot_mapping: torch.Tensor, cache: PagedKvCache,
                                     layer: int, prepared: PreparedAttention,
@@ -349,16 +408,21 @@ def paged_attention_append_prepared(q: torch.Tensor, k: torch.Tensor, v: torch.T
     if _is_quantised(cache):
         # Two calls; what the second would refuse is refused before the first, and
         # its workspace is there before rows are written.
-        check_on_device(cache.k[0], q, out, prepared.block_table, prepared.seqlens_q)
-        if (q.data_ptr() | out.data_ptr()) & 15:
-            raise ValueError("q and out must be 16-byte aligned")
-        if prepared.block_table.shape[1] == 0 or prepared.flags & ~(ATTN_DETERMINISTIC |
-                                                                    ATTN_NO_DECODE_ROWS):
-            raise ValueError(f"a block table of no columns, or unknown flags {prepared.flags:#x}")
+        _check_second(cache, q, out, prepared)
         if b and not _workspace(cache, prepared, b, num_heads, max_q, max_k, q.device,
                                 stream)[0]:
             raise ValueError(lib().vapi_kv_last_error().decode())
         write_rows_indexed(cache, layer, k, v, slot_mapping, stream=stream)
+        return paged_attention_prepared(q, cache, layer, prepared, softmax_scale,
+                                        window_size_left, window_size_right, out=out,
+                                        stream=stream, sinks=sinks)
+    if b and prepared.shared_bytes(cache, num_heads):
+        # Two calls here too; the shared prefixes' is refused before rows are written.
+        _check_second(cache, q, out, prepared)
+        prepared.grow(prepared.shared_bytes(cache, num_heads), q.device, stream)
+        check(lib().vapi_kv_append(cache.pool, layer, k.data_ptr(), v.data_ptr(),
+                                   slot_mapping.data_ptr(), k.shape[0], stream_handle(stream)))
+        keep_for(stream, k, v, slot_mapping)
         return paged_attention_prepared(q, cache, layer, prepared, softmax_scale,
                                         window_size_left, window_size_right, out=out,
                                         stream=stream, sinks=sinks)

@@ -17,6 +17,7 @@
 #include <mutex>
 
 #include "attn_common.hpp"
+#include "attn_shared.hpp"
 
 namespace vk {
 
@@ -179,7 +180,8 @@ static int paged_attention_impl(const vapi_kv_pool* pool, uint32_t layer, const 
                                 size_t workspace_bytes, vapi_stream_t stream,
                                 const NewRows* fuse, uint32_t flags,
                                 const PrefillSeqs* pf = nullptr, uint32_t sinks = 0,
-                                bool checks_only = false);
+                                bool checks_only = false,
+                                const vapi_kv_prefixes* prefixes = nullptr);
 
 // The workspace a call cannot run without: the decode's (unless the call
 // launches no decode kernel) or the VALU kernel's split partials.
@@ -194,6 +196,12 @@ static size_t required_workspace(const vapi_kv_pool* pool, uint32_t batch, uint3
     return generic_workspace_bytes(batch, pool->num_kv_heads, group, pool->head_dim,
                                    std::max(max_seqlen_q, 1u), max_seqlen_k);
   return skip_decode ? 0 : decode_ws_for(pool, batch, num_heads);
+}
+
+// Where a call with shared prefixes keeps its tiles' part of the workspace.
+static size_t shared_offset(const vapi_kv_pool* pool, uint32_t batch, uint32_t num_heads) {
+  if (!mfma16_ok(pool, num_heads)) return 0;
+  return std::max<size_t>((decode_ws_for(pool, batch, num_heads) + 255) & ~(size_t)255, 256);
 }
 
 // A batch the caller says has no decode rows (and which is not a fused decode
@@ -285,6 +293,44 @@ int vapi_paged_attention_sinks(const vapi_kv_pool* pool, uint32_t layer, const v
                               max_blocks, max_seqlen_q, max_seqlen_k, num_heads, scale,
                               window_left, window_right, workspace, workspace_bytes, stream,
                               nullptr, flags, prefill_seqs ? &pf : nullptr, sinks);
+}
+
+size_t vapi_paged_attention_shared_workspace_size(const vapi_kv_pool* pool, uint32_t batch,
+                                                  uint32_t n_prefill, uint32_t num_heads,
+                                                  uint32_t max_seqlen_q, uint32_t max_seqlen_k,
+                                                  const vapi_kv_prefixes* prefixes) {
+  const char* who = "vapi_paged_attention_shared_workspace_size";
+  if (check_pool(pool, who) || batch == 0) return 0;
+  if (!pool->v || num_heads == 0 || num_heads % pool->num_kv_heads || !mfma16_ok(pool, num_heads)) {
+    set_error("%s: not a 16-bit K/V pool of heads, a head_dim and a block_size that it takes", who);
+    return 0;
+  }
+  const uint32_t kvh = pool->num_kv_heads, G = num_heads / kvh, D = decode_dim(pool->head_dim);
+  const uint32_t pf_n = max_seqlen_q > 1 ? std::min(n_prefill, batch) : 0;
+  if (shared_check(prefixes, batch, kvh, G, D, pf_n, max_seqlen_q, max_seqlen_k, who)) return 0;
+  return shared_offset(pool, batch, num_heads) +
+         shared_workspace_bytes(prefixes, batch, kvh, G, D, pf_n, max_seqlen_q);
+}
+
+int vapi_paged_attention_shared(const vapi_kv_pool* pool, uint32_t layer, const void* q, void* out,
+                                const uint32_t* cu_seqlens_q, const uint32_t* cu_seqlens_k,
+                                const uint32_t* block_table, uint32_t batch, uint32_t max_blocks,
+                                uint32_t max_seqlen_q, uint32_t max_seqlen_k, uint32_t num_heads,
+                                float scale, int32_t window_left, int32_t window_right,
+                                uint32_t sinks, uint32_t flags, const uint32_t* prefill_seqs,
+                                uint32_t n_prefill, const vapi_kv_prefixes* prefixes,
+                                void* workspace, size_t workspace_bytes, vapi_stream_t stream) {
+  if (n_prefill > batch)
+    VK_FAIL(VAPI_KV_EINVAL, "vapi_paged_attention_shared: %u prefill sequences in a batch of %u",
+            n_prefill, batch);
+  if (n_prefill && !prefill_seqs)
+    VK_FAIL(VAPI_KV_EINVAL, "vapi_paged_attention_shared: null prefill_seqs");
+  if (!prefixes) VK_FAIL(VAPI_KV_EINVAL, "vapi_paged_attention_shared: null prefixes");
+  const PrefillSeqs pf{prefill_seqs, n_prefill};
+  return paged_attention_impl(pool, layer, q, out, cu_seqlens_q, cu_seqlens_k, block_table, batch,
+                              max_blocks, max_seqlen_q, max_seqlen_k, num_heads, scale,
+                              window_left, window_right, workspace, workspace_bytes, stream,
+                              nullptr, flags, prefill_seqs ? &pf : nullptr, sinks, false, prefixes);
 }
 
 int vapi_paged_attention_append_sinks(
@@ -437,7 +483,8 @@ static int paged_attention_impl(const vapi_kv_pool* pool, uint32_t layer, const 
                                 int32_t window_left, int32_t window_right, void* workspace,
                                 size_t workspace_bytes, vapi_stream_t stream,
                                 const NewRows* fuse, uint32_t flags, const PrefillSeqs* pf,
-                                uint32_t sinks, bool checks_only) {
+                                uint32_t sinks, bool checks_only,
+                                const vapi_kv_prefixes* prefixes) {
   if (int rc = check_pool(pool, "vapi_paged_attention")) return rc;
   if (!pool->v) VK_FAIL(VAPI_KV_EINVAL, "vapi_paged_attention: a K-only pool has no V to attend over");
   if (layer >= pool->num_layers)
@@ -482,8 +529,21 @@ static int paged_attention_impl(const vapi_kv_pool* pool, uint32_t layer, const 
       prefill_f32_items(pf_n, pool->num_kv_heads, num_heads / pool->num_kv_heads,
                         max_seqlen_q) > (sinks ? 0x7FFFFFFFull : 0xFFFFFFFFull))
     VK_FAIL(VAPI_KV_EUNSUP, "vapi_paged_attention: prefill batch too large for one launch");
-  const size_t need =
+  size_t need =
       required_workspace(pool, batch, num_heads, max_seqlen_q, max_seqlen_k, skip_decode);
+  const size_t shared_off = shared_offset(pool, batch, num_heads);
+  const uint32_t shared_pf = max_seqlen_q > 1 ? pf_n : 0;
+  if (prefixes) {
+    if (!mfma16_ok(pool, num_heads))
+      VK_FAIL(VAPI_KV_EUNSUP, "vapi_paged_attention_shared: not a 16-bit pool of a head_dim and "
+              "block_size that it takes");
+    const uint32_t G = num_heads / pool->num_kv_heads, D = decode_dim(pool->head_dim);
+    if (int rc = shared_check(prefixes, batch, pool->num_kv_heads, G, D, shared_pf, max_seqlen_q,
+                              max_seqlen_k, "vapi_paged_attention_shared"))
+      return rc;
+    need = shared_off + shared_workspace_bytes(prefixes, batch, pool->num_kv_heads, G, D, shared_pf,
+                                               max_seqlen_q);
+  }
   if (workspace_bytes < need || (need && !workspace))
     VK_FAIL(VAPI_KV_ESPACE, "vapi_paged_attention: workspace %zu bytes < %zu",
             workspace_bytes, need);
@@ -538,6 +598,7 @@ static int paged_attention_impl(const vapi_kv_pool* pool, uint32_t layer, const 
   a.wl = window_arg(window_left);
   a.wr = window_arg(window_right);
   a.sinks = sinks_arg(sinks, a.wl);
+  a.shared = nullptr;
   a.deterministic = (flags & VAPI_ATTN_DETERMINISTIC) ? 1u : 0u;
   a.pf_min_q = 2;
   a.pf_seqs = listed ? pf->seqs : nullptr;
@@ -561,6 +622,19 @@ static int paged_attention_impl(const vapi_kv_pool* pool, uint32_t layer, const 
     const bool bf16 = pool->dtype == VAPI_KV_BF16;
     const uint32_t D = decode_dim(g.d);
     a.num_waves = decode_num_waves();
+    if (prefixes) {
+      dec.num_waves = a.num_waves;
+      dec.shared = prefixes->start;
+      dec.pf_min_q = skip_decode ? 1 : 2;
+      decode_bind(dec, workspace, D);
+      const SharedArgs sh =
+          shared_args(prefixes, dec, D, shared_pf, max_seqlen_q, (char*)workspace + shared_off);
+      if (!skip_decode) launch_decode_shared(dec, D, bf16, s);
+      launch_shared_tiles(dec, sh, D, bf16, s);
+      launch_shared_merge(dec, sh, D, bf16, !skip_decode, s);
+      VK_LAUNCHED("paged_attention_shared");
+      return 0;
+    }
     const size_t off = std::max<size_t>((need + 255) & ~(size_t)255, 256);
     const bool room = workspace && workspace_bytes > off;
     // Decode rows and prefill rows in one step: both kernels in one launch.

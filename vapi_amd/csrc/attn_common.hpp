@@ -78,6 +78,9 @@ struct AttnArgs {
   uint32_t q_sign;     // 0x80008000 when scale < 0: XOR into packed 16-bit Q words
   int32_t wl, wr;
   int32_t sinks;  // first keys that wl does not hide (0 without a left window)
+  // Keys at the front of each sequence that another kernel attends for a group of
+  // them (null: none); their partials and this sequence's are joined afterwards.
+  const uint32_t* shared;
   uint32_t deterministic;  // decode: fixed equal XCD shares, no share update
   uint32_t pf_min_q;       // prefill: rows with len_q >= this (2, or 1 when no decode launch)
   // prefill: the sequences its grid covers, u32[pf_seqs_n] (null: 0 ..

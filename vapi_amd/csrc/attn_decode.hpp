@@ -60,17 +60,40 @@ constexpr uint32_t kBalStats = 64;
 constexpr uint32_t kMinStepsPerWave = 8;  // launches that move the shares
 constexpr uint32_t kStatWords = 4;
 
+// What a decode row of sequence s attends here: keys [lo, len_k) and the first
+// `sinks`. The shared keys of a sequence are attended elsewhere, its sinks with
+// them (shared_keys).
+struct RowSpan {
+  int32_t lo, sinks;
+  uint32_t shared;
+};
+// The keys that sequences share, of `keys` named: none where sinks pass them.
+__device__ __forceinline__ int32_t shared_keys(const AttnArgs& a, uint32_t keys) {
+  return (int32_t)keys < a.sinks ? 0 : (int32_t)keys;
+}
+template <bool kShared>
+__device__ __forceinline__ RowSpan row_span(const AttnArgs& a, uint32_t s, int32_t len_k) {
+  RowSpan w{a.wl >= 0 ? max(0, len_k - 1 - a.wl) : 0, a.sinks, 0u};
+  if constexpr (kShared) {
+    const int32_t n = shared_keys(a, a.shared[s]);
+    if (n > 0) w.lo = max(w.lo, n), w.sinks = 0, w.shared = 1;
+  }
+  return w;
+}
+
 // Steps of sequence s (0 for rows that are not decode rows). KS: keys per step
 // (a power of two; 32 but for the streams of 8-bit pools).
-template <int KS = 32, bool kSinks = false>
+// (kShared: the steps past its shared keys.)
+template <int KS = 32, bool kSinks = false, bool kShared = false>
 __device__ __forceinline__ uint32_t decode_steps(const AttnArgs& a,
                                                  const uint32_t* __restrict__ cu_q,
                                                  const uint32_t* __restrict__ cu_k, uint32_t s) {
   if (cu_q[s + 1] - cu_q[s] != 1) return 0;
   const int32_t len_k = (int32_t)(cu_k[s + 1] - cu_k[s]);
   if (len_k <= 0) return 0;
-  const int32_t lo = a.wl >= 0 ? max(0, len_k - 1 - a.wl) : 0;
-  const KeySteps<kSinks> ks(lo, len_k - 1, a.sinks, KS);
+  const RowSpan w = row_span<kShared>(a, s, len_k);
+  if (kShared && w.lo >= len_k) return 0;
+  const KeySteps<kSinks> ks(w.lo, len_k - 1, w.sinks, KS);
   return (uint32_t)(ks.last - ks.start) / KS + 1;
 }
 
@@ -144,7 +167,8 @@ __device__ __forceinline__ void group_bounds(const float (&w)[kGroups], uint32_t
 // Where global step t lives.
 struct DecodePos {
   uint32_t seq, kh, q0;
-  int32_t key0, len_k, lo;
+  int32_t key0, len_k, lo, sinks;
+  uint32_t shared;     // its front keys are attended elsewhere
   uint32_t seg_first;  // key0 is the segment's first step (a word, not a bool: no stack copy)
   uint32_t fuse;       // fused append: key len_k - 1 is read from the new rows
 };
@@ -152,7 +176,7 @@ struct DecodePos {
 // kvh_plan: the kv heads the step order counts (a.kvh, or with a split
 // group's parts side by side the pool heads: then the position is part
 // `part` of pool head kp, virtual head kp * n + part).
-template <int KS = 32, bool kSinks = false>
+template <int KS = 32, bool kSinks = false, bool kShared = false>
 __device__ __forceinline__ DecodePos locate(const AttnArgs& a, const uint32_t* __restrict__ cu_q,
                                             const uint32_t* __restrict__ cu_k, const uint32_t* P,
                                             const uint32_t* FZ, uint32_t t,
@@ -173,8 +197,9 @@ __device__ __forceinline__ DecodePos locate(const AttnArgs& a, const uint32_t* _
   const uint32_t ks = local - kp * nst;
   p.q0 = cu_q[p.seq];
   p.len_k = (int32_t)(cu_k[p.seq + 1] - cu_k[p.seq]);
-  p.lo = a.wl >= 0 ? max(0, p.len_k - 1 - a.wl) : 0;
-  const KeySteps<kSinks> steps(p.lo, p.len_k - 1, a.sinks, KS);
+  const RowSpan w = row_span<kShared>(a, p.seq, p.len_k);
+  p.lo = w.lo, p.sinks = w.sinks, p.shared = w.shared;
+  const KeySteps<kSinks> steps(p.lo, p.len_k - 1, p.sinks, KS);
   p.key0 = steps.key(steps.start + KS * (int32_t)ks);
   p.seg_first = ks == 0;
   p.fuse = FZ ? FZ[lo_i] : 0u;
@@ -185,7 +210,7 @@ __device__ __forceinline__ DecodePos locate(const AttnArgs& a, const uint32_t* _
 // or kv head 0 of the next sequence that has decode steps. A wave's slice
 // is contiguous, so the step after a segment's last is always this one,
 // and a wave that moves on from a finished segment needs no search.
-template <int KS = 32, bool kSinks = false>
+template <int KS = 32, bool kSinks = false, bool kShared = false>
 __device__ __forceinline__ DecodePos next_segment(const AttnArgs& a,
                                                   const uint32_t* __restrict__ cu_q,
                                                   const uint32_t* __restrict__ cu_k,
@@ -204,10 +229,11 @@ __device__ __forceinline__ DecodePos next_segment(const AttnArgs& a,
     p.kh = cur.kh % n;
     p.q0 = cu_q[s];
     p.len_k = (int32_t)(cu_k[s + 1] - cu_k[s]);
-    p.lo = a.wl >= 0 ? max(0, p.len_k - 1 - a.wl) : 0;
+    const RowSpan w = row_span<kShared>(a, s, p.len_k);
+    p.lo = w.lo, p.sinks = w.sinks, p.shared = w.shared;
     p.fuse = FZ ? FZ[s] : 0u;
   }
-  p.key0 = kSinks ? 0 : p.lo & ~(KS - 1);
+  p.key0 = kSinks && p.sinks ? 0 : p.lo & ~(KS - 1);
   p.seg_first = 1u;
   return p;
 }
@@ -331,9 +357,10 @@ __device__ __forceinline__ void flush_piece(const AttnArgs& a, const DecodePos& 
 // loads; ordinary ones for a group split into virtual kv heads, whose
 // parts read the same tiles at about the same time on one XCD (the plan
 // puts a pool head's parts side by side), so all but the first hit in L2.
-// kSinks: a.sinks keys (at least one) before the left window.
+// kSinks: a.sinks keys may stay visible before the left window. kShared: a.shared
+// says which keys are not attended here; their rows' results are all partials.
 template <typename T, int D, bool kFuse, bool kPad = false, int DL = D / 16, bool kNt = true,
-          bool kSinks = false>
+          bool kSinks = false, bool kShared = false>
 __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
                                                    const uint32_t* __restrict__ cu_q,
                                                    const uint32_t* __restrict__ cu_k,
@@ -361,7 +388,7 @@ __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
     const uint32_t per = (B + NT - 1) / NT;
     const uint32_t b0 = min(tid * per, B), b1 = min(b0 + per, B);
     uint32_t sum = 0;
-    for (uint32_t s = b0; s < b1; ++s) sum += decode_steps<32, kSinks>(a, cu_q, cu_k, s) * kvh_plan;
+    for (uint32_t s = b0; s < b1; ++s) sum += decode_steps<32, kSinks, kShared>(a, cu_q, cu_k, s) * kvh_plan;
     uint32_t inc = sum;  // inclusive scan within the wave
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -374,7 +401,7 @@ __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
     for (uint32_t w = 0; w < wave; ++w) run += wave_tot[w];
     for (uint32_t s = b0; s < b1; ++s) {
       P[s] = run;
-      const uint32_t ns = decode_steps<32, kSinks>(a, cu_q, cu_k, s);
+      const uint32_t ns = decode_steps<32, kSinks, kShared>(a, cu_q, cu_k, s);
       run += ns * kvh_plan;
       if (kFuse) FZ[s] = ns ? fused_row(a, cu_q, cu_k, table, s) : 0u;
     }
@@ -416,7 +443,7 @@ __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
 
   uint32_t t = t_begin;
   const uint32_t col = lane & 15, g = lane >> 4;
-  DecodePos pos = locate<32, kSinks>(a, cu_q, cu_k, P, FZ, t, kvh_plan, n_parts, part);
+  DecodePos pos = locate<32, kSinks, kShared>(a, cu_q, cu_k, P, FZ, t, kvh_plan, n_parts, part);
   // The Q^T operand of the current segment lives in LDS (read back every
   // step) to keep the K/V buffers in registers.
   constexpr bool kF32 = sizeof(T) == 4;
@@ -469,17 +496,17 @@ __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
     // and hold the wave's end for a memory round trip.
     DecodePos nxt = pos;
     if (same_piece) {
-      nxt.key0 = next_step<kSinks>(pos.key0, pos.lo, a.sinks);
+      nxt.key0 = next_step<kSinks>(pos.key0, pos.lo, pos.sinks);
       nxt.seg_first = false;
     } else if (more) {
-      nxt = next_segment<32, kSinks>(a, cu_q, cu_k, P, FZ, pos, n_parts);
+      nxt = next_segment<32, kSinks, kShared>(a, cu_q, cu_k, P, FZ, pos, n_parts);
     } else {
       nxt.seq = 0;
       nxt.key0 = 0;
       nxt.len_k = 1;
       nxt.fuse = 0;
     }
-    const int32_t lo = pos.lo, len_k = pos.len_k, key0 = pos.key0;
+    const int32_t lo = pos.lo, len_k = pos.len_k, key0 = pos.key0, sinks = pos.sinks;
     if constexpr (kF32) {
       // kn, vn are kc, vc: each half is refilled with the next step's once
       // it has been computed (16 KiB in flight per wave, as 16-bit steps).
@@ -495,14 +522,14 @@ __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
         if (kSinks && key0 < lo) {  // (see below)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (!row_sees<kSinks>(key0 + 16 * tt + 4 * (int32_t)g + i, lo, len_k, a.sinks))
+            if (!row_sees<kSinks>(key0 + 16 * tt + 4 * (int32_t)g + i, lo, len_k, sinks))
 #pragma unroll
               for (int h = 0; h < D / 64; ++h)
                 vc.h[tt].v[i][h] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
         attend_half_f32<D, DL>(kc.h[tt], vc.h[tt], qf, o, m_run, l_run, a.scale_log2, [&](int i) {
           const int32_t key = key0 + 16 * tt + 4 * (int32_t)g + i;
-          return row_sees<kSinks>(key, lo, len_k, a.sinks);
+          return row_sees<kSinks>(key, lo, len_k, sinks);
         });
         load_halves(kn, vn, nxt, tt);
       }
@@ -514,14 +541,14 @@ __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
       for (int c = 0; c < D / 32; ++c) qf[c] = qs[c * 64 + lane];
       const uint4 pf = attend_qk<T, D, KCL>(kc, qf, o, m_run, l_run, a.scale_log2, g, [&](int tt, int i) {
         const int32_t key = key0 + 16 * tt + 4 * (int32_t)g + i;
-        return row_sees<kSinks>(key, lo, len_k, a.sinks);
+        return row_sees<kSinks>(key, lo, len_k, sinks);
       });
       // Between the sinks and the window keys weigh 0, whatever their V holds
       // (infinities too).
       if (kSinks && key0 < lo) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (!row_sees<kSinks>(key0 + 16 * (j >> 2) + 4 * (int32_t)g + (j & 3), lo, len_k, a.sinks))
+          if (!row_sees<kSinks>(key0 + 16 * (j >> 2) + 4 * (int32_t)g + (j & 3), lo, len_k, sinks))
 #pragma unroll
             for (int w = 0; w < DPL / 2; ++w) vc.v[j].w[w] = 0u;
       }
@@ -533,8 +560,8 @@ __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
         if (piece_first) a.seg_ranges[2 * seg] = r;
         if (seg_ends) a.seg_ranges[2 * seg + 1] = r;
       }
-      flush_piece<T, D, kPad>(a, pos, piece_first && seg_ends, r * n_parts + seg, o, m_run, l_run,
-                              col, g);
+      flush_piece<T, D, kPad>(a, pos, piece_first && seg_ends && !(kShared && pos.shared),
+                              r * n_parts + seg, o, m_run, l_run, col, g);
       if (!more) return false;
       m_run = kNegBig;
       l_run = 0.f;
@@ -688,7 +715,8 @@ __device__ __forceinline__ void store_outputs(T* dst, uint32_t n, const float (&
 // combined through LDS.
 // Workgroup `bid` of `nbid` (kMergeWaves waves); workgroups from merge_wgs
 // on copy the fused append's new rows.
-template <typename T, int D, bool kFuse, int WPS, bool kPad = false>
+// (kShared: the rows with shared keys are joined elsewhere.)
+template <typename T, int D, bool kFuse, int WPS, bool kPad = false, bool kShared = false>
 __device__ __forceinline__ void decode_merge_body(const AttnArgs& a, uint32_t nwg,
                                                   uint32_t merge_wgs, uint32_t bid,
                                                   uint32_t nbid, uint32_t ns = 1) {
@@ -727,6 +755,7 @@ __device__ __forceinline__ void decode_merge_body(const AttnArgs& a, uint32_t nw
   const bool skip = (q1 - q0 != 1) | ((int32_t)(k1 - k0) <= 0) | (r0 >= r1) |
                     (r1 >= nwg * kDecodeWavesPerWG);
   if (skip) return;
+  if (kShared && shared_keys(a, a.shared[seq]) > 0) return;
   const uint32_t G = a.group, seg = segi;
   const uint32_t E = G * D / 64 / ns;
   const uint32_t e_lane = (slice * 64 + lane) * E;

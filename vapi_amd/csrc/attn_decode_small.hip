@@ -117,7 +117,7 @@ __global__ __launch_bounds__(64 * kSmallWaves, 1) void paged_decode_small(
   p.len_k = (int32_t)(cu_k[p.seq + 1] - cu_k[p.seq]);
   if (cu_q[p.seq + 1] - p.q0 != 1 || p.len_k <= 0) return;
   const int32_t lo = a.wl >= 0 ? max(0, p.len_k - 1 - a.wl) : 0, len_k = p.len_k;
-  p.lo = lo;
+  p.lo = lo, p.sinks = a.sinks, p.shared = 0;
   // This workgroup's steps: all of the row's, or its split's, by position.
   const KeySteps<kSinks> ks(lo, len_k - 1, a.sinks, 32);
   int32_t at = ks.start, end = ks.last + 32;

@@ -23,92 +23,6 @@
 
 namespace vk {
 
-// ---- K and V staged by direct global-to-LDS loads --------------------------
-//
-// Rows keep the pool's order (key rows of D elements); each row's 16-byte
-// chunks are XOR-swizzled by a function of the row index (pf_swz) so that
-// the fragment reads below spread over the LDS banks. V^T fragments for O^T = V^T P^T are read
-// transposed from the V rows with ds_read_b64_tr_b16: for a 16-lane group,
-// lane i receives element i % 4 of the 64-bit chunk addressed by lane
-// 4 j + i / 4, for j = 0..3 (measured on gfx950), so lane 4 j + q pointing
-// at key row k0 + j, columns 4 q .. 4 q + 3 hands lane i the column of d
-// (i) over keys k0 .. k0 + 3. A d tile of 16 columns then lands in the
-// MFMA's A rows in order (d = 16 t + m), and the output O^T holds row col
-// at d = 16 t + 4 g + i.
-// Issues the step at s0 into buffer b with W waves (8, or 4 in the mixed
-// launch): each thread moves D / (16 W) 16-byte chunks of K and as many of
-// V (D = 128, 256), or with 8 waves one of K or V (D = 64: waves 0-3 K,
-// waves 4-7 V), with 4 waves one of each. LDS slot t of a tensor holds the chunk its swizzled
-// position names; a wave's 64 slots are contiguous, as the load writes them.
-// rd: what is read for keys hidden from every row.
-// kPad (a head_dim a.hd below D, a multiple of 8): a chunk at or past a.hd
-// lies outside the key's row, so its slot is filled from the row's chunk 0
-// instead (the K fragment reads zero those chunks; the V columns past a.hd
-// only reach output columns that are never stored).
-template <typename T, int D, int W, bool kPad, typename Reads>
-__device__ __forceinline__ void pf_dma(uint16_t* kdst, uint16_t* vdst, const uint32_t* __restrict__ tab,
-                                       const T* kb, const T* vb, const AttnArgs& a, int32_t s0,
-                                       const Reads& rd, uint32_t tid, uint32_t wave) {
-  constexpr uint32_t CPR = D / 8;
-  using ConstU32 = const __attribute__((address_space(4))) uint32_t;
-  const int32_t ts0 = rd.tile(s0), ts1 = rd.tile(s0 + 16);
-  const uint32_t c0 = min((uint32_t)ts0 >> a.bs_shift, a.max_blocks - 1);
-  const uint32_t c1 = min((uint32_t)ts1 >> a.bs_shift, a.max_blocks - 1);
-  const uint32_t blk0 = min(((ConstU32*)tab)[c0], a.last_blk);
-  const uint32_t blk1 = min(((ConstU32*)tab)[c1], a.last_blk);
-  const uint64_t off0 = (uint64_t)blk0 * a.blk_e + (uint64_t)((uint32_t)ts0 & (a.block_size - 1)) * a.tok_e;
-  const uint64_t off1 = (uint64_t)blk1 * a.blk_e + (uint64_t)((uint32_t)ts1 & (a.block_size - 1)) * a.tok_e;
-  auto one = [&](const T* base_t, uint16_t* buf, uint32_t slot, uint32_t wslot0)
-                 __attribute__((always_inline)) {
-    const uint32_t r = slot / CPR, pos = slot % CPR;
-    uint32_t p = pos ^ pf_swz<D>(r);
-    if (kPad && 8 * p >= a.hd) p = 0;
-    // A wave's slots cover 64 / CPR whole rows of one 16-key tile.
-    const bool second = __builtin_amdgcn_readfirstlane(r) >= 16;
-    const T* base = base_t + (second ? off1 : off0);
-    const uint32_t kk = rd.row((int32_t)(r & 15), second ? ts1 : ts0);
-    __builtin_amdgcn_global_load_lds((const void*)(base + kk * a.tok_e + 8 * p),
-                                     (LdsVoid*)(buf + wslot0 * 8), 16, 0, 0);
-  };
-  if constexpr (D >= 128) {
-#pragma unroll
-    for (int j = 0; j < D / (16 * W); ++j) {
-      one(kb, kdst, tid + 64 * W * j, 64 * wave + 64 * W * j);
-      one(vb, vdst, tid + 64 * W * j, 64 * wave + 64 * W * j);
-    }
-  } else if constexpr (W == 8) {
-    if (wave < 4) one(kb, kdst, tid, 64 * wave);
-    else one(vb, vdst, tid - 256, 64 * (wave - 4));
-  } else {
-    one(kb, kdst, tid, 64 * wave);
-    one(vb, vdst, tid, 64 * wave);
-  }
-}
-
-// Four ds_read_b64_tr_b16 issued without waiting (results valid only after
-// a later lgkm wait that names the same registers).
-__device__ __forceinline__ void ds_read_tr16_issue4(uint2 (&r)[4], const uint32_t (&addr)[4]) {
-  __asm__ volatile(
-      "ds_read_b64_tr_b16 %0, %4\n\t"
-      "ds_read_b64_tr_b16 %1, %5\n\t"
-      "ds_read_b64_tr_b16 %2, %6\n\t"
-      "ds_read_b64_tr_b16 %3, %7"
-      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
-      : "v"(addr[0]), "v"(addr[1]), "v"(addr[2]), "v"(addr[3])
-      : "memory");
-}
-// Waits until at most N LDS/scalar-memory operations are in flight; the
-// registers of the batch that completes are named so that no use of them
-// moves above the wait.
-template <int N>
-__device__ __forceinline__ void lgkm_wait(uint2 (&r)[4]) {
-  __asm__ volatile("s_waitcnt lgkmcnt(%4)"
-                   : "+v"(r[0]), "+v"(r[1]), "+v"(r[2]), "+v"(r[3])
-                   : "n"(N)
-                   : "memory");
-}
-
-
 // One item (W waves): query tile it.qt of a sequence and kv head. kSplit 0:
 // all of it, to the output (compiled without the shares' arithmetic); 1: its
 // steps [u0, u1) of c shares, the rows' (m, l, o) to the partial `pb`; 2: the

@@ -178,7 +178,7 @@ __device__ __forceinline__ void q8_attend(const Q8Step<D, KS>& st, const uint4 (
 
 // The stream: decode_stream_body's plan and pieces over 8-bit steps. (The plan is
 // written out here, without the fused append: what changes there changes here.)
-template <typename T, int F, int D, bool kPad, bool kNt, bool kSinks>
+template <typename T, int F, int D, bool kPad, bool kNt, bool kSinks, bool kShared = false>
 __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void q8_decode_stream(
     AttnArgs a, Q8Scales sc, const uint32_t* __restrict__ cu_q, const uint32_t* __restrict__ cu_k,
     const uint32_t* __restrict__ table) {
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void q8_de
     const uint32_t per = (B + NT - 1) / NT;
     const uint32_t b0 = min(tid * per, B), b1 = min(b0 + per, B);
     uint32_t sum = 0;
-    for (uint32_t s = b0; s < b1; ++s) sum += decode_steps<KS, kSinks>(a, cu_q, cu_k, s) * kvh_plan;
+    for (uint32_t s = b0; s < b1; ++s) sum += decode_steps<KS, kSinks, kShared>(a, cu_q, cu_k, s) * kvh_plan;
     uint32_t inc = sum;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void q8_de
     for (uint32_t w = 0; w < wave; ++w) run += wave_tot[w];
     for (uint32_t s = b0; s < b1; ++s) {
       P[s] = run;
-      run += decode_steps<KS, kSinks>(a, cu_q, cu_k, s) * kvh_plan;
+      run += decode_steps<KS, kSinks, kShared>(a, cu_q, cu_k, s) * kvh_plan;
     }
     if (tid == NT - 1) P[B] = run;
     __syncthreads();
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void q8_de
   const uint32_t t_end = bounds[x] + (uint32_t)(((uint64_t)(jr + 1) * len) / nr);
 
   uint32_t t = t_begin;
-  DecodePos pos = locate<KS, kSinks>(a, cu_q, cu_k, P, nullptr, t, kvh_plan, n_parts, part);
+  DecodePos pos = locate<KS, kSinks, kShared>(a, cu_q, cu_k, P, nullptr, t, kvh_plan, n_parts, part);
   uint4* qs = q_lds[wave];
   q8_load_q<T, D, kPad>(qs, a, pos, lane, col, g);
   bool piece_first = pos.seg_first;
@@ -256,10 +256,10 @@ __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void q8_de
     // (The last step's loads point at one cached row, as in the 16-bit stream.)
     DecodePos nxt = pos;
     if (same_piece) {
-      nxt.key0 = next_step<kSinks, KS>(pos.key0, pos.lo, a.sinks);
+      nxt.key0 = next_step<kSinks, KS>(pos.key0, pos.lo, pos.sinks);
       nxt.seg_first = false;
     } else if (more) {
-      nxt = next_segment<KS, kSinks>(a, cu_q, cu_k, P, nullptr, pos, n_parts);
+      nxt = next_segment<KS, kSinks, kShared>(a, cu_q, cu_k, P, nullptr, pos, n_parts);
     } else {
       nxt.seq = 0;
       nxt.key0 = 0;
@@ -270,15 +270,15 @@ __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void q8_de
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) qf[c] = qs[c * 64 + lane];
     q8_attend<T, F, D, KS, true, kSinks>(cur, qf, o, m_run, l_run, a.scale_log2, pos.key0, pos.lo,
-                                 pos.len_k, a.sinks, g);
+                                         pos.len_k, pos.sinks, g);
     if (!same_piece) {
       const uint32_t seg = pos.seq * a.kvh + pos.kh;
       if (lane == 0) {
         if (piece_first) a.seg_ranges[2 * seg] = r;
         if (seg_ends) a.seg_ranges[2 * seg + 1] = r;
       }
-      flush_piece<T, D, kPad>(a, pos, piece_first && seg_ends, r * n_parts + seg, o, m_run, l_run,
-                              col, g);
+      flush_piece<T, D, kPad>(a, pos, piece_first && seg_ends && !(kShared && pos.shared),
+                              r * n_parts + seg, o, m_run, l_run, col, g);
       if (!more) return false;
       m_run = kNegBig;
       l_run = 0.f;
