@@ -373,7 +373,7 @@ typedef struct vapi_kv_prefixes {
  * tables differ attends the first one's blocks.
  *
  * f16 and bf16 pools with head_dim a multiple of 8 up to 256 and block_size a power of
- * two from 16, up to 256 query heads per kv head, 4,096 sequences and 4,096 groups and
+ * two from 16, up to 256 query heads per kv head, 4,096 sequences and 1,024 groups and
  * prefill sequences together (else VAPI_KV_EUNSUP: such a batch runs
  * vapi_paged_attention_sinks). The workspace has no optional part: all that
  * vapi_paged_attention_shared_workspace_size returns, by the same rules as
@@ -716,6 +716,24 @@ int vapi_kv_q8_attention_sinks(const vapi_kv_q8_pool* pool, uint32_t layer, cons
                                int32_t window_left, int32_t window_right, uint32_t sinks,
                                uint32_t flags, const uint32_t* prefill_seqs, uint32_t n_prefill,
                                void* workspace, size_t workspace_bytes, vapi_stream_t stream);
+
+/* vapi_kv_q8_attention over a batch with shared prefixes (see
+ * vapi_paged_attention_shared). The shared keys' codes, and those of the listed
+ * prefill sequences' own keys, are expanded in the workspace once: n_groups *
+ * max_keys and n_prefill * max_seqlen_k keys of the layer in the pool's dtype. */
+size_t vapi_kv_q8_attention_shared_workspace_size(const vapi_kv_q8_pool* pool, uint32_t batch,
+                                                  uint32_t n_prefill, uint32_t num_heads,
+                                                  uint32_t max_seqlen_q, uint32_t max_seqlen_k,
+                                                  const vapi_kv_prefixes* prefixes);
+int vapi_kv_q8_attention_shared(const vapi_kv_q8_pool* pool, uint32_t layer, const void* q,
+                                void* out, const uint32_t* cu_seqlens_q,
+                                const uint32_t* cu_seqlens_k, const uint32_t* block_table,
+                                uint32_t batch, uint32_t max_blocks, uint32_t max_seqlen_q,
+                                uint32_t max_seqlen_k, uint32_t num_heads, float scale,
+                                int32_t window_left, int32_t window_right, uint32_t sinks,
+                                uint32_t flags, const uint32_t* prefill_seqs, uint32_t n_prefill,
+                                const vapi_kv_prefixes* prefixes, void* workspace,
+                                size_t workspace_bytes, vapi_stream_t stream);
 
 /* ---- attention weights and eviction ---------------------------------------- */
 

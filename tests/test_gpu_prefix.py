@@ -65,7 +65,7 @@ def make(groups, alone, heads, kvh, d, dtype, bs=16, layout="HND", fmt="none", s
 
 def prepare(batch, cache, heads, plan, deterministic=False):
     prep = PreparedAttention.from_batch(batch, DEV, deterministic=deterministic)
-    prep.prefixes = PrefixPlan(plan, batch.cu_seqlens_q, batch.batch_size(), DEV)
+    prep.prefixes = PrefixPlan(plan, batch.cu_seqlens_q, batch.cu_seqlens_k, DEV)
     return prep
 
 
@@ -85,7 +85,9 @@ def decode(n, lo, hi, seed):
 
 GEOMETRIES = [(8, 2, 128, BF16, "none"), (4, 4, 64, F16, "none"), (6, 2, 256, BF16, "none"),
               (3, 1, 96, F16, "none"), (28, 4, 128, BF16, "none"), (71, 1, 64, BF16, "none"),
-              (16, 1, 80, F16, "none"), (33, 1, 256, F16, "none")]
+              (16, 1, 80, F16, "none"), (33, 1, 256, F16, "none"),
+              (8, 2, 128, BF16, "e4m3"), (4, 4, 64, F16, "int8"), (40, 2, 80, BF16, "int8"),
+              (6, 2, 256, F16, "e4m3")]
 
 
 @pytest.mark.parametrize("heads,kvh,d,dtype,fmt", GEOMETRIES)
@@ -109,7 +111,7 @@ def test_several_queries_and_mixed_steps(heads, kvh, d, dtype, fmt):
 
 
 @pytest.mark.parametrize("left,sinks", [(20, 0), (20, 3), (130, 8), (300, 50), (40, 200), (1000, 1)])
-@pytest.mark.parametrize("heads,kvh,d,dtype,fmt", GEOMETRIES[:4])
+@pytest.mark.parametrize("heads,kvh,d,dtype,fmt", GEOMETRIES[:4] + GEOMETRIES[8:10])
 def test_windows_and_sinks(left, sinks, heads, kvh, d, dtype, fmt):
     """Windows that hide some of the prefix, all of it, or part of it from some
     sequences; sinks that pass a short prefix."""
@@ -191,13 +193,20 @@ def test_equal_calls_give_equal_bits():
 
 
 def test_the_step_finds_its_prefixes():
-    cache, q, batch, plan = make([(40, decode(6, 1, 200, 1)), (70, decode(3, 1, 20, 2))],
+    cache, q, batch, plan = make([(200, decode(60, 1, 200, 1)), (70, decode(3, 1, 20, 2))],
                                  decode(3, 1, 400, 3), 8, 2, 128, F16)
     prep = PreparedAttention.from_batch(batch, DEV, cache, 8, share_prefixes=True)
     assert sorted((sorted(m), n) for m, n in prep.prefixes.groups) == sorted(
         (sorted(m), n) for m, n in plan)
+    # 59 x 3,200 keys of 1 KiB are worth it; not behind a short window.
+    assert prep.shared_bytes(cache, 8) > 0 and prep.shared_bytes(cache, 8, 100) == 0
     got = paged_attention_prepared(q, cache, 0, prep, 0.1)
     assert_close(got, reference(q, cache, batch, 0.1, None, 0, 0), F16)
+    few = make([(40, decode(6, 1, 200, 1))], [], 8, 2, 128, F16)
+    prep = PreparedAttention.from_batch(few[2], DEV, few[0], 8, share_prefixes=True)
+    assert prep.prefixes is not None and prep.shared_bytes(few[0], 8) == 0
+    got = paged_attention_prepared(few[1], few[0], 0, prep, 0.1)
+    assert_close(got, reference(few[1], few[0], few[2], 0.1, None, 0, 0), F16)
     # Nothing to share: the ordinary call.
     lone = make([], decode(3, 1, 400, 3), 8, 2, 128, F16)
     assert PreparedAttention.from_batch(lone[2], DEV, lone[0], 8,
@@ -207,13 +216,17 @@ def test_the_step_finds_its_prefixes():
 def test_pools_that_take_no_prefixes_run_the_ordinary_call():
     cache, q, batch, plan = make([(70, decode(6, 1, 200, 1))], [(1, 30)], 8, 2, 64, F32)
     prep = PreparedAttention.from_batch(batch, DEV, cache, 8, share_prefixes=True)
-    assert prep.prefixes is not None and prep.shared_bytes(cache, 8) == 0
+    prep.prefixes.min_bytes = (0, 0)  # whatever it saves
+    prep.sharing.clear()
+    assert prep.shared_bytes(cache, 8) == 0 and b"16-bit" in lib().vapi_kv_last_error()
     got = paged_attention_prepared(q, cache, 0, prep, 0.1)
     assert_close(got, reference(q, cache, batch, 0.1, None, 0, 0), F32)
 
 
-def test_a_write_and_its_attention():
-    cache, q, batch, plan = make([(20, [(1, 20), (1, 33), (4, 9)])], [(1, 50)], 8, 2, 64, BF16)
+@pytest.mark.parametrize("fmt", ["none", "e4m3"])
+def test_a_write_and_its_attention(fmt):
+    cache, q, batch, plan = make([(20, [(1, 20), (1, 33), (4, 9)])], [(1, 50)], 8, 2, 64, BF16,
+                                 fmt=fmt)
     cq, ck = batch.cu_seqlens_q, batch.cu_seqlens_k
     slots = [t[p // 16] * 16 + p % 16 for i, t in enumerate(batch.block_tables)
              for p in range(ck[i + 1] - ck[i] - (cq[i + 1] - cq[i]), ck[i + 1] - ck[i])]
@@ -241,6 +254,10 @@ def test_layers_of_different_geometry_in_one_step():
                          max_seqlen_q=1, max_seqlen_k=850)
     prep = PreparedAttention.from_batch(batch, DEV, cache, 4, share_prefixes=True)
     assert prep.prefixes.groups == [([0, 1, 2], 800)]
+    prep.prefixes.min_bytes = (0, 0)  # whatever it saves
+    prep.sharing.clear()
+    prep.reserve(cache, 4, DEV)
+    assert all(prep.sharing.values())
     for layer, (kvh, d) in enumerate(((2, 64), (1, 128), (2, 256))):
         one = PagedKvCache(1, 80, 16, kvh, d, BF16)
         one.k[0].copy_(cache.k[layer])
@@ -332,7 +349,7 @@ def test_refusals():
         PreparedAttention.from_batch(batch, DEV, share_prefixes=True)
     for bad in ([([0, 0], 64)], [([0, 1], 64), ([1], 16)], [([0, 2], 64)], [([0, 1], 0)]):
         with pytest.raises(ValueError):
-            PrefixPlan(bad, batch.cu_seqlens_q, 2, DEV)
+            PrefixPlan(bad, batch.cu_seqlens_q, batch.cu_seqlens_k, DEV)
     prep = prepare(batch, cache, 8, [([0, 1], 64)])
     prep.prefixes.arg.max_keys = 1 << 20
     assert prep.shared_bytes(cache, 8) == 0 and b"prefix" in lib().vapi_kv_last_error()

@@ -41,6 +41,7 @@ EXPORTS = (
     "vapi_paged_attention_prepared", "vapi_paged_attention_prepared_workspace_size",
     "vapi_kv_q8_append", "vapi_kv_q8_gather", "vapi_kv_q8_attention",
     "vapi_kv_q8_attention_workspace_size",
+    "vapi_kv_q8_attention_shared", "vapi_kv_q8_attention_shared_workspace_size",
     "vapi_paged_attention_shared", "vapi_paged_attention_shared_workspace_size",
     "vapi_paged_attention_sinks", "vapi_paged_attention_append_sinks",
     "vapi_kv_q8_attention_sinks",
@@ -217,6 +218,9 @@ def lib():
     L.vapi_kv_q8_attention_sinks.argtypes = [_q8p] + sinks
     L.vapi_paged_attention_shared_workspace_size.argtypes = [_poolp] + [_u32] * 5 + [_pp]
     L.vapi_paged_attention_shared_workspace_size.restype = _sz
+    L.vapi_kv_q8_attention_shared_workspace_size.argtypes = [_q8p] + [_u32] * 5 + [_pp]
+    L.vapi_kv_q8_attention_shared_workspace_size.restype = _sz
+    L.vapi_kv_q8_attention_shared.argtypes = [_q8p] + sinks[:-3] + [_pp] + sinks[-3:]
     L.vapi_paged_attention_shared.argtypes = [_poolp] + sinks[:-3] + [_pp] + sinks[-3:]
     L.vapi_paged_attention_append_sinks.argtypes = [_poolp, _u32, _vp, _vp, _vp] + sinks
     L.vapi_kv_attention_weights_workspace_size.argtypes = [_u32] * 7

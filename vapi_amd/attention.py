@@ -151,7 +151,7 @@ class PreparedAttention:
                    prefill_seqs=cu_seqlens(pf if pf.size else [0], device),
                    n_prefill=int(pf.size))
         if share_prefixes:
-            prep.prefixes = PrefixPlan.from_batch(batch, cache.block_size, device)
+            prep.prefixes = PrefixPlan.from_batch(batch, cache, num_heads, device)
         if cache is not None and num_heads is not None:
             prep.reserve(cache, num_heads, device)
         return prep
@@ -185,20 +185,25 @@ class PreparedAttention:
             self.streams.clear()
         return ws
 
-    def shared_bytes(self, cache, num_heads: int) -> int:
+    def shared_bytes(self, cache, num_heads: int, window_left: int | None = None) -> int:
         """The workspace of a layer's attention over the step's shared prefixes;
-        0 where it runs without them."""
+        0 where it runs without them: the pool takes none, or they save less than
+        their partial results cost (PrefixPlan.worth_it)."""
         if self.prefixes is None:
             return 0
         key = (cache.num_kv_heads, cache.head_dim, cache.block_size, cache.dtype, num_heads,
-               getattr(cache, "fmt", None))
+               getattr(cache, "fmt", None), window_left)
         if key not in self.sharing:
-            b = self.seqlens_q.shape[0] - 1
-            listed = self.prefill_seqs is not None and not self.flags & ATTN_NO_DECODE_ROWS
-            args = (b, self.n_prefill if listed else b, num_heads, max(self.max_seqlen_q, 1),
-                    max(self.max_seqlen_k, 1), self.prefixes.ptr)
-            self.sharing[key] = (0 if _is_quantised(cache) else
-                                 lib().vapi_paged_attention_shared_workspace_size(cache.pool, *args))
+            need = 0
+            if self.prefixes.worth_it(cache, window_left):
+                b = self.seqlens_q.shape[0] - 1
+                listed = self.prefill_seqs is not None and not self.flags & ATTN_NO_DECODE_ROWS
+                args = (b, self.n_prefill if listed else b, num_heads, max(self.max_seqlen_q, 1),
+                        max(self.max_seqlen_k, 1), self.prefixes.ptr)
+                need = (lib().vapi_kv_q8_attention_shared_workspace_size(cache.q8, *args)
+                        if _is_quantised(cache) else
+                        lib().vapi_paged_attention_shared_workspace_size(cache.pool, *args))
+            self.sharing[key] = need
         return self.sharing[key]
 
     def keep_for(self, stream) -> None:
@@ -296,7 +301,7 @@ def paged_attention_prepared(q: torch.Tensor, cache: PagedKvCache, layer: int,
     max_k = max(int(prepared.max_seqlen_k), 1)
     mask = (float(softmax_scale), -1 if window_size_left is None else int(window_size_left),
             -1 if window_size_right is None else int(window_size_right))
-    shared = prepared.shared_bytes(cache, num_heads) if b else 0
+    shared = prepared.shared_bytes(cache, num_heads, window_size_left) if b else 0
     mask += (sinks, prepared.flags) if sinks or shared else (prepared.flags,)
     args = (cache.pool, layer, q.data_ptr(), out.data_ptr(), prepared.seqlens_q.data_ptr(),
             prepared.seqlens_k.data_ptr(), prepared.block_table.data_ptr(), b,
@@ -309,6 +314,9 @@ def paged_attention_prepared(q: torch.Tensor, cache: PagedKvCache, layer: int,
     if shared:
         check_on_device(q, out, prepared.block_table, prepared.seqlens_q)
         fn = lib().vapi_paged_attention_shared
+        if _is_quantised(cache):
+            check_on_device(q, cache.k[0])
+            fn, args = lib().vapi_kv_q8_attention_shared, (cache.q8,) + args[1:]
         args += (prepared.prefixes.ptr,)
         _run_shared(lambda ptr, size: fn(*args, ptr, size, handle), prepared, shared, q.device,
                     stream)
@@ -409,17 +417,20 @@ def paged_attention_append_prepared(q: torch.Tensor, k: torch.Tensor, v: torch.T
         # Two calls; what the second would refuse is refused before the first, and
         # its workspace is there before rows are written.
         _check_second(cache, q, out, prepared)
-        if b and not _workspace(cache, prepared, b, num_heads, max_q, max_k, q.device,
-                                stream)[0]:
+        shared = prepared.shared_bytes(cache, num_heads, window_size_left) if b else 0
+        if shared:
+            prepared.grow(shared, q.device, stream)
+        elif b and not _workspace(cache, prepared, b, num_heads, max_q, max_k, q.device,
+                                  stream)[0]:
             raise ValueError(lib().vapi_kv_last_error().decode())
         write_rows_indexed(cache, layer, k, v, slot_mapping, stream=stream)
         return paged_attention_prepared(q, cache, layer, prepared, softmax_scale,
                                         window_size_left, window_size_right, out=out,
                                         stream=stream, sinks=sinks)
-    if b and prepared.shared_bytes(cache, num_heads):
+    if b and prepared.shared_bytes(cache, num_heads, window_size_left):
         # Two calls here too; the shared prefixes' is refused before rows are written.
         _check_second(cache, q, out, prepared)
-        prepared.grow(prepared.shared_bytes(cache, num_heads), q.device, stream)
+        prepared.grow(prepared.shared_bytes(cache, num_heads, window_size_left), q.device, stream)
         check(lib().vapi_kv_append(cache.pool, layer, k.data_ptr(), v.data_ptr(),
                                    slot_mapping.data_ptr(), k.shape[0], stream_handle(stream)))
         keep_for(stream, k, v, slot_mapping)

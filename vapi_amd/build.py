@@ -70,7 +70,7 @@ NO_SCRATCH = {"attn_prefill.hip": ("paged_prefill_tiled", "paged_mixed_stream"),
               "attn_decode.hip": ("paged_decode_stream",),
               "attn_decode_small.hip": ("paged_decode_small",),
               "attn_prefill_f32.hip": ("paged_prefill_f32",),
-              "attn_shared.hip": ("paged_shared_tiles",),
+              "attn_shared.hip": ("paged_shared_stream",),
               "attn_q8.hip": ("q8_decode_stream", "q8_decode_small"),
               "kv_weights.hip": ("weights_lse", "weights_sum")}
 

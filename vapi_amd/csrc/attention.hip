@@ -628,10 +628,8 @@ static int paged_attention_impl(const vapi_kv_pool* pool, uint32_t layer, const 
       dec.pf_min_q = skip_decode ? 1 : 2;
       decode_bind(dec, workspace, D);
       const SharedArgs sh =
-          shared_args(prefixes, dec, D, shared_pf, max_seqlen_q, (char*)workspace + shared_off);
-      if (!skip_decode) launch_decode_shared(dec, D, bf16, s);
-      launch_shared_tiles(dec, sh, D, bf16, s);
-      launch_shared_merge(dec, sh, D, bf16, !skip_decode, s);
+          shared_args(prefixes, dec, D, shared_pf, (char*)workspace + shared_off);
+      launch_shared(dec, sh, D, bf16, !skip_decode, s);
       VK_LAUNCHED("paged_attention_shared");
       return 0;
     }

@@ -712,6 +712,10 @@ struct KeyReads {
     last = sink ? min(sinks - 1, khi) : khi;
     hole = mid ? klo : 0;
   }
+  // Whether all keys of the step at s0 are read as they are.
+  __device__ __forceinline__ bool whole(int32_t s0) const {
+    return s0 >= first && s0 + 31 <= last && (s0 >= hole || s0 + 31 < sinks);
+  }
   // The 16-key tile read for the one at s, and the row of it for row r.
   __device__ __forceinline__ int32_t tile(int32_t s) const {
     return max(min(s, last & ~15), first & ~15);
@@ -725,6 +729,7 @@ struct KeyReads {
 // The same for one row's decode, which masks hidden keys' V itself.
 struct RowReads {
   int32_t last;
+  __device__ __forceinline__ bool whole(int32_t s0) const { return s0 + 31 <= last; }
   __device__ __forceinline__ int32_t tile(int32_t s) const { return min(s, last & ~15); }
   __device__ __forceinline__ uint32_t row(int32_t r, int32_t ts) const {
     return (uint32_t)min(r, last - ts);

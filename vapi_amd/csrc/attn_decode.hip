@@ -4,13 +4,12 @@
 namespace vk {
 
 template <typename T, int D, bool kFuse, bool kPad = false, int DL = D / 16, bool kNt = true,
-          bool kSinks = false, bool kShared = false>
+          bool kSinks = false>
 __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void paged_decode_stream(
     AttnArgs a, const uint32_t* __restrict__ cu_q, const uint32_t* __restrict__ cu_k,
     const uint32_t* __restrict__ table) {
   extern __shared__ uint32_t P[];
-  decode_stream_body<T, D, kFuse, kPad, DL, kNt, kSinks, kShared>(a, cu_q, cu_k, table, P,
-                                                                   blockIdx.x,
+  decode_stream_body<T, D, kFuse, kPad, DL, kNt, kSinks>(a, cu_q, cu_k, table, P, blockIdx.x,
                                                  gridDim.x);
 }
 
@@ -260,31 +259,6 @@ void launch_decode(AttnArgs a, void* workspace, uint32_t head_dim, uint32_t dtyp
 #undef VK_DECL
 #undef VK_DEC_PAD
   }
-}
-
-// The stream over the keys past a.shared (a bound to its workspace; at most
-// kMaxPlanSeqs sequences).
-void launch_decode_shared(const AttnArgs& a, uint32_t head_dim, bool bf16, hipStream_t s) {
-  const dim3 grid(a.num_waves / kDecodeWavesPerWG), block(64 * kDecodeWavesPerWG);
-  const size_t lds = (a.batch + 1) * sizeof(uint32_t);
-#define VK_DSH(T, DD)                                                                     \
-  do {                                                                                    \
-    constexpr auto once = paged_decode_stream<T, DD, false, false, DD / 16, true, true, true>;      \
-    constexpr auto once_pad = paged_decode_stream<T, DD, false, true, DD / 16, true, true, true>;   \
-    constexpr auto parts = paged_decode_stream<T, DD, false, true, DD / 16, false, true, true>;     \
-    hipLaunchKernelGGL(a.kv_parts.d > 1 ? parts : a.hd != DD ? once_pad : once, grid, block, \
-                       lds, s, a, a.cu_q, a.cu_k, a.table);                               \
-  } while (0)
-  if (bf16) {
-    if (head_dim == 256) VK_DSH(bf16_t, 256);
-    else if (head_dim == 128) VK_DSH(bf16_t, 128);
-    else VK_DSH(bf16_t, 64);
-  } else {
-    if (head_dim == 256) VK_DSH(f16_t, 256);
-    else if (head_dim == 128) VK_DSH(f16_t, 128);
-    else VK_DSH(f16_t, 64);
-  }
-#undef VK_DSH
 }
 
 }  // namespace vk

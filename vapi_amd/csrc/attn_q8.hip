@@ -23,6 +23,7 @@
 #include <algorithm>
 
 #include "attn_decode.hpp"
+#include "attn_shared.hpp"
 #include "q8.hpp"
 
 namespace vk {
@@ -409,8 +410,31 @@ __global__ __launch_bounds__(64 * q8_small_waves<D>(), 1) void q8_decode_small(
 
 // ---- prefill: codes expanded into the workspace ----------------------------------
 
-// One block and kv head of a listed sequence: K and V codes to values of T in
-// an HND pool whose blocks are (list entry, block of the sequence).
+// One block and kv head: K and V codes to values of T, rows `to` x block_size .. of an
+// HND pool.
+template <typename T, int F>
+__device__ __forceinline__ void q8_expand_block(const AttnArgs& a, const Q8Scales& sc, uint32_t blk,
+                                                uint32_t h, uint64_t to, T* k_out, T* v_out) {
+  const uint32_t upr = a.hd / 16, units = a.block_size * upr;
+  const float s[2] = {sc.k[(uint64_t)blk * sc.sblk + h], sc.v[(uint64_t)blk * sc.sblk + h]};
+  const uint64_t src = blk * a.blk_e + h * a.head_e;
+  const uint64_t dst = to * a.block_size * a.hd;
+  for (uint32_t i = threadIdx.x; i < 2 * units; i += 256) {
+    const bool v = i >= units;
+    const uint32_t u = v ? i - units : i;
+    const uint32_t off = u / upr, c = u - off * upr;
+    const uint4 w = *(const uint4*)((v ? a.v : a.k) + src + (uint64_t)off * a.tok_e + 16 * c);
+    const float sv = s[v];
+    const uint2 p0 = q8_expand4<T, F, true>(w.x, sv), p1 = q8_expand4<T, F, true>(w.y, sv);
+    const uint2 p2 = q8_expand4<T, F, true>(w.z, sv), p3 = q8_expand4<T, F, true>(w.w, sv);
+    uint4* out = (uint4*)((v ? v_out : k_out) + dst) + 2 * u;
+    out[0] = make_uint4(p0.x, p0.y, p1.x, p1.y);
+    out[1] = make_uint4(p2.x, p2.y, p3.x, p3.y);
+  }
+}
+
+// One block and kv head of a listed sequence, into a pool whose blocks are (list entry,
+// block of the sequence).
 template <typename T, int F>
 __global__ __launch_bounds__(256) void q8_expand_kernel(AttnArgs a, Q8Scales sc, T* k_out,
                                                         T* v_out, uint32_t* table_out,
@@ -430,22 +454,27 @@ __global__ __launch_bounds__(256) void q8_expand_kernel(AttnArgs a, Q8Scales sc,
   if (h == 0 && threadIdx.x == 0) table_out[(uint64_t)seq * mb + j] = to;
   const uint32_t blk =
       min(a.table[(uint64_t)seq * a.max_blocks + min(j, a.max_blocks - 1)], a.last_blk);
-  const uint32_t upr = a.hd / 16, units = a.block_size * upr;
-  const float s[2] = {sc.k[(uint64_t)blk * sc.sblk + h], sc.v[(uint64_t)blk * sc.sblk + h]};
-  const uint64_t src = blk * a.blk_e + h * a.head_e;
-  const uint64_t dst = ((uint64_t)to * gridDim.y + h) * a.block_size * a.hd;
-  for (uint32_t i = threadIdx.x; i < 2 * units; i += 256) {
-    const bool v = i >= units;
-    const uint32_t u = v ? i - units : i;
-    const uint32_t off = u / upr, c = u - off * upr;
-    const uint4 w = *(const uint4*)((v ? a.v : a.k) + src + (uint64_t)off * a.tok_e + 16 * c);
-    const float sv = s[v];
-    const uint2 p0 = q8_expand4<T, F, true>(w.x, sv), p1 = q8_expand4<T, F, true>(w.y, sv);
-    const uint2 p2 = q8_expand4<T, F, true>(w.z, sv), p3 = q8_expand4<T, F, true>(w.w, sv);
-    uint4* out = (uint4*)((v ? v_out : k_out) + dst) + 2 * u;
-    out[0] = make_uint4(p0.x, p0.y, p1.x, p1.y);
-    out[1] = make_uint4(p2.x, p2.y, p3.x, p3.y);
-  }
+  q8_expand_block<T, F>(a, sc, blk, h, (uint64_t)to * gridDim.y + h, k_out, v_out);
+}
+
+// The same for a call with shared prefixes: block blockIdx.x of the nodes' blocks (mbg
+// of each group, then mbo of each listed sequence), of those that its tiles read.
+template <typename T, int F>
+__global__ __launch_bounds__(256) void q8_expand_nodes_kernel(AttnArgs a, SharedArgs sh,
+                                                              Q8Scales sc, T* k_out, T* v_out,
+                                                              uint32_t* table_out, uint32_t mbg,
+                                                              uint32_t mbo) {
+  const uint32_t to = blockIdx.x, h = blockIdx.y, n_g = sh.n_groups * mbg;
+  const uint32_t node = to < n_g ? to / mbg : sh.n_groups + (to - n_g) / mbo;
+  const uint32_t j = to < n_g ? to % mbg : (to - n_g) % mbo;
+  const ShNode n = sh_node(a, sh, node);
+  if (n.tokens == 0 || j * a.block_size >= (uint32_t)n.k1 ||
+      (j + 1) * a.block_size <= (uint32_t)(n.k0 & ~31))
+    return;
+  if (h == 0 && threadIdx.x == 0) table_out[(uint64_t)node * sh.table_width + j] = to;
+  const uint32_t blk =
+      min(a.table[(uint64_t)n.seq * a.max_blocks + min(j, a.max_blocks - 1)], a.last_blk);
+  q8_expand_block<T, F>(a, sc, blk, h, (uint64_t)to * gridDim.y + h, k_out, v_out);
 }
 
 static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -468,6 +497,28 @@ static Q8ExpandWs q8_expand_ws(const vapi_kv_q8_pool* p, uint32_t batch, uint32_
   Q8ExpandWs w;
   w.table = 0;
   w.k = up256((size_t)batch * mb * sizeof(uint32_t));
+  w.v = w.k + buf;
+  w.total = w.v + buf;
+  return w;
+}
+
+// The same of a call with shared prefixes: mbg blocks a group, mbo a listed sequence.
+struct Q8NodeWs {
+  size_t table, k, v, total;
+  uint64_t blocks;
+  uint32_t mbg, mbo, width;
+};
+static Q8NodeWs q8_node_ws(const vapi_kv_q8_pool* p, const vapi_kv_prefixes* x, uint32_t n_pf,
+                           uint32_t max_k) {
+  Q8NodeWs w;
+  const uint32_t n_groups = x->n_rows ? x->n_groups : 0;
+  w.mbg = n_groups ? (uint32_t)(((uint64_t)x->max_keys + p->block_size - 1) / p->block_size) : 0;
+  w.mbo = n_pf ? (uint32_t)(((uint64_t)max_k + p->block_size - 1) / p->block_size) : 0;
+  w.width = std::max(std::max(w.mbg, w.mbo), 1u);
+  w.blocks = (uint64_t)n_groups * w.mbg + (uint64_t)n_pf * w.mbo;
+  const size_t buf = up256(w.blocks * p->block_size * p->num_kv_heads * p->head_dim * 2);
+  w.table = 0;
+  w.k = up256(((size_t)n_groups + n_pf) * w.width * sizeof(uint32_t));
   w.v = w.k + buf;
   w.total = w.v + buf;
   return w;
@@ -498,6 +549,20 @@ static int q8_check_sizes(const vapi_kv_q8_pool* p, uint32_t num_heads, uint32_t
   return 0;
 }
 
+// And for its shared prefixes.
+static int q8_check_shared(const vapi_kv_q8_pool* p, uint32_t num_heads, uint32_t batch,
+                           uint32_t n_pf, uint32_t max_q, uint32_t max_k,
+                           const vapi_kv_prefixes* x, const char* who) {
+  const uint32_t kvh = p->num_kv_heads;
+  if (int rc = shared_check(x, batch, kvh, num_heads / kvh, q8_dim(p->head_dim), n_pf, max_q, max_k,
+                            who))
+    return rc;
+  if (q8_node_ws(p, x, n_pf, max_k).blocks > 0xFFFFFFull)
+    VK_FAIL(VAPI_KV_EUNSUP, "%s: shared prefixes of %u groups too long for one launch", who,
+            x->n_groups);
+  return 0;
+}
+
 template <typename T, int F, int D>
 static void launch_q8_stream_d(const AttnArgs& c, const Q8Scales& sc, uint32_t nwg, size_t lds,
                                hipStream_t s) {
@@ -518,6 +583,23 @@ static void launch_q8_stream_d(const AttnArgs& c, const Q8Scales& sc, uint32_t n
   else if (once) VK_Q8S(false, true);
   else VK_Q8S(false, false);
 #undef VK_Q8S
+}
+
+// The stream over the rows' own keys (at most 4,096 sequences; a bound to its workspace).
+template <typename T, int F>
+static void launch_q8_shared_stream(const AttnArgs& a, const Q8Scales& sc, uint32_t D,
+                                    hipStream_t s) {
+  const dim3 grid(a.num_waves / kDecodeWavesPerWG), block(64 * kDecodeWavesPerWG);
+  const size_t lds = (a.batch + 1) * sizeof(uint32_t);
+  const bool once = a.kv_parts.d == 1 && (a.tok_e == a.hd || a.hd % 128 == 0);
+#define VK_Q8H(DD)                                                                    \
+  hipLaunchKernelGGL((once ? q8_decode_stream<T, F, DD, true, true, true, true>       \
+                           : q8_decode_stream<T, F, DD, true, false, true, true>),    \
+                     grid, block, lds, s, a, sc, a.cu_q, a.cu_k, a.table)
+  if (D == 256) VK_Q8H(256);
+  else if (D == 128) VK_Q8H(128);
+  else VK_Q8H(64);
+#undef VK_Q8H
 }
 
 template <typename T, int F>
@@ -610,9 +692,27 @@ static void launch_q8_expand(const AttnArgs& a, const Q8Scales& sc, char* ws, co
                      sc, (T*)(ws + w.k), (T*)(ws + w.v), (uint32_t*)(ws + w.table), mb);
 }
 
+template <typename T, int F>
+static void launch_q8_expand_nodes(const AttnArgs& a, const SharedArgs& sh, const Q8Scales& sc,
+                                   char* ws, const Q8NodeWs& w, uint32_t kvh, hipStream_t s) {
+  if (w.blocks)
+    hipLaunchKernelGGL((q8_expand_nodes_kernel<T, F>), dim3((uint32_t)w.blocks, kvh), dim3(256), 0,
+                       s, a, sh, sc, (T*)(ws + w.k), (T*)(ws + w.v), (uint32_t*)(ws + w.table),
+                       w.mbg, w.mbo);
+}
+
 }  // namespace vk
 
 using namespace vk;
+
+static int q8_attention(const vapi_kv_q8_pool* pool, uint32_t layer, const void* q, void* out,
+                        const uint32_t* cu_seqlens_q, const uint32_t* cu_seqlens_k,
+                        const uint32_t* block_table, uint32_t batch, uint32_t max_blocks,
+                        uint32_t max_seqlen_q, uint32_t max_seqlen_k, uint32_t num_heads,
+                        float scale, int32_t window_left, int32_t window_right, uint32_t sinks,
+                        uint32_t flags, const uint32_t* prefill_seqs, uint32_t n_prefill,
+                        const vapi_kv_prefixes* prefixes, void* workspace, size_t workspace_bytes,
+                        vapi_stream_t stream);
 
 extern "C" {
 
@@ -640,10 +740,10 @@ int vapi_kv_q8_attention(const vapi_kv_q8_pool* pool, uint32_t layer, const void
                          float scale, int32_t window_left, int32_t window_right, uint32_t flags,
                          const uint32_t* prefill_seqs, uint32_t n_prefill, void* workspace,
                          size_t workspace_bytes, vapi_stream_t stream) {
-  return vapi_kv_q8_attention_sinks(pool, layer, q, out, cu_seqlens_q, cu_seqlens_k, block_table,
-                                    batch, max_blocks, max_seqlen_q, max_seqlen_k, num_heads,
-                                    scale, window_left, window_right, 0, flags, prefill_seqs,
-                                    n_prefill, workspace, workspace_bytes, stream);
+  return q8_attention(pool, layer, q, out, cu_seqlens_q, cu_seqlens_k, block_table, batch,
+                      max_blocks, max_seqlen_q, max_seqlen_k, num_heads, scale, window_left,
+                      window_right, 0, flags, prefill_seqs, n_prefill, nullptr, workspace,
+                      workspace_bytes, stream);
 }
 
 int vapi_kv_q8_attention_sinks(const vapi_kv_q8_pool* pool, uint32_t layer, const void* q,
@@ -654,6 +754,56 @@ int vapi_kv_q8_attention_sinks(const vapi_kv_q8_pool* pool, uint32_t layer, cons
                                int32_t window_left, int32_t window_right, uint32_t sinks,
                                uint32_t flags, const uint32_t* prefill_seqs, uint32_t n_prefill,
                                void* workspace, size_t workspace_bytes, vapi_stream_t stream) {
+  return q8_attention(pool, layer, q, out, cu_seqlens_q, cu_seqlens_k, block_table, batch,
+                      max_blocks, max_seqlen_q, max_seqlen_k, num_heads, scale, window_left,
+                      window_right, sinks, flags, prefill_seqs, n_prefill, nullptr, workspace,
+                      workspace_bytes, stream);
+}
+
+size_t vapi_kv_q8_attention_shared_workspace_size(const vapi_kv_q8_pool* pool, uint32_t batch,
+                                                  uint32_t n_prefill, uint32_t num_heads,
+                                                  uint32_t max_seqlen_q, uint32_t max_seqlen_k,
+                                                  const vapi_kv_prefixes* prefixes) {
+  const char* who = "vapi_kv_q8_attention_shared_workspace_size";
+  n_prefill = max_seqlen_q > 1 ? std::min(n_prefill, batch) : 0;
+  max_seqlen_k = std::max(max_seqlen_k, 1u);
+  if (check_q8_pool(pool, 0, who) || batch == 0 ||
+      q8_check_sizes(pool, num_heads, n_prefill, max_seqlen_q, max_seqlen_k, who) ||
+      q8_check_shared(pool, num_heads, batch, n_prefill, max_seqlen_q, max_seqlen_k, prefixes, who))
+    return 0;
+  const uint32_t kvh = pool->num_kv_heads;
+  return std::max(up256(q8_decode_ws(pool, batch, num_heads)), (size_t)256) +
+         q8_node_ws(pool, prefixes, n_prefill, max_seqlen_k).total +
+         shared_workspace_bytes(prefixes, batch, kvh, num_heads / kvh, q8_dim(pool->head_dim),
+                                n_prefill, max_seqlen_q);
+}
+
+int vapi_kv_q8_attention_shared(const vapi_kv_q8_pool* pool, uint32_t layer, const void* q,
+                                void* out, const uint32_t* cu_seqlens_q,
+                                const uint32_t* cu_seqlens_k, const uint32_t* block_table,
+                                uint32_t batch, uint32_t max_blocks, uint32_t max_seqlen_q,
+                                uint32_t max_seqlen_k, uint32_t num_heads, float scale,
+                                int32_t window_left, int32_t window_right, uint32_t sinks,
+                                uint32_t flags, const uint32_t* prefill_seqs, uint32_t n_prefill,
+                                const vapi_kv_prefixes* prefixes, void* workspace,
+                                size_t workspace_bytes, vapi_stream_t stream) {
+  if (!prefixes) VK_FAIL(VAPI_KV_EINVAL, "vapi_kv_q8_attention_shared: null prefixes");
+  return q8_attention(pool, layer, q, out, cu_seqlens_q, cu_seqlens_k, block_table, batch,
+                      max_blocks, max_seqlen_q, max_seqlen_k, num_heads, scale, window_left,
+                      window_right, sinks, flags, prefill_seqs, n_prefill, prefixes, workspace,
+                      workspace_bytes, stream);
+}
+
+}  // extern "C"
+
+static int q8_attention(const vapi_kv_q8_pool* pool, uint32_t layer, const void* q, void* out,
+                        const uint32_t* cu_seqlens_q, const uint32_t* cu_seqlens_k,
+                        const uint32_t* block_table, uint32_t batch, uint32_t max_blocks,
+                        uint32_t max_seqlen_q, uint32_t max_seqlen_k, uint32_t num_heads,
+                        float scale, int32_t window_left, int32_t window_right, uint32_t sinks,
+                        uint32_t flags, const uint32_t* prefill_seqs, uint32_t n_prefill,
+                        const vapi_kv_prefixes* prefixes, void* workspace, size_t workspace_bytes,
+                        vapi_stream_t stream) {
   const char* who = "vapi_kv_q8_attention";
   if (int rc = check_q8_pool(pool, layer, who)) return rc;
   if (num_heads == 0 || num_heads % pool->num_kv_heads)
@@ -681,10 +831,20 @@ int vapi_kv_q8_attention_sinks(const vapi_kv_q8_pool* pool, uint32_t layer, cons
   const uint32_t pf_n = !prefill ? 0 : listed ? n_prefill : batch;
   if (int rc = q8_check_sizes(pool, num_heads, pf_n, max_seqlen_q, max_seqlen_k, who)) return rc;
   const uint64_t mb = ((uint64_t)max_seqlen_k + pool->block_size - 1) / pool->block_size;
-  const size_t dec_ws = skip_decode ? 0 : q8_decode_ws(pool, batch, num_heads);
+  const size_t dec_ws =
+      skip_decode && !prefixes ? 0 : q8_decode_ws(pool, batch, num_heads);
   const size_t off = std::max(up256(dec_ws), (size_t)256);
   const Q8ExpandWs w = pf_n ? q8_expand_ws(pool, batch, pf_n, max_seqlen_k) : Q8ExpandWs{0, 0, 0, 0};
-  const size_t need = pf_n ? off + w.total : dec_ws;
+  size_t need = pf_n ? off + w.total : dec_ws;
+  Q8NodeWs nw{};
+  if (prefixes) {
+    if (int rc = q8_check_shared(pool, num_heads, batch, pf_n, max_seqlen_q, max_seqlen_k, prefixes,
+                                 who))
+      return rc;
+    nw = q8_node_ws(pool, prefixes, pf_n, max_seqlen_k);
+    need = off + nw.total + shared_workspace_bytes(prefixes, batch, pool->num_kv_heads, G, D, pf_n,
+                                                   max_seqlen_q);
+  }
   if (workspace_bytes < need || (need && !workspace))
     VK_FAIL(VAPI_KV_ESPACE, "%s: workspace %zu bytes < %zu", who, workspace_bytes, need);
 
@@ -735,13 +895,34 @@ int vapi_kv_q8_attention_sinks(const vapi_kv_q8_pool* pool, uint32_t layer, cons
     else if (e4m3) FN<f16_t, VAPI_KV_Q8_E4M3>(__VA_ARGS__);             \
     else FN<f16_t, VAPI_KV_Q8_INT8>(__VA_ARGS__);                       \
   } while (0)
+  AttnArgs dec = a;
+  if (parts > 1) {
+    dec.kvh = a.kvh * parts;
+    dec.group = (G + parts - 1) / parts;
+    dec.kv_parts = FastDiv(parts);
+  }
+  if (prefixes) {
+    // The stream over the rows' own codes; the codes of the nodes expanded, and the
+    // 16-bit tiles over them.
+    dec.shared = prefixes->start;
+    decode_bind(dec, workspace, D);
+    char* ws = (char*)workspace + off;
+    SharedArgs sh = shared_args(prefixes, dec, D, pf_n, ws + nw.total);
+    sh.tables = (const uint32_t*)(ws + nw.table);
+    sh.table_width = nw.width;
+    sh.last_blk = nw.blocks ? (uint32_t)nw.blocks - 1 : 0;
+    sh.k = ws + nw.k, sh.v = ws + nw.v;
+    sh.tok_e = g.d;
+    sh.head_e = (uint64_t)g.block_size * g.d;
+    sh.blk_e = sh.head_e * g.kvh;
+    if (!skip_decode) VK_Q8(launch_q8_shared_stream, dec, sc, D, s);
+    VK_Q8(launch_q8_expand_nodes, dec, sh, sc, ws, nw, g.kvh, s);
+    launch_shared_tiles(dec, sh, D, bf16, s);
+    launch_shared_merge(dec, sh, D, bf16, !skip_decode, s);
+    VK_LAUNCHED(who);
+    return 0;
+  }
   if (!skip_decode) {
-    AttnArgs dec = a;
-    if (parts > 1) {
-      dec.kvh = a.kvh * parts;
-      dec.group = (G + parts - 1) / parts;
-      dec.kv_parts = FastDiv(parts);
-    }
     // (The partials of a split lie past the balance block, as the stream's.)
     const SmallPlan small = q8_small_plan(dec, D, max_seqlen_k, dec_ws - kDecodeBalanceBytes);
     if (small.ok)
@@ -770,5 +951,3 @@ int vapi_kv_q8_attention_sinks(const vapi_kv_q8_pool* pool, uint32_t layer, cons
   VK_LAUNCHED(who);
   return 0;
 }
-
-}  // extern "C"

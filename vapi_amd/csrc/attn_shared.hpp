@@ -14,8 +14,8 @@
 // A merge then joins each row's partials.
 //
 // Tiles are cut into ranges of equal work, one workgroup each: the work of a launch
-// is the run of 32-key steps over (kv head, node, row tile), and range r takes its
-// r-th part. Tiles whose rows are joined with others' results (groups', and those of
+// is the run of 32-key steps over (kv head, node, row tile), kShTileSteps more to a
+// tile, and range r takes its r-th part. Tiles whose rows are joined with others' results (groups', and those of
 // sequences with shared keys) write partials even where a range holds all of them;
 // the others write the output there. With `before` the number of such joined tiles
 // before a tile in step order, a piece's partial is slot 2 r + before, + 1 if it is
@@ -34,15 +34,29 @@ constexpr uint32_t kShThreads = 64 * kShWaves;
 template <int D>
 constexpr int sh_row_tiles() { return D == 256 ? 1 : 2; }
 constexpr uint32_t sh_rows(uint32_t d) { return 16u * (d == 256 ? 1 : 2) * kShWaves; }
-constexpr uint32_t kShMinSteps = 4;       // of a range, in launches of few steps
-constexpr uint32_t kShMaxNodes = 4096;    // their plan is in LDS
+constexpr uint32_t kShMinSteps = 8;       // of a range, in launches of few steps
+// What a tile costs beside its steps (its rows, its first loads, its results: 5-6 us, a
+// step 1-1.4): counted as work, so that ranges of many short tiles are not the longest.
+constexpr uint32_t kShTileSteps = 5;
+constexpr uint32_t kShMaxNodes = 1024;    // their plan is in LDS
 constexpr uint32_t kShMaxRanges = 512;
 
-struct ShTile {
+struct __attribute__((aligned(16))) ShTile {
   uint32_t valid, r0, r1;  // the ranges that hold it
-  uint32_t node, tile, kh;
-  uint32_t slot0, before;  // its first piece's slot; of range r's, for r > r0: 2 r + before
+  uint32_t tile;
+  uint32_t kh, slot0, before;  // its first piece's slot; of range r's, for r > r0: 2 r + before
+  uint32_t seq;                // own nodes: the sequence; groups: ~0
+  uint32_t first, tokens;      // the node's rows
+  uint32_t pad[2];
 };
+// A query of a group as the merge needs it.
+struct __attribute__((aligned(16))) ShQuery {
+  uint32_t q;     // its row of q, ~0: none
+  uint32_t seq;
+  uint32_t kind;  // where its own keys' partials are: ShOwn
+  uint32_t tok;   // its number among its sequence's queries
+};
+enum ShOwn : uint32_t { kOwnNone, kOwnStream, kOwnTiles };
 
 struct SharedArgs {
   // Groups, in device memory: group i's queries are entries offsets[i] ..
@@ -50,7 +64,8 @@ struct SharedArgs {
   const uint32_t *offsets, *rows, *seqs, *keys;
   uint32_t n_groups, n_rows;
   uint32_t n_nodes;     // the groups, then the sequences of a.pf_seqs
-  uint32_t max_joined;  // joined tiles of a kv head, at most
+  uint32_t max_joined;   // joined tiles of a kv head, at most
+  uint32_t max_grouped;  // the groups' of them (the first, in step order)
   uint32_t ranges;
   // Blocks of node i at tables[i * table_width ..] (null: a.table's rows).
   const uint32_t* tables;
@@ -59,11 +74,14 @@ struct SharedArgs {
   const char *k, *v;  // the pool they lie in
   uint64_t blk_e, head_e;
   uint32_t tok_e;
-  // Workspace: the joined tiles of a kv head, joined tiles, ranges' open tiles; the
-  // first tile of a sequence's own node; partials.
-  uint32_t* n_joined;
+  uint32_t lds_rows;  // whether every query of the groups has an entry in LDS
+  // Workspace: the groups' tiles of a kv head; joined tiles, max_grouped of each kv head
+  // for the groups and then the rest for each; the ranges' open tiles; the first joined
+  // tile of a sequence's own node; the groups' queries; partials.
+  uint32_t* n_grouped;
   ShTile *joined, *open;
   uint32_t* own;
+  ShQuery* queries;
   char* part;
 };
 
@@ -108,12 +126,16 @@ __device__ __forceinline__ uint32_t sh_node_steps(const AttnArgs& a, const ShNod
 }
 
 // The plan, in LDS: tiles, steps and joined tiles of the nodes before each (n_nodes + 1
-// of each, one array after the other).
+// of each, one array after the other), then the nodes.
+constexpr size_t sh_plan_bytes(uint32_t n_nodes) {
+  return 3 * ((size_t)n_nodes + 1) * sizeof(uint32_t) + n_nodes * sizeof(ShNode);
+}
 __device__ __forceinline__ void sh_plan(const AttnArgs& a, const SharedArgs& sh, uint32_t rows,
                                         uint32_t* tiles) {
   __shared__ uint32_t tot[3][kShWaves];
   const uint32_t N1 = sh.n_nodes + 1;
   uint32_t *steps = tiles + N1, *joined = steps + N1;
+  ShNode* nodes = (ShNode*)(joined + N1);
   const uint32_t tid = threadIdx.x, lane = tid & 63;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t per = (sh.n_nodes + kShThreads - 1) / kShThreads;
@@ -122,9 +144,10 @@ __device__ __forceinline__ void sh_plan(const AttnArgs& a, const SharedArgs& sh,
   for (uint32_t i = i0; i < i1; ++i) {
     const ShNode n = sh_node(a, sh, i);
     const uint32_t nt = (uint32_t)(((uint64_t)n.tokens * a.g_real + rows - 1) / rows);
-    const uint32_t ns = nt * sh_node_steps(a, n, i < sh.n_groups);
+    const uint32_t ns = nt * (sh_node_steps(a, n, i < sh.n_groups) + kShTileSteps);
     const uint32_t nj = i < sh.n_groups || n.k0 > 0 ? nt : 0u;
     tiles[i] = nt, steps[i] = ns, joined[i] = nj;
+    nodes[i] = n;
     sum[0] += nt, sum[1] += ns, sum[2] += nj;
   }
 #pragma unroll
@@ -153,29 +176,111 @@ __device__ __forceinline__ void sh_plan(const AttnArgs& a, const SharedArgs& sh,
   __syncthreads();
 }
 
-// The query of row r of a node: its row of q, sequence and position (false: none).
-struct ShRow {
-  uint32_t q, seq, head;  // head: of the kv head's group
-  int32_t pos, len_k;
+// Entry e of the groups' lists: its row of q (~0: it names none), its sequence, and the
+// keys that its mask leaves.
+struct ShEntry {
+  uint32_t q, seq;
+  int32_t lo, hi;
 };
-__device__ __forceinline__ bool sh_row(const AttnArgs& a, const SharedArgs& sh, const ShNode& n,
-                                       bool group, uint32_t r, ShRow& w) {
-  const uint32_t G = a.g_real, j = r / G;
-  if (j >= n.tokens) return false;
-  w.head = r - j * G;
-  w.q = group ? sh.rows[n.first + j] : n.first + j;
-  w.seq = group ? sh.seqs[n.first + j] : n.seq;
-  if (w.seq >= a.batch) return false;
-  const uint32_t q0 = a.cu_q[w.seq], len_q = a.cu_q[w.seq + 1] - q0;
-  w.len_k = (int32_t)(a.cu_k[w.seq + 1] - a.cu_k[w.seq]);
-  w.pos = w.len_k - (int32_t)len_q + (int32_t)(w.q - q0);
-  return w.q - q0 < len_q;
+__device__ __forceinline__ ShEntry sh_entry(const AttnArgs& a, const SharedArgs& sh, uint32_t e,
+                                            ShQuery* info = nullptr) {
+  ShEntry x{sh.rows[e], sh.seqs[e], 0, -1};
+  const bool in = x.seq < a.batch;
+  const uint32_t s = in ? x.seq : 0;
+  const uint32_t q0 = a.cu_q[s], len_q = a.cu_q[s + 1] - q0;
+  const int32_t len_k = (int32_t)(a.cu_k[s + 1] - a.cu_k[s]);
+  const uint32_t tok = x.q - q0;
+  if (!in || tok >= len_q) x.q = ~0u;
+  else key_range(len_k - (int32_t)len_q + (int32_t)tok, len_k, a.wl, a.wr, x.lo, x.hi);
+  if (info) {
+    const bool past = len_k > shared_keys(a, a.shared[s]);
+    *info = ShQuery{x.q, s, len_q >= a.pf_min_q ? kOwnTiles : past ? kOwnStream : kOwnNone, tok};
+  }
+  return x;
 }
 
+// A thread's chunks are the same rows and columns of every step (ShSlots), so that a
+// step whose keys are all read as they are costs no address arithmetic per lane.
+template <int D, int W, bool kPad>
+struct ShSlots {
+  static constexpr uint32_t CPR = D / 8;             // chunks a row
+  static constexpr int N = D >= 128 ? D / (16 * W) : 1;
+  static_assert((64 * W / CPR) % 8 == 0 || N == 1, "slots of a thread are 8 or 16 rows apart");
+  uint32_t r0, col[N], off[N];  // off: bytes from the 16-key tile's first row
+  __device__ __forceinline__ ShSlots(uint32_t tid, uint32_t tok_e, uint32_t hd) {
+    const uint32_t slot0 = D >= 128 || W == 4 ? tid : tid & 255;  // (W == 8, D == 64: see issue)
+    r0 = slot0 / CPR;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const uint32_t r = r0 + (64 * W / CPR) * j;
+      uint32_t p = (slot0 % CPR) ^ pf_swz<D>(r);
+      if (kPad && 8 * p >= hd) p = 0;
+      col[j] = 8 * p;
+      off[j] = ((r & 15) * tok_e + 8 * p) * 2;
+    }
+  }
+};
+template <typename T, int D, int W, bool kPad, typename Reads>
+__device__ __forceinline__ void sh_issue(const ShSlots<D, W, kPad>& sl, uint16_t* kdst,
+                                         uint16_t* vdst, const T* kb, const T* vb, uint32_t blk0,
+                                         uint32_t blk1, uint64_t blk_e, uint32_t tok_e,
+                                         uint32_t block_size, int32_t s0, const Reads& rd,
+                                         uint32_t wave) {
+  constexpr uint32_t CPR = D / 8;
+  const int32_t ts0 = rd.tile(s0), ts1 = rd.tile(s0 + 16);
+  const uint64_t off0 = (uint64_t)blk0 * blk_e + (uint64_t)((uint32_t)ts0 & (block_size - 1)) * tok_e;
+  const uint64_t off1 = (uint64_t)blk1 * blk_e + (uint64_t)((uint32_t)ts1 & (block_size - 1)) * tok_e;
+  auto all = [&](auto whole) __attribute__((always_inline)) {
+    auto one = [&](const T* base_t, uint16_t* buf, int j, uint32_t wslot0)
+                   __attribute__((always_inline)) {
+      // A wave's slots cover 64 / CPR whole rows of one 16-key tile.
+      const bool second = wslot0 / CPR >= 16;
+      const char* base = (const char*)(base_t + (second ? off1 : off0));
+      uint32_t off = sl.off[j];
+      if constexpr (!decltype(whole)::value) {
+        const uint32_t r = sl.r0 + (64 * W / CPR) * j;
+        off = (rd.row((int32_t)(r & 15), second ? ts1 : ts0) * tok_e + sl.col[j]) * 2;
+      }
+      __builtin_amdgcn_global_load_lds((const void*)(base + off), (LdsVoid*)(buf + wslot0 * 8), 16, 0,
+                                       0);
+    };
+    if constexpr (D >= 128) {
+#pragma unroll
+      for (int j = 0; j < D / (16 * W); ++j) {
+        one(kb, kdst, j, 64 * wave + 64 * W * j);
+        one(vb, vdst, j, 64 * wave + 64 * W * j);
+      }
+    } else if constexpr (W == 8) {
+      if (wave < 4) one(kb, kdst, 0, 64 * wave);
+      else one(vb, vdst, 0, 64 * (wave - 4));
+    } else {
+      one(kb, kdst, 0, 64 * wave);
+      one(vb, vdst, 0, 64 * wave);
+    }
+  };
+  if (rd.whole(s0)) all(std::true_type{});
+  else all(std::false_type{});
+}
+
+// Four ds_read_b64_tr_b16 issued without waiting (results valid only after a later
+// lgkm wait that names the same registers): the d tiles at a0 and a1, their keys 0 .. 15
+// and, 16 rows on (the swizzle repeats), 16 .. 31.
+template <int D>
+__device__ __forceinline__ void sh_read_tr16(uint2 (&r)[4], uint32_t a0, uint32_t a1) {
+  __asm__ volatile(
+      "ds_read_b64_tr_b16 %0, %4\n\t"
+      "ds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+      "ds_read_b64_tr_b16 %2, %5\n\t"
+      "ds_read_b64_tr_b16 %3, %5 offset:%6"
+      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
+      : "v"(a0), "v"(a1), "n"(16 * D * 2)
+      : "memory");
+}
 // Counts [u0, u1) of the c of a node's tile at kv head kh (its share of the steps),
 // to the partial `pb`, or to the output if pb is null.
 template <typename T, int D, bool kPad>
 __device__ __forceinline__ void sh_piece(const AttnArgs& a, const SharedArgs& sh, uint32_t node,
+                                         const ShNode* nodes, const ShEntry* entries,
                                          uint32_t tile, uint32_t kh, uint32_t u0, uint32_t u1,
                                          uint32_t c, char* pb) {
   constexpr int RT = sh_row_tiles<D>(), W = kShWaves, KC = D / 32, DT = D / 16;
@@ -184,83 +289,129 @@ __device__ __forceinline__ void sh_piece(const AttnArgs& a, const SharedArgs& sh
   // (Three separate objects a tensor: see prefill_piece.)
   __shared__ __attribute__((aligned(16))) uint16_t kb0[32 * D], kb1[32 * D], kb2[32 * D];
   __shared__ __attribute__((aligned(16))) uint16_t vb0[32 * D], vb1[32 * D], vb2[32 * D];
-  __shared__ int4 span[W];
+  __shared__ int2 span[W];
   const bool group = node < sh.n_groups;
-  const ShNode n = sh_node(a, sh, node);
+  ShNode n;
+  n.first = __builtin_amdgcn_readfirstlane(nodes[node].first);
+  n.tokens = __builtin_amdgcn_readfirstlane(nodes[node].tokens);
+  n.seq = __builtin_amdgcn_readfirstlane(nodes[node].seq);
+  n.k0 = __builtin_amdgcn_readfirstlane(nodes[node].k0);
+  n.k1 = __builtin_amdgcn_readfirstlane(nodes[node].k1);
   const uint32_t tid = threadIdx.x, lane = tid & 63;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t col = lane & 15, g = lane >> 4;
   const uint32_t row0 = tile * kRows + wave * 16 * RT;
   const int32_t sinks = n.k0 ? 0 : a.sinks;
 
+  const uint32_t* __restrict__ tab =
+      sh.tables ? sh.tables + (uint64_t)node * sh.table_width
+                : a.table + (uint64_t)n.seq * a.max_blocks;
+  const uint32_t width = (sh.tables ? sh.table_width : a.max_blocks) - 1;
+  const T* kb = (const T*)sh.k + kh * sh.head_e;
+  const T* vb = (const T*)sh.v + kh * sh.head_e;
+  // The keys [klo, khi] that the tile's rows see, this share of their steps, and the
+  // share's first two on their way.
+  int32_t klo = 0, khi = -1, s0_ = 0, s_last = -32;
+  KeySteps<true> ks(0, 0, 0, 32);
+  // A step's blocks are looked up a step before its loads are issued, so that a wave
+  // does not wait for the table there.
+  auto lookup = [&](int32_t at) __attribute__((always_inline)) {
+    using ConstU32 = const __attribute__((address_space(4))) uint32_t;
+    const KeyReads rd(ks, at, klo, khi, sinks);
+    const int32_t s0 = ks.key(at);
+    return make_uint2(((ConstU32*)tab)[min((uint32_t)rd.tile(s0) >> a.bs_shift, width)],
+                      ((ConstU32*)tab)[min((uint32_t)rd.tile(s0 + 16) >> a.bs_shift, width)]);
+  };
+  const ShSlots<D, W, kPad> slots(tid, sh.tok_e, a.hd);
+  auto load = [&](uint16_t* kd, uint16_t* vd, int32_t at, uint2 blk) __attribute__((always_inline)) {
+    sh_issue<T, D, W, kPad>(slots, kd, vd, kb, vb, min(blk.x, sh.last_blk),
+                            min(blk.y, sh.last_blk), sh.blk_e, sh.tok_e, a.block_size, ks.key(at),
+                            KeyReads(ks, at, klo, khi, sinks), wave);
+  };
+  uint2 blk{0, 0};  // of the step whose loads are issued next
+  auto begin = [&](int32_t lo_, int32_t hi_) __attribute__((always_inline)) {
+    klo = lo_, khi = hi_;
+    ks = KeySteps<true>(klo, khi, sinks, 32);
+    const uint32_t all = khi >= klo ? (uint32_t)ks.last / 32 + 1 : 0u;
+    s0_ = 32 * (int32_t)pf_step_at(u0, c, all);
+    s_last = 32 * (int32_t)pf_step_at(u1, c, all) - 32;
+    if (s0_ <= s_last) {  // (uniform)
+      const uint2 b0 = lookup(s0_), b1 = lookup(min(s0_ + 32, s_last));
+      blk = lookup(min(s0_ + 64, s_last));
+      load(kb0, vb0, s0_, b0);
+      load(kb1, vb1, min(s0_ + 32, s_last), b1);
+    }
+  };
+  // Without a left window the keys follow from the node: the first loads need not wait
+  // for the rows' lengths (shared keys past a row's position are masked).
+  if (a.wl < 0) {
+    const uint32_t r_end = min((tile + 1) * kRows, n.tokens * a.g_real);
+    const int32_t p_last = n.k1 - (int32_t)n.tokens + (int32_t)((r_end - 1) / a.g_real);
+    begin(n.k0, group || a.wr < 0 ? n.k1 - 1 : min(n.k1 - 1, p_last + a.wr));
+  }
+
   // This lane's rows: what they see, and Q^T.
   uint4 qf[RT][KC];
   int32_t lo[RT], cnt[RT];
-  // Over the workgroup's rows: the least and largest first key + 1, last key + 2.
-  constexpr uint32_t kNone = 0x7FFFFFFFu;
-  uint32_t ext[4] = {kNone, 0u, kNone, 0u};
+  // Over the wave's rows: their largest first key + 1, least last key + 2; over those
+  // and the other waves': the least first key + 1, the largest last key + 2.
+  uint32_t lo_min = 0x7FFFFFFFu, lo_max = 0u, hi_min = 0x7FFFFFFFu, hi_max = 0u;
+  const T* qrow[RT];
+  bool live[RT];
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
-    ShRow w;
-    const bool live = sh_row(a, sh, n, group, row0 + 16 * t + col, w);
+    const uint32_t r = row0 + 16 * t + col, j = r / a.g_real;
+    const bool in = j < n.tokens;
+    uint32_t wq = n.first + (in ? j : 0);
+    int32_t wlo, hi;
+    key_range(n.k1 - (int32_t)n.tokens + (int32_t)j, n.k1, a.wl, a.wr, wlo, hi);
+    if (group && in) {
+      const uint32_t e = wq;
+      if (sh.lds_rows) {
+        wq = entries[e].q, wlo = entries[e].lo, hi = entries[e].hi;
+      } else {
+        const ShEntry x = sh_entry(a, sh, e);
+        wq = x.q, wlo = x.lo, hi = x.hi;
+      }
+    }
+    live[t] = in && wq != ~0u;
     lo[t] = 0, cnt[t] = 0;
-    if (live) {
-      int32_t hi;
-      key_range(w.pos, w.len_k, a.wl, a.wr, lo[t], hi);
-      lo[t] = max(lo[t], n.k0);
+    if (live[t]) {
+      lo[t] = max(wlo, n.k0);
       hi = max(min(hi, n.k1 - 1), -1);
       cnt[t] = max(hi - lo[t] + 1, 0);
       const uint32_t l1 = (uint32_t)lo[t] + 1, h2 = (uint32_t)(hi + 2);
-      ext[0] = min(ext[0], l1), ext[1] = max(ext[1], l1);
-      ext[2] = min(ext[2], h2), ext[3] = max(ext[3], h2);
+      lo_min = min(lo_min, l1), lo_max = max(lo_max, l1);
+      hi_min = min(hi_min, h2), hi_max = max(hi_max, h2);
     }
-    const T* qrow = (const T*)a.q +
-                    ((uint64_t)(live ? w.q : 0) * a.num_heads + kh * a.g_real + (live ? w.head : 0)) *
-                        (kPad ? a.hd : D);
+    qrow[t] = (const T*)a.q + ((uint64_t)(live[t] ? wq : 0) * a.num_heads + kh * a.g_real +
+                               (live[t] ? r - j * a.g_real : 0)) * (kPad ? a.hd : D);
+  }
+  auto least = [](uint32_t x, uint32_t y) { return min(x, y); };
+  auto most = [](uint32_t x, uint32_t y) { return max(x, y); };
+  const int32_t full_lo = (int32_t)__builtin_amdgcn_readfirstlane(wave_reduce(lo_max, most)) - 1;
+  const int32_t full_hi = (int32_t)__builtin_amdgcn_readfirstlane(wave_reduce(hi_min, least)) - 2;
+  const bool active = full_lo >= 0;  // a wave without rows only loads
+  if (a.wl >= 0) {
+    const uint32_t e0 = wave_reduce(lo_min, least), e1 = wave_reduce(hi_max, most);
+    if (lane == 0) span[wave] = make_int2((int32_t)e0, (int32_t)e1);
+    __syncthreads();
+    int2 e = span[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) e.x = min(e.x, span[w].x), e.y = max(e.y, span[w].y);
+    begin(__builtin_amdgcn_readfirstlane(e.x) - 1, __builtin_amdgcn_readfirstlane(e.y) - 2);
+  }
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
 #pragma unroll
     for (int x = 0; x < KC; ++x) {
       uint4 u = make_uint4(0, 0, 0, 0);
-      if (live && (!kPad || 32 * x + 8 * g < a.hd)) {
-        u = *(const uint4*)(qrow + 32 * x + 8 * g);
+      if (live[t] && (!kPad || 32 * x + 8 * g < a.hd)) {
+        u = *(const uint4*)(qrow[t] + 32 * x + 8 * g);
         u.x ^= a.q_sign, u.y ^= a.q_sign, u.z ^= a.q_sign, u.w ^= a.q_sign;
       }
       qf[t][x] = u;
     }
-  }
-  {
-    auto least = [](uint32_t x, uint32_t y) { return min(x, y); };
-    auto most = [](uint32_t x, uint32_t y) { return max(x, y); };
-    const uint32_t e0 = wave_reduce(ext[0], least), e1 = wave_reduce(ext[1], most);
-    const uint32_t e2 = wave_reduce(ext[2], least), e3 = wave_reduce(ext[3], most);
-    if (lane == 0) span[wave] = make_int4((int32_t)e0, (int32_t)e1, (int32_t)e2, (int32_t)e3);
-  }
-  __syncthreads();
-  int4 e = span[0];
-#pragma unroll
-  for (int w = 1; w < W; ++w) {
-    e.x = min(e.x, span[w].x), e.y = max(e.y, span[w].y);
-    e.z = min(e.z, span[w].z), e.w = max(e.w, span[w].w);
-  }
-  // Keys that some row sees [klo, khi], and that all rows see [full_lo, full_hi].
-  const int32_t klo = __builtin_amdgcn_readfirstlane(e.x) - 1;
-  const int32_t full_lo = __builtin_amdgcn_readfirstlane(e.y) - 1;
-  const int32_t full_hi = __builtin_amdgcn_readfirstlane(e.z) - 2;
-  const int32_t khi = __builtin_amdgcn_readfirstlane(e.w) - 2;
-  const KeySteps<true> ks(klo, khi, sinks, 32);
-  const int32_t all = full_lo >= 0 && khi >= klo ? ks.last / 32 + 1 : 0;
-  const int32_t a0 = (int32_t)pf_step_at(u0, c, (uint32_t)all);
-  const int32_t a1 = (int32_t)pf_step_at(u1, c, (uint32_t)all);
-  int32_t s0_ = 32 * a0;
-  const int32_t s_last = 32 * a1 - 32;
-
-  const uint32_t* __restrict__ tab =
-      sh.tables ? sh.tables + (uint64_t)node * sh.table_width
-                : a.table + (uint64_t)n.seq * a.max_blocks;
-  AttnArgs p = a;  // (the fields that loads use)
-  p.blk_e = sh.blk_e, p.head_e = sh.head_e, p.tok_e = sh.tok_e, p.last_blk = sh.last_blk;
-  p.max_blocks = sh.tables ? sh.table_width : a.max_blocks;
-  const T* kb = (const T*)sh.k + kh * sh.head_e;
-  const T* vb = (const T*)sh.v + kh * sh.head_e;
 
   float m_run[RT], l_run[RT];
   floatx4 o[RT][DT];
@@ -271,23 +422,15 @@ __device__ __forceinline__ void sh_piece(const AttnArgs& a, const SharedArgs& sh
 #pragma unroll
     for (int k = 0; k < DT; ++k) o[t][k] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
-  uint32_t k_off[2][KC];
+  uint32_t k_off[KC];
 #pragma unroll
-  for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-    for (int x = 0; x < KC; ++x) k_off[tt][x] = pf_chunk<D>(16 * tt + col, 4 * x + g);
+  for (int x = 0; x < KC; ++x) k_off[x] = pf_chunk<D>(col, 4 * x + g);
   const uint32_t vj = col >> 2, vq = col & 3;
-  uint32_t v_off[DT][2];
+  uint32_t v_off[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t)
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      v_off[t][h] = pf_chunk<D>(16 * h + 4 * g + vj, 2 * t + (vq >> 1)) + 4 * (vq & 1);
+    v_off[t] = 2 * (pf_chunk<D>(4 * g + vj, 2 * t + (vq >> 1)) + 4 * (vq & 1));
 
-  auto load = [&](uint16_t* kd, uint16_t* vd, int32_t at) __attribute__((always_inline)) {
-    pf_dma<T, D, W, kPad>(kd, vd, tab, kb, vb, p, ks.key(at), KeyReads(ks, at, klo, khi, sinks), tid,
-                          wave);
-  };
   // The 32-key step of prefill_piece: scores, online softmax, O^T += V^T P^T, the
   // step after next on its way.
   auto step = [&](auto cur) __attribute__((always_inline)) {
@@ -297,18 +440,20 @@ __device__ __forceinline__ void sh_piece(const AttnArgs& a, const SharedArgs& sh
     uint16_t* const knext = B == 0 ? kb2 : B == 1 ? kb0 : kb1;
     uint16_t* const vnext = B == 0 ? vb2 : B == 1 ? vb0 : vb1;
     const int32_t at = __builtin_amdgcn_readfirstlane(s0_), s0 = ks.key(at);
-    load(knext, vnext, min(at + 64, s_last));
+    load(knext, vnext, min(at + 64, s_last), blk);
+    blk = lookup(min(at + 96, s_last));
+    s0_ += 32;
+    if (!active) {
+      wait_vmcnt<kLoadsPerStep>();
+      ring_barrier();
+      return;
+    }
     const bool masked = !(s0 >= full_lo && s0 + 31 <= full_hi);
     const uint32_t vbase = lds_addr(vbuf);
     constexpr int NB = (DT + 1) / 2;
     uint2 r[NB][4];
     auto issue = [&](int b) __attribute__((always_inline)) {
-      uint32_t ad[4];
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) ad[2 * k + h] = vbase + 2 * v_off[2 * b + k][h];
-      ds_read_tr16_issue4(r[b], ad);
+      sh_read_tr16<D>(r[b], vbase + v_off[2 * b], vbase + v_off[2 * b + 1]);
     };
     float sc[RT][8];
     {
@@ -318,7 +463,7 @@ __device__ __forceinline__ void sh_piece(const AttnArgs& a, const SharedArgs& sh
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
         for (int x = 0; x < KC; ++x) {
-          kt.k[tt][x] = *(const uint4*)(kbuf + k_off[tt][x]);
+          kt.k[tt][x] = *(const uint4*)(kbuf + k_off[x] + 16 * D * tt);
           if (kPad && 32 * x + 8 * g >= a.hd) kt.k[tt][x] = make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
@@ -375,11 +520,8 @@ __device__ __forceinline__ void sh_piece(const AttnArgs& a, const SharedArgs& sh
     }
     wait_vmcnt<kLoadsPerStep>();
     ring_barrier();
-    s0_ += 32;
   };
   if (s0_ <= s_last) {  // (uniform)
-    load(kb0, vb0, s0_);
-    load(kb1, vb1, min(s0_ + 32, s_last));
     wait_vmcnt<kLoadsPerStep>();
     ring_barrier();
     while (true) {
@@ -420,18 +562,28 @@ __device__ __forceinline__ void sh_piece(const AttnArgs& a, const SharedArgs& sh
   }
 }
 
-// Workgroup `bid` of sh.ranges. lds: 3 (n_nodes + 1) words.
+// Workgroup `bid` of sh.ranges. lds: sh_plan_bytes, and with sh.lds_rows an entry for
+// each of the groups' queries: read while nothing else runs yet, where a round trip to
+// memory is short (beside the stream at work it takes 4 to 5 us).
 template <typename T, int D, bool kPad>
 __device__ __forceinline__ void sh_range(const AttnArgs& a, const SharedArgs& sh, uint32_t* lds,
                                          uint32_t bid) {
   constexpr uint32_t kRows = sh_rows(D);
   const uint32_t N = sh.n_nodes, kvh = sh_heads(a);
   const uint32_t *tiles = lds, *steps = lds + N + 1, *joined = steps + N + 1;
+  const ShNode* nodes = (const ShNode*)(joined + N + 1);
+  ShEntry* entries = (ShEntry*)(nodes + N);
+  if (sh.lds_rows)
+    for (uint32_t e = threadIdx.x; e < sh.n_rows; e += kShThreads) entries[e] = sh_entry(a, sh, e);
+  for (uint32_t e = bid * kShThreads + threadIdx.x; e < sh.n_rows; e += sh.ranges * kShThreads)
+    sh_entry(a, sh, e, sh.queries + e);
   sh_plan(a, sh, kRows, lds);
   const uint32_t S = __builtin_amdgcn_readfirstlane(steps[N]);
   const uint32_t n_joined = __builtin_amdgcn_readfirstlane(joined[N]);
-  const bool fits = n_joined <= sh.max_joined;  // (as every plan of the host's)
-  if (bid == 0 && threadIdx.x == 0) *sh.n_joined = fits ? n_joined : 0u;
+  const uint32_t n_grouped = __builtin_amdgcn_readfirstlane(joined[sh.n_groups]);
+  const uint32_t max_own = sh.max_joined - sh.max_grouped;
+  const bool fits = n_grouped <= sh.max_grouped && n_joined - n_grouped <= max_own;  // (every plan)
+  if (bid == 0 && threadIdx.x == 0) *sh.n_grouped = fits ? n_grouped : 0u;
   const uint64_t total = (uint64_t)S * kvh;
   const uint32_t nr = (uint32_t)min((uint64_t)sh.ranges, (total + kShMinSteps - 1) / kShMinSteps);
   if (bid >= nr || !fits) {
@@ -467,15 +619,18 @@ __device__ __forceinline__ void sh_range(const AttnArgs& a, const SharedArgs& sh
     const bool whole = u0 == 0 && u1 == c;
     if (u0 == 0 && (joins || !whole) && threadIdx.x == 0) {
       const uint32_t last = (uint32_t)min(((at + c) * nr + total - 1) / total, (uint64_t)nr) - 1;
-      const ShTile d{1u, r, last, node, tile, kh, slot, before};
-      (joins ? sh.joined[before] : sh.open[r]) = d;
-      if (joins && node >= sh.n_groups && kh == 0 && tile == 0) {
-        const uint32_t li = node - sh.n_groups;
-        sh.own[a.pf_seqs ? a.pf_seqs[li] : li] = j0;
-      }
+      const bool group = node < sh.n_groups;
+      const uint32_t t = j0 + tile;  // of the kv head's joined tiles
+      uint4* d = (uint4*)(!joins  ? sh.open + r
+                          : group ? sh.joined + kh * sh.max_grouped + t
+                                  : sh.joined + kvh * sh.max_grouped + kh * max_own + (t - n_grouped));
+      d[0] = make_uint4(1u, r, last, tile);
+      d[1] = make_uint4(kh, slot, before, group ? ~0u : nodes[node].seq);
+      d[2] = make_uint4(nodes[node].first, nodes[node].tokens, 0u, 0u);
+      if (joins && !group && kh == 0 && tile == 0) sh.own[nodes[node].seq] = j0 - n_grouped;
     }
     open = open || (u0 == 0 && !joins && !whole);
-    sh_piece<T, D, kPad>(a, sh, node, tile, kh, u0, u1, c,
+    sh_piece<T, D, kPad>(a, sh, node, nodes, entries, tile, kh, u0, u1, c,
                          joins || !whole ? sh.part + (uint64_t)slot * pf_part_bytes(kRows, D)
                                          : nullptr);
     after = 1;
@@ -497,90 +652,44 @@ __device__ __forceinline__ void sh_range(const AttnArgs& a, const SharedArgs& sh
   if (!open && threadIdx.x == 0) sh.open[r].valid = 0;
 }
 
-// Joins the partials of the rows of row block `block` of item `i` (the joined tiles of
-// all kv heads, at most kvh * max_joined of them, then the ranges' open tiles): thread
+// Joins the partials of the rows of row block `block` of item `i` (the groups' tiles of
+// all kv heads, at most kvh * max_grouped of them, then the ranges' open tiles): thread
 // (row, four outputs). nwg: the decode's workgroups.
 template <typename T, int D>
 __device__ __forceinline__ void sh_merge(const AttnArgs& a, const SharedArgs& sh, uint32_t nwg,
                                          uint32_t i, uint32_t block) {
   constexpr uint32_t kRows = sh_rows(D), kTpr = D / 4, kRpw = 256 / kTpr;
-  const uint32_t n_joined = *sh.n_joined, kvh = sh_heads(a);
-  const uint32_t most = sh.max_joined * kvh;
-  if (i < most && i >= n_joined * kvh) return;
-  const ShTile d = i < most ? sh.joined[i] : sh.open[i - most];
-  if (!d.valid || d.node >= sh.n_nodes) return;
-  const uint32_t kh = d.kh, G = a.g_real;
+  const uint32_t kvh = sh_heads(a), most = sh.max_grouped * kvh, G = a.g_real;
+  const bool group = i < most;
+  const uint32_t n_grouped = *sh.n_grouped;
+  const ShTile d = group ? sh.joined[i] : sh.open[i - most];
+  if (group ? i % sh.max_grouped >= n_grouped : !d.valid) return;
+  const uint32_t kh = d.kh;
   const uint32_t row = block * kRpw + threadIdx.x / kTpr, dq = (threadIdx.x % kTpr) * 4;
-  const bool group = d.node < sh.n_groups;
-  const ShNode n = sh_node(a, sh, d.node);
-  if (!group && n.k0 > 0) return;  // joined with its group's
-  ShRow w;
-  if (!sh_row(a, sh, n, group, d.tile * kRows + row, w) || dq >= a.hd) return;
+  const uint32_t r = d.tile * kRows + row, tok = r / G, head = r - tok * G;
+  if (tok >= d.tokens || dq >= a.hd) return;
+  ShQuery w{d.first + tok, d.seq, kOwnNone, tok};
+  if (group) w = sh.queries[d.first + tok];
   const uint64_t stride = pf_part_bytes(kRows, D);
-  // The partials: ranges d.r0 .. d.r1 of this tile, then of the sequence's own keys:
-  // ranges of its tile, or the decode stream's of its segment.
-  uint32_t np = d.r1 - d.r0 + 1, no = 0;
-  ShTile e{};  // the own tile
-  uint32_t orow = 0;
   auto slot_of = [](const ShTile& t, uint32_t j) { return j ? 2 * (t.r0 + j) + t.before : t.slot0; };
-  uint64_t sl = 0;           // or the stream's first
-  bool stream = false;
-  if (group) {
-    const uint32_t first = a.cu_q[w.seq], len_q = a.cu_q[w.seq + 1] - first;
-    if (len_q < a.pf_min_q) {
-      if (w.len_k > shared_keys(a, a.shared[w.seq])) {
-        const uint32_t v = w.head / a.group;  // the virtual kv head of the group's part
-        const uint32_t seg = w.seq * a.kvh + kh * a.kv_parts.d + v;
-        const uint2 rr = *(const uint2*)(a.seg_ranges + 2 * seg);
-        if (rr.y < nwg * kDecodeWavesPerWG && rr.x <= rr.y) {
-          stream = true;
-          no = rr.y - rr.x + 1;
-          sl = ((uint64_t)rr.x * a.kv_parts.d + seg) * a.group + (w.head - v * a.group);
-        }
-      }
-    } else {
-      const uint32_t r = (w.q - first) * G + w.head;
-      const uint32_t t = sh.own[w.seq] + r / kRows;
-      if (t < n_joined) {
-        e = sh.joined[kh * n_joined + t];
-        // (A sequence that the list leaves out has no tile of its own.)
-        if (e.node >= sh.n_groups && e.node < sh.n_nodes && e.tile == r / kRows &&
-            sh_node(a, sh, e.node).seq == w.seq) {
-          no = e.r1 - e.r0 + 1;
-          orow = r % kRows;
-        }
-      }
-    }
-  }
   constexpr uint32_t kB = 8;  // partials per round trip
   float M = kNegBig, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (uint32_t s0 = 0; s0 < np + no; s0 += kB) {
-    float2 ml[kB];
-    float4 x[kB];
-    float by[kB];
+  float2 ml[kB];
+  float4 x[kB];
+  // Partials [j0, j0 + kB) of the n at (m, l) pm(j) and o px(j).
+  auto fetch = [&](uint32_t j0, uint32_t n, auto at) __attribute__((always_inline)) {
 #pragma unroll
     for (uint32_t u = 0; u < kB; ++u) {
-      const bool in = s0 + u < np + no;
-      const uint32_t j = in ? s0 + u : 0;
-      const bool own_part = j >= np;
+      const bool in = j0 + u < n;
       const float *pm, *px;
-      if (own_part && stream) {
-        const uint64_t slot = sl + (uint64_t)(j - np) * a.kv_parts.d * a.group;
-        pm = a.ws_ml + slot * 2;
-        px = a.ws_o + slot * D + dq;
-      } else {
-        const char* pb =
-            sh.part + (uint64_t)(own_part ? slot_of(e, j - np) : slot_of(d, j)) * stride;
-        const uint32_t rw = own_part ? orow : row;
-        pm = (const float*)(pb + (uint64_t)rw * 8);
-        px = (const float*)(pb + (uint64_t)kRows * 8) + (uint64_t)rw * D + dq;
-      }
+      at(in ? j0 + u : j0, pm, px);
       ml[u] = *(const float2*)pm;
       x[u] = *(const float4*)px;
-      // Tiles' partials hold o / l, the stream's o.
-      by[u] = own_part && stream ? 1.f : ml[u].y;
       if (!in) ml[u].y = 0.f;
     }
+  };
+  // Joins what was fetched. kNormed: it is o / l (tiles'), else o (the stream's).
+  auto join = [&](bool normed) __attribute__((always_inline)) {
     float Mn = M;
 #pragma unroll
     for (uint32_t u = 0; u < kB; ++u)
@@ -592,14 +701,67 @@ __device__ __forceinline__ void sh_merge(const AttnArgs& a, const SharedArgs& sh
 #pragma unroll
     for (uint32_t u = 0; u < kB; ++u) {
       if (!(ml[u].y > 0.f)) continue;  // a share with no visible key (its o is stale)
-      const float e = fast_exp2(ml[u].x - Mn), wgt = by[u] * e;
+      const float e = fast_exp2(ml[u].x - Mn), wgt = normed ? ml[u].y * e : e;
       L += ml[u].y * e;
       o[0] += x[u].x * wgt, o[1] += x[u].y * wgt, o[2] += x[u].z * wgt, o[3] += x[u].w * wgt;
     }
     M = Mn;
+  };
+  auto of_tile = [&](const ShTile& t, uint32_t r) {
+    return [&, r](uint32_t j, const float*& pm, const float*& px) {
+      const char* pb = sh.part + (uint64_t)slot_of(t, j) * stride;
+      pm = (const float*)(pb + (uint64_t)r * 8);
+      px = (const float*)(pb + (uint64_t)kRows * 8) + (uint64_t)r * D + dq;
+    };
+  };
+  // The tile's partials are on their way while the row's own are looked up.
+  const uint32_t np = d.r1 - d.r0 + 1;
+  fetch(0, np, of_tile(d, row));
+  if (w.q == ~0u) return;
+  // Its own keys: ranges of its tile, or the decode stream's of its segment.
+  uint32_t no = 0, orow = 0;
+  ShTile e{};
+  uint64_t sl = 0;
+  const bool stream = w.kind == kOwnStream;
+  if (stream) {
+    const uint32_t v = head / a.group;  // the virtual kv head of the group's part
+    const uint32_t seg = w.seq * a.kvh + kh * a.kv_parts.d + v;
+    const uint2 rr = *(const uint2*)(a.seg_ranges + 2 * seg);
+    if (rr.y < nwg * kDecodeWavesPerWG && rr.x <= rr.y) {
+      no = rr.y - rr.x + 1;
+      sl = ((uint64_t)rr.x * a.kv_parts.d + seg) * a.group + (head - v * a.group);
+    }
+  } else if (w.kind == kOwnTiles) {
+    const uint32_t row_own = w.tok * G + head, max_own = sh.max_joined - sh.max_grouped;
+    const uint32_t t = sh.own[w.seq] + row_own / kRows;
+    if (t < max_own) {
+      e = sh.joined[most + kh * max_own + t];
+      // (A sequence that the list leaves out has no tile of its own.)
+      if (e.valid && e.seq == w.seq && e.kh == kh && e.tile == row_own / kRows && e.r0 <= e.r1 &&
+          e.r1 < sh.ranges) {
+        no = e.r1 - e.r0 + 1;
+        orow = row_own % kRows;
+      }
+    }
+  }
+  join(true);
+  for (uint32_t j0 = kB; j0 < np; j0 += kB) {
+    fetch(j0, np, of_tile(d, row));
+    join(true);
+  }
+  for (uint32_t j0 = 0; j0 < no; j0 += kB) {
+    if (stream)
+      fetch(j0, no, [&](uint32_t j, const float*& pm, const float*& px) {
+        const uint64_t slot = sl + (uint64_t)j * a.kv_parts.d * a.group;
+        pm = a.ws_ml + slot * 2;
+        px = a.ws_o + slot * D + dq;
+      });
+    else
+      fetch(j0, no, of_tile(e, orow));
+    join(!stream);
   }
   const float inv = L > 0.f ? 1.f / L : 0.f;
-  T* dst = (T*)a.out + ((uint64_t)w.q * a.num_heads + kh * G + w.head) * a.hd + dq;
+  T* dst = (T*)a.out + ((uint64_t)w.q * a.num_heads + kh * G + head) * a.hd + dq;
   *(uint2*)dst = make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
 }
 
@@ -614,10 +776,12 @@ int shared_check(const vapi_kv_prefixes* p, uint32_t batch, uint32_t kvh, uint32
                  uint32_t head_dim, uint32_t n_pf, uint32_t max_q, uint32_t max_k, const char* who);
 // The groups and `ws` of a call over a's pool (a: the decode's arguments).
 SharedArgs shared_args(const vapi_kv_prefixes* p, const AttnArgs& a, uint32_t head_dim,
-                       uint32_t n_pf, uint32_t max_q, char* ws);
-// The decode stream over the rows' own keys.
-void launch_decode_shared(const AttnArgs& a, uint32_t head_dim, bool bf16, hipStream_t s);
-// The tiles of a launch; then the merge of their partials and the stream's.
+                       uint32_t n_pf, char* ws);
+// The decode rows' own keys (`decode`: the batch may have such rows), the tiles, and
+// the merge of their partials.
+void launch_shared(const AttnArgs& a, const SharedArgs& sh, uint32_t head_dim, bool bf16,
+                   bool decode, hipStream_t s);
+// Its parts, where another kernel streams the decode rows.
 void launch_shared_tiles(const AttnArgs& a, const SharedArgs& sh, uint32_t head_dim, bool bf16,
                          hipStream_t s);
 void launch_shared_merge(const AttnArgs& a, const SharedArgs& sh, uint32_t head_dim, bool bf16,

@@ -15,22 +15,27 @@ import torch
 
 from ._lib import Prefixes
 
-# Keys that need not be read again, times kv heads not counted, from which a group is
-# worth its partial results; and the most queries a sequence brings to one (more fill
-# tiles of their own).
-MIN_SAVED_KEYS = 1024
-MAX_QUERIES = 64
+# Sharing costs a fixed 15 to 25 us a layer against the ordinary call (tiles, partial
+# results, their merge), which this many bytes of K and V take to read: 8 sequences
+# over 2,000 keys (57 MB saved, 32 q / 8 kv heads) 29 us shared, 14 not; 32 over 1,000
+# (126 MB) 33 and 34; 64 over 1,000 (256 MB) 41 and 55. An 8-bit cache's shared codes
+# are expanded first.
+MIN_SAVED_BYTES = 128 << 20
+MIN_SAVED_BYTES_Q8 = 128 << 20
+# Rows (queries times query heads of a kv head) that a sequence brings to a group at
+# most. More fill tiles by themselves, and read the prefix for many rows at once anyway:
+# 16 sequences over 2,000 keys (32 kv heads), 64 queries each: 109 us shared, 147 not;
+# 128 each: 182 and 151; 8 sequences (8 kv heads, 4 query heads each), 64: 72 and 40.
+MAX_ROWS = 64
 
 
 def find_shared_prefixes(block_tables, lens_q, lens_k, block_size: int,
-                         min_saved: int = MIN_SAVED_KEYS,
-                         max_queries: int = MAX_QUERIES) -> list[tuple[list[int], int]]:
+                         max_queries: int) -> list[tuple[list[int], int]]:
     """Groups (members, shared keys) of sequences whose tables begin with the same
     blocks, each sequence in at most one: of all ways to group along the tree of
     common prefixes the one that saves the most key reads, (members - 1) * keys a
-    group, counting groups of at least `min_saved`. Whole blocks within every
-    member's context are shared. Sequences of more than `max_queries` queries are
-    left out."""
+    group. Whole blocks within every member's context are shared. Sequences of more
+    than `max_queries` queries are left out."""
     tables = [np.asarray(t, dtype=np.int64)[:max(int(lk), 0) // block_size]
               for t, lk in zip(block_tables, lens_k)]
     live = [i for i, t in enumerate(tables) if len(t) and 1 <= lens_q[i] <= max_queries]
@@ -41,38 +46,49 @@ def find_shared_prefixes(block_tables, lens_q, lens_k, block_size: int,
         for i in members:
             if len(tables[i]) > depth:
                 out.setdefault(int(tables[i][depth]), []).append(i)
-        return out
+        return list(out.values())
 
-    def best(members, depth):
-        """The saved keys and the groups of sequences that agree up to `depth` blocks."""
-        if len(members) < 2:
-            return 0, []
+    def common(members, depth):
+        """How many blocks the members, alike in the first `depth`, have in common."""
         first = tables[members[0]]
         same = min(len(tables[i]) for i in members)
         for i in members[1:]:
             differ = np.nonzero(tables[i][depth:same] != first[depth:same])[0]
-            same = min(same, depth + int(differ[0]) if differ.size else same)
-        saved, groups = 0, []
-        for part in by_block(members, same).values():
-            s, g = best(part, same)
-            saved, groups = saved + s, groups + g
-        whole = (len(members) - 1) * same * block_size
-        if whole >= max(saved, min_saved, 1):
-            return whole, [(members, same * block_size)]
-        return saved, groups
+            if differ.size:
+                same = depth + int(differ[0])
+        return same
 
+    # Depth first, parents before children (without recursion: prefixes nest as deep as
+    # there are sequences); then the better of each node and what its children found.
+    nodes, todo = [], [(part, 0, -1) for part in by_block(live, 0) if len(part) > 1]
+    while todo:
+        members, depth, parent = todo.pop()
+        same = common(members, depth)
+        nodes.append([members, same, parent, 0, []])
+        todo += [(part, same, len(nodes) - 1) for part in by_block(members, same) if len(part) > 1]
     groups = []
-    for part in by_block(live, 0).values():
-        groups += best(part, 0)[1]
+    for members, same, parent, saved, found in reversed(nodes):
+        whole = (len(members) - 1) * same * block_size
+        if whole >= saved:
+            saved, found = whole, [(members, same * block_size)]
+        if parent < 0:
+            groups += found
+        else:
+            nodes[parent][3] += saved
+            nodes[parent][4] = nodes[parent][4] + found
     return groups
 
 
 class PrefixPlan:
-    """The groups of a step and their device lists (vapi_kv_prefixes)."""
+    """The groups of a step and their device lists (vapi_kv_prefixes). `min_bytes`:
+    the K and V bytes of a layer that sharing has to save there (16-bit, 8-bit)."""
 
-    def __init__(self, groups, cu_seqlens_q, batch: int, device):
+    def __init__(self, groups, cu_seqlens_q, cu_seqlens_k, device, min_bytes=(0, 0)):
         cq = np.asarray(cu_seqlens_q, dtype=np.int64)
+        lens_k = np.diff(np.asarray(cu_seqlens_k, dtype=np.int64))
+        batch = len(lens_k)
         self.groups = [(list(map(int, m)), int(n)) for m, n in groups]
+        self.min_bytes = min_bytes
         start = np.zeros(max(batch, 1), np.int64)
         rows, seqs, offsets = [], [], [0]
         for members, keys in self.groups:
@@ -84,6 +100,8 @@ class PrefixPlan:
                 rows += range(int(cq[s]), int(cq[s + 1]))
                 seqs += [s] * int(cq[s + 1] - cq[s])
             offsets.append(len(rows))
+        # Keys past the prefix, a member's on average: what of it a window leaves.
+        self.past = [float(np.mean(lens_k[m])) - n if m else 0.0 for m, n in self.groups]
         keys = [n for _, n in self.groups]
         lists = [np.asarray(a or [0], dtype=np.int64) for a in (offsets, rows, seqs, keys)] + [start]
         sizes = np.cumsum([0] + [len(a) for a in lists])
@@ -93,10 +111,31 @@ class PrefixPlan:
                             n_groups=len(self.groups), n_rows=len(rows), max_keys=max(keys or [0]))
         self.ptr = ctypes.pointer(self.arg)
 
+    def saved_keys(self, window_left: int | None = None) -> float:
+        """Key reads that sharing saves a kv head, about (behind a left window only what
+        it leaves of the prefix counts)."""
+        total = 0.0
+        for (members, keys), past in zip(self.groups, self.past):
+            if window_left is not None and window_left >= 0:
+                keys = min(max(window_left + 1 - past, 0.0), keys)
+            total += (len(members) - 1) * keys
+        return total
+
+    def worth_it(self, cache, window_left: int | None = None) -> bool:
+        fmt = getattr(cache, "fmt", None)
+        size = 1 if fmt else torch.empty((), dtype=cache.dtype).element_size()
+        saved = self.saved_keys(window_left) * 2 * cache.num_kv_heads * cache.head_dim * size
+        return saved >= self.min_bytes[1 if fmt else 0]
+
     @classmethod
-    def from_batch(cls, batch, block_size: int, device, **limits) -> "PrefixPlan | None":
-        """The plan of a ForwardBatch; None where sharing saves nothing. `limits`:
-        find_shared_prefixes' min_saved and max_queries."""
+    def from_batch(cls, batch, cache, num_heads: int | None, device) -> "PrefixPlan | None":
+        """The plan of a ForwardBatch over `cache`, for layers that it pays for; None
+        where no two sequences share a block. Without `num_heads`, single queries are
+        grouped only."""
+        heads = getattr(cache, "num_kv_heads", None) or min(
+            s[1] for s in cache.layouts if s[0] == "kv")
+        queries = max(MAX_ROWS * heads // num_heads, 1) if num_heads else 1
         groups = find_shared_prefixes(batch.block_tables, np.diff(batch.cu_seqlens_q),
-                                      np.diff(batch.cu_seqlens_k), block_size, **limits)
-        return cls(groups, batch.cu_seqlens_q, batch.batch_size(), device) if groups else None
+                                      np.diff(batch.cu_seqlens_k), cache.block_size, queries)
+        return cls(groups, batch.cu_seqlens_q, batch.cu_seqlens_k, device,
+                   (MIN_SAVED_BYTES, MIN_SAVED_BYTES_Q8)) if groups else None
