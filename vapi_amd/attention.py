@@ -75,16 +75,20 @@ class ForwardBatch:
             _ptr(li), len(self.logits_indices), num_blocks, block_size))
 
 
-def pack_block_tables(batch: ForwardBatch, device) -> torch.Tensor:
-    """[batch, max_blocks] u32 (as int32 bits), rows padded with their own
-    last block (attention.rs:42-62)."""
+def _packed_tables(batch: ForwardBatch) -> np.ndarray:
     offs, data = _ragged(batch.block_tables)
     b = len(batch.block_tables)
     width = max([len(t) for t in batch.block_tables] + [1])
     out = np.zeros((max(b, 1), width), dtype=np.uint32)
     w = check(lib().vapi_pack_block_tables(b, _ptr(offs), _ptr(data), _ptr(out), out.size))
     assert w == width
-    return torch.from_numpy(out[:b].view(np.int32)).to(device)
+    return out[:b]
+
+
+def pack_block_tables(batch: ForwardBatch, device) -> torch.Tensor:
+    """[batch, max_blocks] u32 (as int32 bits), rows padded with their own
+    last block (attention.rs:42-62)."""
+    return torch.from_numpy(_packed_tables(batch).view(np.int32)).to(device)
 
 
 def cu_seqlens(values, device) -> torch.Tensor:
@@ -143,7 +147,8 @@ class PreparedAttention:
         if lens_q.size and not np.any(lens_q == 1):
             flags |= ATTN_NO_DECODE_ROWS
         pf = np.nonzero(lens_q > 1)[0]
-        prep = cls(block_table=pack_block_tables(batch, device),
+        packed = _packed_tables(batch)
+        prep = cls(block_table=torch.from_numpy(packed.view(np.int32)).to(device),
                    seqlens_q=cu_seqlens(batch.cu_seqlens_q, device),
                    seqlens_k=cu_seqlens(batch.cu_seqlens_k, device),
                    max_seqlen_q=int(batch.max_seqlen_q),
@@ -151,7 +156,7 @@ class PreparedAttention:
                    prefill_seqs=cu_seqlens(pf if pf.size else [0], device),
                    n_prefill=int(pf.size))
         if share_prefixes:
-            prep.prefixes = PrefixPlan.from_batch(batch, cache, num_heads, device)
+            prep.prefixes = PrefixPlan.from_batch(batch, cache, num_heads, device, packed)
         if cache is not None and num_heads is not None:
             prep.reserve(cache, num_heads, device)
         return prep
@@ -284,8 +289,8 @@ def paged_attention_prepared(q: torch.Tensor, cache: PagedKvCache, layer: int,
     unlimited (flash convention); the default right window 0 is causal.
     `sinks`: a sequence's first keys that stay visible behind its left window
     (vapi_paged_attention_sinks). A step prepared with share_prefixes reads
-    shared prefixes once (vapi_paged_attention_shared). `cache` may be a HybridKvCache (`layer` then names one of its K/V layers)
-    or a QuantKvCache."""
+    shared prefixes once (vapi_paged_attention_shared). `cache` may be a
+    HybridKvCache (`layer` then names one of its K/V layers) or a QuantKvCache."""
     cache, layer = _per_layer(cache, layer)
     if q.dim() != 3 or q.shape[2] != cache.head_dim:
         raise ValueError(f"q must be (tokens, heads, {cache.head_dim}), got {tuple(q.shape)}")

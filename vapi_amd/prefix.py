@@ -36,7 +36,7 @@ def find_shared_prefixes(block_tables, lens_q, lens_k, block_size: int,
     common prefixes the one that saves the most key reads, (members - 1) * keys a
     group. Whole blocks within every member's context are shared. Sequences of more
     than `max_queries` queries are left out."""
-    tables = [np.asarray(t, dtype=np.int64)[:max(int(lk), 0) // block_size]
+    tables = [np.asarray(t)[:max(int(lk), 0) // block_size]
               for t, lk in zip(block_tables, lens_k)]
     live = [i for i, t in enumerate(tables) if len(t) and 1 <= lens_q[i] <= max_queries]
 
@@ -128,14 +128,19 @@ class PrefixPlan:
         return saved >= self.min_bytes[1 if fmt else 0]
 
     @classmethod
-    def from_batch(cls, batch, cache, num_heads: int | None, device) -> "PrefixPlan | None":
+    def from_batch(cls, batch, cache, num_heads: int | None, device,
+                   packed=None) -> "PrefixPlan | None":
         """The plan of a ForwardBatch over `cache`, for layers that it pays for; None
         where no two sequences share a block. Without `num_heads`, single queries are
-        grouped only."""
+        grouped only. `packed`: the batch's tables as rows of an array, if at hand (128
+        tables of 2,068 entries take 15 ms as lists, 1 ms as rows)."""
+        tables = batch.block_tables
+        if packed is not None:
+            tables = [row[:len(t)] for row, t in zip(packed, tables)]
         heads = getattr(cache, "num_kv_heads", None) or min(
             s[1] for s in cache.layouts if s[0] == "kv")
         queries = max(MAX_ROWS * heads // num_heads, 1) if num_heads else 1
-        groups = find_shared_prefixes(batch.block_tables, np.diff(batch.cu_seqlens_q),
+        groups = find_shared_prefixes(tables, np.diff(batch.cu_seqlens_q),
                                       np.diff(batch.cu_seqlens_k), cache.block_size, queries)
         return cls(groups, batch.cu_seqlens_q, batch.cu_seqlens_k, device,
                    (MIN_SAVED_BYTES, MIN_SAVED_BYTES_Q8)) if groups else None
