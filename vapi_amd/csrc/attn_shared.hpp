@@ -540,6 +540,8 @@ __device__ __forceinline__ void sh_piece(const AttnArgs& a, const SharedArgs& sh
     const float lt = wave_sum_g(l_run[t]);
     const float inv = lt > 0.f ? 1.f / lt : 0.f;
     const uint32_t row = wave * 16 * RT + 16 * t + col;  // of the tile
+    const uint32_t r = tile * kRows + row, j = r / a.g_real;
+    if (j >= n.tokens) continue;
     if (pb) {
       // Per row (m in scaled log2 units, l), then o / l (pf_part_bytes).
       if (g == 0) *(float2*)(pb + (uint64_t)row * 8) = make_float2(m_run[t], lt);
@@ -550,8 +552,6 @@ __device__ __forceinline__ void sh_piece(const AttnArgs& a, const SharedArgs& sh
                                                       o[t][k][2] * inv, o[t][k][3] * inv);
       continue;
     }
-    const uint32_t r = tile * kRows + row, j = r / a.g_real;
-    if (j >= n.tokens) continue;
     T* orow = (T*)a.out + ((uint64_t)(n.first + j) * a.num_heads + kh * a.g_real + (r - j * a.g_real)) *
                               (kPad ? a.hd : D);
 #pragma unroll
@@ -680,12 +680,12 @@ __device__ __forceinline__ void sh_merge(const AttnArgs& a, const SharedArgs& sh
   auto fetch = [&](uint32_t j0, uint32_t n, auto at) __attribute__((always_inline)) {
 #pragma unroll
     for (uint32_t u = 0; u < kB; ++u) {
-      const bool in = j0 + u < n;
+      ml[u].y = 0.f;
+      if (j0 + u >= n) continue;
       const float *pm, *px;
-      at(in ? j0 + u : j0, pm, px);
+      at(j0 + u, pm, px);
       ml[u] = *(const float2*)pm;
       x[u] = *(const float4*)px;
-      if (!in) ml[u].y = 0.f;
     }
   };
   // Joins what was fetched. kNormed: it is o / l (tiles'), else o (the stream's).
