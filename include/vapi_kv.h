@@ -718,9 +718,8 @@ int vapi_kv_q8_attention_sinks(const vapi_kv_q8_pool* pool, uint32_t layer, cons
                                void* workspace, size_t workspace_bytes, vapi_stream_t stream);
 
 /* vapi_kv_q8_attention over a batch with shared prefixes (see
- * vapi_paged_attention_shared). The shared keys' codes, and those of the listed
- * prefill sequences' own keys, are expanded in the workspace once: n_groups *
- * max_keys and n_prefill * max_seqlen_k keys of the layer in the pool's dtype. */
+ * vapi_paged_attention_shared). Prefill sequences and groups read the codes
+ * themselves: nothing is expanded in the workspace. */
 size_t vapi_kv_q8_attention_shared_workspace_size(const vapi_kv_q8_pool* pool, uint32_t batch,
                                                   uint32_t n_prefill, uint32_t num_heads,
                                                   uint32_t max_seqlen_q, uint32_t max_seqlen_k,

@@ -216,7 +216,7 @@ def test_the_step_finds_its_prefixes():
 def test_pools_that_take_no_prefixes_run_the_ordinary_call():
     cache, q, batch, plan = make([(70, decode(6, 1, 200, 1))], [(1, 30)], 8, 2, 64, F32)
     prep = PreparedAttention.from_batch(batch, DEV, cache, 8, share_prefixes=True)
-    prep.prefixes.min_bytes = (0, 0)  # whatever it saves
+    prep.prefixes.min_bytes = 0  # whatever it saves
     prep.sharing.clear()
     assert prep.shared_bytes(cache, 8) == 0 and b"16-bit" in lib().vapi_kv_last_error()
     got = paged_attention_prepared(q, cache, 0, prep, 0.1)
@@ -254,7 +254,7 @@ def test_layers_of_different_geometry_in_one_step():
                          max_seqlen_q=1, max_seqlen_k=850)
     prep = PreparedAttention.from_batch(batch, DEV, cache, 4, share_prefixes=True)
     assert prep.prefixes.groups == [([0, 1, 2], 800)]
-    prep.prefixes.min_bytes = (0, 0)  # whatever it saves
+    prep.prefixes.min_bytes = 0  # whatever it saves
     prep.sharing.clear()
     prep.reserve(cache, 4, DEV)
     assert all(prep.sharing.values())

@@ -39,7 +39,7 @@ COMMON_FLAGS = [
 
 SOURCES = ["kv_ops.hip", "attention.hip", "attn_decode.hip", "attn_decode_small.hip",
            "attn_prefill.hip", "attn_prefill_f32.hip", "attn_generic.hip", "q8_ops.hip",
-           "attn_q8.hip", "attn_shared.hip", "kv_weights.hip", "kv_evict.hip", "host.cpp", "spill.cpp"]
+           "attn_q8.hip", "attn_q8_shared.hip", "attn_shared.hip", "kv_weights.hip", "kv_evict.hip", "host.cpp", "spill.cpp"]
 
 # Matrix products into the registers that the vector unit reads; through the
 # accumulation ones each score is copied once (the 8-bit decode 76.6 -> 75.2 us
@@ -58,6 +58,8 @@ EXTRA_FLAGS = {"attn_decode.hip": ["-fno-honor-nans", "-Rpass-analysis=kernel-re
                "attn_shared.hip": ["-fno-honor-nans", "-Rpass-analysis=kernel-resource-usage"],
                "attn_q8.hip": ["-fno-honor-nans", *VGPR_FORM,
                                "-Rpass-analysis=kernel-resource-usage"],
+               "attn_q8_shared.hip": ["-fno-honor-nans", *VGPR_FORM,
+                                      "-Rpass-analysis=kernel-resource-usage"],
                "kv_weights.hip": ["-fno-honor-nans", *VGPR_FORM,
                                   "-Rpass-analysis=kernel-resource-usage"]}
 
@@ -72,6 +74,7 @@ NO_SCRATCH = {"attn_prefill.hip": ("paged_prefill_tiled", "paged_mixed_stream"),
               "attn_prefill_f32.hip": ("paged_prefill_f32",),
               "attn_shared.hip": ("paged_shared_stream",),
               "attn_q8.hip": ("q8_decode_stream", "q8_decode_small"),
+              "attn_q8_shared.hip": ("q8_shared_stream",),
               "kv_weights.hip": ("weights_lse", "weights_sum")}
 
 # Half of a CU's 160 KiB of LDS less the dynamic part (4 bytes for each of the

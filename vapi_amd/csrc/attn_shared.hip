@@ -129,9 +129,6 @@ SharedArgs shared_args(const vapi_kv_prefixes* p, const AttnArgs& a, uint32_t he
   sh.max_joined = (uint32_t)joined_tiles(p, a.g_real, head_dim, n_pf);
   sh.max_grouped = (uint32_t)grouped_tiles(p, a.g_real, head_dim);
   sh.ranges = shared_ranges(p, a.kvh / a.kv_parts.d, a.g_real, head_dim, n_pf);
-  sh.last_blk = a.last_blk;
-  sh.k = a.k, sh.v = a.v;
-  sh.blk_e = a.blk_e, sh.head_e = a.head_e, sh.tok_e = a.tok_e;
   const SharedWs w = shared_ws(a.batch, a.kvh / a.kv_parts.d, head_dim, sh.max_joined,
                                p->n_rows);
   sh.lds_rows =
@@ -158,11 +155,15 @@ SharedArgs shared_args(const vapi_kv_prefixes* p, const AttnArgs& a, uint32_t he
     }                                                            \
   } while (0)
 
-static void launch_shared_stream(const AttnArgs& a, const SharedArgs& sh, uint32_t head_dim,
-                                 bool bf16, uint32_t nwg, uint32_t ranges, hipStream_t s) {
+size_t shared_lds(const AttnArgs& a, const SharedArgs& sh, uint32_t nwg, uint32_t ranges) {
   const size_t plan =
       sh_plan_bytes(sh.n_nodes) + (sh.lds_rows ? sh.n_rows * sizeof(ShEntry) : 0);
-  const size_t lds = std::max(ranges ? plan : 0, nwg ? (a.batch + 1) * sizeof(uint32_t) : 0);
+  return std::max(ranges ? plan : 0, nwg ? (a.batch + 1) * sizeof(uint32_t) : 0);
+}
+
+static void launch_shared_stream(const AttnArgs& a, const SharedArgs& sh, uint32_t head_dim,
+                                 bool bf16, uint32_t nwg, uint32_t ranges, hipStream_t s) {
+  const size_t lds = shared_lds(a, sh, nwg, ranges);
   // (A group of query heads in parts reads its keys with ordinary loads: launch_stream.)
 #define VK_SHT(T, DD)                                                                            \
   do {                                                                                           \
@@ -174,11 +175,6 @@ static void launch_shared_stream(const AttnArgs& a, const SharedArgs& sh, uint32
   } while (0)
   VK_SH_ALL(VK_SHT);
 #undef VK_SHT
-}
-
-void launch_shared_tiles(const AttnArgs& a, const SharedArgs& sh, uint32_t head_dim, bool bf16,
-                         hipStream_t s) {
-  launch_shared_stream(a, sh, head_dim, bf16, 0, sh.ranges, s);
 }
 
 void launch_shared(const AttnArgs& a, const SharedArgs& sh, uint32_t head_dim, bool bf16,

@@ -26,6 +26,7 @@
 
 #include "attn_decode.hpp"
 #include "attn_prefill.hpp"
+#include "q8.hpp"
 
 namespace vk {
 
@@ -67,13 +68,8 @@ struct SharedArgs {
   uint32_t max_joined;   // joined tiles of a kv head, at most
   uint32_t max_grouped;  // the groups' of them (the first, in step order)
   uint32_t ranges;
-  // Blocks of node i at tables[i * table_width ..] (null: a.table's rows).
-  const uint32_t* tables;
-  uint32_t table_width;
-  uint32_t last_blk;
-  const char *k, *v;  // the pool they lie in
-  uint64_t blk_e, head_e;
-  uint32_t tok_e;
+  const float *ks, *vs;  // 8-bit pools: the layer's scales, sblk a block
+  uint32_t sblk;
   uint32_t lds_rows;  // whether every query of the groups has an entry in LDS
   // Workspace: the groups' tiles of a kv head; joined tiles, max_grouped of each kv head
   // for the groups and then the rest for each; the ranges' open tiles; the first joined
@@ -262,6 +258,16 @@ __device__ __forceinline__ void sh_issue(const ShSlots<D, W, kPad>& sl, uint16_t
   else all(std::false_type{});
 }
 
+// A thread's codes of a step: 16 of a row at a time (D == 64: of K in the first half of
+// the workgroup, of V in the other), and the scales of their block.
+template <int D>
+struct ShCodes {
+  static constexpr uint32_t CPR = D / 16;     // chunks of 16 codes a row
+  static constexpr int N = D == 256 ? 2 : 1;  // chunks of a tensor
+  uint4 k[N], v[N];
+  float ks[N], vs[N];
+};
+
 // Four ds_read_b64_tr_b16 issued without waiting (results valid only after a later
 // lgkm wait that names the same registers): the d tiles at a0 and a1, their keys 0 .. 15
 // and, 16 rows on (the swizzle repeats), 16 .. 31.
@@ -277,8 +283,15 @@ __device__ __forceinline__ void sh_read_tr16(uint2 (&r)[4], uint32_t a0, uint32_
       : "memory");
 }
 // Counts [u0, u1) of the c of a node's tile at kv head kh (its share of the steps),
-// to the partial `pb`, or to the output if pb is null.
-template <typename T, int D, bool kPad>
+// to the partial `pb`, or to the output if pb is null. F: the format of an 8-bit pool's
+// codes, kShValues where the pool holds values of T. Codes come through registers, three
+// steps ahead, and are expanded into the ring a step before they are used (exactly: every
+// code times its scale is a value of T): 128 columns of 32 keys are 16 codes of K and of V
+// a thread. (Expanded by a launch of its own into a 16-bit pool in the workspace, 32
+// sequences over 5,008 keys, 32 kv heads, took 26 us more: 41 MB read, 82 written, 82
+// read again.)
+constexpr int kShValues = -1;
+template <typename T, int D, bool kPad, int F>
 __device__ __forceinline__ void sh_piece(const AttnArgs& a, const SharedArgs& sh, uint32_t node,
                                          const ShNode* nodes, const ShEntry* entries,
                                          uint32_t tile, uint32_t kh, uint32_t u0, uint32_t u1,
@@ -286,6 +299,8 @@ __device__ __forceinline__ void sh_piece(const AttnArgs& a, const SharedArgs& sh
   constexpr int RT = sh_row_tiles<D>(), W = kShWaves, KC = D / 32, DT = D / 16;
   constexpr uint32_t kRows = 16 * RT * W;
   constexpr int kLoadsPerStep = D >= 128 ? 2 * D / (16 * W) : 2;
+  constexpr bool kCodes = F != kShValues;
+  using E = std::conditional_t<kCodes, uint8_t, T>;  // of the pool
   // (Three separate objects a tensor: see prefill_piece.)
   __shared__ __attribute__((aligned(16))) uint16_t kb0[32 * D], kb1[32 * D], kb2[32 * D];
   __shared__ __attribute__((aligned(16))) uint16_t vb0[32 * D], vb1[32 * D], vb2[32 * D];
@@ -303,12 +318,10 @@ __device__ __forceinline__ void sh_piece(const AttnArgs& a, const SharedArgs& sh
   const uint32_t row0 = tile * kRows + wave * 16 * RT;
   const int32_t sinks = n.k0 ? 0 : a.sinks;
 
-  const uint32_t* __restrict__ tab =
-      sh.tables ? sh.tables + (uint64_t)node * sh.table_width
-                : a.table + (uint64_t)n.seq * a.max_blocks;
-  const uint32_t width = (sh.tables ? sh.table_width : a.max_blocks) - 1;
-  const T* kb = (const T*)sh.k + kh * sh.head_e;
-  const T* vb = (const T*)sh.v + kh * sh.head_e;
+  const uint32_t* __restrict__ tab = a.table + (uint64_t)n.seq * a.max_blocks;
+  const uint32_t width = a.max_blocks - 1;
+  const E* kb = (const E*)a.k + kh * a.head_e;
+  const E* vb = (const E*)a.v + kh * a.head_e;
   // The keys [klo, khi] that the tile's rows see, this share of their steps, and the
   // share's first two on their way.
   int32_t klo = 0, khi = -1, s0_ = 0, s_last = -32;
@@ -322,11 +335,64 @@ __device__ __forceinline__ void sh_piece(const AttnArgs& a, const SharedArgs& sh
     return make_uint2(((ConstU32*)tab)[min((uint32_t)rd.tile(s0) >> a.bs_shift, width)],
                       ((ConstU32*)tab)[min((uint32_t)rd.tile(s0 + 16) >> a.bs_shift, width)]);
   };
-  const ShSlots<D, W, kPad> slots(tid, sh.tok_e, a.hd);
+  const ShSlots<D, W, kPad> slots(tid, a.tok_e, a.hd);
   auto load = [&](uint16_t* kd, uint16_t* vd, int32_t at, uint2 blk) __attribute__((always_inline)) {
-    sh_issue<T, D, W, kPad>(slots, kd, vd, kb, vb, min(blk.x, sh.last_blk),
-                            min(blk.y, sh.last_blk), sh.blk_e, sh.tok_e, a.block_size, ks.key(at),
-                            KeyReads(ks, at, klo, khi, sinks), wave);
+    if constexpr (!kCodes)
+      sh_issue<T, D, W, kPad>(slots, kd, vd, kb, vb, min(blk.x, a.last_blk), min(blk.y, a.last_blk),
+                              a.blk_e, a.tok_e, a.block_size, ks.key(at),
+                              KeyReads(ks, at, klo, khi, sinks), wave);
+  };
+  using Codes = ShCodes<D>;
+  Codes c0, c1, c2;
+  const uint32_t slot_c = D == 64 ? tid & 127 : tid, row_c = slot_c / Codes::CPR;
+  const uint32_t col_c = slot_c % Codes::CPR;  // in chunks
+  auto load_codes = [&](Codes& x, int32_t at, uint2 blk) __attribute__((always_inline)) {
+    using ConstF32 = const __attribute__((address_space(4))) float;
+    const KeyReads rd(ks, at, klo, khi, sinks);
+    const int32_t s0 = ks.key(at);
+    const uint32_t d = kPad && 16 * col_c >= a.hd ? 0 : 16 * col_c;
+#pragma unroll
+    for (int j = 0; j < Codes::N; ++j) {
+      // (A wave's rows lie in one 16-key tile, so in one block.)
+      const bool second = D == 256 ? j == 1 : D == 128 ? wave >= 2 : wave & 1;
+      const uint32_t b = min(second ? blk.y : blk.x, a.last_blk);
+      const int32_t ts = rd.tile(second ? s0 + 16 : s0);
+      const uint64_t off = (uint64_t)b * a.blk_e +
+                           (uint64_t)((uint32_t)ts & (a.block_size - 1)) * a.tok_e +
+                           (rd.row((int32_t)(row_c & 15), ts) * a.tok_e + d);
+      const uint64_t si = (uint64_t)b * sh.sblk + kh;
+      if constexpr (D == 64) {
+        x.k[j] = *(const uint4*)((wave < 2 ? kb : vb) + off);
+        x.ks[j] = ((ConstF32*)(wave < 2 ? sh.ks : sh.vs))[si];
+      } else {
+        x.k[j] = *(const uint4*)(kb + off), x.v[j] = *(const uint4*)(vb + off);
+        x.ks[j] = ((ConstF32*)sh.ks)[si], x.vs[j] = ((ConstF32*)sh.vs)[si];
+      }
+    }
+  };
+  auto expand = [&](const Codes& x, uint16_t* kd, uint16_t* vd) __attribute__((always_inline)) {
+    auto put = [&](uint16_t* buf, int j, uint4 w, float s) __attribute__((always_inline)) {
+      const uint32_t r = row_c + 16 * j;
+      const uint2 e0 = q8_expand4<T, F, true>(w.x, s), e1 = q8_expand4<T, F, true>(w.y, s);
+      const uint2 e2 = q8_expand4<T, F, true>(w.z, s), e3 = q8_expand4<T, F, true>(w.w, s);
+      *(uint4*)(buf + pf_chunk<D>(r, 2 * col_c)) = make_uint4(e0.x, e0.y, e1.x, e1.y);
+      *(uint4*)(buf + pf_chunk<D>(r, 2 * col_c + 1)) = make_uint4(e2.x, e2.y, e3.x, e3.y);
+    };
+#pragma unroll
+    for (int j = 0; j < Codes::N; ++j) {
+      if constexpr (D == 64) {
+        if (wave < 2) put(kd, j, x.k[j], x.ks[j]);
+        else put(vd, j, x.k[j], x.ks[j]);
+      } else {
+        put(kd, j, x.k[j], x.ks[j]), put(vd, j, x.v[j], x.vs[j]);
+      }
+    }
+  };
+  // The next step's rows are in the ring, all waves'.
+  auto ring_ready = [&]() __attribute__((always_inline)) {
+    if constexpr (kCodes) __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    else wait_vmcnt<kLoadsPerStep>();
+    ring_barrier();
   };
   uint2 blk{0, 0};  // of the step whose loads are issued next
   auto begin = [&](int32_t lo_, int32_t hi_) __attribute__((always_inline)) {
@@ -337,9 +403,17 @@ __device__ __forceinline__ void sh_piece(const AttnArgs& a, const SharedArgs& sh
     s_last = 32 * (int32_t)pf_step_at(u1, c, all) - 32;
     if (s0_ <= s_last) {  // (uniform)
       const uint2 b0 = lookup(s0_), b1 = lookup(min(s0_ + 32, s_last));
-      blk = lookup(min(s0_ + 64, s_last));
-      load(kb0, vb0, s0_, b0);
-      load(kb1, vb1, min(s0_ + 32, s_last), b1);
+      const uint2 b2 = lookup(min(s0_ + 64, s_last));
+      if constexpr (kCodes) {
+        blk = lookup(min(s0_ + 96, s_last));
+        load_codes(c0, s0_, b0);
+        load_codes(c1, min(s0_ + 32, s_last), b1);
+        load_codes(c2, min(s0_ + 64, s_last), b2);
+      } else {
+        blk = b2;
+        load(kb0, vb0, s0_, b0);
+        load(kb1, vb1, min(s0_ + 32, s_last), b1);
+      }
     }
   };
   // Without a left window the keys follow from the node: the first loads need not wait
@@ -440,12 +514,18 @@ __device__ __forceinline__ void sh_piece(const AttnArgs& a, const SharedArgs& sh
     uint16_t* const knext = B == 0 ? kb2 : B == 1 ? kb0 : kb1;
     uint16_t* const vnext = B == 0 ? vb2 : B == 1 ? vb0 : vb1;
     const int32_t at = __builtin_amdgcn_readfirstlane(s0_), s0 = ks.key(at);
-    load(knext, vnext, min(at + 64, s_last), blk);
-    blk = lookup(min(at + 96, s_last));
+    if constexpr (kCodes) {
+      Codes& x = B == 0 ? c1 : B == 1 ? c2 : c0;
+      expand(x, B == 0 ? kb1 : B == 1 ? kb2 : kb0, B == 0 ? vb1 : B == 1 ? vb2 : vb0);
+      load_codes(x, min(at + 128, s_last), blk);
+      blk = lookup(min(at + 160, s_last));
+    } else {
+      load(knext, vnext, min(at + 64, s_last), blk);
+      blk = lookup(min(at + 96, s_last));
+    }
     s0_ += 32;
     if (!active) {
-      wait_vmcnt<kLoadsPerStep>();
-      ring_barrier();
+      ring_ready();
       return;
     }
     const bool masked = !(s0 >= full_lo && s0 + 31 <= full_hi);
@@ -518,12 +598,15 @@ __device__ __forceinline__ void sh_piece(const AttnArgs& a, const SharedArgs& sh
         for (int t = 0; t < RT; ++t) o[t][2 * b + k] = mfma16x16x32<T>(vf, pf[t], o[t][2 * b + k]);
       }
     }
-    wait_vmcnt<kLoadsPerStep>();
-    ring_barrier();
+    ring_ready();
   };
   if (s0_ <= s_last) {  // (uniform)
-    wait_vmcnt<kLoadsPerStep>();
-    ring_barrier();
+    if constexpr (kCodes) {
+      expand(c0, kb0, vb0);
+      load_codes(c0, min(s0_ + 96, s_last), blk);
+      blk = lookup(min(s0_ + 128, s_last));
+    }
+    ring_ready();
     while (true) {
       step(std::integral_constant<int, 0>{});
       if (s0_ > s_last) break;
@@ -565,7 +648,7 @@ __device__ __forceinline__ void sh_piece(const AttnArgs& a, const SharedArgs& sh
 // Workgroup `bid` of sh.ranges. lds: sh_plan_bytes, and with sh.lds_rows an entry for
 // each of the groups' queries: read while nothing else runs yet, where a round trip to
 // memory is short (beside the stream at work it takes 4 to 5 us).
-template <typename T, int D, bool kPad>
+template <typename T, int D, bool kPad, int F = kShValues>
 __device__ __forceinline__ void sh_range(const AttnArgs& a, const SharedArgs& sh, uint32_t* lds,
                                          uint32_t bid) {
   constexpr uint32_t kRows = sh_rows(D);
@@ -630,7 +713,7 @@ __device__ __forceinline__ void sh_range(const AttnArgs& a, const SharedArgs& sh
       if (joins && !group && kh == 0 && tile == 0) sh.own[nodes[node].seq] = j0 - n_grouped;
     }
     open = open || (u0 == 0 && !joins && !whole);
-    sh_piece<T, D, kPad>(a, sh, node, nodes, entries, tile, kh, u0, u1, c,
+    sh_piece<T, D, kPad, F>(a, sh, node, nodes, entries, tile, kh, u0, u1, c,
                          joins || !whole ? sh.part + (uint64_t)slot * pf_part_bytes(kRows, D)
                                          : nullptr);
     after = 1;
@@ -781,10 +864,12 @@ SharedArgs shared_args(const vapi_kv_prefixes* p, const AttnArgs& a, uint32_t he
 // the merge of their partials.
 void launch_shared(const AttnArgs& a, const SharedArgs& sh, uint32_t head_dim, bool bf16,
                    bool decode, hipStream_t s);
-// Its parts, where another kernel streams the decode rows.
-void launch_shared_tiles(const AttnArgs& a, const SharedArgs& sh, uint32_t head_dim, bool bf16,
-                         hipStream_t s);
+// The same over an 8-bit pool (sh.ks, sh.vs and sh.sblk set).
+void launch_q8_shared(const AttnArgs& a, const SharedArgs& sh, uint32_t head_dim, bool bf16,
+                      bool e4m3, bool decode, hipStream_t s);
+// Their merge, and the dynamic LDS of a launch of nwg and `ranges` workgroups.
 void launch_shared_merge(const AttnArgs& a, const SharedArgs& sh, uint32_t head_dim, bool bf16,
                          bool decode, hipStream_t s);
+size_t shared_lds(const AttnArgs& a, const SharedArgs& sh, uint32_t nwg, uint32_t ranges);
 
 }  // namespace vk

@@ -18,10 +18,9 @@ from ._lib import Prefixes
 # Sharing costs a fixed 15 to 25 us a layer against the ordinary call (tiles, partial
 # results, their merge), which this many bytes of K and V take to read: 8 sequences
 # over 2,000 keys (57 MB saved, 32 q / 8 kv heads) 29 us shared, 14 not; 32 over 1,000
-# (126 MB) 33 and 34; 64 over 1,000 (256 MB) 41 and 55. An 8-bit cache's shared codes
-# are expanded first.
+# (126 MB) 33 and 34; 64 over 1,000 (256 MB) 41 and 55. In e4m3: 16 over 4,000 (123 MB)
+# 33 and 34; 64 over 1,000 (128 MB) 38 and 36; 16 over 2,000 (32 kv heads, 246 MB) 30 and 56.
 MIN_SAVED_BYTES = 128 << 20
-MIN_SAVED_BYTES_Q8 = 128 << 20
 # Rows (queries times query heads of a kv head) that a sequence brings to a group at
 # most. More fill tiles by themselves, and read the prefix for many rows at once anyway:
 # 16 sequences over 2,000 keys (32 kv heads), 64 queries each: 109 us shared, 147 not;
@@ -81,9 +80,9 @@ def find_shared_prefixes(block_tables, lens_q, lens_k, block_size: int,
 
 class PrefixPlan:
     """The groups of a step and their device lists (vapi_kv_prefixes). `min_bytes`:
-    the K and V bytes of a layer that sharing has to save there (16-bit, 8-bit)."""
+    the K and V bytes that sharing has to save in a layer."""
 
-    def __init__(self, groups, cu_seqlens_q, cu_seqlens_k, device, min_bytes=(0, 0)):
+    def __init__(self, groups, cu_seqlens_q, cu_seqlens_k, device, min_bytes: int = 0):
         cq = np.asarray(cu_seqlens_q, dtype=np.int64)
         lens_k = np.diff(np.asarray(cu_seqlens_k, dtype=np.int64))
         batch = len(lens_k)
@@ -122,10 +121,9 @@ class PrefixPlan:
         return total
 
     def worth_it(self, cache, window_left: int | None = None) -> bool:
-        fmt = getattr(cache, "fmt", None)
-        size = 1 if fmt else torch.empty((), dtype=cache.dtype).element_size()
+        size = 1 if getattr(cache, "fmt", None) else torch.empty((), dtype=cache.dtype).element_size()
         saved = self.saved_keys(window_left) * 2 * cache.num_kv_heads * cache.head_dim * size
-        return saved >= self.min_bytes[1 if fmt else 0]
+        return saved >= self.min_bytes
 
     @classmethod
     def from_batch(cls, batch, cache, num_heads: int | None, device,
@@ -143,4 +141,4 @@ class PrefixPlan:
         groups = find_shared_prefixes(tables, np.diff(batch.cu_seqlens_q),
                                       np.diff(batch.cu_seqlens_k), cache.block_size, queries)
         return cls(groups, batch.cu_seqlens_q, batch.cu_seqlens_k, device,
-                   (MIN_SAVED_BYTES, MIN_SAVED_BYTES_Q8)) if groups else None
+                   MIN_SAVED_BYTES) if groups else None
