@@ -373,13 +373,13 @@ typedef struct vapi_kv_prefixes {
  * tables differ attends the first one's blocks.
  *
  * f16 and bf16 pools with head_dim a multiple of 8 up to 256 and block_size a power of
- * two from 16, up to 256 query heads per kv head, 4,096 sequences and 1,024 groups and
+ * two from 16, up to 256 query heads per kv head, 4,096 sequences and 1,000 groups and
  * prefill sequences together (else VAPI_KV_EUNSUP: such a batch runs
  * vapi_paged_attention_sinks). The workspace has no optional part: all that
  * vapi_paged_attention_shared_workspace_size returns, by the same rules as
  * vapi_paged_attention's and usable by its calls too; that size is 0 where the call
- * would be refused (vapi_kv_last_error says why). No counterpart in the reference, which reads a shared
- * prefix once for each sequence (attention.rs:90-163).
+ * would be refused (vapi_kv_last_error says why). No counterpart in the reference,
+ * which reads a shared prefix once for each sequence (attention.rs:90-163).
  */
 size_t vapi_paged_attention_shared_workspace_size(const vapi_kv_pool* pool, uint32_t batch,
                                                   uint32_t n_prefill, uint32_t num_heads,

@@ -155,6 +155,12 @@ def test_long_prefixes_and_large_batches(dtype, d):
           d, dtype)
 
 
+@pytest.mark.parametrize("d,fmt", [(256, "none"), (256, "e4m3"), (64, "none")])
+def test_as_many_groups_as_a_call_takes(d, fmt):
+    check([(1, [(1, 1 + i % 7), (1, 2 + i % 5)]) for i in range(1000)], [(1, 40)], 2, 1, d, BF16,
+          fmt=fmt)
+
+
 def test_prompts_fill_many_tiles():
     """Long prompts beside a group: whole tiles, open ones and joined ones."""
     check([(40, [(1, 20), (200, 300), (64, 64)])], [(700, 900), (300, 300), (1, 2000)], 16, 4, 128,

@@ -186,7 +186,8 @@ def test_shared_prefixes_refuse(q8):
         assert size(make(), 4, 0, 8, 1, 100, bad) == 0
     none = ctypes.POINTER(_lib.Prefixes)()
     assert call(fn, make(), none) == _lib.EINVAL and b"null prefixes" in L.vapi_kv_last_error()
-    assert call(fn, make(), prefixes(n_groups=2000)) == _lib.EUNSUP
+    assert call(fn, make(), prefixes(n_groups=1001)) == _lib.EUNSUP
+    assert call(fn, make(), prefixes(n_groups=1000)) == _lib.ESPACE
     big = HEAD[:5] + [5000, 8]
     assert call(fn, make(), ok, head=big) == _lib.EUNSUP
     assert call(fn, make(), prefixes(n_rows=1 << 31)) == _lib.EUNSUP

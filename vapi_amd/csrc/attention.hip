@@ -605,6 +605,7 @@ static int paged_attention_impl(const vapi_kv_pool* pool, uint32_t layer, const 
   a.pf_seqs_n = pf_n;
   a.pf_order = kPfListOrder;
   a.kv_parts = FastDiv(1);
+  a.plan_parts = 1;
   a.g_real = a.group;
   a.hd = g.d;
   const hipStream_t s = hs(stream);
@@ -616,6 +617,7 @@ static int paged_attention_impl(const vapi_kv_pool* pool, uint32_t layer, const 
     dec.kvh = a.kvh * parts;
     dec.group = (a.group + parts - 1) / parts;
     dec.kv_parts = FastDiv(parts);
+    dec.plan_parts = parts;
   }
 
   if (mfma16_ok(pool, num_heads)) {

@@ -100,6 +100,10 @@ struct AttnArgs {
   // kernel's D (a multiple of 8 up to 256) at the next of 64, 128 or 256:
   // elements d >= hd are loaded as zeros and not stored.
   uint32_t hd;
+  // How many (virtual) kv heads, one after the other, the stream's plan gives to as
+  // many waves side by side, over the same keys: the parts of a group, or heads whose
+  // rows share cache lines.
+  uint32_t plan_parts;
 };
 
 // A prefill work item: query tile qt of list entry li (sequence seq, its rows

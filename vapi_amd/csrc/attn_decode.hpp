@@ -803,7 +803,7 @@ __device__ __forceinline__ void decode_merge_body(const AttnArgs& a, uint32_t nw
       for (int u = 0; u < R; ++u) {
         const uint32_t pc = w + u * WPS;
         const bool in = pc <= r1;
-        const uint64_t sl = ((uint64_t)pc * a.kv_parts.d + seg) * G;
+        const uint64_t sl = ((uint64_t)pc * a.plan_parts + seg) * G;
         const float* po = a.ws_o + sl * D + e_lane + j0;
         if (in && n == 8) {
           const float4 v0 = *(const float4*)po, v1 = *(const float4*)(po + 4);

@@ -180,7 +180,7 @@ __device__ __forceinline__ void q8_stream_body(const AttnArgs& a, const Q8Scales
   const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t B = a.batch;
-  const uint32_t n_parts = a.kv_parts.d, kvh_plan = a.kvh / n_parts;
+  const uint32_t n_parts = a.plan_parts, kvh_plan = a.kvh / n_parts;
   const uint32_t t_entry = (uint32_t)__builtin_amdgcn_s_memrealtime();
   {
     constexpr uint32_t NT = 64 * kDecodeWavesPerWG;

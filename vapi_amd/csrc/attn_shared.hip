@@ -109,12 +109,14 @@ int shared_check(const vapi_kv_prefixes* p, uint32_t batch, uint32_t kvh, uint32
   if (batch > decode_max_plan_seqs() || (uint64_t)p->n_groups + n_pf > kShMaxNodes)
     VK_FAIL(VAPI_KV_EUNSUP, "%s: %u sequences, %u groups and %u prefill sequences", who, batch,
             p->n_groups, n_pf);
-  // Steps of a kv head and workgroups of the merge stay in 32 bits.
+  // Steps of a kv head and threads of the merge (16 workgroups a joined tile) stay in
+  // 32 bits.
   const uint64_t rows = sh_rows(head_dim), joined = joined_tiles(p, group, head_dim, n_pf);
   const uint64_t tiles =
       (uint64_t)p->n_rows * group / rows + p->n_groups +
       n_pf * (((uint64_t)max_q * group + rows - 1) / rows);
-  if (tiles * ((uint64_t)max_k / 32 + 4 + kShTileSteps) > 0xFFFFFFFFull || (joined + 1) * kvh > 0xFFFFFFull)
+  if (tiles * ((uint64_t)max_k / 32 + 4 + kShTileSteps) > 0xFFFFFFFFull ||
+      (joined + 1) * kvh > 0x7FFFFull)
     VK_FAIL(VAPI_KV_EUNSUP, "%s: too many queries for one launch", who);
   return 0;
 }

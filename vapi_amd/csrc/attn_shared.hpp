@@ -39,7 +39,8 @@ constexpr uint32_t kShMinSteps = 8;       // of a range, in launches of few step
 // What a tile costs beside its steps (its rows, its first loads, its results: 5-6 us, a
 // step 1-1.4): counted as work, so that ranges of many short tiles are not the longest.
 constexpr uint32_t kShTileSteps = 5;
-constexpr uint32_t kShMaxNodes = 1024;    // their plan is in LDS
+// Their plan (32 bytes each) is in LDS, beside 128 KiB of queries and ring at D = 256.
+constexpr uint32_t kShMaxNodes = 1000;
 constexpr uint32_t kShMaxRanges = 512;
 
 struct __attribute__((aligned(16))) ShTile {
