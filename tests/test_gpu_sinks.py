@@ -137,6 +137,18 @@ def test_a_full_batch_of_single_tokens(dtype, fmt, d):
     assert got.shape == again.shape
 
 
+@pytest.mark.parametrize("dtype,fmt,heads,kvh,d", [
+    (F16, "int8", 16, 16, 96), (BF16, "e4m3", 12, 6, 96), (BF16, "int8", 15, 15, 80),
+    (F16, "e4m3", 8, 8, 48), (BF16, "e4m3", 4, 4, 160), (F16, "int8", 34, 2, 96)])
+def test_rows_that_share_cache_lines(dtype, fmt, heads, kvh, d):
+    """Token-major 8-bit rows that are no whole lines: 1, 2, 3, 4 or 8 heads to a walk."""
+    r = np.random.default_rng(d + heads)
+    lens = r.integers(1, 700, 136).tolist() + [1, 2, 3, 900]
+    got = check([1] * 140, lens, heads, kvh, d, dtype, 250, 20, fmt=fmt, layout="NHD", det=True)
+    again = check([1] * 140, lens, heads, kvh, d, dtype, 250, 20, fmt=fmt, layout="NHD", det=True)
+    assert torch.equal(got, again)
+
+
 @pytest.mark.parametrize("left,sinks", [(0, 1), (20, 4), (63, 33), (64, 70), (300, 5), (31, 900)])
 @pytest.mark.parametrize("dtype,fmt,heads,kvh,d", [
     (BF16, "none", 8, 2, 128), (F16, "none", 4, 4, 64), (BF16, "none", 2, 1, 256),
