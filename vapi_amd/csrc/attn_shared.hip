@@ -23,7 +23,7 @@ __global__ __launch_bounds__(kShThreads, D == 256 ? 1 : 2) void paged_shared_str
 
 // Workgroups 0 .. merge_wgs - 1 join the stream's partials of rows without shared
 // keys, the others those of tiles.
-template <typename T, int D, int WPS, bool kPad>
+template <typename T, int D, int WPS, bool kPad, int NV>
 __global__ __launch_bounds__(256) void paged_shared_merge(AttnArgs a, SharedArgs sh, uint32_t nwg,
                                                           uint32_t merge_wgs, uint32_t ns) {
   if (blockIdx.x < merge_wgs) {
@@ -31,15 +31,15 @@ __global__ __launch_bounds__(256) void paged_shared_merge(AttnArgs a, SharedArgs
     return;
   }
   // A workgroup to each row block of a group's tile, one to an open tile.
-  constexpr uint32_t kBlocks = sh_rows(D) / (256 / (D / 4));
+  constexpr uint32_t kBlocks = sh_rows(D) / sh_merge_rows(D, NV);
   const uint32_t i = blockIdx.x - merge_wgs, most = sh.max_grouped * sh_heads(a);
   if (i < most * kBlocks) {
-    sh_merge<T, D>(a, sh, nwg, i / kBlocks, i % kBlocks);
+    sh_merge<T, D, NV>(a, sh, nwg, i / kBlocks, i % kBlocks);
     return;
   }
   const uint32_t r = i - most * kBlocks;
   if (sh.open[r].valid)
-    for (uint32_t b = 0; b < kBlocks; ++b) sh_merge<T, D>(a, sh, nwg, most + r, b);
+    for (uint32_t b = 0; b < kBlocks; ++b) sh_merge<T, D, NV>(a, sh, nwg, most + r, b);
 }
 
 // Dynamic LDS with which two workgroups still share a CU (at head_dim 128, where the
@@ -197,14 +197,25 @@ void launch_shared_merge(const AttnArgs& a, const SharedArgs& sh, uint32_t head_
   bool wide = false;
   const uint32_t all = decode_merge_wgs(a.batch, a.kvh, &wide, ns);
   const uint32_t merge_wgs = decode ? all : 0u, nwg = a.num_waves / kDecodeWavesPerWG;
-  const uint32_t blocks = sh_rows(head_dim) / (256 / (head_dim / 4));
+  // Four outputs a thread and eight partials a round trip, or where those workgroups do
+  // not all run at once (four to a CU) eight and four: half the chains of lists, tiles
+  // and partials. Us, with four / eight outputs: 1,050 queries of 28 sequences (32 heads,
+  // 9 tiles a head) 21.7 / 14.5; 64 single queries 8.5 / 9.8, three groups 9.0 / 10.7.
+  const uint32_t tiles = sh.max_grouped * (a.kvh / a.kv_parts.d);
+  const int nv = tiles * (sh_rows(head_dim) / sh_merge_rows(head_dim, 1)) > 1024 ? 2 : 1;
+  const uint32_t blocks = sh_rows(head_dim) / sh_merge_rows(head_dim, nv);
   // (Without sequences of their own tiles, no range has an open one.)
-  const dim3 grid(merge_wgs + sh.max_grouped * (a.kvh / a.kv_parts.d) * blocks +
+  const dim3 grid(merge_wgs + tiles * blocks +
                   (sh.n_nodes > sh.n_groups ? sh.ranges : 0u));
-#define VK_SHM2(T, DD, WPS)                                                                    \
-  hipLaunchKernelGGL((a.hd != DD ? paged_shared_merge<T, DD, WPS, true>                        \
-                                 : paged_shared_merge<T, DD, WPS, false>),                     \
+#define VK_SHM3(T, DD, WPS, NV)                                                   \
+  hipLaunchKernelGGL((a.hd != DD ? paged_shared_merge<T, DD, WPS, true, NV>        \
+                                 : paged_shared_merge<T, DD, WPS, false, NV>),     \
                      grid, dim3(256), 0, s, a, sh, nwg, merge_wgs, ns)
+#define VK_SHM2(T, DD, WPS)          \
+  do {                               \
+    if (nv > 1) VK_SHM3(T, DD, WPS, 2); \
+    else VK_SHM3(T, DD, WPS, 1);     \
+  } while (0)
 #define VK_SHM(T, DD)                          \
   do {                                         \
     if (wide) VK_SHM2(T, DD, (int)kMergeWaves); \
@@ -213,6 +224,7 @@ void launch_shared_merge(const AttnArgs& a, const SharedArgs& sh, uint32_t head_
   VK_SH_ALL(VK_SHM);
 #undef VK_SHM
 #undef VK_SHM2
+#undef VK_SHM3
 }
 
 }  // namespace vk

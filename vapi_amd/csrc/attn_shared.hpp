@@ -736,13 +736,16 @@ __device__ __forceinline__ void sh_range(const AttnArgs& a, const SharedArgs& sh
   if (!open && threadIdx.x == 0) sh.open[r].valid = 0;
 }
 
+// Rows of a workgroup of the merge: threads of four outputs (NV == 1) or eight.
+constexpr uint32_t sh_merge_rows(uint32_t d, int nv) { return 256 / (d / (4 * nv)); }
+
 // Joins the partials of the rows of row block `block` of item `i` (the groups' tiles of
 // all kv heads, at most kvh * max_grouped of them, then the ranges' open tiles): thread
-// (row, four outputs). nwg: the decode's workgroups.
-template <typename T, int D>
+// (row, 4 NV outputs). nwg: the decode's workgroups.
+template <typename T, int D, int NV>
 __device__ __forceinline__ void sh_merge(const AttnArgs& a, const SharedArgs& sh, uint32_t nwg,
                                          uint32_t i, uint32_t block) {
-  constexpr uint32_t kRows = sh_rows(D), kTpr = D / 4, kRpw = 256 / kTpr;
+  constexpr uint32_t kRows = sh_rows(D), kTpr = D / (4 * NV), kRpw = sh_merge_rows(D, NV);
   const uint32_t kvh = sh_heads(a), most = sh.max_grouped * kvh, G = a.g_real;
   const bool group = i < most;
   const uint32_t n_grouped = *sh.n_grouped;
@@ -756,10 +759,12 @@ __device__ __forceinline__ void sh_merge(const AttnArgs& a, const SharedArgs& sh
   if (group) w = sh.queries[d.first + tok];
   const uint64_t stride = pf_part_bytes(kRows, D);
   auto slot_of = [](const ShTile& t, uint32_t j) { return j ? 2 * (t.r0 + j) + t.before : t.slot0; };
-  constexpr uint32_t kB = 8;  // partials per round trip
-  float M = kNegBig, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  constexpr uint32_t kB = 8 / NV;  // partials per round trip
+  // The second four outputs are D / 2 on (past a.hd: the first again, not stored).
+  const uint32_t d2 = NV > 1 && dq + D / 2 < a.hd ? D / 2 : 0;
+  float M = kNegBig, L = 0.f, o[4 * NV] = {};
   float2 ml[kB];
-  float4 x[kB];
+  float4 x[kB][NV];
   // Partials [j0, j0 + kB) of the n at (m, l) pm(j) and o px(j).
   auto fetch = [&](uint32_t j0, uint32_t n, auto at) __attribute__((always_inline)) {
 #pragma unroll
@@ -769,7 +774,8 @@ __device__ __forceinline__ void sh_merge(const AttnArgs& a, const SharedArgs& sh
       const float *pm, *px;
       at(j0 + u, pm, px);
       ml[u] = *(const float2*)pm;
-      x[u] = *(const float4*)px;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) x[u][v] = *(const float4*)(px + v * d2);
     }
   };
   // Joins what was fetched. kNormed: it is o / l (tiles'), else o (the stream's).
@@ -781,13 +787,17 @@ __device__ __forceinline__ void sh_merge(const AttnArgs& a, const SharedArgs& sh
     const float f = fast_exp2(M - Mn);
     L *= f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] *= f;
+    for (int i = 0; i < 4 * NV; ++i) o[i] *= f;
 #pragma unroll
     for (uint32_t u = 0; u < kB; ++u) {
       if (!(ml[u].y > 0.f)) continue;  // a share with no visible key (its o is stale)
       const float e = fast_exp2(ml[u].x - Mn), wgt = normed ? ml[u].y * e : e;
       L += ml[u].y * e;
-      o[0] += x[u].x * wgt, o[1] += x[u].y * wgt, o[2] += x[u].z * wgt, o[3] += x[u].w * wgt;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        o[4 * v] += x[u][v].x * wgt, o[4 * v + 1] += x[u][v].y * wgt;
+        o[4 * v + 2] += x[u][v].z * wgt, o[4 * v + 3] += x[u][v].w * wgt;
+      }
     }
     M = Mn;
   };
@@ -846,7 +856,11 @@ __device__ __forceinline__ void sh_merge(const AttnArgs& a, const SharedArgs& sh
   }
   const float inv = L > 0.f ? 1.f / L : 0.f;
   T* dst = (T*)a.out + ((uint64_t)w.q * a.num_heads + kh * G + head) * a.hd + dq;
-  *(uint2*)dst = make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+    if (v == 0 || d2)
+      *(uint2*)(dst + v * d2) = make_uint2(pack2<T>(o[4 * v] * inv, o[4 * v + 1] * inv),
+                                           pack2<T>(o[4 * v + 2] * inv, o[4 * v + 3] * inv));
 }
 
 // ---- launch (attn_shared.hip) ----------------------------------------------------
