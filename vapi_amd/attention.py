@@ -296,7 +296,7 @@ def paged_attention_prepared(q: torch.Tensor, cache: PagedKvCache, layer: int,
         raise ValueError(f"q must be (tokens, heads, {cache.head_dim}), got {tuple(q.shape)}")
     if q.dtype != cache.dtype:
         raise ValueError(f"q is {q.dtype} but the cache is {cache.dtype}")
-    sinks = sinks_arg(sinks)
+    sinks = sinks_arg(sinks) if sinks else 0
     q = contiguous_on(stream, q)
     if out is None:
         out = empty_on(stream, q)
@@ -304,13 +304,15 @@ def paged_attention_prepared(q: torch.Tensor, cache: PagedKvCache, layer: int,
     num_heads = q.shape[1]
     max_q = max(int(prepared.max_seqlen_q), 1)
     max_k = max(int(prepared.max_seqlen_k), 1)
-    mask = (float(softmax_scale), -1 if window_size_left is None else int(window_size_left),
-            -1 if window_size_right is None else int(window_size_right))
-    shared = prepared.shared_bytes(cache, num_heads, window_size_left) if b else 0
-    mask += (sinks, prepared.flags) if sinks or shared else (prepared.flags,)
+    shared = 0
+    if prepared.prefixes is not None and b:
+        shared = prepared.shared_bytes(cache, num_heads, window_size_left)
+    flags = (sinks, prepared.flags) if sinks or shared else (prepared.flags,)
     args = (cache.pool, layer, q.data_ptr(), out.data_ptr(), prepared.seqlens_q.data_ptr(),
             prepared.seqlens_k.data_ptr(), prepared.block_table.data_ptr(), b,
-            prepared.block_table.shape[1], max_q, max_k, num_heads) + mask
+            prepared.block_table.shape[1], max_q, max_k, num_heads, float(softmax_scale),
+            -1 if window_size_left is None else int(window_size_left),
+            -1 if window_size_right is None else int(window_size_right), *flags)
     handle = stream_handle(stream)
     if _is_quantised(cache) or sinks or shared:
         listed = prepared.prefill_seqs is not None
@@ -410,7 +412,7 @@ def paged_attention_append_prepared(q: torch.Tensor, k: torch.Tensor, v: torch.T
                          f"got {tuple(k.shape)} and {tuple(v.shape)}")
     if slot_mapping.numel() != k.shape[0] or slot_mapping.element_size() != 4:
         raise ValueError("slot_mapping must hold one 32-bit slot per row")
-    sinks = sinks_arg(sinks)
+    sinks = sinks_arg(sinks) if sinks else 0
     q, k, v = (contiguous_on(stream, t) for t in (q, k, v))
     if out is None:
         out = empty_on(stream, q)
@@ -432,7 +434,8 @@ def paged_attention_append_prepared(q: torch.Tensor, k: torch.Tensor, v: torch.T
         return paged_attention_prepared(q, cache, layer, prepared, softmax_scale,
                                         window_size_left, window_size_right, out=out,
                                         stream=stream, sinks=sinks)
-    if b and prepared.shared_bytes(cache, num_heads, window_size_left):
+    if prepared.prefixes is not None and b and \
+            prepared.shared_bytes(cache, num_heads, window_size_left):
         # Two calls here too; the shared prefixes' is refused before rows are written.
         _check_second(cache, q, out, prepared)
         prepared.grow(prepared.shared_bytes(cache, num_heads, window_size_left), q.device, stream)

@@ -531,7 +531,7 @@ static int paged_attention_impl(const vapi_kv_pool* pool, uint32_t layer, const 
     VK_FAIL(VAPI_KV_EUNSUP, "vapi_paged_attention: prefill batch too large for one launch");
   size_t need =
       required_workspace(pool, batch, num_heads, max_seqlen_q, max_seqlen_k, skip_decode);
-  const size_t shared_off = shared_offset(pool, batch, num_heads);
+  size_t shared_off = 0;
   const uint32_t shared_pf = max_seqlen_q > 1 ? pf_n : 0;
   if (prefixes) {
     if (!mfma16_ok(pool, num_heads))
@@ -541,6 +541,7 @@ static int paged_attention_impl(const vapi_kv_pool* pool, uint32_t layer, const 
     if (int rc = shared_check(prefixes, batch, pool->num_kv_heads, G, D, shared_pf, max_seqlen_q,
                               max_seqlen_k, "vapi_paged_attention_shared"))
       return rc;
+    shared_off = shared_offset(pool, batch, num_heads);
     need = shared_off + shared_workspace_bytes(prefixes, batch, pool->num_kv_heads, G, D, shared_pf,
                                                max_seqlen_q);
   }
