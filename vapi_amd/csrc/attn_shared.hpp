@@ -15,13 +15,20 @@
 //
 // Tiles are cut into ranges of equal work, one workgroup each: the work of a launch
 // is the run of 32-key steps over (kv head, node, row tile), kShTileSteps more to a
-// tile, and range r takes its r-th part. Tiles whose rows are joined with others' results (groups', and those of
-// sequences with shared keys) write partials even where a range holds all of them;
-// the others write the output there. With `before` the number of such joined tiles
-// before a tile in step order, a piece's partial is slot 2 r + before, + 1 if it is
-// not the first of its range: slots grow from one written piece to the next, so they
-// are distinct. The piece that starts a tile describes it for the merge: the joined
-// tile number `before`, or range r's open tile (a range leaves at most one open).
+// tile, and range r takes its r-th part. Tiles whose rows are joined with others'
+// results (groups', and those of sequences with shared keys) write partials even where
+// a range holds all of them; the others write the output there. With `before` the
+// number of such joined tiles before a tile in step order, a piece's partial is slot
+// 2 r + before, + 1 if it is not the first of its range: slots grow from one written
+// piece to the next, so they are distinct and nothing is atomic. The piece that starts
+// a tile describes it for the merge: the joined tile number `before`, or range r's open
+// tile (a range leaves at most one open).
+//
+// Measured, us a call (without sharing), 32 q / 8 kv heads of 128 in bf16: 64 sequences
+// over 4,096 shared keys 42.6 (172), 4-8 queries each of 16 over 3,200 45.6 (72); 64 q
+// heads, 128 sequences over 32,768 224-230 (2,485), 620 TFLOP/s. Long prefixes are bound
+// by the tiles' step (25% MFMA, 29% VALU, waits at 2 waves a SIMD), short ones by round
+// trips, 4-10 us each while the stream keeps HBM's queues full, and by the merge, 6-15.
 #pragma once
 
 #include "attn_decode.hpp"
