@@ -139,9 +139,11 @@ def test_a_full_batch_of_single_tokens(dtype, fmt, d):
 
 @pytest.mark.parametrize("dtype,fmt,heads,kvh,d", [
     (F16, "int8", 16, 16, 96), (BF16, "e4m3", 12, 6, 96), (BF16, "int8", 15, 15, 80),
-    (F16, "e4m3", 8, 8, 48), (BF16, "e4m3", 4, 4, 160), (F16, "int8", 34, 2, 96)])
+    (F16, "e4m3", 8, 8, 48), (BF16, "e4m3", 4, 4, 160), (F16, "int8", 34, 2, 96),
+    (BF16, "none", 8, 8, 80), (F16, "none", 12, 6, 96), (F32, "none", 9, 3, 80),
+    (F32, "none", 8, 8, 16), (BF16, "none", 4, 4, 200), (F16, "none", 40, 2, 72)])
 def test_rows_that_share_cache_lines(dtype, fmt, heads, kvh, d):
-    """Token-major 8-bit rows that are no whole lines: 1, 2, 3, 4 or 8 heads to a walk."""
+    """Token-major rows that are no whole lines: 1, 2, 3, 4 or 8 heads to a walk."""
     r = np.random.default_rng(d + heads)
     lens = r.integers(1, 700, 136).tolist() + [1, 2, 3, 900]
     got = check([1] * 140, lens, heads, kvh, d, dtype, 250, 20, fmt=fmt, layout="NHD", det=True)

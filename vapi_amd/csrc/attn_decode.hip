@@ -20,12 +20,12 @@ __global__ __launch_bounds__(64 * kDecodeWavesPerWG, kDecodeWGsPerCU) void paged
 // and 74.0 us); every other call with streaming loads.
 template <typename T, int D, bool F, bool PAD, int DL>
 static void launch_stream(const AttnArgs& c, uint32_t nwg, size_t lds, hipStream_t s) {
-  // Sinks (no fused append): all d tiles live.
+  // Sinks (no fused append): all d tiles live; heads side by side share lines as parts do.
   if constexpr (!F) {
     if (c.sinks) {
       constexpr auto once = paged_decode_stream<T, D, false, PAD, D / 16, true, true>;
       constexpr auto shared = paged_decode_stream<T, D, false, PAD, D / 16, false, true>;
-      hipLaunchKernelGGL(c.kv_parts.d > 1 ? shared : once, dim3(nwg),
+      hipLaunchKernelGGL(c.plan_parts > 1 ? shared : once, dim3(nwg),
                          dim3(64 * kDecodeWavesPerWG), lds, s, c, c.cu_q, c.cu_k, c.table);
       return;
     }
@@ -167,6 +167,7 @@ void launch_decode(AttnArgs a, void* workspace, uint32_t head_dim, uint32_t dtyp
     c.cu_q = a.cu_q + b0;
     c.cu_k = a.cu_k + b0;
     c.table = a.table + (uint64_t)b0 * a.max_blocks;
+    if (c.sinks) c.plan_parts = line_heads(c, c.hd * (dtype == VAPI_KV_F32 ? 4 : 2));
     decode_bind(c, workspace, head_dim);
     // Fused append: the first chunk's merge launch also writes the new rows
     // (every chunk's stream reads a row's new key from the new rows).

@@ -40,6 +40,7 @@
 // exactly once.
 #pragma once
 #include <cstdlib>
+#include <numeric>
 #include <type_traits>
 
 #include "attn_common.hpp"
@@ -376,7 +377,8 @@ __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
   // A group split into n virtual kv heads: steps are counted per pool
   // head, each of n neighbouring waves walking one part (n = 1: the
   // virtual heads are the pool's).
-  const uint32_t n_parts = a.kv_parts.d;
+  // (With sinks, whole heads too: line_heads.)
+  const uint32_t n_parts = kSinks && !kShared ? a.plan_parts : a.kv_parts.d;
   const uint32_t kvh_plan = a.kvh / n_parts;
   // The shared 100 MHz clock at entry: XCDs start the grid up to ~2.5 us
   // apart, and the shares account for it.
@@ -881,6 +883,18 @@ __device__ __forceinline__ void decode_merge_body(const AttnArgs& a, uint32_t nw
       store(e_lane + j0, n, O, L);
     }
   }
+}
+
+// Heads that one walk over the keys takes side by side (plan_parts), of rows of `row`
+// bytes: as many as fill whole lines where a token's heads are neighbours and a row is
+// no whole line. 2,000 + 20 keys a row, one head at a time / these: 24 rows, 32 kv heads
+// of 80 in bf16 81 / 65 us, of 96 in f16 77 / 70; 64 rows, 8 of 80 96 / 78, 4 of 80 in f32
+// 87 / 85; whole lines (128 in bf16) 90 either way. (Calls with sinks; the others keep
+// their ranges of keys, and with them how their sums round.)
+inline uint32_t line_heads(const AttnArgs& a, uint32_t row) {
+  return a.kv_parts.d > 1 ? a.kv_parts.d
+         : a.tok_e == a.hd ? 1
+                           : std::gcd(a.kvh, kLine / std::gcd(row, kLine));
 }
 
 // Workgroups of a decode's merge launch for `batch` sequences (without a

@@ -21,7 +21,6 @@
 // chunk of 512 queries uses each expanded value 2,048 times (4 query heads a kv
 // head); the expansion moves 5 bytes a code (1 in, 2 out, 2 back in).
 #include <algorithm>
-#include <numeric>
 
 #include "attn_q8.hpp"
 #include "attn_shared.hpp"
@@ -236,15 +235,6 @@ static int q8_check_sizes(const vapi_kv_q8_pool* p, uint32_t num_heads, uint32_t
                pf_n * mb > 0xFFFFFFull))
     VK_FAIL(VAPI_KV_EUNSUP, "%s: prefill batch too large for one launch", who);
   return 0;
-}
-
-// Heads that one walk over the keys takes side by side: as many as fill whole lines
-// where a token's heads are neighbours and a row is no whole line. 24 rows behind a
-// window of 1,000 keys, 32 kv heads of 96: 315 MB read and 60.9 us a head at a time,
-// 161 MB (150 are needed) and 51-53 four at a time. (Calls with sinks; the others keep
-// their ranges of keys, and with them how their sums round.)
-static uint32_t q8_line_heads(const AttnArgs& a) {
-  return q8_read_once(a) ? 1 : std::gcd(a.kvh, 128 / std::gcd(a.hd, 128u));
 }
 
 template <typename T, int F, int D>
@@ -553,7 +543,9 @@ static int q8_attention(const vapi_kv_q8_pool* pool, uint32_t layer, const void*
     dec.kv_parts = FastDiv(parts);
     dec.plan_parts = parts;
   } else if (a.sinks) {
-    dec.plan_parts = q8_line_heads(a);
+    // 24 rows behind a window of 1,000 keys, 32 kv heads of 96: 315 MB read and 60.9 us
+    // a head at a time, 161 MB (150 are needed) and 51-53 four at a time.
+    dec.plan_parts = line_heads(a, a.hd);
   }
   if (prefixes) {
     dec.shared = prefixes->start;
