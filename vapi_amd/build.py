@@ -39,7 +39,8 @@ COMMON_FLAGS = [
 
 SOURCES = ["kv_ops.hip", "attention.hip", "attn_decode.hip", "attn_decode_small.hip",
            "attn_prefill.hip", "attn_prefill_f32.hip", "attn_generic.hip", "q8_ops.hip",
-           "attn_q8.hip", "attn_q8_shared.hip", "attn_shared.hip", "kv_weights.hip", "kv_evict.hip", "host.cpp", "spill.cpp"]
+           "attn_q8.hip", "attn_q8_shared.hip", "attn_shared.hip", "kv_weights.hip",
+           "kv_evict.hip", "host.cpp", "spill.cpp"]
 
 # Matrix products into the registers that the vector unit reads; through the
 # accumulation ones each score is copied once (the 8-bit decode 76.6 -> 75.2 us

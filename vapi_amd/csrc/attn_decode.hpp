@@ -390,7 +390,8 @@ __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
     const uint32_t per = (B + NT - 1) / NT;
     const uint32_t b0 = min(tid * per, B), b1 = min(b0 + per, B);
     uint32_t sum = 0;
-    for (uint32_t s = b0; s < b1; ++s) sum += decode_steps<32, kSinks, kShared>(a, cu_q, cu_k, s) * kvh_plan;
+    for (uint32_t s = b0; s < b1; ++s)
+      sum += decode_steps<32, kSinks, kShared>(a, cu_q, cu_k, s) * kvh_plan;
     uint32_t inc = sum;  // inclusive scan within the wave
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {

@@ -129,7 +129,8 @@ __device__ __forceinline__ void lgkm_wait(uint2 (&r)[6]) {
 }
 
 // RT row tiles of one wave in f32 MFMAs, straight from the pool over the steps at
-// positions s0 .. s_last of ks (none if s_last < s0): rows row0 .. of a sequence (its len_q * G rows are nrows). `pb`:
+// positions s0 .. s_last of ks (none if s_last < s0): rows row0 .. of a sequence (its
+// len_q * G rows are nrows). `pb`:
 // the wave's item's partials of a key split ((m, l), then o / l per row,
 // prow0 the wave's first row in the item's part_rows), or null for the output.
 template <int D, int RT, bool kPad, int CL, bool kAhead, bool kSinks>
@@ -195,7 +196,9 @@ __device__ __forceinline__ void f32_rows(const AttnArgs& a, const uint32_t* __re
           const int32_t key = h0 + 4 * (int32_t)g, top = sink_end(t);
           const uint32_t base = (uint32_t)(key - lo[t]), n = cnt[t];
           attend_half_f32<D, CL>(kt, vt, qf[t], o[t], m_run[t], l_run[t], a.scale_log2,
-                                 [&](int i) { return base + (uint32_t)i < n || (kSinks && key + i < top); });
+                                 [&](int i) {
+                                   return base + (uint32_t)i < n || (kSinks && key + i < top);
+                                 });
         }
       }
     } else {
@@ -218,7 +221,9 @@ __device__ __forceinline__ void f32_rows(const AttnArgs& a, const uint32_t* __re
             const int32_t top = sink_end(t);
             const uint32_t base = (uint32_t)(key - lo[t]), n = cnt[t];
             attend_half_f32<D, CL>(kt.h[tt], vt.h[tt], qf[t], o[t], m_run[t], l_run[t], a.scale_log2,
-                               [&](int i) { return base + (uint32_t)i < n || (kSinks && key + i < top); });
+                               [&](int i) {
+                                 return base + (uint32_t)i < n || (kSinks && key + i < top);
+                               });
           }
           load_half_f32<D, false, kPad, CL>(kt.h[tt], vt.h[tt], tab, kb, vb, a, key_next, tt,
                                             reads(s_next), col, g);
@@ -527,9 +532,9 @@ __device__ __forceinline__ void x3_piece(const AttnArgs& a, const uint32_t* __re
   if (__builtin_amdgcn_readfirstlane(outside_lds)) {
 #pragma unroll 1
     for (uint32_t t = 0; t < (uint32_t)RT; ++t)
-      f32_rows<D, 1, kPad, D / 16, false, kSinks>(a, tab, kh, q0, nrows, row0 + 16 * t, offset, len_k, ks,
-                                          s_first, s_last, klo, khi, kSplit ? pb : nullptr,
-                                          wrow0 + 16 * t, kPf32Rows);
+      f32_rows<D, 1, kPad, D / 16, false, kSinks>(a, tab, kh, q0, nrows, row0 + 16 * t, offset,
+                                                  len_k, ks, s_first, s_last, klo, khi,
+                                                  kSplit ? pb : nullptr, wrow0 + 16 * t, kPf32Rows);
     return;
   }
 #pragma unroll
@@ -643,8 +648,9 @@ __global__ __launch_bounds__(64 * kPfF32Waves, 1) void paged_prefill_f32(
   char* const pb = kSplit ? (char*)part + ((uint64_t)(rest * qtiles + qt) * n_split + split) *
                                               pf_part_bytes(16 * RT, D)
                           : nullptr;
-  f32_rows<D, RT, kPad, CL, true, kSinks>(a, a.table + (uint64_t)seq * a.max_blocks, kh, q0, nrows, row0, offset,
-                            len_k, ks, s0, s_last, klo, khi, pb, 0, 16 * RT);
+  f32_rows<D, RT, kPad, CL, true, kSinks>(a, a.table + (uint64_t)seq * a.max_blocks, kh, q0, nrows,
+                                          row0, offset, len_k, ks, s0, s_last, klo, khi, pb, 0,
+                                          16 * RT);
 }
 
 

@@ -187,7 +187,8 @@ __device__ __forceinline__ void q8_stream_body(const AttnArgs& a, const Q8Scales
     const uint32_t per = (B + NT - 1) / NT;
     const uint32_t b0 = min(tid * per, B), b1 = min(b0 + per, B);
     uint32_t sum = 0;
-    for (uint32_t s = b0; s < b1; ++s) sum += decode_steps<KS, kSinks, kShared>(a, cu_q, cu_k, s) * kvh_plan;
+    for (uint32_t s = b0; s < b1; ++s)
+      sum += decode_steps<KS, kSinks, kShared>(a, cu_q, cu_k, s) * kvh_plan;
     uint32_t inc = sum;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -228,7 +229,8 @@ __device__ __forceinline__ void q8_stream_body(const AttnArgs& a, const Q8Scales
   const uint32_t t_end = bounds[x] + (uint32_t)(((uint64_t)(jr + 1) * len) / nr);
 
   uint32_t t = t_begin;
-  DecodePos pos = locate<KS, kSinks, kShared>(a, cu_q, cu_k, P, nullptr, t, kvh_plan, n_parts, part);
+  DecodePos pos =
+      locate<KS, kSinks, kShared>(a, cu_q, cu_k, P, nullptr, t, kvh_plan, n_parts, part);
   uint4* qs = q_lds[wave];
   q8_load_q<T, D, kPad>(qs, a, pos, lane, col, g);
   bool piece_first = pos.seg_first;

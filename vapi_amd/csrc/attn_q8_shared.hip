@@ -28,8 +28,9 @@ static void launch_q8_shared_stream(const AttnArgs& a, const SharedArgs& sh, uin
                                     uint32_t nwg, uint32_t ranges, hipStream_t s) {
   const size_t lds = shared_lds(a, sh, nwg, ranges);
   const bool once = q8_read_once(a);
-#define VK_Q8H(DD)                                                                       \
-  hipLaunchKernelGGL((once ? q8_shared_stream<T, F, DD, true> : q8_shared_stream<T, F, DD, false>), \
+#define VK_Q8H(DD)                                                          \
+  hipLaunchKernelGGL((once ? q8_shared_stream<T, F, DD, true>               \
+                           : q8_shared_stream<T, F, DD, false>),            \
                      dim3(nwg + ranges), dim3(kShThreads), lds, s, a, sh, nwg)
   if (D == 256) VK_Q8H(256);
   else if (D == 128) VK_Q8H(128);

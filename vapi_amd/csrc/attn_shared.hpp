@@ -643,8 +643,8 @@ __device__ __forceinline__ void sh_piece(const AttnArgs& a, const SharedArgs& sh
                                                       o[t][k][2] * inv, o[t][k][3] * inv);
       continue;
     }
-    T* orow = (T*)a.out + ((uint64_t)(n.first + j) * a.num_heads + kh * a.g_real + (r - j * a.g_real)) *
-                              (kPad ? a.hd : D);
+    const uint64_t head = (uint64_t)(n.first + j) * a.num_heads + kh * a.g_real + (r - j * a.g_real);
+    T* orow = (T*)a.out + head * (kPad ? a.hd : D);
 #pragma unroll
     for (int k = 0; k < DT; ++k)
       if (!kPad || 16 * k + 4 * g < a.hd)
@@ -714,7 +714,8 @@ __device__ __forceinline__ void sh_range(const AttnArgs& a, const SharedArgs& sh
       const uint32_t t = j0 + tile;  // of the kv head's joined tiles
       uint4* d = (uint4*)(!joins  ? sh.open + r
                           : group ? sh.joined + kh * sh.max_grouped + t
-                                  : sh.joined + kvh * sh.max_grouped + kh * max_own + (t - n_grouped));
+                                  : sh.joined + kvh * sh.max_grouped + kh * max_own +
+                                        (t - n_grouped));
       d[0] = make_uint4(1u, r, last, tile);
       d[1] = make_uint4(kh, slot, before, group ? ~0u : nodes[node].seq);
       d[2] = make_uint4(nodes[node].first, nodes[node].tokens, 0u, 0u);
