@@ -37,6 +37,26 @@ void plan_list_parts(uint32_t n_seqs, uint32_t kvh, uint32_t qtiles, uint32_t* o
     pf_list_part(i, n_seqs, kvh, qtiles, out[3 * i], out[3 * i + 1], out[3 * i + 2]);
 }
 
+// The 32-key steps of rows that see [klo, khi] and the first `sinks` of [0, khi]: the
+// keys they stand for and the keys that are read for those, 32 of each a step. Returns
+// the number of steps.
+uint32_t plan_key_steps(int32_t klo, int32_t khi, int32_t sinks, uint32_t most, int32_t* keys,
+                        int32_t* read) {
+  klo = window_first(klo, khi, 32);
+  const KeySteps<true> ks(klo, khi, sinks, 32);
+  const uint32_t all = (uint32_t)(ks.last / 32 + 1);
+  for (uint32_t i = 0; i < all && i < most; ++i) {
+    const KeyReads rd(ks, 32 * (int32_t)i, klo, khi, sinks);
+    const int32_t s0 = ks.key(32 * (int32_t)i);
+    for (int32_t r = 0; r < 32; ++r) {
+      const int32_t ts = rd.tile(s0 + (r & 16));
+      keys[32 * i + r] = s0 + r;
+      read[32 * i + r] = rd.whole(s0) ? s0 + r : ts + (int32_t)rd.row(r & 15, ts);
+    }
+  }
+  return all;
+}
+
 }  // extern "C"
 
 namespace {

@@ -72,3 +72,13 @@ def item_order(n_seqs, qtiles, kvh):
     _lib().plan_list_parts(ctypes.c_uint32(n_seqs), ctypes.c_uint32(kvh), ctypes.c_uint32(qtiles),
                            out)
     return [tuple(out[3 * i:3 * i + 3]) for i in range(n_seqs * qtiles * kvh)]
+
+
+def key_steps(klo, khi, sinks, most=4096):
+    """The keys that the steps of rows seeing [klo, khi] and the first `sinks` of
+    [0, khi] stand for, and those read for them."""
+    keys, read = ((ctypes.c_int32 * (32 * most))() for _ in range(2))
+    i32 = ctypes.c_int32
+    n = _lib().plan_key_steps(i32(klo), i32(khi), i32(sinks), ctypes.c_uint32(most), keys, read)
+    assert n <= most
+    return list(keys[:32 * n]), list(read[:32 * n])

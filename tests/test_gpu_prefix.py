@@ -397,3 +397,30 @@ def test_refusals():
     prep.flags = 0x80
     with pytest.raises(VapiKvError):
         paged_attention_prepared(q, cache, 0, prep, 0.1)
+
+
+# Groups whose members all lie further past the prefix than the left window of 41 keys
+# reaches, by one key or many, so that a tile of theirs sees its sinks only; prefixes of
+# whole steps of 32 keys and not; one group beside another that is in reach.
+PAST = [
+    [(8, [(1, 42), (1, 150), (1, 77)])],
+    [(9, [(1, 60), (4, 90), (1, 43), (2, 45), (30, 75)])],
+    [(8, [(1, 100), (3, 47)]), (5, [(1, 3), (1, 300), (2, 41)])],
+    [(3, [(1, 50 + 3 * i) for i in range(80)]), (12, [(5, 46 + i) for i in range(20)])],
+]
+
+
+@pytest.mark.parametrize("groups", PAST)
+@pytest.mark.parametrize("sinks", [1, 5, 32, 40])
+@pytest.mark.parametrize("heads,kvh,d,dtype,fmt", [
+    (8, 8, 64, BF16, "none"), (8, 2, 128, F16, "none"), (4, 1, 256, BF16, "none"),
+    (28, 1, 128, BF16, "none"), (71, 1, 64, F16, "none"), (6, 3, 96, BF16, "none"),
+    (2, 2, 128, BF16, "e4m3"), (28, 1, 64, F16, "int8"), (71, 1, 256, BF16, "int8"),
+    (4, 1, 256, F16, "e4m3")])
+def test_sinks_of_a_prefix_that_no_window_reaches(groups, sinks, heads, kvh, d, dtype, fmt):
+    check(groups, [(1, 200), (3, 30)], heads, kvh, d, dtype, 40, sinks, fmt=fmt)
+
+
+def test_sinks_alone_behind_a_right_window():
+    for right in (3, None):
+        check(PAST[1], [], 8, 2, 128, BF16, 40, 5, right=right)

@@ -6,8 +6,8 @@ import heapq
 import numpy as np
 import pytest
 
-from prefill_plan import (BY_CLASS, LIST_ORDER, LIST_PARTS, SEQUENCES, check_walk, item_order, route,
-                          tile_order)
+from prefill_plan import (BY_CLASS, LIST_ORDER, LIST_PARTS, SEQUENCES, check_walk, item_order,
+                          key_steps, route, tile_order)
 
 
 def equal(f32, n, heads, kvh, q, k, d=128):
@@ -223,3 +223,21 @@ def test_short_sequences_keep_list_order():
         # A sequence on two XCDs at most, where each holds a sequence or more.
         if n >= 8:
             assert max(sum(any(s == q for _, q in x) for x in xcds) for s in range(n)) <= 2
+
+
+def test_steps_hold_every_visible_key_once_and_read_no_hidden_one():
+    """Sinks and windows of every phase, windows past all the keys (klo > khi) and rows
+    without any (khi < 0) among them."""
+    rng = np.random.default_rng(3)
+    cases = [(4172, 4095, 4), (2200, 1999, 4), (2200, 1999, 0), (5, 4, 3), (32, 31, 32),
+             (0x7FFFFFFE, -2, 4), (0, -1, 9), (100, 99, 100)]
+    for _ in range(3000):
+        khi = int(rng.integers(-2, 300))
+        klo = int(rng.integers(0, 400))
+        cases.append((klo, khi, int(rng.integers(0, max(khi + 1, 0) + 1))))
+    for klo, khi, sinks in cases:
+        keys, read = key_steps(klo, khi, sinks)
+        seen = {k for k in range(khi + 1) if k >= klo or k < sinks}
+        assert seen <= set(keys) and len(keys) == len(set(keys)), (klo, khi, sinks)
+        assert sorted({k // 32 for k in keys}) == sorted({k // 32 for k in seen}), (klo, khi, sinks)
+        assert set(read) <= seen and all(r == k for k, r in zip(keys, read) if k in seen)

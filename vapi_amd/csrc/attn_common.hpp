@@ -702,35 +702,7 @@ __device__ __forceinline__ floatx4 mfma16x16x4f32(float a, float b, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// What a tile of rows reads of its steps: keys hidden from all of them re-read one
-// that is visible (their zero weights then meet values that count anyway). Sinks'
-// steps (positions before ks.hop) hold keys [0, sinks), the window's [klo, khi];
-// `hole` is klo where sinks end in the window's first step, else 0.
-struct KeyReads {
-  int32_t first, last, hole, sinks;
-  __device__ __forceinline__ KeyReads(const KeySteps<true>& ks, int32_t at, int32_t klo, int32_t khi,
-                                      int32_t sinks_)
-      : sinks(sinks_) {
-    const bool sink = at < ks.hop, mid = sinks > (klo & ~31);
-    first = sink || mid ? 0 : klo;
-    last = sink ? min(sinks - 1, khi) : khi;
-    hole = mid ? klo : 0;
-  }
-  // Whether all keys of the step at s0 are read as they are.
-  __device__ __forceinline__ bool whole(int32_t s0) const {
-    return s0 >= first && s0 + 31 <= last && (s0 >= hole || s0 + 31 < sinks);
-  }
-  // The 16-key tile read for the one at s, and the row of it for row r.
-  __device__ __forceinline__ int32_t tile(int32_t s) const {
-    return max(min(s, last & ~15), first & ~15);
-  }
-  __device__ __forceinline__ uint32_t row(int32_t r, int32_t ts) const {
-    int32_t k = max(min(r, last - ts), first - ts);
-    if (hole && ts + k >= sinks && ts + k < hole) k = (ts < sinks ? sinks - 1 : hole) - ts;
-    return (uint32_t)k;
-  }
-};
-// The same for one row's decode, which masks hidden keys' V itself.
+// What one row's decode, which masks hidden keys' V itself, reads (KeyReads).
 struct RowReads {
   int32_t last;
   __device__ __forceinline__ bool whole(int32_t s0) const { return s0 + 31 <= last; }

@@ -404,9 +404,10 @@ __device__ __forceinline__ void sh_piece(const AttnArgs& a, const SharedArgs& sh
   };
   uint2 blk{0, 0};  // of the step whose loads are issued next
   auto begin = [&](int32_t lo_, int32_t hi_) __attribute__((always_inline)) {
-    klo = lo_, khi = hi_;
+    // (Windows past all of the node's keys leave the sinks' steps, or none.)
+    klo = window_first(lo_, hi_, 32), khi = hi_;
     ks = KeySteps<true>(klo, khi, sinks, 32);
-    const uint32_t all = khi >= klo ? (uint32_t)ks.last / 32 + 1 : 0u;
+    const uint32_t all = (uint32_t)(ks.last / 32 + 1);
     s0_ = 32 * (int32_t)pf_step_at(u0, c, all);
     s_last = 32 * (int32_t)pf_step_at(u1, c, all) - 32;
     if (s0_ <= s_last) {  // (uniform)

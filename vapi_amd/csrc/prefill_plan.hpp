@@ -50,6 +50,39 @@ struct KeySteps {
   }
   VK_HD int32_t key(int32_t at) const { return kSinks && at >= hop ? at + gap : at; }
 };
+// Where the windows of rows over keys [0, khi] begin: at klo, or past all of those keys
+// (klo > khi) at the first step behind them, so that KeySteps walks the sinks' steps
+// and no others.
+VK_HD int32_t window_first(int32_t klo, int32_t khi, int32_t step) {
+  return klo <= khi ? klo : (khi + step) & ~(step - 1);
+}
+// What a tile of rows reads of its steps: keys hidden from all of them re-read one
+// that is visible (their zero weights then meet values that count anyway). Sinks'
+// steps (positions before ks.hop) hold keys [0, sinks), the window's [klo, khi];
+// `hole` is klo where sinks end in the window's first step, else 0.
+struct KeyReads {
+  int32_t first, last, hole, sinks;
+  VK_HD KeyReads(const KeySteps<true>& ks, int32_t at, int32_t klo, int32_t khi, int32_t sinks_)
+      : sinks(sinks_) {
+    const bool sink = at < ks.hop, mid = sinks > (klo & ~31);
+    first = sink || mid ? 0 : klo;
+    last = sink ? pf_min(sinks - 1, khi) : khi;
+    hole = mid ? klo : 0;
+  }
+  // Whether all keys of the step at s0 are read as they are.
+  VK_HD bool whole(int32_t s0) const {
+    return s0 >= first && s0 + 31 <= last && (s0 >= hole || s0 + 31 < sinks);
+  }
+  // The 16-key tile read for the one at s, and the row of it for row r.
+  VK_HD int32_t tile(int32_t s) const {
+    return pf_max(pf_min(s, last & ~15), first & ~15);
+  }
+  VK_HD uint32_t row(int32_t r, int32_t ts) const {
+    int32_t k = pf_max(pf_min(r, last - ts), first - ts);
+    if (hole && ts + k >= sinks && ts + k < hole) k = (ts < sinks ? sinks - 1 : hole) - ts;
+    return (uint32_t)k;
+  }
+};
 
 // How a launch's items are ordered (prefill_item says why).
 constexpr uint32_t kLine = 128;  // bytes of an L2 line
