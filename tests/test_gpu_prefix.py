@@ -424,3 +424,13 @@ def test_sinks_of_a_prefix_that_no_window_reaches(groups, sinks, heads, kvh, d, 
 def test_sinks_alone_behind_a_right_window():
     for right in (3, None):
         check(PAST[1], [], 8, 2, 128, BF16, 40, 5, right=right)
+
+
+@pytest.mark.parametrize("fmt,dtype", [("e4m3", BF16), ("int8", BF16), ("int8", F16), ("none", F16)])
+@pytest.mark.parametrize("heads,kvh,d", [(4, 1, 64), (2, 2, 64), (8, 8, 64), (32, 32, 96),
+                                         (24, 12, 96), (8, 8, 80), (12, 3, 80), (34, 2, 80)])
+def test_sinks_over_rows_that_share_cache_lines(heads, kvh, d, fmt, dtype):
+    """Token-major pools, members (and others) whose own keys span several of the
+    stream's ranges."""
+    check([(70, decode(24, 1, 1500, d)), (4, [(1, 900), (3, 700), (1, 1)])], decode(8, 1, 2500, 3),
+          heads, kvh, d, dtype, 1200, 20, fmt=fmt, layout="NHD")

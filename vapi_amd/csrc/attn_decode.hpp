@@ -307,6 +307,13 @@ __device__ __forceinline__ void load_step_v(VTile<D>& st, const AttnArgs& a,
 }
 
 
+// The slot (of a.group rows) of the partial that range r leaves of segment seg, for the
+// streams that write it and the merges that read it: `parts` segments walk the keys side
+// by side (plan_parts), so that a segment's partials are `parts` slots apart.
+__device__ __forceinline__ uint32_t stream_slot(uint32_t parts, uint32_t r, uint32_t seg) {
+  return r * parts + seg;
+}
+
 // Write a finished piece of segment (p.seq, p.kh): the final output if the
 // piece is the whole segment, else a partial in slot `slot`.
 template <typename T, int D, bool kPad = false>
@@ -377,7 +384,8 @@ __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
   // A group split into n virtual kv heads: steps are counted per pool
   // head, each of n neighbouring waves walking one part (n = 1: the
   // virtual heads are the pool's).
-  // (With sinks, whole heads too: line_heads.)
+  // (With sinks, whole heads too: line_heads. Beside tiles of shared prefixes the two
+  // are the same, and plan_parts costs registers that this kernel does not have.)
   const uint32_t n_parts = kSinks && !kShared ? a.plan_parts : a.kv_parts.d;
   const uint32_t kvh_plan = a.kvh / n_parts;
   // The shared 100 MHz clock at entry: XCDs start the grid up to ~2.5 us
@@ -564,7 +572,7 @@ __device__ __forceinline__ void decode_stream_body(const AttnArgs& a,
         if (seg_ends) a.seg_ranges[2 * seg + 1] = r;
       }
       flush_piece<T, D, kPad>(a, pos, piece_first && seg_ends && !(kShared && pos.shared),
-                              r * n_parts + seg, o, m_run, l_run, col, g);
+                              stream_slot(n_parts, r, seg), o, m_run, l_run, col, g);
       if (!more) return false;
       m_run = kNegBig;
       l_run = 0.f;
@@ -806,7 +814,7 @@ __device__ __forceinline__ void decode_merge_body(const AttnArgs& a, uint32_t nw
       for (int u = 0; u < R; ++u) {
         const uint32_t pc = w + u * WPS;
         const bool in = pc <= r1;
-        const uint64_t sl = ((uint64_t)pc * a.plan_parts + seg) * G;
+        const uint64_t sl = (uint64_t)stream_slot(a.plan_parts, pc, seg) * G;
         const float* po = a.ws_o + sl * D + e_lane + j0;
         if (in && n == 8) {
           const float4 v0 = *(const float4*)po, v1 = *(const float4*)(po + 4);

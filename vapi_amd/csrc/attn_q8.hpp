@@ -270,7 +270,7 @@ __device__ __forceinline__ void q8_stream_body(const AttnArgs& a, const Q8Scales
         if (seg_ends) a.seg_ranges[2 * seg + 1] = r;
       }
       flush_piece<T, D, kPad>(a, pos, piece_first && seg_ends && !(kShared && pos.shared),
-                              r * n_parts + seg, o, m_run, l_run, col, g);
+                              stream_slot(n_parts, r, seg), o, m_run, l_run, col, g);
       if (!more) return false;
       m_run = kNegBig;
       l_run = 0.f;

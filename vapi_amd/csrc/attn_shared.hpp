@@ -832,7 +832,7 @@ __device__ __forceinline__ void sh_merge(const AttnArgs& a, const SharedArgs& sh
     const uint2 rr = *(const uint2*)(a.seg_ranges + 2 * seg);
     if (rr.y < nwg * kDecodeWavesPerWG && rr.x <= rr.y) {
       no = rr.y - rr.x + 1;
-      sl = ((uint64_t)rr.x * a.kv_parts.d + seg) * a.group + (head - v * a.group);
+      sl = (uint64_t)stream_slot(a.plan_parts, rr.x, seg) * a.group + (head - v * a.group);
     }
   } else if (w.kind == kOwnTiles) {
     const uint32_t row_own = w.tok * G + head, max_own = sh.max_joined - sh.max_grouped;
@@ -855,7 +855,7 @@ __device__ __forceinline__ void sh_merge(const AttnArgs& a, const SharedArgs& sh
   for (uint32_t j0 = 0; j0 < no; j0 += kB) {
     if (stream)
       fetch(j0, no, [&](uint32_t j, const float*& pm, const float*& px) {
-        const uint64_t slot = sl + (uint64_t)j * a.kv_parts.d * a.group;
+        const uint64_t slot = sl + (uint64_t)j * a.plan_parts * a.group;
         pm = a.ws_ml + slot * 2;
         px = a.ws_o + slot * D + dq;
       });
