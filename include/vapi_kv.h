@@ -316,10 +316,11 @@ int vapi_paged_attention_prepared(const vapi_kv_pool* pool, uint32_t layer, cons
  * and without a left window sinks change nothing. Any pool that
  * vapi_paged_attention takes, the same workspace, the same flags; prefill_seqs ==
  * NULL with n_prefill == 0 covers every sequence. Keys between the sinks and the
- * windows of a step's queries are not read (up to the 31 next to either), so their
- * blocks may be given to others (the table's entries then name any block), and what
- * V holds where no query of a sequence looks does not reach the output. No counterpart in the
- * reference, whose windows hide all that lies before them (attention.rs:179-194).
+ * windows of a step's queries are not read (up to the 31 next to either; up to the 63
+ * over 8-bit pools), so the blocks that hold only such keys may be given to others (the
+ * table's entries then name any block), and what V holds where no query of a sequence
+ * looks does not reach the output. No counterpart in the reference, whose windows hide
+ * all that lies before them (attention.rs:179-194).
  */
 int vapi_paged_attention_sinks(const vapi_kv_pool* pool, uint32_t layer, const void* q, void* out,
                                const uint32_t* cu_seqlens_q, const uint32_t* cu_seqlens_k,

@@ -434,3 +434,31 @@ def test_sinks_over_rows_that_share_cache_lines(heads, kvh, d, fmt, dtype):
     stream's ranges."""
     check([(70, decode(24, 1, 1500, d)), (4, [(1, 900), (3, 700), (1, 1)])], decode(8, 1, 2500, 3),
           heads, kvh, d, dtype, 1200, 20, fmt=fmt, layout="NHD")
+
+
+@pytest.mark.parametrize("heads,kvh,d,dtype,fmt", [
+    (8, 2, 128, BF16, "e4m3"), (8, 2, 128, BF16, "int8"), (4, 4, 64, F16, "int8"),
+    (6, 2, 256, F16, "e4m3")])
+def test_what_no_query_sees_of_codes_does_not_matter(heads, kvh, d, dtype, fmt):
+    """Codes that are NaN where no query looks, and scales of any value in blocks of those."""
+    members = [(1, 20), (1, 150), (1, 7), (3, 90)]
+    cache, q, batch, plan = make([(8, members), (9, [(1, 60), (1, 400)])], [(1, 300)], heads, kvh, d,
+                                 dtype, fmt=fmt)
+    left, sinks, bs = 33, 10, 16
+    want = reference(q, cache, batch, 0.1, left, 0, sinks)
+    cq, ck = batch.cu_seqlens_q, batch.cu_seqlens_k
+    seen = set()
+    for i, table in enumerate(batch.block_tables):
+        lk = ck[i + 1] - ck[i]
+        first = max(lk - (cq[i + 1] - cq[i]) - left, 0)
+        seen |= {table[p // bs] * bs + p % bs for p in range(lk) if p < sinks or p >= first}
+    hidden = torch.ones(cache.num_slots(), dtype=torch.bool)
+    hidden[list(seen)] = False
+    hidden = hidden.view(-1, bs).to(DEV)
+    whole = hidden.all(dim=1)
+    for c, s in ((cache.k[0], cache.k_scale[0]), (cache.v[0], cache.v_scale[0])):
+        c.view(torch.uint8).masked_fill_(hidden[:, None, :, None], 0x7F)
+        s.masked_fill_(whole[:, None], float("nan"))
+    got = paged_attention_prepared(q, cache, 0, prepare(batch, cache, heads, plan), 0.1, left, 0,
+                                   sinks=sinks)
+    assert_close(got, want, dtype)

@@ -327,3 +327,34 @@ def test_refusals():
     with pytest.raises(VapiKvError):
         paged_attention(torch.zeros(2, 3, 64, dtype=BF16, device=DEV), cache, 0, batch, 0.1,
                         sliding_window=9, sinks=1)
+
+
+@pytest.mark.parametrize("dtype,fmt,heads,kvh,d,layout", [
+    (BF16, "e4m3", 8, 2, 128, "HND"), (BF16, "int8", 8, 2, 128, "HND"),
+    (F16, "e4m3", 4, 4, 64, "NHD"), (F16, "int8", 12, 4, 80, "NHD"),
+    (BF16, "int8", 4, 2, 256, "NHD"), (F16, "e4m3", 6, 2, 256, "HND")])
+@pytest.mark.parametrize("lens_q", [[1] * 6, [1] * 80, [5, 1, 1, 90, 1, 3]])
+def test_what_no_query_sees_of_codes_does_not_matter(dtype, fmt, heads, kvh, d, layout, lens_q):
+    """Codes that are NaN between the sinks and the windows, scales of any value in the
+    blocks that lie there whole, and table entries there that name any block."""
+    lens_k = [40 + 37 * i % 900 + n for i, n in enumerate(lens_q)]
+    cache, q, batch = make(lens_q, lens_k, heads, kvh, d, dtype, fmt=fmt, layout=layout)
+    left, sinks, bs = 33, 10, 16
+    want = reference(q, cache, batch, 0.1, left, 0, sinks)
+    bad = [float("nan"), float("inf"), -float("inf"), -1.0, 0.0]
+    codes = [t[0].view(torch.uint8) for t in (cache.k, cache.v)]
+    for i, table in enumerate(batch.block_tables):
+        first = max(lens_k[i] - lens_q[i] - left, 0)
+        for key in range(sinks, first):
+            for c in codes:
+                c.select(0, table[key // bs]).select(1 if layout == "HND" else 0,
+                                                     key % bs).fill_(0x7F)
+        for b in range(1, first // bs):
+            cache.k_scale[0][table[b]] = bad[(i + b) % 5]
+            cache.v_scale[0][table[b]] = bad[b % 5]
+        # (64 keys a step: the next three blocks on either side may be read.)
+        for b in range(1 + 3, first // bs - 3):
+            table[b] = 0xFFFFFFFF if b % 2 else 0
+    got = paged_attention_prepared(q, cache, 0, PreparedAttention.from_batch(batch, DEV), 0.1, left,
+                                   0, sinks=sinks)
+    assert_close(got, want, dtype)

@@ -110,12 +110,27 @@ __device__ __forceinline__ void q8_load(Q8Step<D, KS>& st, const AttnArgs& a, co
 // stream's measured shares move from call to call, changes no rounding of P (of
 // 64 x 256-8,192 keys 0.03% of the outputs differed between calls, 45% without;
 // 74.5 us either way).
+// kSinks: keys between the sinks and the window weigh 0, whatever their V and its scale
+// hold (st is changed).
 template <typename T, int F, int D, int KS, bool kWhole, bool kSinks>
-__device__ __forceinline__ void q8_attend(const Q8Step<D, KS>& st, const uint4 (&qf)[D / 32],
+__device__ __forceinline__ void q8_attend(Q8Step<D, KS>& st, const uint4 (&qf)[D / 32],
                                           floatx4 (&o)[D / 16], float& m_run, float& l_run,
                                           float scale_log2, int32_t key0, int32_t lo,
                                           int32_t len_k, int32_t sinks, uint32_t g) {
   constexpr int NT = KS / 16, DPL = D / 16;
+  if (kSinks && key0 < lo) {
+#pragma unroll
+    for (int tt = 0; tt < NT; ++tt) {
+      const int32_t k0 = key0 + 16 * tt;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (!row_sees<kSinks>(k0 + 4 * (int32_t)g + i, lo, len_k, sinks))
+#pragma unroll
+          for (int w = 0; w < D / 64; ++w) st.v[tt][i][w] = 0u;
+      // (A tile lies in one block: one that holds a visible key has its scale.)
+      if (k0 >= sinks && k0 + 15 < lo) st.vs[tt] = 1.f;
+    }
+  }
   float s[4 * NT];
   float mx = -INFINITY;
 #pragma unroll
