@@ -462,3 +462,16 @@ def test_what_no_query_sees_of_codes_does_not_matter(heads, kvh, d, dtype, fmt):
     got = paged_attention_prepared(q, cache, 0, prepare(batch, cache, heads, plan), 0.1, left, 0,
                                    sinks=sinks)
     assert_close(got, want, dtype)
+
+
+@pytest.mark.parametrize("fmt", ["none", "e4m3"])
+@pytest.mark.parametrize("n_groups,n_rows", [(0, 8), (3, 0), (0, 0)])
+def test_lists_of_nothing_are_not_read(n_groups, n_rows, fmt):
+    """Rows without groups and groups without rows: the call takes null lists for them."""
+    cache, q, batch, _ = make([], [(1, 300), (1, 20), (3, 90), (1, 2000)], 8, 2, 128, BF16, fmt=fmt)
+    prep = prepare(batch, cache, 8, [])
+    a = prep.prefixes.arg
+    a.n_groups, a.n_rows, a.rows, a.seqs, a.keys = n_groups, n_rows, None, None, None
+    assert prep.shared_bytes(cache, 8) > 0
+    got = paged_attention_prepared(q, cache, 0, prep, 0.1)
+    assert_close(got, reference(q, cache, batch, 0.1, None, 0, 0), BF16)

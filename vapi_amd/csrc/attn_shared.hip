@@ -125,8 +125,9 @@ SharedArgs shared_args(const vapi_kv_prefixes* p, const AttnArgs& a, uint32_t he
                        uint32_t n_pf, char* ws) {
   SharedArgs sh{};
   sh.offsets = p->offsets, sh.rows = p->rows, sh.seqs = p->seqs, sh.keys = p->keys;
+  // (Groups without rows or rows without groups are neither: their lists may be null.)
   sh.n_groups = p->n_rows ? p->n_groups : 0;
-  sh.n_rows = p->n_rows;
+  sh.n_rows = p->n_groups ? p->n_rows : 0;
   sh.n_nodes = sh.n_groups + n_pf;
   sh.max_joined = (uint32_t)joined_tiles(p, a.g_real, head_dim, n_pf);
   sh.max_grouped = (uint32_t)grouped_tiles(p, a.g_real, head_dim);
