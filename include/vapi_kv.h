@@ -367,9 +367,9 @@ typedef struct vapi_kv_prefixes {
  * the order of f32 sums and the rounding of probabilities to the pool's dtype, with
  * each group's shared keys read once for all of its queries instead of once for each
  * sequence. Any lengths, windows and sinks; sequences in no group, decode rows and
- * prefill rows as there. prefill_seqs lists the sequences with len_q > 1 (NULL with
- * n_prefill == 0: all of them); a sequence with len_q > 1 that it leaves out gets no
- * output, or one without its own keys. Like the block table the lists are trusted:
+ * prefill rows as there. prefill_seqs lists the sequences with len_q > 1, each once
+ * (NULL with n_prefill == 0: all of them); a sequence with len_q > 1 that it leaves out
+ * gets no output, or in a group one without its own keys. Like the block table the lists are trusted:
  * entries that name no query of the batch are left out, and a group whose sequences'
  * tables differ attends the first one's blocks.
  *

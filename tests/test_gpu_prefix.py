@@ -475,3 +475,27 @@ def test_lists_of_nothing_are_not_read(n_groups, n_rows, fmt):
     assert prep.shared_bytes(cache, 8) > 0
     got = paged_attention_prepared(q, cache, 0, prep, 0.1)
     assert_close(got, reference(q, cache, batch, 0.1, None, 0, 0), BF16)
+
+
+@pytest.mark.parametrize("heads,kvh,d,dtype,fmt", [GEOMETRIES[0], GEOMETRIES[2], GEOMETRIES[9]])
+@pytest.mark.parametrize("left_out", [0, 2, 4])
+def test_sequences_that_the_prefill_list_leaves_out(left_out, heads, kvh, d, dtype, fmt):
+    """They end with the shared keys, whatever an earlier call left in the workspace."""
+    members = [(5, 40), (1, 60), (40, 300), (1, 5), (9, 9)]
+    cache, q, batch, plan = make([(12, members)], [(30, 80), (1, 200)], heads, kvh, d, dtype, fmt=fmt,
+                                 shuffle=False)
+    prep = prepare(batch, cache, heads, plan)
+    want, top = reference(q, cache, batch, 0.1, None, 0, 0)
+    got = paged_attention_prepared(q, cache, 0, prep, 0.1)
+    assert_close(got, (want, top), dtype)
+    prep.prefill_seqs = torch.tensor([s for s in (0, 2, 4, 5) if s != left_out], dtype=torch.int32,
+                                     device=DEV)
+    prep.n_prefill = 3
+    got = paged_attention_prepared(q, cache, 0, prep, 0.1)
+    lens = np.diff(batch.cu_seqlens_k)
+    lens[left_out] = 12 * 16
+    short = ForwardBatch(cu_seqlens_q=batch.cu_seqlens_q, block_tables=batch.block_tables,
+                         cu_seqlens_k=np.concatenate([[0], np.cumsum(lens)]).tolist())
+    rows = slice(batch.cu_seqlens_q[left_out], batch.cu_seqlens_q[left_out + 1])
+    want[rows] = reference(q, cache, short, 0.1, None, None, 0)[0][rows]
+    assert_close(got, (want, top), dtype)

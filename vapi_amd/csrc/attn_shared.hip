@@ -136,7 +136,7 @@ SharedArgs shared_args(const vapi_kv_prefixes* p, const AttnArgs& a, uint32_t he
                                p->n_rows);
   sh.lds_rows =
       sh.n_rows && sh_plan_bytes(sh.n_nodes) + sh.n_rows * sizeof(ShEntry) <= kShPlanLds;
-  sh.n_grouped = (uint32_t*)ws;
+  sh.n_tiles = (uint32_t*)ws;
   sh.joined = (ShTile*)(ws + w.joined);
   sh.open = (ShTile*)(ws + w.open);
   sh.own = (uint32_t*)(ws + w.own);

@@ -79,10 +79,12 @@ struct SharedArgs {
   const float *ks, *vs;  // 8-bit pools: the layer's scales, sblk a block
   uint32_t sblk;
   uint32_t lds_rows;  // whether every query of the groups has an entry in LDS
-  // Workspace: the groups' tiles of a kv head; joined tiles, max_grouped of each kv head
-  // for the groups and then the rest for each; the ranges' open tiles; the first joined
-  // tile of a sequence's own node; the groups' queries; partials.
-  uint32_t* n_grouped;
+  // Workspace: the joined tiles of a kv head, {the groups', the sequences' own}; joined
+  // tiles, max_grouped of each kv head for the groups and then the rest for each; the
+  // ranges' open tiles; the first joined tile of a sequence's own node (of sequences that
+  // have one: what the others' words hold is of earlier calls); the groups' queries;
+  // partials.
+  uint32_t* n_tiles;
   ShTile *joined, *open;
   uint32_t* own;
   ShQuery* queries;
@@ -675,7 +677,8 @@ __device__ __forceinline__ void sh_range(const AttnArgs& a, const SharedArgs& sh
   const uint32_t n_grouped = __builtin_amdgcn_readfirstlane(joined[sh.n_groups]);
   const uint32_t max_own = sh.max_joined - sh.max_grouped;
   const bool fits = n_grouped <= sh.max_grouped && n_joined - n_grouped <= max_own;  // (every plan)
-  if (bid == 0 && threadIdx.x == 0) *sh.n_grouped = fits ? n_grouped : 0u;
+  if (bid == 0 && threadIdx.x == 0)
+    *(uint2*)sh.n_tiles = fits ? make_uint2(n_grouped, n_joined - n_grouped) : make_uint2(0u, 0u);
   const uint64_t total = (uint64_t)S * kvh;
   const uint32_t nr = (uint32_t)min((uint64_t)sh.ranges, (total + kShMinSteps - 1) / kShMinSteps);
   if (bid >= nr || !fits) {
@@ -757,9 +760,9 @@ __device__ __forceinline__ void sh_merge(const AttnArgs& a, const SharedArgs& sh
   constexpr uint32_t kRows = sh_rows(D), kTpr = D / (4 * NV), kRpw = sh_merge_rows(D, NV);
   const uint32_t kvh = sh_heads(a), most = sh.max_grouped * kvh, G = a.g_real;
   const bool group = i < most;
-  const uint32_t n_grouped = *sh.n_grouped;
+  const uint2 n_tiles = *(const uint2*)sh.n_tiles;
   const ShTile d = group ? sh.joined[i] : sh.open[i - most];
-  if (group ? i % sh.max_grouped >= n_grouped : !d.valid) return;
+  if (group ? i % sh.max_grouped >= n_tiles.x : !d.valid) return;
   const uint32_t kh = d.kh;
   const uint32_t row = block * kRpw + threadIdx.x / kTpr, dq = (threadIdx.x % kTpr) * 4;
   const uint32_t r = d.tile * kRows + row, tok = r / G, head = r - tok * G;
@@ -837,11 +840,11 @@ __device__ __forceinline__ void sh_merge(const AttnArgs& a, const SharedArgs& sh
   } else if (w.kind == kOwnTiles) {
     const uint32_t row_own = w.tok * G + head, max_own = sh.max_joined - sh.max_grouped;
     const uint32_t t = sh.own[w.seq] + row_own / kRows;
-    if (t < max_own) {
+    // (The call's own tiles, all of them written: a sequence that the list of prefill
+    // sequences leaves out has none among them, whatever `own` holds for it.)
+    if (t < n_tiles.y) {
       e = sh.joined[most + kh * max_own + t];
-      // (A sequence that the list leaves out has no tile of its own.)
-      if (e.valid && e.seq == w.seq && e.kh == kh && e.tile == row_own / kRows && e.r0 <= e.r1 &&
-          e.r1 < sh.ranges) {
+      if (e.seq == w.seq && e.tile == row_own / kRows) {
         no = e.r1 - e.r0 + 1;
         orow = row_own % kRows;
       }
