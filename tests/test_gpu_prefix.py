@@ -499,3 +499,49 @@ def test_sequences_that_the_prefill_list_leaves_out(left_out, heads, kvh, d, dty
     rows = slice(batch.cu_seqlens_q[left_out], batch.cu_seqlens_q[left_out + 1])
     want[rows] = reference(q, cache, short, 0.1, None, None, 0)[0][rows]
     assert_close(got, (want, top), dtype)
+
+
+@pytest.mark.parametrize("heads,kvh,d,dtype,fmt", [GEOMETRIES[0], GEOMETRIES[5], GEOMETRIES[11]])
+@pytest.mark.parametrize("members,many", [(3, 1), (150, 1), (5, 300), (1100, 1)])
+def test_entries_that_name_no_query_are_left_out(members, many, heads, kvh, d, dtype, fmt):
+    """The first of a group among them, and all of one: a sequence past the batch, one that
+    has ended and whose table names nothing, a row that is not the sequence's."""
+    if members * heads > 16000:
+        heads = kvh  # (the reference's time)
+    groups = [(6, [(1, 1 + i % 50) for i in range(members)])]
+    groups += [(1, [(1, 1 + i % 9), (1, 3)]) for i in range(many)]
+    cache, q, batch, plan = make(groups + [(3, [(0, 5), (0, 9)])], [(0, 0), (1, 40)], heads, kvh, d,
+                                 dtype, fmt=fmt, shuffle=False)
+    want = reference(q, cache, batch, 0.1, None, 0, 0)
+    n, ended = len(batch.block_tables), members + 2 * many
+    batch.block_tables[ended] = [0] * 4  # what a finished request leaves
+    prep = prepare(batch, cache, heads, plan)
+    a, words = prep.prefixes.arg, prep.prefixes.lists.cpu().numpy().view(np.uint32)
+
+    def at(p, count):
+        i = (p - prep.prefixes.lists.data_ptr()) // 4
+        return words[i:i + count].tolist()
+
+    offsets, rows, seqs = at(a.offsets, a.n_groups + 1), at(a.rows, a.n_rows), at(a.seqs, a.n_rows)
+    dead = [(0, n), (0, ended), (0xFFFFFFFF, 0), (0, n - 1), (0xFFFFFFFF, 0xFFFFFFFF)]
+    new = [[], [], [0]]
+    for g in range(a.n_groups):
+        front = dead * 30 if g == 0 else dead[g % 5:g % 5 + 1] * (g % 2)
+        some = list(zip(rows, seqs))[offsets[g]:offsets[g + 1]]
+        if not some:  # the group without queries: entries that name none
+            front = dead * 2
+        for row, seq in front + some[:2] + dead + some[2:]:
+            new[0].append(row)
+            new[1].append(seq)
+        new[2].append(len(new[0]))
+    lists = [new[2], new[0], new[1], at(a.keys, a.n_groups), at(a.start, n)]
+    sizes = np.cumsum([0] + [len(x) for x in lists])
+    prep.prefixes.lists = torch.from_numpy(
+        np.concatenate(lists).astype(np.uint32).view(np.int32)).to(DEV)
+    ptr = [prep.prefixes.lists.data_ptr() + 4 * int(x) for x in sizes]
+    a.offsets, a.rows, a.seqs, a.keys, a.start = ptr[:5]
+    a.n_rows = len(new[0])
+    assert prep.shared_bytes(cache, heads) > 0
+    out = torch.full_like(q, float("nan"))
+    got = paged_attention_prepared(q, cache, 0, prep, 0.1, out=out)
+    assert_close(got, want, dtype)

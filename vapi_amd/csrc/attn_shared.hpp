@@ -96,7 +96,7 @@ __device__ __forceinline__ uint32_t sh_heads(const AttnArgs& a) { return a.kvh /
 
 struct ShNode {
   uint32_t first, tokens;  // rows of its queries: entries of rows, or rows of q
-  uint32_t seq;            // own nodes: the sequence; groups: one of theirs
+  uint32_t seq;            // own nodes: the sequence; groups: one of theirs (sh_plan)
   int32_t k0, k1;          // its keys
 };
 __device__ __forceinline__ ShNode sh_node(const AttnArgs& a, const SharedArgs& sh, uint32_t i) {
@@ -106,8 +106,7 @@ __device__ __forceinline__ ShNode sh_node(const AttnArgs& a, const SharedArgs& s
     n.first = e0;
     n.k1 = shared_keys(a, sh.keys[i]);
     if (e1 <= e0 || n.k1 <= 0) return n;
-    n.seq = sh.seqs[e0];
-    if (n.seq < a.batch) n.tokens = e1 - e0;
+    n.tokens = e1 - e0;
     return n;
   }
   n.seq = a.pf_seqs ? a.pf_seqs[i - sh.n_groups] : i - sh.n_groups;
@@ -131,13 +130,38 @@ __device__ __forceinline__ uint32_t sh_node_steps(const AttnArgs& a, const ShNod
   return (uint32_t)ks.last / 32 + 1;
 }
 
+// Entry e of the groups' lists: its row of q (~0: it names none), its sequence, and the
+// keys that its mask leaves.
+struct ShEntry {
+  uint32_t q, seq;
+  int32_t lo, hi;
+};
+__device__ __forceinline__ ShEntry sh_entry(const AttnArgs& a, const SharedArgs& sh, uint32_t e,
+                                            ShQuery* info = nullptr) {
+  ShEntry x{sh.rows[e], sh.seqs[e], 0, -1};
+  const bool in = x.seq < a.batch;
+  const uint32_t s = in ? x.seq : 0;
+  const uint32_t q0 = a.cu_q[s], len_q = a.cu_q[s + 1] - q0;
+  const int32_t len_k = (int32_t)(a.cu_k[s + 1] - a.cu_k[s]);
+  const uint32_t tok = x.q - q0;
+  if (!in || tok >= len_q) x.q = ~0u;
+  else key_range(len_k - (int32_t)len_q + (int32_t)tok, len_k, a.wl, a.wr, x.lo, x.hi);
+  if (info) {
+    const bool past = len_k > shared_keys(a, a.shared[s]);
+    *info = ShQuery{x.q, s, len_q >= a.pf_min_q ? kOwnTiles : past ? kOwnStream : kOwnNone, tok};
+  }
+  return x;
+}
+
 // The plan, in LDS: tiles, steps and joined tiles of the nodes before each (n_nodes + 1
-// of each, one array after the other), then the nodes.
+// of each, one array after the other), then the nodes. `entries`: the groups' queries, if
+// they are in LDS. A group's keys are those of the sequence of its first entry that names
+// a query (none: of any).
 constexpr size_t sh_plan_bytes(uint32_t n_nodes) {
   return 3 * ((size_t)n_nodes + 1) * sizeof(uint32_t) + n_nodes * sizeof(ShNode);
 }
 __device__ __forceinline__ void sh_plan(const AttnArgs& a, const SharedArgs& sh, uint32_t rows,
-                                        uint32_t* tiles) {
+                                        uint32_t* tiles, const ShEntry* entries) {
   __shared__ uint32_t tot[3][kShWaves];
   const uint32_t N1 = sh.n_nodes + 1;
   uint32_t *steps = tiles + N1, *joined = steps + N1;
@@ -179,30 +203,27 @@ __device__ __forceinline__ void sh_plan(const AttnArgs& a, const SharedArgs& sh,
     }
     if (tid == kShThreads - 1) arr[sh.n_nodes] = run;
   }
-  __syncthreads();
-}
-
-// Entry e of the groups' lists: its row of q (~0: it names none), its sequence, and the
-// keys that its mask leaves.
-struct ShEntry {
-  uint32_t q, seq;
-  int32_t lo, hi;
-};
-__device__ __forceinline__ ShEntry sh_entry(const AttnArgs& a, const SharedArgs& sh, uint32_t e,
-                                            ShQuery* info = nullptr) {
-  ShEntry x{sh.rows[e], sh.seqs[e], 0, -1};
-  const bool in = x.seq < a.batch;
-  const uint32_t s = in ? x.seq : 0;
-  const uint32_t q0 = a.cu_q[s], len_q = a.cu_q[s + 1] - q0;
-  const int32_t len_k = (int32_t)(a.cu_k[s + 1] - a.cu_k[s]);
-  const uint32_t tok = x.q - q0;
-  if (!in || tok >= len_q) x.q = ~0u;
-  else key_range(len_k - (int32_t)len_q + (int32_t)tok, len_k, a.wl, a.wr, x.lo, x.hi);
-  if (info) {
-    const bool past = len_k > shared_keys(a, a.shared[s]);
-    *info = ShQuery{x.q, s, len_q >= a.pf_min_q ? kOwnTiles : past ? kOwnStream : kOwnNone, tok};
+  auto entry = [&](uint32_t e) { return sh.lds_rows ? entries[e] : sh_entry(a, sh, e); };
+  for (uint32_t i = i0; i < i0 + per; ++i) {
+    ShEntry x{0, 0, 0, 0};
+    if (i < min(i1, sh.n_groups) && nodes[i].tokens) {
+      x = entry(nodes[i].first);
+      nodes[i].seq = x.q != ~0u ? x.seq : 0u;
+    }
+    // Groups whose first entry names none, one after the other by all of the wave.
+    for (uint64_t dead = __ballot(x.q == ~0u); dead; dead &= dead - 1) {
+      const uint32_t node = __shfl(i, __builtin_ctzll(dead));
+      const uint32_t first = nodes[node].first, end = first + nodes[node].tokens;
+      for (uint32_t e = first; e < end; e += 64) {
+        const ShEntry y = entry(min(e + lane, end - 1));
+        const uint64_t live = __ballot(y.q != ~0u);
+        if (!live) continue;
+        if (lane == (uint32_t)__builtin_ctzll(live)) nodes[node].seq = y.seq;
+        break;
+      }
+    }
   }
-  return x;
+  __syncthreads();
 }
 
 // A thread's chunks are the same rows and columns of every step (ShSlots), so that a
@@ -671,7 +692,7 @@ __device__ __forceinline__ void sh_range(const AttnArgs& a, const SharedArgs& sh
     for (uint32_t e = threadIdx.x; e < sh.n_rows; e += kShThreads) entries[e] = sh_entry(a, sh, e);
   for (uint32_t e = bid * kShThreads + threadIdx.x; e < sh.n_rows; e += sh.ranges * kShThreads)
     sh_entry(a, sh, e, sh.queries + e);
-  sh_plan(a, sh, kRows, lds);
+  sh_plan(a, sh, kRows, lds, entries);
   const uint32_t S = __builtin_amdgcn_readfirstlane(steps[N]);
   const uint32_t n_joined = __builtin_amdgcn_readfirstlane(joined[N]);
   const uint32_t n_grouped = __builtin_amdgcn_readfirstlane(joined[sh.n_groups]);
