@@ -545,3 +545,29 @@ def test_entries_that_name_no_query_are_left_out(members, many, heads, kvh, d, d
     out = torch.full_like(q, float("nan"))
     got = paged_attention_prepared(q, cache, 0, prep, 0.1, out=out)
     assert_close(got, want, dtype)
+
+
+@pytest.mark.parametrize("heads,kvh,d,dtype,fmt", [
+    (8, 2, 128, BF16, "none"), (4, 4, 64, F16, "none"), (6, 2, 256, BF16, "none"),
+    (8, 2, 128, BF16, "e4m3"), (32, 32, 96, F16, "none")])
+@pytest.mark.parametrize("where", ["prefix", "own"])
+def test_a_nan_key_stays_with_the_rows_that_see_it(where, heads, kvh, d, dtype, fmt):
+    """A NaN in the shared keys reaches every member's outputs, one in a member's own keys
+    that member's."""
+    members = [(1, 50), (1, 900), (4, 70), (1, 33), (30, 60)]
+    cache, q, batch, plan = make([(40, members)], [(1, 200), (5, 90)], heads, kvh, d, dtype, fmt=fmt,
+                                 shuffle=False)
+    want, top = reference(q, cache, batch, 0.1, None, 0, 0)
+    key = 300 if where == "prefix" else 640 + 5
+    block = batch.block_tables[1][key // 16]
+    if fmt == "none":
+        cache.k[0][block, 0, key % 16] = float("nan")
+    else:
+        cache.k[0].view(torch.uint8)[block, 0, key % 16] = 0x7F
+    got = paged_attention_prepared(q, cache, 0, prepare(batch, cache, heads, plan), 0.1)
+    rows = slice(0, 37) if where == "prefix" else slice(1, 2)
+    group = heads // kvh
+    assert torch.isnan(got[rows, :group]).all()
+    got[rows, :group] = 0.0
+    want[rows, :group] = 0.0
+    assert_close(got, (want, top), dtype)

@@ -358,3 +358,30 @@ def test_what_no_query_sees_of_codes_does_not_matter(dtype, fmt, heads, kvh, d, 
     got = paged_attention_prepared(q, cache, 0, PreparedAttention.from_batch(batch, DEV), 0.1, left,
                                    0, sinks=sinks)
     assert_close(got, want, dtype)
+
+
+@pytest.mark.parametrize("dtype,fmt,heads,kvh,d", [
+    (BF16, "none", 8, 2, 128), (F16, "none", 4, 4, 64), (BF16, "none", 4, 1, 256),
+    (F32, "none", 8, 2, 128), (BF16, "e4m3", 8, 2, 128), (F16, "none", 4, 2, 20)])
+@pytest.mark.parametrize("lens_q", [[1, 1], [1] * 40, [3, 40], [300, 200, 100]])
+@pytest.mark.parametrize("where", ["sink", "window"])
+def test_a_nan_key_stays_with_the_rows_that_see_it(dtype, fmt, heads, kvh, d, lens_q, where):
+    """However a row's keys are split over workgroups: NaN scores leave NaN, in no other row."""
+    lens_k = [2500 + 11 * i for i in range(len(lens_q))]
+    cache, q, batch = make(lens_q, lens_k, heads, kvh, d, dtype, fmt=fmt)
+    left, sinks, bs = 1000, 3, 16
+    want, top = reference(q, cache, batch, 0.1, left, 0, sinks)
+    lq, lk, table = lens_q[1], lens_k[1], batch.block_tables[1]
+    key = 1 if where == "sink" else lk - lq - 700  # every query of the sequence sees it
+    if fmt == "none":
+        cache.k[0][table[key // bs], 0, key % bs] = float("nan")
+    else:
+        cache.k[0].view(torch.uint8)[table[key // bs], 0, key % bs] = 0x7F
+    got = paged_attention_prepared(q, cache, 0, PreparedAttention.from_batch(batch, DEV), 0.1, left,
+                                   0, sinks=sinks)
+    rows = slice(batch.cu_seqlens_q[1], batch.cu_seqlens_q[2])
+    group = heads // kvh
+    assert torch.isnan(got[rows, :group]).all()
+    got[rows, :group] = 0.0
+    want[rows, :group] = 0.0
+    assert_close(got, (want, top), dtype)

@@ -703,7 +703,7 @@ __device__ __forceinline__ void store_outputs(T* dst, uint32_t n, const float (&
                                               const float (&L)[8]) {
   float v[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = L[j] > 0.f ? O[j] / L[j] : 0.f;
+  for (int j = 0; j < 8; ++j) v[j] = weighs(L[j]) ? O[j] / L[j] : 0.f;
   if constexpr (sizeof(T) == 4) {
     if (n == 8 && ((uintptr_t)dst & 15) == 0) {
       ((float4*)dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
@@ -787,7 +787,7 @@ __device__ __forceinline__ void decode_merge_body(const AttnArgs& a, uint32_t nw
       for (int j = 0; j < 8; ++j) {
         const uint32_t ej = e + j, d = ej % D;
         if (j < (int)n && d < hd)
-          orow[(ej / D) * hd + d] = from_f32<T>(L[j] > 0.f ? O[j] / L[j] : 0.f);
+          orow[(ej / D) * hd + d] = from_f32<T>(weighs(L[j]) ? O[j] / L[j] : 0.f);
       }
     } else {
       store_outputs<T>(orow + e, n, O, L);
@@ -827,8 +827,8 @@ __device__ __forceinline__ void decode_merge_body(const AttnArgs& a, uint32_t nw
         const float2 x0 = in ? *(const float2*)(a.ws_ml + (sl + h0) * 2) : make_float2(kNegBig, 0.f);
         const float2 x1 = in ? *(const float2*)(a.ws_ml + (sl + h1) * 2) : make_float2(kNegBig, 0.f);
         // Partials with l = 0 weigh nothing, whatever their m and o hold.
-        mm[u][0] = x0.y > 0.f ? x0.x : kNegBig, ll[u][0] = x0.y;
-        mm[u][1] = x1.y > 0.f ? x1.x : kNegBig, ll[u][1] = x1.y;
+        mm[u][0] = weighs(x0.y) ? x0.x : kNegBig, ll[u][0] = x0.y;
+        mm[u][1] = weighs(x1.y) ? x1.x : kNegBig, ll[u][1] = x1.y;
       }
       float f[2], e[R][2];
 #pragma unroll
@@ -840,7 +840,7 @@ __device__ __forceinline__ void decode_merge_body(const AttnArgs& a, uint32_t nw
         float Ln = Lh[h] * f[h];
 #pragma unroll
         for (int u = 0; u < R; ++u) {
-          e[u][h] = ll[u][h] > 0.f ? fast_exp2(mm[u][h] - Mn) : 0.f;
+          e[u][h] = weighs(ll[u][h]) ? fast_exp2(mm[u][h] - Mn) : 0.f;
           Ln += ll[u][h] * e[u][h];
         }
         Mh[h] = Mn, Lh[h] = Ln;
@@ -882,7 +882,7 @@ __device__ __forceinline__ void decode_merge_body(const AttnArgs& a, uint32_t nw
         }
         const uint32_t e = e_lane + j0 + j;
         if (j < n && e < e_end && (!kPad || e % D < hd))
-          orow[kPad ? (e / D) * hd + e % D : e] = from_f32<T>(Lj > 0.f ? Oj / Lj : 0.f);
+          orow[kPad ? (e / D) * hd + e % D : e] = from_f32<T>(weighs(Lj) ? Oj / Lj : 0.f);
       }
       __syncthreads();  // the LDS is reused by the next eight outputs
     } else {

@@ -361,12 +361,12 @@ __global__ __launch_bounds__(64 * kSmallWaves) void paged_decode_small_merge(
         }
         float Mn = M;
 #pragma unroll
-        for (uint32_t u = 0; u < kB; ++u) Mn = fmaxf(Mn, ml[u].y > 0.f ? ml[u].x : kNegBig);
+        for (uint32_t u = 0; u < kB; ++u) Mn = fmaxf(Mn, weighs(ml[u].y) ? ml[u].x : kNegBig);
         const float f = fast_exp2(M - Mn);
         L *= f, x.x *= f, x.y *= f, x.z *= f, x.w *= f;
 #pragma unroll
         for (uint32_t u = 0; u < kB; ++u) {
-          if (!(ml[u].y > 0.f)) continue;  // a share without keys, or past the last
+          if (!weighs(ml[u].y)) continue;  // a share without keys, or past the last
           const float w = fast_exp2(ml[u].x - Mn);
           L += ml[u].y * w;
           x.x += y[u].x * w, x.y += y[u].y * w, x.z += y[u].z * w, x.w += y[u].w * w;

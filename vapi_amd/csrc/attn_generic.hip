@@ -412,14 +412,14 @@ __global__ __launch_bounds__(kGenThreads) void paged_attn_generic_merge(
     float Mn = M;
 #pragma unroll
     for (int u = 0; u < kB; ++u)
-      if (l[u] > 0.f) Mn = fmaxf(Mn, m[u]);
+      if (weighs(l[u])) Mn = fmaxf(Mn, m[u]);
     const float f = __expf(M - Mn);
     L *= f;
 #pragma unroll
     for (int i = 0; i < kMaxDPer; ++i) o[i] *= f;
 #pragma unroll
     for (int u = 0; u < kB; ++u) {
-      if (!(l[u] > 0.f)) continue;  // a chunk no key of this row is visible in
+      if (!weighs(l[u])) continue;  // a chunk no key of this row is visible in
       const float e = __expf(m[u] - Mn);
       L += l[u] * e;
 #pragma unroll

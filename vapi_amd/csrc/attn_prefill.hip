@@ -390,14 +390,14 @@ __device__ __forceinline__ void prefill_merge_rows(const AttnArgs& a, uint32_t s
     float Mn = M;
 #pragma unroll
     for (uint32_t u = 0; u < kB; ++u)
-      if (ml[u].y > 0.f) Mn = fmaxf(Mn, ml[u].x);
+      if (weighs(ml[u].y)) Mn = fmaxf(Mn, ml[u].x);
     const float f = fast_exp2(M - Mn);
     L *= f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] *= f;
 #pragma unroll
     for (uint32_t u = 0; u < kB; ++u) {
-      if (!(ml[u].y > 0.f)) continue;  // a share with no visible key (its o is stale)
+      if (!weighs(ml[u].y)) continue;  // a share with no visible key (its o is stale)
       const float e = fast_exp2(ml[u].x - Mn);
       const float w = ml[u].y * e;  // the partial's o is o / l
       L += w;
