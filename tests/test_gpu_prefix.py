@@ -571,3 +571,18 @@ def test_a_nan_key_stays_with_the_rows_that_see_it(where, heads, kvh, d, dtype, 
     got[rows, :group] = 0.0
     want[rows, :group] = 0.0
     assert_close(got, (want, top), dtype)
+
+
+@pytest.mark.parametrize("fmt", ["none", "e4m3"])
+def test_a_plan_on_another_device_is_refused(fmt):
+    cache, q, batch, plan = make([(4, [(1, 5), (1, 9)])], [], 8, 2, 64, BF16, fmt=fmt)
+    prep = prepare(batch, cache, 8, plan)
+    prep.prefixes = PrefixPlan(plan, batch.cu_seqlens_q, batch.cu_seqlens_k, "cpu")
+    with pytest.raises(ValueError, match="cpu"):
+        paged_attention_prepared(q, cache, 0, prep, 0.1)
+    before = cache.k[0].clone()
+    k = torch.zeros(2, 2, 64, device=DEV, dtype=BF16)
+    with pytest.raises(ValueError, match="cpu"):
+        paged_attention_append_prepared(q, k, k, scatter_index(np.array([0, 1]), DEV), cache, 0, prep,
+                                        0.1)
+    assert torch.equal(before.view(torch.uint8), cache.k[0].view(torch.uint8))

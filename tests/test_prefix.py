@@ -197,3 +197,16 @@ def test_shared_prefixes_refuse(q8):
             assert size(p, 4, 0, 8, 1, 100, ok) == 0
     # A step that shares nothing, or has no groups, is an ordinary one.
     assert size(make(), 4, 0, 8, 1, 100, prefixes(n_groups=0, n_rows=0)) > 0
+
+
+def test_a_plan_of_another_batch_is_refused():
+    cache = PagedKvCache(1, 8, 16, 8, 128, layout="HND", device="cpu")
+    batch = batch_of([[1, 2], [1, 3], [1, 4]], [1] * 3, [20] * 3)
+    prep = PreparedAttention.from_batch(batch, "cpu")
+    prep.prefixes = PrefixPlan([([0, 1], 16)], batch.cu_seqlens_q, batch.cu_seqlens_k, "cpu")
+    assert prep.shared_bytes(cache, 32) > 0
+    for n in (2, 4):
+        cu = list(range(n + 1))
+        prep.prefixes = PrefixPlan([([0, 1], 16)], cu, [20 * x for x in cu], "cpu")
+        with pytest.raises(ValueError, match="sequences in a step of 3"):
+            prep.shared_bytes(cache, 32)

@@ -196,6 +196,9 @@ class PreparedAttention:
         their partial results cost (PrefixPlan.worth_it)."""
         if self.prefixes is None:
             return 0
+        if self.prefixes.batch != self.seqlens_q.shape[0] - 1:
+            raise ValueError(f"shared prefixes of {self.prefixes.batch} sequences in a step of "
+                             f"{self.seqlens_q.shape[0] - 1}")
         key = (cache.num_kv_heads, cache.head_dim, cache.block_size, cache.dtype, num_heads,
                getattr(cache, "fmt", None), window_left)
         if key not in self.sharing:
@@ -319,7 +322,7 @@ def paged_attention_prepared(q: torch.Tensor, cache: PagedKvCache, layer: int,
         args += (prepared.prefill_seqs.data_ptr() if listed else None,
                  prepared.n_prefill if listed else 0)
     if shared:
-        check_on_device(q, out, prepared.block_table, prepared.seqlens_q)
+        check_on_device(q, out, prepared.block_table, prepared.seqlens_q, prepared.prefixes.lists)
         fn = lib().vapi_paged_attention_shared
         if _is_quantised(cache):
             check_on_device(q, cache.k[0])
@@ -377,7 +380,8 @@ def paged_attention(q, cache, layer, batch: ForwardBatch, softmax_scale,
 def _check_second(cache, q, out, prepared: PreparedAttention) -> None:
     """What an attention refuses that follows a write as a second call."""
     check_on_device(q, out, prepared.block_table, prepared.seqlens_q,
-                    *(cache.k[:1] if _is_quantised(cache) else ()))
+                    *(cache.k[:1] if _is_quantised(cache) else ()),
+                    *((prepared.prefixes.lists,) if prepared.prefixes else ()))
     if (q.data_ptr() | out.data_ptr()) & 15:
         raise ValueError("q and out must be 16-byte aligned")
     if prepared.block_table.shape[1] == 0 or prepared.flags & ~(ATTN_DETERMINISTIC |

@@ -85,7 +85,7 @@ class PrefixPlan:
     def __init__(self, groups, cu_seqlens_q, cu_seqlens_k, device, min_bytes: int = 0):
         cq = np.asarray(cu_seqlens_q, dtype=np.int64)
         lens_k = np.diff(np.asarray(cu_seqlens_k, dtype=np.int64))
-        batch = len(lens_k)
+        batch = self.batch = len(lens_k)
         self.groups = [(list(map(int, m)), int(n)) for m, n in groups]
         self.min_bytes = min_bytes
         start = np.zeros(max(batch, 1), np.int64)
