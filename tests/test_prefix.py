@@ -210,3 +210,22 @@ def test_a_plan_of_another_batch_is_refused():
         prep.prefixes = PrefixPlan([([0, 1], 16)], cu, [20 * x for x in cu], "cpu")
         with pytest.raises(ValueError, match="sequences in a step of 3"):
             prep.shared_bytes(cache, 32)
+
+
+def test_a_step_whose_plan_or_lengths_change_asks_again():
+    cache = PagedKvCache(1, 8, 16, 8, 128, layout="HND", device="cpu")
+    batch = batch_of([[1, 2]] * 40, [4] * 40, [20] * 40)
+    prep = PreparedAttention.from_batch(batch, "cpu")
+
+    def plan(n):
+        return PrefixPlan([(list(range(n)), 16)], batch.cu_seqlens_q, batch.cu_seqlens_k, "cpu")
+
+    prep.prefixes = plan(2)
+    few = prep.shared_bytes(cache, 32)
+    prep.prefixes = plan(40)
+    many = prep.shared_bytes(cache, 32)
+    assert 0 < few < many
+    prep.n_prefill = 1  # the others' queries have no tiles of their own
+    assert 0 < prep.shared_bytes(cache, 32) < many
+    prep.max_seqlen_k = 15  # fewer keys than the prefix: refused
+    assert prep.shared_bytes(cache, 32) == 0

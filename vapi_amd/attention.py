@@ -126,7 +126,7 @@ class PreparedAttention:
     workspaces: list = field(default_factory=list)  # the attention's earlier ones
     streams: set = field(default_factory=set)  # handles keep_for has seen
     prefixes: PrefixPlan | None = None
-    sharing: dict = field(default_factory=dict)  # shares()'s answers
+    sharing: dict = field(default_factory=dict)  # shared_bytes()'s answers
 
     @classmethod
     def from_batch(cls, batch: ForwardBatch, device, cache=None, num_heads: int | None = None,
@@ -200,7 +200,8 @@ class PreparedAttention:
             raise ValueError(f"shared prefixes of {self.prefixes.batch} sequences in a step of "
                              f"{self.seqlens_q.shape[0] - 1}")
         key = (cache.num_kv_heads, cache.head_dim, cache.block_size, cache.dtype, num_heads,
-               getattr(cache, "fmt", None), window_left)
+               getattr(cache, "fmt", None), window_left, self.prefixes, self.flags,
+               self.n_prefill, self.max_seqlen_q, self.max_seqlen_k)
         if key not in self.sharing:
             need = 0
             if self.prefixes.worth_it(cache, window_left):
