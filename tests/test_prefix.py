@@ -225,7 +225,8 @@ def test_a_step_whose_plan_or_lengths_change_asks_again():
     prep.prefixes = plan(40)
     many = prep.shared_bytes(cache, 32)
     assert 0 < few < many
-    prep.n_prefill = 1  # the others' queries have no tiles of their own
+    # (Without a decode row the call covers every sequence, whatever the list.)
+    prep.flags, prep.n_prefill = 0, 1  # the others' queries have no tiles of their own
     assert 0 < prep.shared_bytes(cache, 32) < many
     prep.max_seqlen_k = 15  # fewer keys than the prefix: refused
     assert prep.shared_bytes(cache, 32) == 0
