@@ -48,13 +48,16 @@ inline int32_t row_window(int32_t wl, int32_t sinks) {
   return wl < 0 || !sinks ? wl : std::min<int32_t>(wl + std::min(sinks, 1 << 29) + 64, 1 << 30);
 }
 // Whether a partial whose exponentials sum to l counts: all but l = 0 (no visible key), NaN
-// of a NaN score among them, so that it reaches the row however its keys were split. (A
-// test of the bits, which the compiler must not see come from a float: the kernels are
-// built without NaN in float compares, and it makes one of those of it.)
+// of a NaN score among them, so that it reaches the row however its keys were split. (Of
+// the bits: the kernels are built without NaN in float compares, and the compiler makes
+// one of those of a float's bits unless that is hidden from it. Loaded sums are tested
+// after all loads of their batch, which the hidden test would wait for one by one: 64
+// decode rows of 256-8,192 keys 122.2 -> 124.0 us, 16 43.3 -> 44.9.)
+__device__ __forceinline__ bool weighs(uint32_t l_bits) { return l_bits != 0u; }
 __device__ __forceinline__ bool weighs(float l) {
   uint32_t bits = __float_as_uint(l);
   asm("" : "+v"(bits));
-  return bits != 0u;
+  return weighs(bits);
 }
 constexpr float kNegBig = -1e30f;  // running-max start: finite, so exp2 never sees inf-inf
 constexpr float kRescaleSlack = 8.0f;  // log2 units the running max may lag by

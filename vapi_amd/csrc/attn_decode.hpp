@@ -826,21 +826,24 @@ __device__ __forceinline__ void decode_merge_body(const AttnArgs& a, uint32_t nw
         }
         const float2 x0 = in ? *(const float2*)(a.ws_ml + (sl + h0) * 2) : make_float2(kNegBig, 0.f);
         const float2 x1 = in ? *(const float2*)(a.ws_ml + (sl + h1) * 2) : make_float2(kNegBig, 0.f);
-        // Partials with l = 0 weigh nothing, whatever their m and o hold.
-        mm[u][0] = weighs(x0.y) ? x0.x : kNegBig, ll[u][0] = x0.y;
-        mm[u][1] = weighs(x1.y) ? x1.x : kNegBig, ll[u][1] = x1.y;
+        mm[u][0] = x0.x, ll[u][0] = x0.y;
+        mm[u][1] = x1.x, ll[u][1] = x1.y;
       }
       float f[2], e[R][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float Mn = Mh[h];
+        // Partials with l = 0 weigh nothing, whatever their m and o hold.
+        bool in[R];
 #pragma unroll
-        for (int u = 0; u < R; ++u) Mn = fmaxf(Mn, mm[u][h]);
+        for (int u = 0; u < R; ++u) in[u] = weighs(ll[u][h]);
+#pragma unroll
+        for (int u = 0; u < R; ++u) Mn = fmaxf(Mn, in[u] ? mm[u][h] : kNegBig);
         f[h] = fast_exp2(Mh[h] - Mn);
         float Ln = Lh[h] * f[h];
 #pragma unroll
         for (int u = 0; u < R; ++u) {
-          e[u][h] = weighs(ll[u][h]) ? fast_exp2(mm[u][h] - Mn) : 0.f;
+          e[u][h] = in[u] ? fast_exp2(mm[u][h] - Mn) : 0.f;
           Ln += ll[u][h] * e[u][h];
         }
         Mh[h] = Mn, Lh[h] = Ln;

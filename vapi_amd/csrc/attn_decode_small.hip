@@ -348,27 +348,28 @@ __global__ __launch_bounds__(64 * kSmallWaves) void paged_decode_small_merge(
     if (part < parts && c < a.group) {
       constexpr uint32_t kB = 8;  // splits per round trip
       for (uint32_t s0 = part; s0 < n_split; s0 += kB * parts) {
-        float2 ml[kB];
+        uint2 ml[kB];  // (bits: weighs)
         float4 y[kB];
 #pragma unroll
         for (uint32_t u = 0; u < kB; ++u) {
           const uint32_t s = s0 + u * parts;
           const bool in = s < n_split;
           const uint64_t slot = ((uint64_t)blockIdx.x * n_split + (in ? s : part)) * a.group + c;
-          ml[u] = *(const float2*)(a.ws_ml + slot * 2);
+          ml[u] = *(const uint2*)(a.ws_ml + slot * 2);
           y[u] = *(const float4*)(a.ws_o + slot * D + d);
-          if (!in) ml[u].y = 0.f;
+          if (!in) ml[u].y = 0u;
         }
         float Mn = M;
 #pragma unroll
-        for (uint32_t u = 0; u < kB; ++u) Mn = fmaxf(Mn, weighs(ml[u].y) ? ml[u].x : kNegBig);
+        for (uint32_t u = 0; u < kB; ++u)
+          Mn = fmaxf(Mn, weighs(ml[u].y) ? __uint_as_float(ml[u].x) : kNegBig);
         const float f = fast_exp2(M - Mn);
         L *= f, x.x *= f, x.y *= f, x.z *= f, x.w *= f;
 #pragma unroll
         for (uint32_t u = 0; u < kB; ++u) {
           if (!weighs(ml[u].y)) continue;  // a share without keys, or past the last
-          const float w = fast_exp2(ml[u].x - Mn);
-          L += ml[u].y * w;
+          const float w = fast_exp2(__uint_as_float(ml[u].x) - Mn);
+          L += __uint_as_float(ml[u].y) * w;
           x.x += y[u].x * w, x.y += y[u].y * w, x.z += y[u].z * w, x.w += y[u].w * w;
         }
         M = Mn;

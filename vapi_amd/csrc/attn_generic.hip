@@ -396,13 +396,14 @@ __global__ __launch_bounds__(kGenThreads) void paged_attn_generic_merge(
 #pragma unroll
   for (int i = 0; i < kMaxDPer; ++i) o[i] = 0.f;
   for (int32_t c0 = c_first; c0 <= c_last; c0 += kB) {
-    float m[kB], l[kB], x[kB][kMaxDPer];
+    float m[kB], x[kB][kMaxDPer];
+    uint32_t l[kB];  // (bits: weighs)
 #pragma unroll
     for (int u = 0; u < kB; ++u) {
       const bool in = c0 + u <= c_last && !skipped(c0 + u);
       const float* pc = part + (base + (in ? c0 + u : c_first)) * stride;
       m[u] = pc[2 * pr];
-      l[u] = in ? pc[2 * pr + 1] : 0.f;
+      l[u] = in ? ((const uint32_t*)pc)[2 * pr + 1] : 0u;
 #pragma unroll
       for (int i = 0; i < kMaxDPer; ++i) {
         const uint32_t d = pd + 16 * i;
@@ -421,7 +422,7 @@ __global__ __launch_bounds__(kGenThreads) void paged_attn_generic_merge(
     for (int u = 0; u < kB; ++u) {
       if (!weighs(l[u])) continue;  // a chunk no key of this row is visible in
       const float e = __expf(m[u] - Mn);
-      L += l[u] * e;
+      L += __uint_as_float(l[u]) * e;
 #pragma unroll
       for (int i = 0; i < kMaxDPer; ++i) o[i] += x[u][i] * e;
     }

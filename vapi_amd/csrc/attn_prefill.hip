@@ -377,20 +377,20 @@ __device__ __forceinline__ void prefill_merge_rows(const AttnArgs& a, uint32_t s
   constexpr uint32_t kB = 8;
   float M = kNegBig, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
   for (uint32_t s0 = 0; s0 < n_split; s0 += kB) {
-    float2 ml[kB];
+    uint2 ml[kB];  // (bits: weighs)
     float4 xb[kB];
 #pragma unroll
     for (uint32_t u = 0; u < kB; ++u) {
       const bool in = s0 + u < n_split;
       const char* pr = partial(in ? s0 + u : s0);
-      ml[u] = *(const float2*)(pr + ml_off);
+      ml[u] = *(const uint2*)(pr + ml_off);
       xb[u] = *(const float4*)(pr + o_off);
-      if (!in) ml[u].y = 0.f;
+      if (!in) ml[u].y = 0u;
     }
     float Mn = M;
 #pragma unroll
     for (uint32_t u = 0; u < kB; ++u)
-      if (weighs(ml[u].y)) Mn = fmaxf(Mn, ml[u].x);
+      if (weighs(ml[u].y)) Mn = fmaxf(Mn, __uint_as_float(ml[u].x));
     const float f = fast_exp2(M - Mn);
     L *= f;
 #pragma unroll
@@ -398,8 +398,8 @@ __device__ __forceinline__ void prefill_merge_rows(const AttnArgs& a, uint32_t s
 #pragma unroll
     for (uint32_t u = 0; u < kB; ++u) {
       if (!weighs(ml[u].y)) continue;  // a share with no visible key (its o is stale)
-      const float e = fast_exp2(ml[u].x - Mn);
-      const float w = ml[u].y * e;  // the partial's o is o / l
+      const float e = fast_exp2(__uint_as_float(ml[u].x) - Mn);
+      const float w = __uint_as_float(ml[u].y) * e;  // the partial's o is o / l
       L += w;
       o[0] += xb[u].x * w, o[1] += xb[u].y * w;
       o[2] += xb[u].z * w, o[3] += xb[u].w * w;

@@ -796,17 +796,17 @@ __device__ __forceinline__ void sh_merge(const AttnArgs& a, const SharedArgs& sh
   // The second four outputs are D / 2 on (past a.hd: the first again, not stored).
   const uint32_t d2 = NV > 1 && dq + D / 2 < a.hd ? D / 2 : 0;
   float M = kNegBig, L = 0.f, o[4 * NV] = {};
-  float2 ml[kB];
+  uint2 ml[kB];  // (bits: weighs)
   float4 x[kB][NV];
   // Partials [j0, j0 + kB) of the n at (m, l) pm(j) and o px(j).
   auto fetch = [&](uint32_t j0, uint32_t n, auto at) __attribute__((always_inline)) {
 #pragma unroll
     for (uint32_t u = 0; u < kB; ++u) {
-      ml[u].y = 0.f;
+      ml[u].y = 0u;
       if (j0 + u >= n) continue;
       const float *pm, *px;
       at(j0 + u, pm, px);
-      ml[u] = *(const float2*)pm;
+      ml[u] = *(const uint2*)pm;
 #pragma unroll
       for (int v = 0; v < NV; ++v) x[u][v] = *(const float4*)(px + v * d2);
     }
@@ -816,7 +816,7 @@ __device__ __forceinline__ void sh_merge(const AttnArgs& a, const SharedArgs& sh
     float Mn = M;
 #pragma unroll
     for (uint32_t u = 0; u < kB; ++u)
-      if (weighs(ml[u].y)) Mn = fmaxf(Mn, ml[u].x);
+      if (weighs(ml[u].y)) Mn = fmaxf(Mn, __uint_as_float(ml[u].x));
     const float f = fast_exp2(M - Mn);
     L *= f;
 #pragma unroll
@@ -824,8 +824,9 @@ __device__ __forceinline__ void sh_merge(const AttnArgs& a, const SharedArgs& sh
 #pragma unroll
     for (uint32_t u = 0; u < kB; ++u) {
       if (!weighs(ml[u].y)) continue;  // a share with no visible key (its o is stale)
-      const float e = fast_exp2(ml[u].x - Mn), wgt = normed ? ml[u].y * e : e;
-      L += ml[u].y * e;
+      const float e = fast_exp2(__uint_as_float(ml[u].x) - Mn), l = __uint_as_float(ml[u].y);
+      const float wgt = normed ? l * e : e;
+      L += l * e;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         o[4 * v] += x[u][v].x * wgt, o[4 * v + 1] += x[u][v].y * wgt;
