@@ -586,3 +586,53 @@ def test_a_plan_on_another_device_is_refused(fmt):
         paged_attention_append_prepared(q, k, k, scatter_index(np.array([0, 1]), DEV), cache, 0, prep,
                                         0.1)
     assert torch.equal(before.view(torch.uint8), cache.k[0].view(torch.uint8))
+
+
+@pytest.mark.parametrize("fmt,layout", [("none", "HND"), ("e4m3", "NHD"), ("int8", "HND")])
+def test_a_write_and_its_attention_behind_a_window_with_sinks(fmt, layout):
+    """A layer's call of a windowed model over shared prefixes, members in and out of the
+    prefix's reach."""
+    members = [(1, 20), (1, 333), (4, 90), (1, 64), (9, 200)]
+    cache, q, batch, plan = make([(20, members), (4, [(1, 300), (2, 400)])], [(1, 50), (3, 3)], 8, 2,
+                                 64, BF16, fmt=fmt, layout=layout)
+    cq, ck = batch.cu_seqlens_q, batch.cu_seqlens_k
+    slots = [t[p // 16] * 16 + p % 16 for i, t in enumerate(batch.block_tables)
+             for p in range(ck[i + 1] - ck[i] - (cq[i + 1] - cq[i]), ck[i + 1] - ck[i])]
+    k, v = (torch.randn(len(slots), 2, 64, device=DEV).to(BF16) for _ in range(2))
+    prep = prepare(batch, cache, 8, plan)
+    got = paged_attention_append_prepared(q, k, v, scatter_index(np.array(slots), DEV), cache, 0,
+                                          prep, 0.125, 63, 0, sinks=4)
+    assert_close(got, reference(q, cache, batch, 0.125, 63, 0, 4), BF16)
+
+
+@pytest.mark.parametrize("fmt", ["none", "int8"])
+def test_a_graph_replays_while_windows_leave_the_prefix(fmt):
+    """Two graphs over one workspace, a windowed layer with sinks and one without a window;
+    the lengths on the device grow until no window reaches the prefix."""
+    cache, q, batch, plan = make([(12, decode(5, 26, 30, 1))], decode(2, 10, 300, 2), 8, 2, 128,
+                                 BF16, shuffle=False, fmt=fmt)
+    spare = [b for b in range(cache.num_slots() // 16)
+             if not any(b in t for t in batch.block_tables)]
+    for i, t in enumerate(batch.block_tables):  # room to grow in blocks of the pool
+        t.append(spare[i % len(spare)])
+    batch.max_seqlen_k += 12
+    prep = prepare(batch, cache, 8, plan, deterministic=True)
+    calls = [(None, 0), (29, 3)]
+    outs, graphs = [torch.empty_like(q) for _ in calls], []
+    for out, (left, sinks) in zip(outs, calls):
+        paged_attention_prepared(q, cache, 0, prep, 0.1, left, 0, out=out, sinks=sinks)
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            paged_attention_prepared(q, cache, 0, prep, 0.1, left, 0, out=out, sinks=sinks)
+    for step in range(4):
+        for out, graph in zip(outs, graphs):
+            out.fill_(float("nan"))
+            graph.replay()
+        torch.cuda.synchronize()
+        for out, (left, sinks) in zip(outs, calls):
+            assert_close(out, reference(q, cache, batch, 0.1, left, 0, sinks), BF16)
+            assert torch.equal(out, paged_attention_prepared(q, cache, 0, prep, 0.1, left, 0,
+                                                             sinks=sinks))
+        torch.cuda.synchronize()
+        batch.cu_seqlens_k = [x + 3 * i for i, x in enumerate(batch.cu_seqlens_k)]
+        prep.seqlens_k.copy_(torch.tensor(batch.cu_seqlens_k, dtype=torch.int32))
