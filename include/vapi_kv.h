@@ -369,9 +369,9 @@ typedef struct vapi_kv_prefixes {
  * sequence. Any lengths, windows and sinks; sequences in no group, decode rows and
  * prefill rows as there. prefill_seqs lists the sequences with len_q > 1, each once
  * (NULL with n_prefill == 0: all of them); a sequence with len_q > 1 that it leaves out
- * gets no output, or in a group one without its own keys. Like the block table the lists are trusted:
- * entries that name no query of the batch are left out, and a group whose sequences'
- * tables differ attends the first one's blocks.
+ * gets no output, or in a group one without its own keys. Like the block table the lists
+ * are trusted: entries that name no query of the batch are left out, and a group whose
+ * sequences' tables differ attends the blocks of its first entry that names one.
  *
  * f16 and bf16 pools with head_dim a multiple of 8 up to 256 and block_size a power of
  * two from 16, up to 256 query heads per kv head, 4,096 sequences and 1,000 groups and

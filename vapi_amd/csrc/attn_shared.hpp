@@ -25,7 +25,7 @@
 // tile (a range leaves at most one open).
 //
 // Measured, us a call (without sharing), 32 q / 8 kv heads of 128 in bf16: 64 sequences
-// over 4,096 shared keys 42.6 (172), 4-8 queries each of 16 over 3,200 45.6 (72); 64 q
+// over 4,096 shared keys 43.2 (172), 4-8 queries each of 16 over 3,200 45.4 (72); 64 q
 // heads, 128 sequences over 32,768 224-230 (2,485), 620 TFLOP/s. Long prefixes are bound
 // by the tiles' step (25% MFMA, 29% VALU, waits at 2 waves a SIMD), short ones by round
 // trips, 4-10 us each while the stream keeps HBM's queues full, and by the merge, 6-15.
