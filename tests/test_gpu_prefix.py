@@ -636,3 +636,10 @@ def test_a_graph_replays_while_windows_leave_the_prefix(fmt):
         torch.cuda.synchronize()
         batch.cu_seqlens_k = [x + 3 * i for i, x in enumerate(batch.cu_seqlens_k)]
         prep.seqlens_k.copy_(torch.tensor(batch.cu_seqlens_k, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("d,fmt", [(128, "none"), (64, "int8"), (256, "e4m3")])
+def test_sinks_of_more_members_than_entries_in_lds(d, fmt):
+    """Tiles past every window beside tiles in reach, their rows looked up one by one."""
+    check([(3, [(1, 42 + i % 30) for i in range(700)] + [(1, 1 + i % 39) for i in range(500)])],
+          [(1, 90)], 2, 1, d, BF16, 40, 5, fmt=fmt, shuffle=False)
